@@ -158,7 +158,12 @@ def exported_symbols():
                                        "mlk_linear_planar_workspace_bytes",
                                        # bound with their structs in forward.py
                                        "mlk_forward_layer_workspace_bytes",
-                                       "mlk_forward_layer_batch"])
+                                       "mlk_forward_layer_batch",
+                                       # and in paged.py
+                                       "mlk_paged_kv_append", "mlk_attention_paged",
+                                       "mlk_attention_paged_workspace_bytes",
+                                       "mlk_attention_packed",
+                                       "mlk_attention_packed_workspace_bytes"])
 
 
 # ------------------------------------------------------------------ runtime

@@ -1,0 +1,449 @@
+// mlk_paged.hip -- new tokens of many sequences into a paged KV cache, RoPE on
+// the way, and the C entries of the attention over it (kernels: mlk_ragged.hip).
+//
+// Append: token row t of sequence s is position p = seq_len[s] - (start[s + 1]
+// - t).  Pair i of a head of q or k turns by p * theta^(-2i / head_dim)
+// (float64 angle, cos, sin and rotation, rounded to float as mlk_rope_f32
+// does, then to the type stored); k and v rows go to page table[s][p /
+// page_size], row p % page_size.  Bound by bytes: it reads q, k and v and
+// writes q and the two cache rows once.
+//
+// One workgroup per token: its first threads evaluate the token's angles into
+// shared memory (every head of q and k turns by the same ones), all threads
+// then move units of 8 elements, 16 or 32 bytes a load.  A unit's 4 pairs are
+// neighbours (normal) or two runs of 4, half a head apart (NeoX).
+#include "mlk_paged.h"
+
+#include <climits>
+#include <cmath>
+
+namespace mlk {
+namespace {
+
+constexpr int kAppendThreads = 256;
+
+struct AppendArgs {
+    Ragged batch;
+    RowsAt rows;
+    const void *k, *v, *q;
+    void* q_out;
+    int64_t k_row, v_row, q_row, q_out_row;
+    int32_t n_heads, n_kv_heads;  // n_heads 0: no q
+    int32_t rope;                 // 0: none, 1: normal, 2: NeoX
+    int32_t* err;
+};
+
+// N elements of T from / to memory, through fp32.
+template <typename T, int N>
+__device__ inline void LoadN(const typename T::Bits* p, float* x) {
+    if constexpr (N == 1) {
+        x[0] = T::Get(*p);
+    } else {
+        typedef typename T::Bits Vec __attribute__((ext_vector_type(N)));
+        const Vec v = *reinterpret_cast<const Vec*>(p);
+#pragma unroll
+        for (int i = 0; i < N; ++i) x[i] = T::Get(v[i]);
+    }
+}
+template <typename T, int N>
+__device__ inline void StoreN(typename T::Bits* p, const float* x) {
+    if constexpr (N == 1) {
+        *p = T::Put(x[0]);
+    } else {
+        typedef typename T::Bits Vec __attribute__((ext_vector_type(N)));
+        Vec v;
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = T::Put(x[i]);
+        *reinterpret_cast<Vec*>(p) = v;
+    }
+}
+
+// PV pairs a unit (4, or 1 for odd sizes and alignments).
+template <typename A, typename C, int PV>
+__global__ __launch_bounds__(kAppendThreads) void PagedAppend(AppendArgs p, const RopeFreqs f) {
+    __shared__ double2 turn[kRopePairs];  // cos, sin of the token's pairs
+    const int tid = static_cast<int>(threadIdx.x);
+    const int32_t t = static_cast<int32_t>(blockIdx.x);
+    const int hd = p.rows.head_dim, half = (hd + 1) / 2;
+    if (t == 0) CheckSeqs(p.batch, p.err);
+    const int s = LastSeq(p.batch, t, [](int32_t a, int) { return a; });
+    Seq q;
+    if (!LoadSeq(p.batch, s, &q) || t < q.t0 || t >= q.t0 + q.n) return;
+    const int32_t pos = q.len - q.n + (t - q.t0);
+    bool bad = false;
+    const int32_t page = PageOf(p.rows, p.batch.table + s * p.batch.table_stride, pos, &bad);
+    if (bad && tid == 0) RaiseFlag(p.err, 1);
+    const int64_t at = PagedRow(p.rows, page, pos);
+    if (p.rope != 0) {
+        for (int i = tid; i < half; i += kAppendThreads) {
+            RopeCosSin(pos, f.inv[i], &turn[i].x, &turn[i].y);
+        }
+        __syncthreads();
+    }
+    typedef typename A::Bits AB;
+    typedef typename C::Bits CB;
+    const AB* rq = static_cast<const AB*>(p.q) + t * p.q_row;
+    const AB* rk = static_cast<const AB*>(p.k) + t * p.k_row;
+    const AB* rv = static_cast<const AB*>(p.v) + t * p.v_row;
+    AB* oq = static_cast<AB*>(p.q_out) + t * p.q_out_row;
+    CB* ok = static_cast<CB*>(const_cast<void*>(p.rows.k)) + at;
+    CB* ov = static_cast<CB*>(const_cast<void*>(p.rows.v)) + at;
+    const int groups = half / PV;
+    const int units = (p.n_heads + 2 * p.n_kv_heads) * groups;
+    for (int u = tid; u < units; u += kAppendThreads) {
+        const int h = u / groups, g = u % groups;
+        const bool is_q = h < p.n_heads, is_v = h >= p.n_heads + p.n_kv_heads;
+        if (!is_q && bad) continue;
+        const int kh = is_v ? h - p.n_heads - p.n_kv_heads : h - p.n_heads;
+        const int64_t o = static_cast<int64_t>(is_q ? h : kh) * hd;
+        const AB* src = (is_q ? rq : is_v ? rv : rk) + o;
+        // the unit's two runs: x0[i] at e0 + i * step, its partner x1[i]
+        const bool apart = p.rope == 2;
+        float x0[PV], x1[PV];
+        int e0, e1;
+        if constexpr (PV == 1) {
+            e0 = apart ? g : 2 * g;
+            e1 = apart ? g + half : 2 * g + 1;
+            x0[0] = A::Get(src[e0]);
+            x1[0] = e1 < hd ? A::Get(src[e1]) : 0.0f;
+        } else {
+            e0 = apart ? PV * g : 2 * PV * g;
+            e1 = apart ? e0 + half : e0 + PV;
+            float a[PV], b[PV];
+            LoadN<A, PV>(src + e0, a);
+            LoadN<A, PV>(src + e1, b);
+#pragma unroll
+            for (int i = 0; i < PV; ++i) {
+                x0[i] = apart ? a[i] : (2 * i < PV ? a[2 * i] : b[2 * i - PV]);
+                x1[i] = apart ? b[i] : (2 * i < PV ? a[2 * i + 1] : b[2 * i + 1 - PV]);
+            }
+        }
+        if (p.rope != 0 && !is_v) {
+#pragma unroll
+            for (int i = 0; i < PV; ++i) {
+                const double2 c = turn[g * PV + i];
+                RopeRotate(x0[i], x1[i], c.x, c.y, &x0[i], &x1[i]);
+            }
+        }
+        if constexpr (PV == 1) {
+            if (is_q) {
+                oq[o + e0] = A::Put(x0[0]);
+                if (e1 < hd) oq[o + e1] = A::Put(x1[0]);
+            } else {
+                CB* d = (is_v ? ov : ok) + o;
+                d[e0] = C::Put(x0[0]);
+                if (e1 < hd) d[e1] = C::Put(x1[0]);
+            }
+        } else {
+            float a[PV], b[PV];
+#pragma unroll
+            for (int i = 0; i < PV; ++i) {
+                a[i] = apart ? x0[i] : (i % 2 ? x1[i / 2] : x0[i / 2]);
+                b[i] = apart ? x1[i] : (i % 2 ? x1[(PV + i) / 2] : x0[(PV + i) / 2]);
+            }
+            if (is_q) {
+                StoreN<A, PV>(oq + o + e0, a);
+                StoreN<A, PV>(oq + o + e1, b);
+            } else {
+                CB* d = (is_v ? ov : ok) + o;
+                StoreN<C, PV>(d + e0, a);
+                StoreN<C, PV>(d + e1, b);
+            }
+        }
+    }
+}
+
+template <typename A, typename C>
+void LaunchAppend(const AppendArgs& p, const RopeFreqs& f, bool wide, hipStream_t s) {
+    const dim3 grid(static_cast<unsigned>(p.batch.n_tokens));
+    if (wide) {
+        hipLaunchKernelGGL((PagedAppend<A, C, 4>), grid, dim3(kAppendThreads), 0, s, p, f);
+    } else {
+        hipLaunchKernelGGL((PagedAppend<A, C, 1>), grid, dim3(kAppendThreads), 0, s, p, f);
+    }
+}
+
+bool KnownType(int32_t t) { return t == MLK_F32 || t == MLK_F16 || t == MLK_BF16; }
+
+}  // namespace
+
+mlk_status CheckElements(const char* fn, const char* name, const void* p, int32_t type) {
+    if (p == nullptr) return Fail(MLK_ERR_INVALID, "%s: %s must not be null", fn, name);
+    if (!Aligned(p, TypeBytes(type))) {
+        return Fail(MLK_ERR_INVALID, "%s: %s must be %d-byte aligned", fn, name, TypeBytes(type));
+    }
+    return MLK_OK;
+}
+
+mlk_status CheckHeads(const char* fn, int32_t n_heads, int32_t n_kv_heads, int32_t head_dim,
+                      float scale) {
+    if (n_heads <= 0 || n_kv_heads <= 0 || n_heads % n_kv_heads != 0) {
+        return Fail(MLK_ERR_INVALID, "%s: n_heads must be a positive multiple of n_kv_heads", fn);
+    }
+    if (n_heads > 65536) {
+        return Fail(MLK_ERR_INVALID, "%s: more than 65536 heads", fn);
+    }
+    if (head_dim < 1 || head_dim > 256) {
+        return Fail(MLK_ERR_INVALID, "%s: head_dim must be in 1..256", fn);
+    }
+    if (!std::isfinite(scale) || scale <= 0.0f) {
+        return Fail(MLK_ERR_INVALID, "%s: scale must be finite and positive", fn);
+    }
+    return MLK_OK;
+}
+
+mlk_status CheckPaged(const char* fn, const mlk_paged_cache* cache, const mlk_paged_batch* batch,
+                      int32_t type, PagedArgs* args) {
+    if (cache == nullptr || batch == nullptr) {
+        return Fail(MLK_ERR_INVALID, "%s: cache and batch must not be null", fn);
+    }
+    const mlk_paged_cache& c = *cache;
+    const mlk_paged_batch& b = *batch;
+    if (!KnownType(type) || !KnownType(c.type)) {
+        return Fail(MLK_ERR_INVALID, "%s: unknown element type", fn);
+    }
+    if (type != MLK_F32 && type != c.type) {
+        return Fail(MLK_ERR_INVALID, "%s: 16-bit activations need a cache of their own type", fn);
+    }
+    if (c.n_kv_heads <= 0 || c.n_kv_heads > 65536) {
+        return Fail(MLK_ERR_INVALID, "%s: n_kv_heads must be in 1..65536", fn);
+    }
+    if (c.head_dim < 1 || c.head_dim > 256) {
+        return Fail(MLK_ERR_INVALID, "%s: head_dim must be in 1..256", fn);
+    }
+    if (c.page_size < 1 || c.page_size > (1 << 20) || (c.page_size & (c.page_size - 1)) != 0) {
+        return Fail(MLK_ERR_INVALID, "%s: page_size must be a power of two up to 2^20", fn);
+    }
+    if (c.n_pages < 1 || c.n_pages > INT32_MAX) {
+        return Fail(MLK_ERR_INVALID, "%s: n_pages must be in 1..2^31 - 1", fn);
+    }
+    const int64_t slot = static_cast<int64_t>(c.n_kv_heads) * c.head_dim;
+    if (c.page_stride < c.page_size * slot || c.page_stride > INT64_MAX / 4 / c.n_pages) {
+        return Fail(MLK_ERR_INVALID,
+                    "%s: page_stride must cover page_size * n_kv_heads * head_dim elements", fn);
+    }
+    mlk_status st = CheckElements(fn, "k pages", c.k, c.type);
+    if (st != MLK_OK) return st;
+    st = CheckElements(fn, "v pages", c.v, c.type);
+    if (st != MLK_OK) return st;
+    if (c.k == c.v) return Fail(MLK_ERR_INVALID, "%s: k and v pages must be distinct", fn);
+    if (b.n_seqs < 0 || b.n_seqs > (1 << 24)) {
+        return Fail(MLK_ERR_INVALID, "%s: n_seqs must be in 0..2^24", fn);
+    }
+    if (b.n_tokens < 0 || b.n_tokens > (1 << 28)) {
+        return Fail(MLK_ERR_INVALID, "%s: n_tokens must be in 0..2^28", fn);
+    }
+    int shift = 0;
+    while ((1 << shift) < c.page_size) ++shift;
+    *args = {};
+    args->rows = {c.k, c.v, c.page_stride, slot, slot, shift, static_cast<int32_t>(c.n_pages),
+                  c.head_dim};
+    if (b.n_seqs == 0 || b.n_tokens == 0) return MLK_OK;  // nothing to do
+    if (b.token_start == nullptr || b.seq_len == nullptr || b.page_table == nullptr) {
+        return Fail(MLK_ERR_INVALID, "%s: token_start, seq_len and page_table must not be null",
+                    fn);
+    }
+    if (!Aligned(b.token_start, 4) || !Aligned(b.seq_len, 4) || !Aligned(b.page_table, 4)) {
+        return Fail(MLK_ERR_INVALID,
+                    "%s: token_start, seq_len and page_table must be 4-byte aligned", fn);
+    }
+    if (b.max_new_tokens < 1 || b.max_seq_len < 1 || b.max_seq_len > (1 << 30)) {
+        return Fail(MLK_ERR_INVALID,
+                    "%s: max_new_tokens must be positive and max_seq_len in 1..2^30", fn);
+    }
+    if (b.table_stride < 1 || b.table_stride > INT32_MAX ||
+        b.max_seq_len > b.table_stride * c.page_size) {
+        return Fail(MLK_ERR_INVALID, "%s: max_seq_len exceeds table_stride * page_size", fn);
+    }
+    int64_t max_new = b.max_new_tokens < b.max_seq_len ? b.max_new_tokens : b.max_seq_len;
+    if (max_new > b.n_tokens) max_new = b.n_tokens;
+    args->batch = {b.token_start, b.seq_len, b.page_table, b.table_stride,
+                   static_cast<int32_t>(b.n_seqs), static_cast<int32_t>(b.n_tokens),
+                   static_cast<int32_t>(max_new), static_cast<int32_t>(b.max_seq_len)};
+    return MLK_OK;
+}
+
+}  // namespace mlk
+
+using namespace mlk;
+
+extern "C" {
+
+mlk_status mlk_paged_kv_append(const mlk_paged_cache* cache, const mlk_paged_batch* batch,
+                               int32_t type, const void* k, int64_t k_row_stride, const void* v,
+                               int64_t v_row_stride, const void* q, int64_t q_row_stride,
+                               void* q_out, int64_t q_out_row_stride, int32_t n_heads,
+                               float theta, int32_t rope_type, int32_t* err, void* stream) {
+    const char* fn = "mlk_paged_kv_append";
+    PagedArgs a;
+    mlk_status st = CheckPaged(fn, cache, batch, type, &a);
+    if (st != MLK_OK) return st;
+    const int32_t hd = cache->head_dim, KV = cache->n_kv_heads;
+    const int64_t slot = static_cast<int64_t>(KV) * hd;
+    st = CheckElements(fn, "k", k, type);
+    if (st != MLK_OK) return st;
+    st = CheckElements(fn, "v", v, type);
+    if (st != MLK_OK) return st;
+    if (k_row_stride < slot || v_row_stride < slot) {
+        return Fail(MLK_ERR_INVALID, "%s: row strides must be at least n_kv_heads * head_dim", fn);
+    }
+    if (!std::isfinite(theta) || theta < 0.0f) {
+        return Fail(MLK_ERR_INVALID, "%s: theta must be finite and not negative", fn);
+    }
+    if (theta != 0.0f) {
+        if (rope_type != MLK_ROPE_NORMAL && rope_type != MLK_ROPE_NEOX) {
+            return Fail(MLK_ERR_INVALID, "%s: unknown rope type %d", fn, rope_type);
+        }
+        if (hd % 2 != 0) return Fail(MLK_ERR_INVALID, "%s: head_dim must be even", fn);
+    } else if (q != nullptr) {
+        return Fail(MLK_ERR_INVALID, "%s: theta 0 rotates nothing: q must be null", fn);
+    }
+    bool wide_q = true;
+    if (q != nullptr) {
+        st = CheckElements(fn, "q", q, type);
+        if (st != MLK_OK) return st;
+        st = CheckElements(fn, "q_out", q_out, type);
+        if (st != MLK_OK) return st;
+        if (n_heads <= 0 || n_heads > 65536) {
+            return Fail(MLK_ERR_INVALID, "%s: n_heads must be in 1..65536", fn);
+        }
+        const int64_t width = static_cast<int64_t>(n_heads) * hd;
+        if (q_row_stride < width || q_out_row_stride < width) {
+            return Fail(MLK_ERR_INVALID, "%s: row strides must be at least n_heads * head_dim",
+                        fn);
+        }
+        if (q_out == q && q_out_row_stride != q_row_stride) {
+            return Fail(MLK_ERR_INVALID, "%s: q in place needs equal row strides", fn);
+        }
+        if (q_out == k || q_out == v || q_out == cache->k || q_out == cache->v) {
+            return Fail(MLK_ERR_INVALID, "%s: q_out may not alias k, v or the pages", fn);
+        }
+        wide_q = q_row_stride % 4 == 0 && q_out_row_stride % 4 == 0 &&
+                 Aligned(q, 4 * TypeBytes(type)) && Aligned(q_out, 4 * TypeBytes(type));
+    }
+    if (k == cache->k || k == cache->v || v == cache->k || v == cache->v) {
+        return Fail(MLK_ERR_INVALID, "%s: k and v may not alias the pages", fn);
+    }
+    if (a.batch.n_seqs == 0) return MLK_OK;
+    const bool neox = theta != 0.0f && rope_type == MLK_ROPE_NEOX;
+    AppendArgs p{};
+    p.batch = a.batch;
+    p.rows = a.rows;
+    p.k = k;
+    p.v = v;
+    p.q = q;
+    p.q_out = q_out;
+    p.k_row = k_row_stride;
+    p.v_row = v_row_stride;
+    p.q_row = q != nullptr ? q_row_stride : 0;
+    p.q_out_row = q != nullptr ? q_out_row_stride : 0;
+    p.n_heads = q != nullptr ? n_heads : 0;
+    p.n_kv_heads = KV;
+    p.rope = theta == 0.0f ? 0 : neox ? 2 : 1;
+    p.err = err;
+    const int ab = TypeBytes(type), cb = TypeBytes(cache->type);
+    const bool wide = hd % 8 == 0 && wide_q && k_row_stride % 4 == 0 && v_row_stride % 4 == 0 &&
+                      cache->page_stride % 4 == 0 && Aligned(k, 4 * ab) && Aligned(v, 4 * ab) &&
+                      Aligned(cache->k, 4 * cb) && Aligned(cache->v, 4 * cb);
+    const RopeFreqs f = p.rope != 0 ? MakeRopeFreqs(theta, hd) : RopeFreqs{};
+    const hipStream_t s = AsStream(stream);
+    if (type == MLK_F32) {
+        if (cache->type == MLK_F32) LaunchAppend<F32, F32>(p, f, wide, s);
+        else if (cache->type == MLK_F16) LaunchAppend<F32, F16>(p, f, wide, s);
+        else LaunchAppend<F32, BF16>(p, f, wide, s);
+    } else if (type == MLK_F16) {
+        LaunchAppend<F16, F16>(p, f, wide, s);
+    } else {
+        LaunchAppend<BF16, BF16>(p, f, wide, s);
+    }
+    return CheckLaunch("PagedAppend");
+}
+
+mlk_status mlk_attention_paged(const mlk_paged_cache* cache, const mlk_paged_batch* batch,
+                               int32_t type, const void* q, int64_t q_row_stride, void* out,
+                               int32_t n_heads, float scale, void* workspace,
+                               size_t workspace_bytes, int32_t* err, void* stream) {
+    const char* fn = "mlk_attention_paged";
+    PagedArgs a;
+    mlk_status st = CheckPaged(fn, cache, batch, type, &a);
+    if (st != MLK_OK) return st;
+    st = CheckHeads(fn, n_heads, cache->n_kv_heads, cache->head_dim, scale);
+    if (st != MLK_OK) return st;
+    st = CheckElements(fn, "q", q, type);
+    if (st != MLK_OK) return st;
+    st = CheckElements(fn, "out", out, type);
+    if (st != MLK_OK) return st;
+    if (q_row_stride < static_cast<int64_t>(n_heads) * cache->head_dim) {
+        return Fail(MLK_ERR_INVALID, "%s: q_row_stride must be at least n_heads * head_dim", fn);
+    }
+    if (out == q || out == cache->k || out == cache->v) {
+        return Fail(MLK_ERR_INVALID, "%s: out may not alias q or the pages", fn);
+    }
+    if (workspace != nullptr && !Aligned(workspace, 16)) {
+        return Fail(MLK_ERR_INVALID, "%s: workspace must be 16-byte aligned", fn);
+    }
+    if (a.batch.n_seqs == 0) return MLK_OK;
+    return Attend({a.batch, a.rows, type, cache->type, q, q_row_stride, out, n_heads,
+                   cache->n_kv_heads, scale, workspace, workspace == nullptr ? 0 : workspace_bytes,
+                   err, AsStream(stream)});
+}
+
+int64_t mlk_attention_paged_workspace_bytes(int64_t n_seqs, int64_t n_tokens,
+                                            int64_t max_new_tokens, int64_t max_seq_len,
+                                            int32_t n_heads, int32_t n_kv_heads,
+                                            int32_t head_dim) {
+    return AttendWorkspace(n_seqs, n_tokens, max_new_tokens, max_seq_len, n_heads, n_kv_heads,
+                           head_dim);
+}
+
+mlk_status mlk_attention_packed(int32_t type, const void* q, int64_t q_row_stride, const void* k,
+                                int64_t k_row_stride, const void* v, int64_t v_row_stride,
+                                const int32_t* seq_start, int64_t n_seqs, int64_t n_tokens,
+                                int64_t max_seq_len, int32_t n_heads, int32_t n_kv_heads,
+                                int32_t head_dim, float scale, void* out, void* workspace,
+                                size_t workspace_bytes, int32_t* err, void* stream) {
+    const char* fn = "mlk_attention_packed";
+    if (!KnownType(type)) return Fail(MLK_ERR_INVALID, "%s: unknown element type", fn);
+    mlk_status st = CheckHeads(fn, n_heads, n_kv_heads, head_dim, scale);
+    if (st != MLK_OK) return st;
+    const char* names[4] = {"q", "k", "v", "out"};
+    const void* ptrs[4] = {q, k, v, out};
+    for (int i = 0; i < 4; ++i) {
+        st = CheckElements(fn, names[i], ptrs[i], type);
+        if (st != MLK_OK) return st;
+    }
+    const int64_t slot = static_cast<int64_t>(n_kv_heads) * head_dim;
+    if (q_row_stride < static_cast<int64_t>(n_heads) * head_dim || k_row_stride < slot ||
+        v_row_stride < slot) {
+        return Fail(MLK_ERR_INVALID, "%s: row strides must be at least heads * head_dim", fn);
+    }
+    if (out == q || out == k || out == v) {
+        return Fail(MLK_ERR_INVALID, "%s: out may not alias q, k or v", fn);
+    }
+    if (n_seqs < 0 || n_seqs > (1 << 24) || n_tokens < 0 || n_tokens > (1 << 28)) {
+        return Fail(MLK_ERR_INVALID, "%s: n_seqs must be in 0..2^24 and n_tokens in 0..2^28", fn);
+    }
+    if (workspace != nullptr && !Aligned(workspace, 16)) {
+        return Fail(MLK_ERR_INVALID, "%s: workspace must be 16-byte aligned", fn);
+    }
+    if (n_seqs == 0 || n_tokens == 0) return MLK_OK;
+    if (seq_start == nullptr || !Aligned(seq_start, 4)) {
+        return Fail(MLK_ERR_INVALID, "%s: seq_start must be a 4-byte aligned device array", fn);
+    }
+    if (max_seq_len < 1) return Fail(MLK_ERR_INVALID, "%s: max_seq_len must be positive", fn);
+    const int32_t T = static_cast<int32_t>(n_tokens);
+    const int32_t most = max_seq_len < n_tokens ? static_cast<int32_t>(max_seq_len) : T;
+    const Ragged b{seq_start, nullptr, nullptr, 0, static_cast<int32_t>(n_seqs), T, most, most};
+    const RowsAt r{k, v, 0, k_row_stride, v_row_stride, 0, 0, head_dim};
+    return Attend({b, r, type, type, q, q_row_stride, out, n_heads, n_kv_heads, scale, workspace,
+                   workspace == nullptr ? 0 : workspace_bytes, err, AsStream(stream)});
+}
+
+int64_t mlk_attention_packed_workspace_bytes(int64_t n_seqs, int64_t n_tokens,
+                                             int64_t max_seq_len, int32_t n_heads,
+                                             int32_t n_kv_heads, int32_t head_dim) {
+    return AttendWorkspace(n_seqs, n_tokens, max_seq_len, max_seq_len, n_heads, n_kv_heads,
+                           head_dim);
+}
+
+}  // extern "C"

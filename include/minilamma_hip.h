@@ -332,6 +332,122 @@ mlk_status mlk_attention_prefill_f32(const float* q, int64_t q_row_stride, const
                                      int64_t layer, int32_t pos0, int64_t n_tokens, float* out,
                                      void* stream);
 
+/* --------------------------------------------------- many sequences at once
+ * A server's attention: the new tokens of several sequences in one batch,
+ * their keys and values in pages of one shared cache, and whole prompts of
+ * different lengths packed in one buffer.  No counterpart in the reference
+ * (one sequence, one contiguous cache). */
+
+/* Element types of activations and caches.  fp32 activations run over a cache
+ * of any type; 16-bit activations over a cache of their own type. */
+typedef enum { MLK_F32 = 0, MLK_F16 = 1, MLK_BF16 = 2 } mlk_float_type;
+
+/* One layer's pages, [n_pages, page_size, n_kv_heads, head_dim] of `type`:
+ * page g's first row is at k + g * page_stride elements.  page_size is a power
+ * of two; page_stride is at least page_size * n_kv_heads * head_dim (more where
+ * other layers' pages lie between). */
+typedef struct {
+    void* k;
+    void* v;
+    int32_t type;       /* mlk_float_type */
+    int32_t page_size;  /* positions a page holds */
+    int64_t n_pages;
+    int64_t page_stride;
+    int32_t n_kv_heads, head_dim;
+} mlk_paged_cache;
+
+/* The new tokens of n_seqs sequences: sequence s brings the token rows
+ * token_start[s] .. token_start[s + 1] - 1 (none is allowed), which are its
+ * last positions, seq_len[s] - count .. seq_len[s] - 1; position j of the
+ * sequence is row j % page_size of page page_table[s * table_stride +
+ * j / page_size].  The three arrays are read on the device, so a captured call
+ * replays with new values within the host's bounds: n_tokens token rows exist
+ * (rows behind token_start[n_seqs] are neither read nor written), no sequence
+ * brings over max_new_tokens, none is longer than max_seq_len
+ * (<= table_stride * page_size).  A sequence outside these bounds, or with more
+ * new tokens than its length, raises *err (NULL: no report; the caller clears
+ * it) and gets nothing written. */
+typedef struct {
+    const int32_t* token_start;  /* device [n_seqs + 1] */
+    const int32_t* seq_len;      /* device [n_seqs] */
+    const int32_t* page_table;   /* device [n_seqs, table_stride] */
+    int64_t n_seqs, n_tokens, table_stride, max_new_tokens, max_seq_len;
+} mlk_paged_batch;
+
+/*
+ * The new tokens' k and v (rows of n_kv_heads * head_dim elements of `type`,
+ * row t at k + t * k_row_stride) into their pages, k rotated on the way and,
+ * where q is not NULL, q (n_heads * head_dim elements a row) rotated into q_out
+ * (of the same type; q_out == q with equal strides rotates in place, otherwise
+ * the two do not overlap).  The rotation is mlk_rope_f32's: angles, cos and sin
+ * in float64, each result rounded once to the type it is stored in.  theta == 0:
+ * k is stored as it is, and q must be NULL.  k and v are only read.  Every
+ * position written belongs to one sequence of the batch (pages shared between
+ * sequences may be read by mlk_attention_paged, not appended to).  A page index
+ * outside [0, n_pages) raises *err and its row is not written.  head_dim 1..256,
+ * even where theta != 0.
+ */
+mlk_status mlk_paged_kv_append(const mlk_paged_cache* cache, const mlk_paged_batch* batch,
+                               int32_t type, const void* k, int64_t k_row_stride, const void* v,
+                               int64_t v_row_stride, const void* q, int64_t q_row_stride,
+                               void* q_out, int64_t q_out_row_stride, int32_t n_heads,
+                               float theta, int32_t rope_type, int32_t* err, void* stream);
+
+/*
+ * Attention of the batch's new tokens over their sequences' pages (the tokens'
+ * own rows already there, e.g. by mlk_paged_kv_append): token row t at
+ * position p of its sequence, query head i on KV head i / (n_heads /
+ * n_kv_heads),
+ *   s_j = scale (q_i . k_j),  w = softmax(s_0 .. s_p),  out[t, i] = sum_j w_j v_j
+ * for one new token per sequence (a decode step), several (a prompt's chunk) or
+ * both in one batch.  q rows and out (dense [n_tokens, n_heads, head_dim]) are
+ * of `type`; out must not overlap q or the pages.  head_dim 1..256.  Scores,
+ * statistics and sums are fp32.  With fp32 activations q and w enter the
+ * products in enough 16-bit pieces that each product is within 2^-20 of
+ * itself; with 16-bit ones w is rounded to that type.  What a token does not
+ * attend to (later positions, the rest of the last page) never changes its
+ * result, whatever bits lie there; a token that attends to a non-finite value
+ * gets non-finite results.  A page index outside [0, n_pages) raises *err and
+ * page 0 is read in its place.
+ *
+ * workspace: optional scratch (16-byte aligned,
+ * mlk_attention_paged_workspace_bytes(); it may differ between calls, its
+ * content does not matter).  With it few rows over long sequences split their
+ * positions over workgroups, the partial sums joined in a fixed order; without
+ * it (NULL or smaller) the call is correct, only slower.
+ */
+mlk_status mlk_attention_paged(const mlk_paged_cache* cache, const mlk_paged_batch* batch,
+                               int32_t type, const void* q, int64_t q_row_stride, void* out,
+                               int32_t n_heads, float scale, void* workspace,
+                               size_t workspace_bytes, int32_t* err, void* stream);
+/* Bytes of that workspace for these bounds on the current device (0: none). */
+int64_t mlk_attention_paged_workspace_bytes(int64_t n_seqs, int64_t n_tokens,
+                                            int64_t max_new_tokens, int64_t max_seq_len,
+                                            int32_t n_heads, int32_t n_kv_heads,
+                                            int32_t head_dim);
+
+/*
+ * Causal attention of whole prompts packed in one buffer: sequence s has the
+ * token rows seq_start[s] .. seq_start[s + 1] - 1 (device [n_seqs + 1],
+ * non-decreasing; empty sequences are allowed), and each row attends to its
+ * own sequence's rows up to itself, as mlk_attention_paged does over pages, with
+ * the same semantics and precision.  q, k, v (rows q_row_stride, k_row_stride,
+ * v_row_stride elements apart: slices of one fused projection are fine) and out
+ * (dense) are of `type`.  Rows behind seq_start[n_seqs] are neither read nor
+ * written; n_tokens and max_seq_len bound them on the host; a sequence outside
+ * the bounds raises *err and gets nothing written.  workspace: as above
+ * (mlk_attention_packed_workspace_bytes()).
+ */
+mlk_status mlk_attention_packed(int32_t type, const void* q, int64_t q_row_stride, const void* k,
+                                int64_t k_row_stride, const void* v, int64_t v_row_stride,
+                                const int32_t* seq_start, int64_t n_seqs, int64_t n_tokens,
+                                int64_t max_seq_len, int32_t n_heads, int32_t n_kv_heads,
+                                int32_t head_dim, float scale, void* out, void* workspace,
+                                size_t workspace_bytes, int32_t* err, void* stream);
+int64_t mlk_attention_packed_workspace_bytes(int64_t n_seqs, int64_t n_tokens,
+                                             int64_t max_seq_len, int32_t n_heads,
+                                             int32_t n_kv_heads, int32_t head_dim);
+
 /* ------------------------------------------------------ batched forward
  * One transformer layer over a batch of tokens: the reference's
  * ForwardLayerDevice (src/forward.cc:337-384) for all tokens at once, i.e.
