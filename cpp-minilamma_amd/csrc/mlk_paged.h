@@ -101,6 +101,6 @@ struct AttendArgs {
 };
 mlk_status Attend(const AttendArgs& a);
 int64_t AttendWorkspace(int64_t n_seqs, int64_t n_tokens, int64_t max_new, int64_t max_len,
-                        int32_t n_heads, int32_t n_kv_heads, int32_t head_dim);
+                        int32_t n_heads, int32_t n_kv_heads, int32_t head_dim, bool packed);
 
 }  // namespace mlk

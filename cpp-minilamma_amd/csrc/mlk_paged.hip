@@ -393,7 +393,7 @@ int64_t mlk_attention_paged_workspace_bytes(int64_t n_seqs, int64_t n_tokens,
                                             int32_t n_heads, int32_t n_kv_heads,
                                             int32_t head_dim) {
     return AttendWorkspace(n_seqs, n_tokens, max_new_tokens, max_seq_len, n_heads, n_kv_heads,
-                           head_dim);
+                           head_dim, false);
 }
 
 mlk_status mlk_attention_packed(int32_t type, const void* q, int64_t q_row_stride, const void* k,
@@ -443,7 +443,7 @@ int64_t mlk_attention_packed_workspace_bytes(int64_t n_seqs, int64_t n_tokens,
                                              int64_t max_seq_len, int32_t n_heads,
                                              int32_t n_kv_heads, int32_t head_dim) {
     return AttendWorkspace(n_seqs, n_tokens, max_seq_len, max_seq_len, n_heads, n_kv_heads,
-                           head_dim);
+                           head_dim, true);
 }
 
 }  // extern "C"

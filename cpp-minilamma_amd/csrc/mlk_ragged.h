@@ -1,0 +1,302 @@
+// mlk_ragged.h -- what the two kernels of ragged attention share: the matrix
+// instructions over 16-bit elements, the split of fp32 values into 16-bit
+// pieces, and the launch parameters.
+//
+// Pieces.  fp32 q and softmax weights w meet 16-bit (or fp32) K and V on the
+// 16-bit matrix cores as sums of 16-bit pieces:
+//   fp16 K, V: 2 fp16 pieces (11 + 11 bits, truncated: within 2^-21 of the value).
+//     q is first scaled by a power of two per row, its largest element to
+//     2^14 .. 2^15, and w by 2^14, so that the second piece of all but tiny
+//     elements is a normal fp16 number; the scales go into the exponent's factor
+//     and cancel in the division by the sum.
+//   bf16 K, V: 3 bf16 pieces, exact (8 + 8 + 8 bits).
+//   fp32 K, V: 3 x 3 bf16 pieces, the 6 products above 2^-21 of q k (the three
+//     dropped ones are below 2^-20).
+// 16-bit q needs no split; its w is rounded to q's type (fp16: scaled as above).
+#pragma once
+
+#include "mlk_paged.h"
+
+#include <cmath>
+#include <type_traits>
+
+namespace mlk {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+
+constexpr float kLog2e = 1.44269504088896340736f;
+
+struct MmaBf {
+    static __device__ f32x16 Mma32(u32x4 a, u32x4 b, f32x16 c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a),
+                                                       __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+    }
+    static __device__ f32x4 Mma16(u32x4 a, u32x4 b, f32x4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a),
+                                                       __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+    }
+    static __device__ uint32_t Round2(float a, float b) {
+        const bf16x2 v = {static_cast<__bf16>(a), static_cast<__bf16>(b)};
+        return __builtin_bit_cast(uint32_t, v);
+    }
+    // 2 values into N pieces each
+    template <int N>
+    static __device__ void Split2(float a, float b, uint32_t (&o)[N]) {
+        if constexpr (N == 1) {
+            o[0] = Round2(a, b);
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                o[i] = PackBf(a, b);
+                if (i + 1 < N) {
+                    a -= __uint_as_float(__float_as_uint(a) & 0xFFFF0000u);
+                    b -= __uint_as_float(__float_as_uint(b) & 0xFFFF0000u);
+                }
+            }
+        }
+    }
+};
+
+struct MmaF16 {
+    static __device__ f32x16 Mma32(u32x4 a, u32x4 b, f32x16 c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a),
+                                                      __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+    }
+    static __device__ f32x4 Mma16(u32x4 a, u32x4 b, f32x4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a),
+                                                      __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+    }
+    static __device__ uint32_t Round2(float a, float b) {
+        const f16x2 v = {static_cast<_Float16>(a), static_cast<_Float16>(b)};
+        return __builtin_bit_cast(uint32_t, v);
+    }
+    template <int N>
+    static __device__ void Split2(float a, float b, uint32_t (&o)[N]) {
+        if constexpr (N == 1) {
+            o[0] = Round2(a, b);
+        } else {
+            static_assert(N == 2);
+            const auto hi = __builtin_amdgcn_cvt_pkrtz(a, b);
+            o[0] = __builtin_bit_cast(uint32_t, hi);
+            o[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(
+                                                    a - static_cast<float>(hi[0]),
+                                                    b - static_cast<float>(hi[1])));
+        }
+    }
+};
+
+// How activations of type A meet a cache of type C: NQ pieces of q and w, NK of
+// K and V; W: w's scale, a power of two; kScaleQ: q scaled per row.
+template <typename A, typename C>
+struct Pieces;
+template <>
+struct Pieces<BF16, BF16> {
+    typedef MmaBf M;
+    static constexpr int NQ = 1, NK = 1, W = 0;
+    static constexpr bool kScaleQ = false;
+};
+template <>
+struct Pieces<F16, F16> {
+    typedef MmaF16 M;
+    static constexpr int NQ = 1, NK = 1, W = 14;
+    static constexpr bool kScaleQ = false;
+};
+template <>
+struct Pieces<F32, F16> {
+    typedef MmaF16 M;
+    static constexpr int NQ = 2, NK = 1, W = 14;
+    static constexpr bool kScaleQ = true;
+};
+template <>
+struct Pieces<F32, BF16> {
+    typedef MmaBf M;
+    static constexpr int NQ = 3, NK = 1, W = 0;
+    static constexpr bool kScaleQ = false;
+};
+template <>
+struct Pieces<F32, F32> {
+    typedef MmaBf M;
+    static constexpr int NQ = 3, NK = 3, W = 0;
+    static constexpr bool kScaleQ = false;
+};
+
+// Eight fp32 values into N operands.
+template <typename M, int N>
+__device__ inline void Split8(const float* x, u32x4 (&o)[N]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        uint32_t w[N];
+        M::template Split2<N>(x[2 * i], x[2 * i + 1], w);
+#pragma unroll
+        for (int p = 0; p < N; ++p) o[p][i] = w[p];
+    }
+}
+
+// Power-of-two exponent that brings a row's largest |q| to 2^14 .. 2^15 (0 for
+// a row of zeros or with a non-finite element).
+__device__ inline int RowExponent(float amax) {
+    const int e = static_cast<int>(__float_as_uint(amax) >> 23);  // amax >= 0; subnormal: 0
+    if (amax == 0.0f || e == 255) return 0;
+    const int s = 14 - (e - 127);
+    return s < 100 ? s : 100;
+}
+
+// Maximum / sum over the lanes l, l ^ 32 (every lane gets it).
+__device__ inline float Max32(float v) {
+    const u32x2 r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false,
+                                                     false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ inline float Sum32(float v) {
+    const u32x2 r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false,
+                                                     false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+// The same over l, l ^ 16.
+__device__ inline float Max16(float v) {
+    const u32x2 r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false,
+                                                     false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ inline float Sum16(float v) {
+    const u32x2 r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false,
+                                                     false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+// ---------------------------------------------------- non-finite V, masked tiles
+// A weight of 0 does not hide an infinity or NaN in a matrix product.  Where a
+// tile has positions that some row does not attend to, V is looked through for
+// non-finite values as it lies in registers, and they are replaced by zeros; a
+// workgroup that met any adds them to the results of the rows that do attend to
+// them, element by element, at its end (adding one twice changes nothing).
+
+// Replaces the non-finite of N dwords' elements by zeros; whether there was one.
+template <typename C, int N>
+__device__ inline bool OnlyFinite(uint32_t* v) {
+    bool any = false;
+    if constexpr (C::kType == MLK_F32) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) any |= (v[i] & 0x7F800000u) == 0x7F800000u;
+        if (any) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) v[i] = (v[i] & 0x7F800000u) == 0x7F800000u ? 0u : v[i];
+        }
+    } else {
+        constexpr uint32_t kExp = C::kType == MLK_F16 ? 0x7C00u : 0x7F80u;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            any |= (v[i] & kExp) == kExp || (v[i] & (kExp << 16)) == (kExp << 16);
+        }
+        if (any) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                if ((v[i] & kExp) == kExp) v[i] &= 0xFFFF0000u;
+                if ((v[i] & (kExp << 16)) == (kExp << 16)) v[i] &= 0x0000FFFFu;
+            }
+        }
+    }
+    return any;
+}
+
+// The sum of the non-finite elements at dim d of positions first .. last of a
+// sequence (0: none); `v` is the KV head's first element.
+template <typename C>
+__device__ inline float NonFiniteSum(const RowsAt& at, const int32_t* table, int64_t t0,
+                                     const typename C::Bits* v, int32_t first, int32_t last,
+                                     int d) {
+    float sum = 0.0f;
+    bool bad = false;
+    for (int32_t j = first; j <= last; ++j) {
+        const int64_t o = table != nullptr ? PagedRow(at, PageOf(at, table, j, &bad), j)
+                                           : (t0 + j) * at.v_row;
+        const float x = C::Get(v[o + d]);
+        if (!__builtin_isfinite(x)) sum += x;
+    }
+    return sum;
+}
+
+// ------------------------------------------------------------ launches
+
+struct RaggedParams {
+    Ragged batch;
+    RowsAt rows;
+    const void* q;
+    int64_t q_row;
+    void* out;
+    int32_t n_heads, n_kv_heads, group;
+    float factor;  // scale * log2 e
+    int32_t vec;   // rows of q, K and V 16-byte aligned, head_dim % 8 == 0
+    // split over positions: chunk c of a row is positions c * chunk .. of it;
+    // partial results (maximum and sum of a row's chunk, then its weighted rows)
+    // where a row has more than one
+    int32_t chunk, n_chunks;
+    float2* part_ml;
+    float* part_o;
+    // sequences of at most this many rows (new tokens * group) are the few-row
+    // kernel's, the others the tile kernel's
+    int32_t few_rows;
+    int32_t* err;
+};
+
+// Rows of a KV head that the few-row kernel takes: two blocks of 16, one where
+// two would not leave registers for the tile in flight.
+inline int FewMost(int head_dim) { return head_dim <= 128 ? 32 : 16; }
+constexpr int kFewKeys = 128;  // positions its workgroup's waves take per step
+
+// Launches on `stream`; type and cache_type choose the instance.
+mlk_status LaunchFew(const RaggedParams& p, int32_t type, int32_t cache_type, hipStream_t stream);
+mlk_status LaunchTile(const RaggedParams& p, int32_t type, int32_t cache_type, hipStream_t stream);
+
+// f.template Run<A, C>() for the types.
+template <typename F>
+mlk_status ByType(int32_t type, int32_t cache_type, const F& f) {
+    if (type == MLK_F16) return f.template Run<F16, F16>();
+    if (type == MLK_BF16) return f.template Run<BF16, BF16>();
+    if (cache_type == MLK_F16) return f.template Run<F32, F16>();
+    if (cache_type == MLK_BF16) return f.template Run<F32, BF16>();
+    return f.template Run<F32, F32>();
+}
+
+// Where the partials of row m of KV head g lie: few-row kernel, by sequence;
+// tile kernel, by token row.
+__device__ inline int64_t FewPartial(const RaggedParams& p, int s, int g, int m) {
+    return ((static_cast<int64_t>(s) * p.n_kv_heads + g) * p.few_rows + m) * p.n_chunks;
+}
+__device__ inline int64_t TilePartial(const RaggedParams& p, int32_t t, int h) {
+    return (static_cast<int64_t>(t) * p.n_heads + h) * p.n_chunks;
+}
+
+// One K or V row chunk of 8 elements at p (nullptr: zeros), the first `left` of
+// them real, as raw bits.
+template <typename C, bool kFull>
+__device__ inline void LoadChunk(const typename C::Bits* p, int left, bool vec, uint32_t* o) {
+    constexpr int NW = sizeof(typename C::Bits) == 4 ? 8 : 4;
+    if (kFull || (vec && left >= 8)) {
+#pragma unroll
+        for (int i = 0; i < NW / 4; ++i) {
+            const u32x4 v = reinterpret_cast<const u32x4*>(p)[i];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[4 * i + e] = v[e];
+        }
+        return;
+    }
+    for (int i = 0; i < NW; ++i) o[i] = 0;
+    if (vec) return;  // head_dim % 8 == 0: nothing here
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        if (i < left) {
+            if constexpr (NW == 8) o[i] = __float_as_uint(p[i]);
+            else o[i / 2] |= static_cast<uint32_t>(p[i]) << (16 * (i % 2));
+        }
+    }
+}
+
+}  // namespace mlk

@@ -1,0 +1,480 @@
+// mlk_ragged_few.hip -- ragged attention of few rows per sequence: decode steps
+// and short chunks, bound by the bytes of K and V.
+//
+// A workgroup takes one sequence, one KV head and one chunk of its positions;
+// its rows are the (new token, query head of the group) pairs, at most 16 * NB,
+// so each K and V row is read once for all of them.  The 4 waves take 32
+// positions each in turn (16 for fp32), with softmax statistics of their own,
+// joined once at the end; several chunks' results are joined by a second kernel.
+//
+// Nothing is staged: both products take their operands from registers as the
+// loads leave them.
+//   S^T = K Q^T (16 positions x 16 rows a matrix instruction): a lane's
+//     operand is 8 neighbouring elements of one K row, a 16-byte load.
+//   O^T = V^T P^T: S^T's result layout (lane l: row l % 16, positions
+//     4 (l / 16) + r) is P^T's operand layout with the positions in the order
+//     16 (j / 4) + 4 (l / 16) + j % 4, j = 0 .. 7.  V^T's operand holds the same
+//     8 positions of one dim; which dim belongs to which of the HD / 16
+//     instructions is free, so lane l takes dims VE (l % 16) .. + VE - 1 of each
+//     of its 8 positions, one load each, and instruction e their e-th: one byte
+//     permute per operand dword.  The results then are runs of VE dims.
+//   fp32 caches multiply in fp32 (v_mfma_f32_16x16x4_f32): 16 rows need 64
+//     TFLOP/s at 8 TB/s, below its rate, and no pieces are formed.
+// A tile's loads are issued when the one before has been used, so each wave
+// keeps one tile (16 KB at head_dim 128) in flight through its arithmetic.
+#include "mlk_ragged.h"
+
+#include <climits>
+
+namespace mlk {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kWaves = kThreads / kWave;
+
+__device__ inline uint32_t LowHalves(uint32_t a, uint32_t b) {
+    return __builtin_amdgcn_perm(b, a, 0x05040100u);
+}
+__device__ inline uint32_t HighHalves(uint32_t a, uint32_t b) {
+    return __builtin_amdgcn_perm(b, a, 0x07060302u);
+}
+
+// K and V operands of one tile in registers, and their loads.
+template <typename C, int HD, bool kFull>
+struct FewTile {
+    static constexpr bool kF32 = std::is_same<C, F32>::value;
+    static constexpr int KT = kF32 ? 16 : 32;        // positions
+    static constexpr int NBK = KT / 16;              // blocks of 16 positions
+    static constexpr int NKW = HD * (kF32 ? 4 : 2) / 16;  // dwords a lane has of a K row (4 lanes a row)
+    static constexpr int NVW = HD * (kF32 ? 4 : 2) / 64;  // and of a V row (16 lanes a row)
+    static constexpr int VE = kF32 ? 4 : (HD >= 128 ? 8 : 4);  // dims a lane's run has
+    static constexpr int NVR = HD / 16 / VE;         // runs
+    static constexpr int NKEY = kF32 ? 4 : 8;        // positions a lane's V operand has
+    typedef typename C::Bits B;
+    uint32_t k[NBK][NKW];
+    uint32_t v[NKEY][NVW];
+
+    // K row at `row`, this lane's dims: 16-bit 32 c + 8 g .. + 7, fp32 16 c + 4 g .. + 3
+    __device__ void LoadK(int b, const B* row, int g, int hd, bool vec) {
+        constexpr int N = kF32 ? 4 : 8, S = 4 * N;
+#pragma unroll
+        for (int c = 0; c < HD / S; ++c) Run<N>(row + S * c + N * g, hd - S * c - N * g, vec, &k[b][4 * c]);
+    }
+    // V row at `row`, dims 16 VE n + VE (l % 16) .. + VE - 1
+    __device__ void LoadV(int j, const B* row, int i16, int hd, bool vec) {
+        constexpr int W = VE * sizeof(B) / 4;
+#pragma unroll
+        for (int n = 0; n < NVR; ++n) {
+            Run<VE>(row + 16 * VE * n + VE * i16, hd - 16 * VE * n - VE * i16, vec, &v[j][W * n]);
+        }
+    }
+    // N elements at p, `left` of them real
+    template <int N>
+    static __device__ void Run(const B* p, int left, bool vec, uint32_t* o) {
+        constexpr int W = N * sizeof(B) / 4;
+        if (kFull || (vec && left >= N)) {
+            if constexpr (W == 4) {
+                const u32x4 x = *reinterpret_cast<const u32x4*>(p);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) o[i] = x[i];
+            } else {
+                const u32x2 x = *reinterpret_cast<const u32x2*>(p);
+                o[0] = x[0];
+                o[1] = x[1];
+            }
+            return;
+        }
+#pragma unroll
+        for (int i = 0; i < W; ++i) o[i] = 0;
+        if (vec) return;  // head_dim is a multiple of 8: nothing real here
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            if (i < left) {
+                if constexpr (kF32) o[i] = __float_as_uint(p[i]);
+                else o[i / 2] |= static_cast<uint32_t>(p[i]) << (16 * (i % 2));
+            }
+        }
+    }
+};
+
+// What addresses a tile needs: the sequence's table or first row.
+struct FewRows {
+    const RowsAt* at;
+    const int32_t* table;  // nullptr: packed
+    int64_t t0;
+    int32_t end;  // positions the workgroup may read: 0 .. end - 1
+};
+
+// Element offsets of position j's K and V rows, lane by lane, clamped to the last.
+__device__ inline void RowOffsets(const FewRows& r, int32_t j, int64_t* ko, int64_t* vo, bool* bad) {
+    j = j < r.end ? j : r.end - 1;
+    if (r.table != nullptr) {
+        *ko = *vo = PagedRow(*r.at, PageOf(*r.at, r.table, j, bad), j);
+    } else {
+        *ko = (r.t0 + j) * r.at->k_row;
+        *vo = (r.t0 + j) * r.at->v_row;
+    }
+}
+
+template <typename A, typename C, int HD, int NB, bool kFull>
+__global__ __launch_bounds__(kThreads) void AttnFew(const RaggedParams p) {
+    typedef Pieces<A, C> P;
+    typedef typename P::M M;
+    typedef FewTile<C, HD, kFull> Tile;
+    typedef typename C::Bits CB;
+    typedef typename A::Bits AB;
+    constexpr bool kF32 = Tile::kF32;
+    constexpr int KT = Tile::KT, NBK = Tile::NBK, NI = HD / 16;
+    constexpr int NQ = kF32 ? 1 : P::NQ;
+    constexpr float kW = kF32 ? 0.0f : static_cast<float>(P::W);
+    constexpr int kOLd = HD + 4;  // row stride of a wave's results in shared memory
+    __shared__ float so[kWaves][16 * NB][kOLd];
+    __shared__ float sm[kWaves][16 * NB], sl[kWaves][16 * NB];
+
+    const int tid = static_cast<int>(threadIdx.x), lane = tid % kWave;
+    const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
+    const int i16 = lane % 16, g4 = lane / 16;
+    const int hd = kFull ? HD : p.rows.head_dim;
+    if (blockIdx.x == 0) CheckSeqs(p.batch, p.err);
+    const int kvh = static_cast<int>(blockIdx.x % p.n_kv_heads);
+    const int64_t rest = blockIdx.x / p.n_kv_heads;
+    const int chunk = static_cast<int>(rest % p.n_chunks);
+    const int s = static_cast<int>(rest / p.n_chunks);
+    Seq q;
+    if (!LoadSeq(p.batch, s, &q)) return;
+    const int rows = q.n * p.group;
+    const int32_t j_begin = chunk * p.chunk;
+    if (rows == 0 || rows > p.few_rows || j_begin >= q.len) return;
+    const int32_t j_end = q.len - j_begin < p.chunk ? q.len : j_begin + p.chunk;
+    const bool split = q.len > p.chunk;
+    const bool vec = kFull || p.vec;
+
+    const FewRows fr{&p.rows,
+                     p.batch.table == nullptr ? nullptr : p.batch.table + s * p.batch.table_stride,
+                     q.t0, j_end};
+    const CB* kb = static_cast<const CB*>(p.rows.k) + static_cast<int64_t>(kvh) * hd;
+    const CB* vb = static_cast<const CB*>(p.rows.v) + static_cast<int64_t>(kvh) * hd;
+
+    // the rows' positions and q operands
+    int32_t pos[NB];
+    float factor[NB];
+    u32x4 qp[NB][kF32 ? HD / 16 : HD / 32][NQ];
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+        const int m = 16 * nb + i16;
+        const bool real = m < rows;
+        const int i = real ? m / p.group : 0;
+        pos[nb] = real ? q.len - q.n + i : -1;
+        const AB* qr = static_cast<const AB*>(p.q) + static_cast<int64_t>(q.t0 + i) * p.q_row +
+                       static_cast<int64_t>(kvh * p.group + (real ? m % p.group : 0)) * hd;
+        factor[nb] = p.factor;
+        if constexpr (kF32) {
+#pragma unroll
+            for (int c = 0; c < HD / 16; ++c) {
+                uint32_t w[4];
+                FewTile<F32, HD, kFull>::template Run<4>(qr + 16 * c + 4 * g4, hd - 16 * c - 4 * g4,
+                                                         vec, w);
+                qp[nb][c][0] = u32x4{w[0], w[1], w[2], w[3]};
+            }
+        } else {
+            uint32_t raw[HD / 32][sizeof(AB) == 4 ? 8 : 4];
+#pragma unroll
+            for (int c = 0; c < HD / 32; ++c) {
+                LoadChunk<A, kFull>(qr + 32 * c + 8 * g4, hd - 32 * c - 8 * g4, vec, raw[c]);
+            }
+            if constexpr (NQ == 1) {
+#pragma unroll
+                for (int c = 0; c < HD / 32; ++c) {
+                    qp[nb][c][0] = u32x4{raw[c][0], raw[c][1], raw[c][2], raw[c][3]};
+                }
+            } else {
+                float up = 1.0f;
+                if constexpr (P::kScaleQ) {
+                    float amax = 0.0f;
+#pragma unroll
+                    for (int c = 0; c < HD / 32; ++c) {
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) {
+                            amax = fmaxf(amax, fabsf(__uint_as_float(raw[c][e])));
+                        }
+                    }
+                    const int e = RowExponent(Max32(Max16(amax)));
+                    up = ldexpf(1.0f, e);
+                    factor[nb] = ldexpf(p.factor, -e);
+                }
+#pragma unroll
+                for (int c = 0; c < HD / 32; ++c) {
+                    float x[8];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) x[e] = __uint_as_float(raw[c][e]) * up;
+                    Split8<M, NQ>(x, qp[nb][c]);
+                }
+            }
+        }
+    }
+
+    Tile tile;
+    bool bad = false;
+    // 16-position blocks whose rows lie evenly apart: whole pages' parts, or packed
+    const bool even = fr.table == nullptr || p.rows.page_shift >= 4;
+    auto block_base = [&](int32_t j, int64_t row) -> int64_t {  // j uniform, j + 15 < end
+        if (fr.table == nullptr) return (fr.t0 + j) * row;
+        return PagedRow(p.rows, PageOf(p.rows, fr.table, j, &bad), j);
+    };
+    auto load_k = [&](int32_t j0) {
+        if (even && j0 + KT <= j_end) {
+#pragma unroll
+            for (int b = 0; b < NBK; ++b) {
+                const CB* base = kb + block_base(j0 + 16 * b, p.rows.k_row);
+                tile.LoadK(b, base + i16 * static_cast<uint32_t>(p.rows.k_row), g4, hd, vec);
+            }
+            return;
+        }
+#pragma unroll
+        for (int b = 0; b < NBK; ++b) {
+            int64_t ko, vo;
+            RowOffsets(fr, j0 + 16 * b + i16, &ko, &vo, &bad);
+            tile.LoadK(b, kb + ko, g4, hd, vec);
+        }
+    };
+    auto load_v = [&](int32_t j0) {
+        if (even && j0 + KT <= j_end) {
+#pragma unroll
+            for (int b = 0; b < NBK; ++b) {
+                const CB* base = vb + block_base(j0 + 16 * b, p.rows.v_row);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    tile.LoadV(4 * b + r, base + r * p.rows.v_row +
+                               (4 * g4) * static_cast<uint32_t>(p.rows.v_row), i16, hd, vec);
+                }
+            }
+            return;
+        }
+#pragma unroll
+        for (int j = 0; j < Tile::NKEY; ++j) {
+            int64_t ko, vo;
+            RowOffsets(fr, j0 + 16 * (j / 4) + 4 * g4 + j % 4, &ko, &vo, &bad);
+            tile.LoadV(j, vb + vo, i16, hd, vec);
+        }
+    };
+
+    f32x4 o[NB][NI];
+    float m[NB], l[NB];
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+        m[nb] = -INFINITY;  // of the scores times the factor
+        l[nb] = 0.0f;       // this lane's part of the sum
+#pragma unroll
+        for (int e = 0; e < NI; ++e) o[nb][e] = f32x4{0, 0, 0, 0};
+    }
+    const int32_t first_pos = q.len - q.n;  // the lowest position of a row
+    bool special = false;                   // met a non-finite V in a masked tile
+
+    int32_t j0 = j_begin + wave * KT;
+    if (j0 < j_end) {
+        load_k(j0);
+        load_v(j0);
+    }
+    for (; j0 < j_end; j0 += kWaves * KT) {
+        const int32_t jn = j0 + kWaves * KT;
+        f32x4 sc[NB][NBK];
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) {
+#pragma unroll
+            for (int b = 0; b < NBK; ++b) {
+                f32x4 a = {0, 0, 0, 0};
+                if constexpr (kF32) {
+#pragma unroll
+                    for (int c = 0; c < HD / 16; ++c) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            a = __builtin_amdgcn_mfma_f32_16x16x4f32(
+                                __uint_as_float(tile.k[b][4 * c + e]),
+                                __uint_as_float(qp[nb][c][0][e]), a, 0, 0, 0);
+                        }
+                    }
+                } else {
+#pragma unroll
+                    for (int c = 0; c < HD / 32; ++c) {
+                        const u32x4 kk = {tile.k[b][4 * c], tile.k[b][4 * c + 1],
+                                          tile.k[b][4 * c + 2], tile.k[b][4 * c + 3]};
+#pragma unroll
+                        for (int n = 0; n < NQ; ++n) a = M::Mma16(kk, qp[nb][c][n], a);
+                    }
+                }
+                sc[nb][b] = a;
+            }
+        }
+        if (jn < j_end) load_k(jn);
+
+        const bool masked = j0 + KT - 1 > first_pos || j0 + KT > j_end;
+        float w[NB][4 * NBK];
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) {
+            float top = -INFINITY;
+#pragma unroll
+            for (int b = 0; b < NBK; ++b) {
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    float x = sc[nb][b][r] * factor[nb];
+                    const int32_t j = j0 + 16 * b + 4 * g4 + r;
+                    if (masked && (j > pos[nb] || j >= j_end)) x = -INFINITY;
+                    w[nb][4 * b + r] = x;
+                    top = fmaxf(top, x);
+                }
+            }
+            top = Max32(Max16(top));
+            const float mn = fmaxf(m[nb], top);
+            const float base = mn == -INFINITY ? 0.0f : mn;
+            if (__ballot(mn != m[nb]) != 0) {
+                const float alpha = __builtin_amdgcn_exp2f(m[nb] - base);
+                l[nb] *= alpha;
+#pragma unroll
+                for (int e = 0; e < NI; ++e) o[nb][e] *= alpha;
+                m[nb] = mn;
+            }
+            float sum = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 4 * NBK; ++i) {
+                w[nb][i] = __builtin_amdgcn_exp2f(w[nb][i] - (base - kW));
+                sum += w[nb][i];
+            }
+            l[nb] += sum;
+        }
+
+        if (masked) {
+#pragma unroll
+            for (int j = 0; j < Tile::NKEY; ++j) {
+                special |= OnlyFinite<C, Tile::NVW>(tile.v[j]);
+            }
+        }
+        if constexpr (kF32) {
+#pragma unroll
+            for (int e = 0; e < NI; ++e) {
+#pragma unroll
+                for (int nb = 0; nb < NB; ++nb) {
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        o[nb][e] = __builtin_amdgcn_mfma_f32_16x16x4f32(
+                            __uint_as_float(tile.v[r][e]), w[nb][r], o[nb][e], 0, 0, 0);
+                    }
+                }
+            }
+        } else {
+            u32x4 wp[NB][NQ];
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb) Split8<M, NQ>(w[nb], wp[nb]);
+#pragma unroll
+            for (int e = 0; e < NI; ++e) {
+                u32x4 a;  // the e-th dim of each of the lane's positions
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const uint32_t x = tile.v[2 * i][e / 2], y = tile.v[2 * i + 1][e / 2];
+                    a[i] = e % 2 ? HighHalves(x, y) : LowHalves(x, y);
+                }
+#pragma unroll
+                for (int nb = 0; nb < NB; ++nb) {
+#pragma unroll
+                    for (int n = 0; n < NQ; ++n) o[nb][e] = M::Mma16(a, wp[nb][n], o[nb][e]);
+                }
+            }
+        }
+        if (jn < j_end) load_v(jn);
+    }
+    if (bad && p.err != nullptr) RaiseFlag(p.err, 1);
+
+    // join the waves: all relative to the largest maximum
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+        const float lt = Sum32(Sum16(l[nb]));
+        if (g4 == 0) {
+            sm[wave][16 * nb + i16] = m[nb];
+            sl[wave][16 * nb + i16] = lt;
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+        const int row = 16 * nb + i16;
+        float top = sm[0][row];
+#pragma unroll
+        for (int w = 1; w < kWaves; ++w) top = fmaxf(top, sm[w][row]);
+        const float f = __builtin_amdgcn_exp2f(m[nb] - (top == -INFINITY ? 0.0f : top));
+#pragma unroll
+        for (int e = 0; e < NI; ++e) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int d = 16 * Tile::VE * (e / Tile::VE) + Tile::VE * (4 * g4 + r) + e % Tile::VE;
+                so[wave][row][d] = o[nb][e][r] * f;
+            }
+        }
+    }
+    special = __syncthreads_or(special);
+    const int32_t masked_from = (first_pos < j_end ? first_pos : j_end) - KT;
+    for (int u = tid; u < rows * HD; u += kThreads) {
+        const int row = u / HD, d = u % HD;
+        if (!kFull && d >= hd) continue;
+        float top = sm[0][row], lt = 0.0f, sum = 0.0f;
+#pragma unroll
+        for (int w = 1; w < kWaves; ++w) top = fmaxf(top, sm[w][row]);
+        const float base = top == -INFINITY ? 0.0f : top;
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) {
+            lt += sl[w][row] * __builtin_amdgcn_exp2f(sm[w][row] - base);
+            sum += so[w][row][d];
+        }
+        const int i = row / p.group, h = kvh * p.group + row % p.group;
+        if (special) {
+            const int32_t last = first_pos + i < j_end ? first_pos + i : j_end - 1;
+            sum += NonFiniteSum<C>(p.rows, fr.table, fr.t0, vb,
+                                   masked_from > j_begin ? masked_from : j_begin, last, d);
+        }
+        if (split) {
+            const int64_t at = FewPartial(p, s, kvh, row) + chunk;
+            p.part_o[at * hd + d] = sum;
+            if (d == 0) p.part_ml[at] = make_float2(top, lt);
+        } else {
+            AB* out = static_cast<AB*>(p.out) +
+                      (static_cast<int64_t>(q.t0 + i) * p.n_heads + h) * hd;
+            out[d] = A::Put(sum / lt);
+        }
+    }
+}
+
+template <typename A, typename C, int HD>
+mlk_status Launch(const RaggedParams& p, dim3 grid, hipStream_t s) {
+    const bool full = p.vec && p.rows.head_dim == HD;
+    if (p.few_rows <= 16) {
+        if (full) hipLaunchKernelGGL((AttnFew<A, C, HD, 1, true>), grid, dim3(kThreads), 0, s, p);
+        else hipLaunchKernelGGL((AttnFew<A, C, HD, 1, false>), grid, dim3(kThreads), 0, s, p);
+    } else if constexpr (HD <= 128) {
+        if (full) hipLaunchKernelGGL((AttnFew<A, C, HD, 2, true>), grid, dim3(kThreads), 0, s, p);
+        else hipLaunchKernelGGL((AttnFew<A, C, HD, 2, false>), grid, dim3(kThreads), 0, s, p);
+    }
+    return CheckLaunch("AttnFew");
+}
+
+struct ByDim {
+    const RaggedParams& p;
+    dim3 grid;
+    hipStream_t stream;
+    template <typename A, typename C>
+    mlk_status Run() const {
+        if (p.rows.head_dim <= 64) return Launch<A, C, 64>(p, grid, stream);
+        if (p.rows.head_dim <= 128) return Launch<A, C, 128>(p, grid, stream);
+        return Launch<A, C, 256>(p, grid, stream);
+    }
+};
+
+}  // namespace
+
+mlk_status LaunchFew(const RaggedParams& p, int32_t type, int32_t cache_type, hipStream_t stream) {
+    const int64_t blocks = static_cast<int64_t>(p.batch.n_seqs) * p.n_chunks * p.n_kv_heads;
+    if (blocks > INT_MAX) {
+        return Fail(MLK_ERR_INVALID, "attention: %lld workgroups exceed the grid",
+                    static_cast<long long>(blocks));
+    }
+    return ByType(type, cache_type, ByDim{p, dim3(static_cast<unsigned>(blocks)), stream});
+}
+
+}  // namespace mlk

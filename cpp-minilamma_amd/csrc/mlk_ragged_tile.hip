@@ -1,0 +1,413 @@
+// mlk_ragged_tile.hip -- ragged attention of many rows per sequence: whole
+// prompts and chunks of them, bound by the matrix cores.
+//
+// A workgroup takes 128 rows of one sequence and KV head -- (token, query head
+// of the group) pairs, so a group's heads share K and V -- and walks the
+// positions its last row attends to, KT at a time.  Each of its 4 waves owns 32
+// rows; the tile's K and V rows are shared through LDS:
+//   S^T = K Q^T  (v_mfma 32x32x16, 32 positions x 32 rows): K rows as they lie,
+//     8 elements a lane; q stays in registers.
+//   softmax: a lane holds 16 of each 32 positions of ONE row, so maximum and sum
+//     are within the lane but for one exchange of the wave's halves, and the
+//     rescale of the results is a plain product.
+//   O^T = V^T P^T: S^T's layout is P^T's operand layout, with the positions of
+//     a lane's half in the order 16 m + 8 (j / 4) + 4 (l / 32) + j % 4; V^T comes
+//     from V's rows by the transposing LDS read (4 positions of 16 dims).
+// The next tile's loads are issued before a tile's products and land in
+// registers; they are written to LDS after them (16-bit caches: two buffers and
+// one barrier a tile; fp32: split into pieces on the way, one buffer).
+// LDS rows are unpadded, their 16-byte chunks permuted by the row so that both
+// K's reads (16 rows of one chunk) and V's (4 rows of 64 bytes) meet each bank
+// once.
+#include "mlk_ragged.h"
+
+#include <climits>
+
+namespace mlk {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kRows = 128;
+
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s16x4* LdsS16x4;
+
+// Row r's chunk permutation (an xor), HD / 8 chunks a row.
+template <int HD>
+__device__ inline int Swizzle(int r) {
+    return HD == 64 ? (((r >> 1) & 1) << 2) | ((r >> 2) & 3) : ((r & 3) << 2) | ((r >> 2) & 3);
+}
+
+template <typename C, int HD>
+struct TileShape {
+    static constexpr int NK = std::is_same<C, F32>::value ? 3 : 1;
+    static constexpr int KT = NK == 3 || HD == 256 ? 32 : 64;
+    static constexpr int NBUF = NK == 3 ? 1 : 2;
+    static constexpr int kPlane = KT * HD;             // elements
+    static constexpr int NCH = KT * HD / 8 / kThreads;  // chunks a thread stages
+    static constexpr int NW = NK == 3 ? 8 : 4;         // dwords a chunk has in memory
+};
+
+template <typename A, typename C, int HD, bool kFull>
+__global__ __launch_bounds__(kThreads) void AttnTile(const RaggedParams p, int n_slots) {
+    typedef Pieces<A, C> P;
+    typedef typename P::M M;
+    typedef TileShape<C, HD> T;
+    typedef typename C::Bits CB;
+    typedef typename A::Bits AB;
+    constexpr int NQ = P::NQ, NK = T::NK, KT = T::KT, NKB = KT / 32, NCH = T::NCH;
+    constexpr int ND = HD / 32, NS = HD / 16;
+    constexpr int kTerms = NQ > NK ? NQ : NK;  // products of pieces i, j: i + j < kTerms
+    __shared__ __align__(16) uint16_t sk[T::NBUF][NK * T::kPlane];
+    __shared__ __align__(16) uint16_t sv[T::NBUF][NK * T::kPlane];
+
+    const int tid = static_cast<int>(threadIdx.x), lane = tid % kWave;
+    const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
+    const int l32 = lane % 32, half = lane / 32;
+    const int hd = kFull ? HD : p.rows.head_dim;
+    const bool vec = kFull || p.vec;
+    if (blockIdx.x == 0) CheckSeqs(p.batch, p.err);
+
+    const int kvh = static_cast<int>(blockIdx.x % p.n_kv_heads);
+    const int64_t rest = blockIdx.x / p.n_kv_heads;
+    const int chunk = static_cast<int>(rest % p.n_chunks);
+    // the longest prefixes first
+    const int64_t slot = n_slots - 1 - rest / p.n_chunks;
+    const int group = p.group;
+    auto first_slot = [group](int32_t start, int s) {
+        return static_cast<int64_t>(start) * group / kRows + s;
+    };
+    const int s = LastSeq(p.batch, slot, first_slot);
+    Seq q;
+    if (!LoadSeq(p.batch, s, &q)) return;
+    const int64_t m0 = (slot - first_slot(q.t0, s)) * kRows;
+    const int64_t rows = static_cast<int64_t>(q.n) * group;
+    if (m0 < 0 || m0 >= rows || rows <= p.few_rows) return;
+    const int64_t m_last = (m0 + kRows < rows ? m0 + kRows : rows) - 1;
+    const int32_t first = q.len - q.n;  // position of the sequence's first new token
+    const int32_t lo = first + static_cast<int32_t>(m0 / group);
+    const int32_t hi = first + static_cast<int32_t>(m_last / group);
+    const int32_t j_begin = chunk * p.chunk;
+    if (j_begin > hi) return;
+    const int32_t j_end = hi + 1 - j_begin < p.chunk ? hi + 1 : j_begin + p.chunk;
+
+    const int32_t* table =
+        p.batch.table == nullptr ? nullptr : p.batch.table + s * p.batch.table_stride;
+    const CB* kb = static_cast<const CB*>(p.rows.k) + static_cast<int64_t>(kvh) * hd;
+    const CB* vb = static_cast<const CB*>(p.rows.v) + static_cast<int64_t>(kvh) * hd;
+
+    // this lane's row
+    const int64_t m = m0 + 32 * wave + l32;
+    const bool real = m < rows;
+    const int32_t tok = real ? static_cast<int32_t>(m / group) : 0;
+    const int h = kvh * group + (real ? static_cast<int>(m % group) : 0);
+    const int32_t pos = real ? first + tok : -1;
+    // positions the wave's rows attend to: some row all below wave_lo, none from wave_hi
+    const int64_t w0 = m0 + 32 * wave;
+    const int32_t wave_lo = w0 <= m_last ? first + static_cast<int32_t>(w0 / group) : -1;
+    const int64_t w1 = w0 + 31 < m_last ? w0 + 31 : m_last;
+    const int32_t wave_hi = w0 <= m_last ? first + static_cast<int32_t>(w1 / group) + 1 : 0;
+
+    float factor = p.factor;
+    u32x4 qf[NS][NQ];
+    {
+        const AB* qr = static_cast<const AB*>(p.q) + static_cast<int64_t>(q.t0 + tok) * p.q_row +
+                       static_cast<int64_t>(h) * hd;
+        uint32_t raw[NS][sizeof(AB) == 4 ? 8 : 4];
+#pragma unroll
+        for (int c = 0; c < NS; ++c) {
+            LoadChunk<A, kFull>(qr + 16 * c + 8 * half, hd - 16 * c - 8 * half, vec, raw[c]);
+        }
+        if constexpr (NQ == 1) {
+#pragma unroll
+            for (int c = 0; c < NS; ++c) qf[c][0] = u32x4{raw[c][0], raw[c][1], raw[c][2], raw[c][3]};
+        } else {
+            float up = 1.0f;
+            if constexpr (P::kScaleQ) {
+                float amax = 0.0f;
+#pragma unroll
+                for (int c = 0; c < NS; ++c) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) amax = fmaxf(amax, fabsf(__uint_as_float(raw[c][e])));
+                }
+                const int e = RowExponent(Max32(amax));
+                up = ldexpf(1.0f, e);
+                factor = ldexpf(p.factor, -e);
+            }
+#pragma unroll
+            for (int c = 0; c < NS; ++c) {
+                float x[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[e] = __uint_as_float(raw[c][e]) * up;
+                Split8<M, NQ>(x, qf[c]);
+            }
+        }
+    }
+
+    // staging: chunk tid + kThreads * i of the tile
+    uint32_t gk[NCH][T::NW], gv[NCH][T::NW];
+    bool bad = false, special = false;
+    auto load = [&](int32_t j0) {
+#pragma unroll
+        for (int i = 0; i < NCH; ++i) {
+            const int idx = tid + kThreads * i, r = idx / (HD / 8), c = idx % (HD / 8);
+            const int32_t j = j0 + r < j_end ? j0 + r : j_end - 1;
+            int64_t ko, vo;
+            if (table != nullptr) {
+                ko = vo = PagedRow(p.rows, PageOf(p.rows, table, j, &bad), j);
+            } else {
+                ko = (static_cast<int64_t>(q.t0) + j) * p.rows.k_row;
+                vo = (static_cast<int64_t>(q.t0) + j) * p.rows.v_row;
+            }
+            LoadChunk<C, kFull>(kb + ko + 8 * c, hd - 8 * c, vec, gk[i]);
+            LoadChunk<C, kFull>(vb + vo + 8 * c, hd - 8 * c, vec, gv[i]);
+        }
+    };
+    auto put = [&](uint16_t* dst, int r, int c, const uint32_t* g) {
+        const int at = r * HD + ((c ^ Swizzle<HD>(r)) * 8);
+        if constexpr (NK == 1) {
+            *reinterpret_cast<u32x4*>(dst + at) = u32x4{g[0], g[1], g[2], g[3]};
+        } else {
+            float x[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] = __uint_as_float(g[e]);
+            u32x4 w[NK];
+            Split8<M, NK>(x, w);
+#pragma unroll
+            for (int n = 0; n < NK; ++n) *reinterpret_cast<u32x4*>(dst + n * T::kPlane + at) = w[n];
+        }
+    };
+    auto store = [&](int32_t j0, int buf) {
+        const bool masked = j0 + KT - 1 > lo || j0 + KT > j_end;
+#pragma unroll
+        for (int i = 0; i < NCH; ++i) {
+            const int idx = tid + kThreads * i, r = idx / (HD / 8), c = idx % (HD / 8);
+            put(sk[buf], r, c, gk[i]);
+            if (masked) special |= OnlyFinite<C, T::NW>(gv[i]);
+            put(sv[buf], r, c, gv[i]);
+        }
+    };
+
+    f32x16 o[ND];
+    float mx = -INFINITY, l = 0.0f;  // of the scores times the factor; this lane's part
+#pragma unroll
+    for (int d = 0; d < ND; ++d) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[d][r] = 0.0f;
+    }
+
+    load(j_begin);
+    store(j_begin, 0);
+    __syncthreads();
+    int buf = 0;
+    for (int32_t j0 = j_begin; j0 < j_end; j0 += KT) {
+        const bool more = j0 + KT < j_end;
+        if (more) load(j0 + KT);
+        if (j0 < wave_hi) {
+            const uint16_t* ks = sk[buf];
+            const uint16_t* vs = sv[buf];
+            f32x16 sc[NKB];
+#pragma unroll
+            for (int b = 0; b < NKB; ++b) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) sc[b][r] = 0.0f;
+            }
+#pragma unroll
+            for (int c = 0; c < NS; ++c) {
+#pragma unroll
+                for (int b = 0; b < NKB; ++b) {
+                    u32x4 kf[NK];
+#pragma unroll
+                    for (int n = 0; n < NK; ++n) {
+                        kf[n] = *reinterpret_cast<const u32x4*>(
+                            ks + n * T::kPlane + (32 * b + l32) * HD +
+                            (((2 * c + half) ^ Swizzle<HD>(l32)) * 8));
+                    }
+#pragma unroll
+                    for (int i = 0; i < NQ; ++i) {
+#pragma unroll
+                        for (int n = 0; n < NK; ++n) {
+                            if (i + n < kTerms) sc[b] = M::Mma32(kf[n], qf[c][i], sc[b]);
+                        }
+                    }
+                }
+            }
+            const bool masked = j0 + KT - 1 > wave_lo || j0 + KT > j_end;
+            if (masked) {
+                const int32_t last = pos < j_end ? pos : j_end - 1;
+#pragma unroll
+                for (int b = 0; b < NKB; ++b) {
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        const int32_t j = j0 + 32 * b + 8 * (r / 4) + 4 * half + r % 4;
+                        if (j > last) sc[b][r] = -INFINITY;
+                    }
+                }
+            }
+            float top = sc[0][0];
+#pragma unroll
+            for (int b = 0; b < NKB; ++b) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) top = fmaxf(top, sc[b][r]);
+            }
+            const float mn = fmaxf(mx, Max32(top) * factor);
+            const float base = mn == -INFINITY ? 0.0f : mn;
+            if (__ballot(mn != mx) != 0) {
+                const float alpha = __builtin_amdgcn_exp2f(mx - base);
+                l *= alpha;
+#pragma unroll
+                for (int d = 0; d < ND; ++d) o[d] *= alpha;
+                mx = mn;
+            }
+            const float off = static_cast<float>(P::W) - base;
+            float sum = 0.0f;
+#pragma unroll
+            for (int b = 0; b < NKB; ++b) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    sc[b][r] = __builtin_amdgcn_exp2f(fmaf(sc[b][r], factor, off));
+                    sum += sc[b][r];
+                }
+            }
+            l += sum;
+            const int i16 = lane % 16, g2 = (lane / 16) % 2;
+#pragma unroll
+            for (int t = 0; t < KT / 16; ++t) {
+                float w[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) w[e] = sc[t / 2][8 * (t % 2) + e];
+                u32x4 wf[NQ];
+                Split8<M, NQ>(w, wf);
+#pragma unroll
+                for (int d = 0; d < ND; ++d) {
+                    u32x4 vf[NK];
+#pragma unroll
+                    for (int n = 0; n < NK; ++n) {
+#pragma unroll
+                        for (int jj = 0; jj < 2; ++jj) {
+                            const int r = 16 * t + 8 * jj + 4 * half + i16 / 4;
+                            const int c = 4 * d + 2 * g2 + (i16 % 4) / 2;
+                            const uint16_t* at = vs + n * T::kPlane + r * HD +
+                                                 ((c ^ Swizzle<HD>(r)) * 8) + 4 * (i16 % 2);
+                            const u32x2 x = __builtin_bit_cast(
+                                u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                           (LdsS16x4)(const_cast<uint16_t*>(at))));
+                            vf[n][2 * jj] = x[0];
+                            vf[n][2 * jj + 1] = x[1];
+                        }
+                    }
+#pragma unroll
+                    for (int i = 0; i < NQ; ++i) {
+#pragma unroll
+                        for (int n = 0; n < NK; ++n) {
+                            if (i + n < kTerms) o[d] = M::Mma32(vf[n], wf[i], o[d]);
+                        }
+                    }
+                }
+            }
+        }
+        if constexpr (T::NBUF == 1) __syncthreads();
+        if (more) store(j0 + KT, T::NBUF == 1 ? 0 : buf ^ 1);
+        __syncthreads();
+        if constexpr (T::NBUF == 2) buf ^= 1;
+    }
+    if (bad && p.err != nullptr) RaiseFlag(p.err, 1);
+    special = __syncthreads_or(special);
+    l = Sum32(l);
+    if (!real || pos < j_begin) return;
+    const int32_t last = pos < j_end ? pos : j_end - 1;
+    const int32_t masked_from = (lo < j_end ? lo : j_end) - KT;
+    const bool split = pos >= p.chunk;
+    const int64_t at = split ? TilePartial(p, q.t0 + tok, h) + chunk : 0;
+    if (split && half == 0) p.part_ml[at] = make_float2(mx, l);
+    const float inv = split ? 1.0f : 1.0f / l;
+    AB* out = static_cast<AB*>(p.out) + (static_cast<int64_t>(q.t0 + tok) * p.n_heads + h) * hd;
+    float* part = p.part_o + at * hd;
+#pragma unroll
+    for (int d = 0; d < ND; ++d) {
+#pragma unroll
+        for (int r4 = 0; r4 < 4; ++r4) {
+            const int dim = 32 * d + 8 * r4 + 4 * half;
+            float x[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[e] = o[d][4 * r4 + e] * inv;
+            if (special) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    if (dim + e < hd) {
+                        x[e] += NonFiniteSum<C>(p.rows, table, q.t0, vb,
+                                                masked_from > j_begin ? masked_from : j_begin, last,
+                                                dim + e);
+                    }
+                }
+            }
+            if (split) {
+                if constexpr (kFull) {
+                    *reinterpret_cast<f32x4*>(part + dim) = f32x4{x[0], x[1], x[2], x[3]};
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        if (dim + e < hd) part[dim + e] = x[e];
+                    }
+                }
+            } else if constexpr (kFull && sizeof(AB) == 4) {
+                *reinterpret_cast<f32x4*>(out + dim) = f32x4{x[0], x[1], x[2], x[3]};
+            } else if constexpr (kFull) {
+                *reinterpret_cast<u32x2*>(out + dim) =
+                    u32x2{static_cast<uint32_t>(A::Put(x[0])) |
+                              (static_cast<uint32_t>(A::Put(x[1])) << 16),
+                          static_cast<uint32_t>(A::Put(x[2])) |
+                              (static_cast<uint32_t>(A::Put(x[3])) << 16)};
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    if (dim + e < hd) out[dim + e] = A::Put(x[e]);
+                }
+            }
+        }
+    }
+}
+
+template <typename A, typename C, int HD>
+mlk_status Launch(const RaggedParams& p, dim3 grid, int n_slots, hipStream_t s) {
+    if (p.vec && p.rows.head_dim == HD) {
+        hipLaunchKernelGGL((AttnTile<A, C, HD, true>), grid, dim3(kThreads), 0, s, p, n_slots);
+    } else {
+        hipLaunchKernelGGL((AttnTile<A, C, HD, false>), grid, dim3(kThreads), 0, s, p, n_slots);
+    }
+    return CheckLaunch("AttnTile");
+}
+
+struct ByDim {
+    const RaggedParams& p;
+    dim3 grid;
+    int n_slots;
+    hipStream_t stream;
+    template <typename A, typename C>
+    mlk_status Run() const {
+        if (p.rows.head_dim <= 64) return Launch<A, C, 64>(p, grid, n_slots, stream);
+        if (p.rows.head_dim <= 128) return Launch<A, C, 128>(p, grid, n_slots, stream);
+        return Launch<A, C, 256>(p, grid, n_slots, stream);
+    }
+};
+
+// Row tiles of a batch: sequence s owns the slots from start[s] * group / kRows
+// + s on, at least as many as it has tiles, whatever the lengths.
+int64_t TileSlots(int64_t n_seqs, int64_t n_tokens, int32_t group) {
+    return n_tokens * group / kRows + n_seqs;
+}
+
+}  // namespace
+
+mlk_status LaunchTile(const RaggedParams& p, int32_t type, int32_t cache_type, hipStream_t stream) {
+    const int64_t slots = TileSlots(p.batch.n_seqs, p.batch.n_tokens, p.group);
+    const int64_t blocks = slots * p.n_chunks * p.n_kv_heads;
+    if (blocks > INT_MAX) {
+        return Fail(MLK_ERR_INVALID, "attention: %lld workgroups exceed the grid",
+                    static_cast<long long>(blocks));
+    }
+    return ByType(type, cache_type, ByDim{p, dim3(static_cast<unsigned>(blocks)),
+                                          static_cast<int>(slots), stream});
+}
+
+}  // namespace mlk
