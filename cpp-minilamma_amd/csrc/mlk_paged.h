@@ -56,7 +56,7 @@ __device__ inline int LastSeq(const Ragged& r, int64_t x, F f) {
     int count = 0;
     for (int s0 = 0; s0 < r.n_seqs; s0 += kWave) {
         const int s = s0 + lane;
-        const bool in = s < r.n_seqs && f(r.start[s], s) <= x;
+        const bool in = s < r.n_seqs && f(ReadIndex(r.start + s), s) <= x;
         const int c = __popcll(__ballot(in));
         count += c;
         if (c < kWave) break;

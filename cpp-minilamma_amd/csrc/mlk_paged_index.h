@@ -29,13 +29,24 @@ struct Seq {
     int32_t t0, n, len;  // first token row, new tokens, length with them
 };
 
+// An element of an array that no kernel writes while it is read here.  On the
+// device the load is from constant memory: with a uniform index it takes the
+// scalar path, and does not queue behind the wave's loads of K and V.
+MLK_HD inline int32_t ReadIndex(const int32_t* p) {
+#ifdef __HIP_DEVICE_COMPILE__
+    return *(const __attribute__((address_space(4))) int32_t*)(p);
+#else
+    return *p;
+#endif
+}
+
 // Sequence s, checked against the host's bounds; false: out of bounds, to be
 // left alone.
 MLK_HD inline bool LoadSeq(const Ragged& r, int s, Seq* q) {
-    const int32_t a = r.start[s], b = r.start[s + 1];
+    const int32_t a = ReadIndex(r.start + s), b = ReadIndex(r.start + s + 1);
     if (a < 0 || b < a || b > r.n_tokens) return false;
     const int32_t n = b - a;
-    const int32_t len = r.len != nullptr ? r.len[s] : n;
+    const int32_t len = r.len != nullptr ? ReadIndex(r.len + s) : n;
     *q = {a, n, len};
     return n <= r.max_new && len >= n && len <= r.max_len;
 }
@@ -54,7 +65,7 @@ struct RowsAt {
 
 // The page of position j, 0 in place of one outside the cache (*bad set).
 MLK_HD inline int32_t PageOf(const RowsAt& a, const int32_t* table_row, int32_t j, bool* bad) {
-    const int32_t g = table_row[j >> a.page_shift];
+    const int32_t g = ReadIndex(table_row + (j >> a.page_shift));
     const bool in = g >= 0 && g < a.n_pages;
     if (!in) *bad = true;
     return in ? g : 0;

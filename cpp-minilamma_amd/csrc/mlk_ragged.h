@@ -179,31 +179,31 @@ __device__ inline float Sum16(float v) {
 // them, element by element, at its end (adding one twice changes nothing).
 
 // Replaces the non-finite of N dwords' elements by zeros; whether there was one.
+// An exponent of all ones is found by the carry of its lowest bit into the sign's
+// place: integer work in vector registers, no lane masks.
 template <typename C, int N>
 __device__ inline bool OnlyFinite(uint32_t* v) {
-    bool any = false;
-    if constexpr (C::kType == MLK_F32) {
+    constexpr uint32_t kExp = C::kType == MLK_F32 ? 0x7F800000u
+                              : C::kType == MLK_F16 ? 0x7C007C00u : 0x7F807F80u;
+    constexpr uint32_t kLow = C::kType == MLK_F32 ? 0x00800000u
+                              : C::kType == MLK_F16 ? 0x04000400u : 0x00800080u;
+    constexpr uint32_t kSign = C::kType == MLK_F32 ? 0x80000000u : 0x80008000u;
+    uint32_t any = 0;
 #pragma unroll
-        for (int i = 0; i < N; ++i) any |= (v[i] & 0x7F800000u) == 0x7F800000u;
-        if (any) {
-#pragma unroll
-            for (int i = 0; i < N; ++i) v[i] = (v[i] & 0x7F800000u) == 0x7F800000u ? 0u : v[i];
-        }
-    } else {
-        constexpr uint32_t kExp = C::kType == MLK_F16 ? 0x7C00u : 0x7F80u;
+    for (int i = 0; i < N; ++i) any |= (v[i] & kExp) + kLow;
+    any &= kSign;
+    if (any != 0) {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            any |= (v[i] & kExp) == kExp || (v[i] & (kExp << 16)) == (kExp << 16);
-        }
-        if (any) {
-#pragma unroll
-            for (int i = 0; i < N; ++i) {
-                if ((v[i] & kExp) == kExp) v[i] &= 0xFFFF0000u;
-                if ((v[i] & (kExp << 16)) == (kExp << 16)) v[i] &= 0x0000FFFFu;
+            const uint32_t hit = ((v[i] & kExp) + kLow) & kSign;
+            if constexpr (C::kType == MLK_F32) {
+                v[i] &= ~static_cast<uint32_t>(static_cast<int32_t>(hit) >> 31);
+            } else {
+                v[i] &= ~((hit >> 15) * 0xFFFFu);
             }
         }
     }
-    return any;
+    return any != 0;
 }
 
 // The sum of the non-finite elements at dim d of positions first .. last of a
@@ -234,10 +234,13 @@ struct RaggedParams {
     int32_t n_heads, n_kv_heads, group;
     float factor;  // scale * log2 e
     int32_t vec;   // rows of q, K and V 16-byte aligned, head_dim % 8 == 0
-    // split over positions: chunk c of a row is positions c * chunk .. of it;
-    // partial results (maximum and sum of a row's chunk, then its weighted rows)
-    // where a row has more than one
+    // tile kernel: chunk c of a row is positions c * chunk .. of it
     int32_t chunk, n_chunks;
+    // few-row kernel: workgroups (0: one per sequence and KV head), and the most KV
+    // heads a workgroup's waves may take side by side
+    int32_t workers, few_heads;
+    // partial results (maximum and sum of a row's part, then its weighted rows)
+    // where a row has more than one part
     float2* part_ml;
     float* part_o;
     // sequences of at most this many rows (new tokens * group) are the few-row
@@ -249,9 +252,12 @@ struct RaggedParams {
 // Rows of a KV head that the few-row kernel takes: two blocks of 16, one where
 // two would not leave registers for the tile in flight.
 inline int FewMost(int head_dim) { return head_dim <= 128 ? 32 : 16; }
-constexpr int kFewKeys = 128;  // positions its workgroup's waves take per step
+constexpr int kFewKeys = 32;   // positions of its unit of work
+constexpr int kFewHeads = 8;   // most KV heads of its workgroup
 
 // Launches on `stream`; type and cache_type choose the instance.
+// Waves of a few-row workgroup: 8, or 4 where the registers of 8 would not do.
+inline int FewWaves(int head_dim, int few_rows) { return head_dim <= 128 && few_rows <= 16 ? 8 : 4; }
 mlk_status LaunchFew(const RaggedParams& p, int32_t type, int32_t cache_type, hipStream_t stream);
 mlk_status LaunchTile(const RaggedParams& p, int32_t type, int32_t cache_type, hipStream_t stream);
 
@@ -265,10 +271,104 @@ mlk_status ByType(int32_t type, int32_t cache_type, const F& f) {
     return f.template Run<F32, F32>();
 }
 
-// Where the partials of row m of KV head g lie: few-row kernel, by sequence;
-// tile kernel, by token row.
-__device__ inline int64_t FewPartial(const RaggedParams& p, int s, int g, int m) {
-    return ((static_cast<int64_t>(s) * p.n_kv_heads + g) * p.few_rows + m) * p.n_chunks;
+// The few-row kernel's work: units of kFewKeys positions, sequence by sequence,
+// block of KV heads by block.  Worker w takes units w * share .. + share - 1,
+// whatever sequences they belong to, so lengths of all kinds load the device
+// evenly; of the (sequence, block) pairs in its range only the first and the last
+// can be other workers' too, so it leaves at most two partial results a row.
+// Everything follows from the lengths on the device: a captured call divides
+// what it finds at its replay.
+struct FewWork {
+    int64_t share;
+    int32_t heads;  // KV heads of a block, a power of two up to kFewHeads
+    // the sequence looked for: its units and those of the sequences before it
+    int64_t before;
+    int32_t s, units;
+};
+
+__device__ inline int32_t FewUnits(const RaggedParams& p, int s) {
+    Seq q;
+    if (s >= p.batch.n_seqs || !LoadSeq(p.batch, s, &q)) return 0;
+    if (q.n == 0 || static_cast<int64_t>(q.n) * p.group > p.few_rows) return 0;
+    return (q.len + kFewKeys - 1) / kFewKeys;
+}
+
+// Units of all sequences, and of those before sequence `upto` (a whole wave;
+// every lane gets them).
+__device__ inline int64_t CountFewUnits(const RaggedParams& p, int upto, int64_t* before) {
+    const int lane = static_cast<int>(threadIdx.x) % kWave;
+    int64_t total = 0;
+    *before = 0;
+    for (int s0 = 0; s0 < p.batch.n_seqs; s0 += kWave) {
+        int64_t u = FewUnits(p, s0 + lane), b = s0 + lane < upto ? u : 0;
+        for (int off = kWave / 2; off > 0; off /= 2) {
+            u += __shfl_xor(u, off, kWave);
+            b += __shfl_xor(b, off, kWave);
+        }
+        total += u;
+        *before += b;
+    }
+    return total;
+}
+
+// How `total` units are divided.  A workgroup's waves take neighbouring heads of
+// the same positions (whole rows of the cache, read once and together) where
+// that leaves every worker kFewRun units or more; else fewer heads and more
+// waves per head, down to one head's positions spread over all waves.
+constexpr int kFewRun = 8;
+__device__ inline void DivideFew(const RaggedParams& p, int64_t total, FewWork* w) {
+    int heads = p.few_heads;
+    while (heads > 1 && total * (p.n_kv_heads / heads) < static_cast<int64_t>(p.workers) * kFewRun) {
+        heads /= 2;
+    }
+    const int64_t share = (total * (p.n_kv_heads / heads) + p.workers - 1) / p.workers;
+    w->heads = heads;
+    w->share = share > kFewRun ? share : kFewRun;
+}
+
+// The sequence of a worker's first unit (a whole wave; false: nothing to do).
+__device__ inline bool FindFewWork(const RaggedParams& p, int64_t worker, FewWork* w) {
+    const int lane = static_cast<int>(threadIdx.x) % kWave;
+    if (p.batch.n_seqs == 1) {
+        w->s = 0;
+        w->before = 0;
+        w->units = FewUnits(p, 0);
+        DivideFew(p, w->units, w);
+        return worker * w->share < static_cast<int64_t>(w->units) * (p.n_kv_heads / w->heads);
+    }
+    int64_t before = 0, total = 0;
+    if (p.batch.n_seqs > kWave) total = CountFewUnits(p, 0, &before);
+    for (int s0 = 0;; s0 += kWave) {
+        const int32_t mine = FewUnits(p, s0 + lane);
+        int64_t sum = mine;  // of lanes 0 .. lane
+        for (int off = 1; off < kWave; off *= 2) {
+            const int64_t v = __shfl_up(sum, off, kWave);
+            if (lane >= off) sum += v;
+        }
+        const int64_t here = __shfl(sum, kWave - 1, kWave);
+        if (s0 == 0) {
+            if (p.batch.n_seqs <= kWave) total = here;
+            DivideFew(p, total, w);
+        }
+        const int64_t blocks = p.n_kv_heads / w->heads, target = worker * w->share;
+        if (target >= total * blocks) return false;
+        const uint64_t past = __ballot((before + sum) * blocks > target);
+        if (past != 0) {
+            const int at = __builtin_ctzll(past);
+            w->s = s0 + at;
+            w->units = __builtin_amdgcn_readlane(mine, at);
+            w->before = before + __shfl(sum, at, kWave) - w->units;
+            return true;
+        }
+        before += here;
+    }
+}
+
+// Where the partial of row m lies: few-row kernel, by worker, place in its range
+// (0: its first pair, 1: its last) and head of the block; tile kernel, by token row.
+__device__ inline int64_t FewPartial(const RaggedParams& p, int64_t worker, int place, int head,
+                                     int m) {
+    return ((worker * 2 + place) * kFewHeads + head) * p.few_rows + m;
 }
 __device__ inline int64_t TilePartial(const RaggedParams& p, int32_t t, int h) {
     return (static_cast<int64_t>(t) * p.n_heads + h) * p.n_chunks;

@@ -15,120 +15,197 @@ namespace {
 
 constexpr int kThreads = 256;
 
-// out = sum_c 2^(m_c - m) o_c / sum_c 2^(m_c - m) l_c over a row's chunks, a wave
-// per row, chunks in order.
-template <typename A, bool kFew>
-__global__ __launch_bounds__(kThreads) void AttnJoin(const RaggedParams p) {
-    const int lane = static_cast<int>(threadIdx.x) % kWave;
-    const int64_t id = static_cast<int64_t>(blockIdx.x) * (kThreads / kWave) +
-                       __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / kWave);
+// out = sum_c 2^(m_c - m) o_c / sum_c 2^(m_c - m) l_c over a row's n chunks.  A
+// group of L lanes (4 dims each) takes every `per_row`-th chunk of a row, the
+// groups' sums are added in order.  What costs is latency, not bytes: the first
+// kAhead chunks of each group are on their way before the maxima are looked at
+// (one 8B decode row over 32 chunks: 21 us with one wave walking them all, 5 us).
+constexpr int kAhead = 4;
+
+template <typename A, int L, bool kFew>
+__global__ __launch_bounds__(kThreads) void AttnJoin(const RaggedParams p, int per_row, int per_seq) {
+    constexpr int NG = kThreads / L;
+    __shared__ f32x4 sums[NG][L];
+    const int lane = static_cast<int>(threadIdx.x) % L, g = static_cast<int>(threadIdx.x) / L;
+    const int rows_here = NG / per_row, part_of = g % per_row;
     const int hd = p.rows.head_dim;
     Seq q;
-    int64_t base;
-    int32_t t, h, n;
+    int64_t base = 0;              // the first part's partial, the second part's
+    int64_t next = 0, step = 1;    // partial, and from there one to the next
+    int32_t t = 0, h = 0, n = 0;   // n 0: no such row, or one part
     if constexpr (kFew) {
-        const int row = static_cast<int>(id % p.few_rows);
-        const int64_t rest = id / p.few_rows;
-        const int kvh = static_cast<int>(rest % p.n_kv_heads);
-        const int64_t s = rest / p.n_kv_heads;
-        if (s >= p.batch.n_seqs || !LoadSeq(p.batch, static_cast<int>(s), &q)) return;
-        const int64_t rows = static_cast<int64_t>(q.n) * p.group;
-        if (rows > p.few_rows || row >= rows || q.len <= p.chunk) return;
-        t = q.t0 + row / p.group;
-        h = kvh * p.group + row % p.group;
-        n = (q.len + p.chunk - 1) / p.chunk;
-        base = FewPartial(p, static_cast<int>(s), kvh, row);
+        // a workgroup's rows are of one sequence, so its waves count together
+        const int s = static_cast<int>(blockIdx.x / per_seq);
+        const int64_t in_seq =
+            static_cast<int64_t>(blockIdx.x % per_seq) * rows_here + g / per_row;
+        const int32_t units = FewUnits(p, s);
+        if (units == 0 || !LoadSeq(p.batch, s, &q)) return;
+        const int64_t real_rows = static_cast<int64_t>(q.n) * p.group;
+        const int row = static_cast<int>(in_seq % real_rows);
+        const int64_t kvh = in_seq / real_rows;
+        // none of the workgroup's rows is one
+        if (static_cast<int64_t>(blockIdx.x % per_seq) * rows_here >= real_rows * p.n_kv_heads) return;
+        int64_t before = 0;
+        FewWork work;
+        DivideFew(p, p.batch.n_seqs == 1 ? units : CountFewUnits(p, s, &before), &work);
+        if (kvh < p.n_kv_heads) {
+            const int64_t u0 = before * (p.n_kv_heads / work.heads) + kvh / work.heads * units;
+            const int64_t w0 = u0 / work.share, w1 = (u0 + units - 1) / work.share;
+            const int head = static_cast<int>(kvh % work.heads);
+            if (w1 > w0) {
+                t = q.t0 + row / p.group;
+                h = static_cast<int>(kvh) * p.group + row % p.group;
+                n = static_cast<int>(w1 - w0) + 1;
+                base = FewPartial(p, w0, u0 == w0 * work.share ? 0 : 1, head, row);
+                next = FewPartial(p, w0 + 1, 0, head, row);
+                step = 2 * kFewHeads * p.few_rows;
+            }
+        }
     } else {
-        if (id >= static_cast<int64_t>(p.batch.n_tokens) * p.n_heads) return;
+        const int64_t id = static_cast<int64_t>(blockIdx.x) * rows_here + g / per_row;
+        // the wave's first row finds the sequence, its others look on from there
         t = static_cast<int32_t>(id / p.n_heads);
         h = static_cast<int32_t>(id % p.n_heads);
-        const int s = LastSeq(p.batch, t, [](int32_t a, int) { return a; });
-        if (!LoadSeq(p.batch, s, &q) || t < q.t0 || t >= q.t0 + q.n) return;
-        const int32_t pos = q.len - q.n + (t - q.t0);
-        if (static_cast<int64_t>(q.n) * p.group <= p.few_rows || pos < p.chunk) return;
-        n = pos / p.chunk + 1;
-        base = TilePartial(p, t, h);
-    }
-    float m = -INFINITY;
-    for (int c = lane; c < n; c += kWave) m = fmaxf(m, p.part_ml[base + c].x);
-    m = WaveMax(m);
-    if (m == -INFINITY) m = 0.0f;
-    float l = 0.0f, o[4] = {0, 0, 0, 0};
-    const float* part = p.part_o + base * hd;
-#pragma unroll 4
-    for (int c = 0; c < n; ++c) {
-        const float2 ml = p.part_ml[base + c];
-        const float f = __builtin_amdgcn_exp2f(ml.x - m);
-        l = fmaf(ml.y, f, l);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int d = lane + kWave * i;
-            if (d < hd) o[i] = fmaf(part[static_cast<int64_t>(c) * hd + d], f, o[i]);
+        int s = LastSeq(p.batch, __builtin_amdgcn_readfirstlane(t), [](int32_t a, int) { return a; });
+        while (s + 1 < p.batch.n_seqs && p.batch.start[s + 1] <= t) ++s;
+        if (t < p.batch.n_tokens && LoadSeq(p.batch, s, &q) && t >= q.t0 && t < q.t0 + q.n) {
+            const int32_t pos = q.len - q.n + (t - q.t0);
+            if (static_cast<int64_t>(q.n) * p.group > p.few_rows && pos >= p.chunk) {
+                n = pos / p.chunk + 1;
+                base = TilePartial(p, t, h);
+                next = base + 1;
+            }
         }
     }
+    const bool wide = hd % 4 == 0;
+    auto part = [&](int c) { return c == 0 ? base : next + (c - 1) * step; };
+    auto dims = [&](int c) {
+        f32x4 x = {0, 0, 0, 0};
+        const float* at = p.part_o + part(c) * hd + 4 * lane;
+        if (wide) {
+            if (4 * lane < hd) x = *reinterpret_cast<const f32x4*>(at);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                if (4 * lane + e < hd) x[e] = at[e];
+            }
+        }
+        return x;
+    };
+    f32x4 ahead[kAhead];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+        const int c = part_of + per_row * i;
+        if (c < n) ahead[i] = dims(c);
+    }
+    float m = -INFINITY;
+    for (int c = lane; c < n; c += L) m = fmaxf(m, p.part_ml[part(c)].x);
+#pragma unroll
+    for (int off = L / 2; off > 0; off /= 2) m = fmaxf(m, __shfl_xor(m, off, kWave));
+    if (m == -INFINITY) m = 0.0f;
+    float l = 0.0f;
+    for (int c = lane; c < n; c += L) {
+        const float2 ml = p.part_ml[part(c)];
+        l = fmaf(ml.y, __builtin_amdgcn_exp2f(ml.x - m), l);
+    }
+#pragma unroll
+    for (int off = L / 2; off > 0; off /= 2) l += __shfl_xor(l, off, kWave);
+    f32x4 o = {0, 0, 0, 0};
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+        const int c = part_of + per_row * i;
+        if (c < n) o += ahead[i] * __builtin_amdgcn_exp2f(p.part_ml[part(c)].x - m);
+    }
+#pragma unroll 4
+    for (int c = part_of + per_row * kAhead; c < n; c += per_row) {
+        o += dims(c) * __builtin_amdgcn_exp2f(p.part_ml[part(c)].x - m);
+    }
+    sums[g][lane] = o;
+    __syncthreads();
+    if (part_of != 0 || n == 0) return;
+    for (int i = 1; i < per_row; ++i) o += sums[g + i][lane];
     typename A::Bits* out =
         static_cast<typename A::Bits*>(p.out) + (static_cast<int64_t>(t) * p.n_heads + h) * hd;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int d = lane + kWave * i;
-        if (d < hd) out[d] = A::Put(o[i] / l);
+    for (int e = 0; e < 4; ++e) {
+        if (4 * lane + e < hd) out[4 * lane + e] = A::Put(o[e] / l);
     }
 }
 
-template <bool kFew>
-mlk_status LaunchJoin(const RaggedParams& p, int32_t type, int64_t waves, hipStream_t s) {
-    const int64_t blocks = (waves + kThreads / kWave - 1) / (kThreads / kWave);
+// per_seq: rows of a sequence (few-row kernel; 0: the tile kernel's, one after
+// the other), `parts` the most a row can have.
+template <typename A, bool kFew>
+mlk_status LaunchJoin(const RaggedParams& p, int64_t rows, int64_t parts, hipStream_t s) {
+    const int groups = p.rows.head_dim <= 128 ? 8 : 4;
+    int per_row = 1;
+    while (per_row < groups && per_row < parts) per_row *= 2;
+    const int64_t per_seq = (rows * per_row + groups - 1) / groups;
+    const int64_t blocks = kFew ? per_seq * p.batch.n_seqs : per_seq;
     if (blocks > 0x7FFFFFFF) return Fail(MLK_ERR_INVALID, "attention: too many rows to join");
     const dim3 grid(static_cast<unsigned>(blocks));
-    if (type == MLK_F32) hipLaunchKernelGGL((AttnJoin<F32, kFew>), grid, dim3(kThreads), 0, s, p);
-    else if (type == MLK_F16) hipLaunchKernelGGL((AttnJoin<F16, kFew>), grid, dim3(kThreads), 0, s, p);
-    else hipLaunchKernelGGL((AttnJoin<BF16, kFew>), grid, dim3(kThreads), 0, s, p);
+    const int n = static_cast<int>(per_seq);
+    if (groups == 8) {
+        hipLaunchKernelGGL((AttnJoin<A, 32, kFew>), grid, dim3(kThreads), 0, s, p, per_row, n);
+    } else {
+        hipLaunchKernelGGL((AttnJoin<A, 64, kFew>), grid, dim3(kThreads), 0, s, p, per_row, n);
+    }
     return CheckLaunch("AttnJoin");
 }
 
-struct Part {
-    bool run = false;
-    int64_t chunk = 0, n_chunks = 1, partials = 0;  // partials: rows times chunks
-    int64_t Bytes(int32_t hd) const {
-        return n_chunks > 1 ? (partials * (4 * hd + 8) + 255) / 256 * 256 : 0;
-    }
-};
+template <bool kFew>
+mlk_status LaunchJoin(const RaggedParams& p, int32_t type, int64_t rows, int64_t parts,
+                      hipStream_t s) {
+    if (type == MLK_F32) return LaunchJoin<F32, kFew>(p, rows, parts, s);
+    if (type == MLK_F16) return LaunchJoin<F16, kFew>(p, rows, parts, s);
+    return LaunchJoin<BF16, kFew>(p, rows, parts, s);
+}
+
 struct Plan {
-    int32_t few_rows = 0;
-    Part few, tile;
+    int64_t few_rows = 0, few_workers = 0, few_partials = 0;
+    bool tile = false;
+    int64_t chunk = 0, n_chunks = 1, tile_partials = 0;
 };
 
-// Chunks of at least `least` positions (and a multiple of it), as many as bring
-// `base` workgroups to about `want`.
-Part Split(int64_t base, int64_t want, int64_t least, int64_t max_len) {
-    Part part;
-    part.run = true;
-    int64_t n = base > 0 ? (want + base - 1) / base : 1;
-    const int64_t most = (max_len + least - 1) / least;
-    if (n > most) n = most;
-    if (n < 1) n = 1;
-    part.chunk = ((max_len + n - 1) / n + least - 1) / least * least;
-    part.n_chunks = (max_len + part.chunk - 1) / part.chunk;
-    return part;
+int64_t PartBytes(int64_t partials, int32_t hd) {
+    return (partials * (4 * hd + 8) + 255) / 256 * 256;
 }
+int64_t PlanBytes(const Plan& plan, int32_t hd) {
+    return PartBytes(plan.few_partials, hd) + PartBytes(plan.tile_partials, hd);
+}
+
+constexpr int64_t kFewUnsplit = 512;   // longest sequences that are not split
+constexpr int64_t kTileLeast = 512;    // positions of a tile row's least chunk
 
 Plan MakePlan(int64_t n_seqs, int64_t n_tokens, int64_t max_new, int64_t max_len, int32_t n_heads,
               int32_t n_kv_heads, int32_t head_dim, bool packed) {
     Plan plan;
     const int64_t group = n_heads / n_kv_heads, cus = ComputeUnits();
     const int64_t most = FewMost(head_dim), max_rows = max_new * group;
-    plan.tile.run = max_rows > most;
+    plan.tile = max_rows > most;
     // a mixed batch of short sequences is left to the tile kernel alone
-    plan.few.run = !plan.tile.run || (!packed && n_seqs > 1 && group <= most && max_len >= 512 &&
-                                      n_tokens < n_seqs * max_new);
-    if (plan.few.run) {
-        plan.few_rows = static_cast<int32_t>(max_rows < most ? max_rows : most);
-        plan.few = Split(n_seqs * n_kv_heads, 3 * cus, 256, max_len);
-        plan.few.partials = n_seqs * n_kv_heads * plan.few_rows * plan.few.n_chunks;
+    if (!plan.tile || (!packed && n_seqs > 1 && group <= 16 && max_len > kFewUnsplit &&
+                       n_tokens < n_seqs * max_new)) {
+        // beside the tile kernel one block of rows, decode steps', is enough
+        const int64_t limit = plan.tile ? 16 : most;
+        plan.few_rows = max_rows < limit ? max_rows : limit;
+        if (max_len > kFewUnsplit) {
+            const int64_t units = n_seqs * n_kv_heads * ((max_len + kFewKeys - 1) / kFewKeys);
+            // 8 waves per compute unit: two such workgroups' loads get in each other's
+            // way (64 bf16 decode rows of the 8B heads: 189 us, with twice as many 213)
+            plan.few_workers = cus * 8 / FewWaves(head_dim, static_cast<int32_t>(plan.few_rows));
+            const int64_t most_workers = (units + kFewRun - 1) / kFewRun;
+            if (plan.few_workers > most_workers) plan.few_workers = most_workers;
+            plan.few_partials = 2 * plan.few_workers * kFewHeads * plan.few_rows;
+        }
     }
-    if (plan.tile.run) {
-        plan.tile = Split((n_tokens * group / 128 + n_seqs) * n_kv_heads, 2 * cus, 512, max_len);
-        plan.tile.partials = n_tokens * n_heads * plan.tile.n_chunks;
+    if (plan.tile) {
+        const int64_t base = (n_tokens * group / 128 + 1) * n_kv_heads;
+        int64_t n = (2 * cus + base - 1) / base;
+        const int64_t longest = (max_len + kTileLeast - 1) / kTileLeast;
+        if (n > longest) n = longest;
+        plan.chunk = ((max_len + n - 1) / n + kTileLeast - 1) / kTileLeast * kTileLeast;
+        plan.n_chunks = (max_len + plan.chunk - 1) / plan.chunk;
+        if (plan.n_chunks > 1) plan.tile_partials = n_tokens * n_heads * plan.n_chunks;
     }
     return plan;
 }
@@ -146,9 +223,9 @@ int64_t AttendWorkspace(int64_t n_seqs, int64_t n_tokens, int64_t max_new, int64
     }
     if (max_new > max_len) max_new = max_len;
     if (max_new > n_tokens) max_new = n_tokens;
-    const Plan plan =
-        MakePlan(n_seqs, n_tokens, max_new, max_len, n_heads, n_kv_heads, head_dim, packed);
-    return plan.few.Bytes(head_dim) + plan.tile.Bytes(head_dim);
+    return PlanBytes(
+        MakePlan(n_seqs, n_tokens, max_new, max_len, n_heads, n_kv_heads, head_dim, packed),
+        head_dim);
 }
 
 mlk_status Attend(const AttendArgs& a) {
@@ -156,11 +233,10 @@ mlk_status Attend(const AttendArgs& a) {
     const Ragged& b = a.batch;
     Plan plan = MakePlan(b.n_seqs, b.n_tokens, b.max_new, b.max_len, a.n_heads, a.n_kv_heads, hd,
                          b.table == nullptr);
-    if (static_cast<int64_t>(a.workspace_bytes) < plan.few.Bytes(hd) + plan.tile.Bytes(hd)) {
-        for (Part* part : {&plan.few, &plan.tile}) {  // no split
-            part->chunk = b.max_len;
-            part->n_chunks = 1;
-        }
+    if (static_cast<int64_t>(a.workspace_bytes) < PlanBytes(plan, hd)) {  // no split
+        plan.few_workers = plan.few_partials = plan.tile_partials = 0;
+        plan.chunk = b.max_len;
+        plan.n_chunks = 1;
     }
     RaggedParams p{};
     p.batch = b;
@@ -175,37 +251,37 @@ mlk_status Attend(const AttendArgs& a) {
     p.vec = hd % 8 == 0 && Multiple8(a.q_row) && Multiple8(a.rows.k_row) &&
             Multiple8(a.rows.v_row) && Multiple8(a.rows.page_stride) && Aligned(a.q, 16) &&
             Aligned(a.rows.k, 16) && Aligned(a.rows.v, 16) && Aligned(a.out, 16);
-    p.few_rows = plan.few_rows;
+    p.few_rows = static_cast<int32_t>(plan.few_rows);
     p.err = a.err;
     char* ws = static_cast<char*>(a.workspace);
-    auto place = [&](const Part& part) {
-        p.chunk = static_cast<int32_t>(part.chunk);
-        p.n_chunks = static_cast<int32_t>(part.n_chunks);
-        p.part_o = nullptr;
-        p.part_ml = nullptr;
-        if (part.n_chunks > 1) {
-            p.part_o = reinterpret_cast<float*>(ws);
-            p.part_ml = reinterpret_cast<float2*>(ws + part.partials * 4 * hd);
-            ws += part.Bytes(hd);
-        }
+    auto place = [&](int64_t partials) {
+        p.part_o = reinterpret_cast<float*>(ws);
+        p.part_ml = reinterpret_cast<float2*>(ws + partials * 4 * hd);
+        ws += PartBytes(partials, hd);
     };
-    if (plan.few.run) {
-        place(plan.few);
+    if (plan.few_rows > 0) {
+        p.workers = static_cast<int32_t>(plan.few_workers);
+        p.few_heads = FewWaves(hd, p.few_rows);
+        while (a.n_kv_heads % p.few_heads != 0) p.few_heads /= 2;
+        if (p.workers > 0) place(plan.few_partials);
         mlk_status st = LaunchFew(p, a.type, a.cache_type, a.stream);
         if (st != MLK_OK) return st;
-        if (p.n_chunks > 1) {
-            st = LaunchJoin<true>(p, a.type, static_cast<int64_t>(b.n_seqs) * a.n_kv_heads * p.few_rows,
-                                  a.stream);
+        if (p.workers > 0) {
+            const int64_t pairs = static_cast<int64_t>(b.n_seqs) * a.n_kv_heads;
+            st = LaunchJoin<true>(p, a.type, static_cast<int64_t>(a.n_kv_heads) * p.few_rows,
+                                  (p.workers + pairs - 1) / pairs + 1, a.stream);
             if (st != MLK_OK) return st;
         }
     }
-    if (plan.tile.run) {
-        place(plan.tile);
+    if (plan.tile) {
+        p.chunk = static_cast<int32_t>(plan.chunk);
+        p.n_chunks = static_cast<int32_t>(plan.n_chunks);
+        if (p.n_chunks > 1) place(plan.tile_partials);
         mlk_status st = LaunchTile(p, a.type, a.cache_type, a.stream);
         if (st != MLK_OK) return st;
         if (p.n_chunks > 1) {
-            st = LaunchJoin<false>(p, a.type, static_cast<int64_t>(b.n_tokens) * a.n_heads, a.stream);
-            if (st != MLK_OK) return st;
+            return LaunchJoin<false>(p, a.type, static_cast<int64_t>(b.n_tokens) * a.n_heads,
+                                     p.n_chunks, a.stream);
         }
     }
     return MLK_OK;

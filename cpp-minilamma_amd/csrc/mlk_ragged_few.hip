@@ -29,9 +29,6 @@
 namespace mlk {
 namespace {
 
-constexpr int kThreads = 256;
-constexpr int kWaves = kThreads / kWave;
-
 __device__ inline uint32_t LowHalves(uint32_t a, uint32_t b) {
     return __builtin_amdgcn_perm(b, a, 0x05040100u);
 }
@@ -74,11 +71,11 @@ struct FewTile {
         constexpr int W = N * sizeof(B) / 4;
         if (kFull || (vec && left >= N)) {
             if constexpr (W == 4) {
-                const u32x4 x = *reinterpret_cast<const u32x4*>(p);
+                const u32x4 x = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p));
 #pragma unroll
                 for (int i = 0; i < 4; ++i) o[i] = x[i];
             } else {
-                const u32x2 x = *reinterpret_cast<const u32x2*>(p);
+                const u32x2 x = __builtin_nontemporal_load(reinterpret_cast<const u32x2*>(p));
                 o[0] = x[0];
                 o[1] = x[1];
             }
@@ -116,8 +113,9 @@ __device__ inline void RowOffsets(const FewRows& r, int32_t j, int64_t* ko, int6
     }
 }
 
-template <typename A, typename C, int HD, int NB, bool kFull>
-__global__ __launch_bounds__(kThreads) void AttnFew(const RaggedParams p) {
+template <typename A, typename C, int HD, int NB, int kWaves, bool kFull>
+__global__ __launch_bounds__(kWaves * kWave) void AttnFew(const RaggedParams p) {
+    constexpr int kThreads = kWaves * kWave;
     typedef Pieces<A, C> P;
     typedef typename P::M M;
     typedef FewTile<C, HD, kFull> Tile;
@@ -136,18 +134,46 @@ __global__ __launch_bounds__(kThreads) void AttnFew(const RaggedParams p) {
     const int i16 = lane % 16, g4 = lane / 16;
     const int hd = kFull ? HD : p.rows.head_dim;
     if (blockIdx.x == 0) CheckSeqs(p.batch, p.err);
-    const int kvh = static_cast<int>(blockIdx.x % p.n_kv_heads);
-    const int64_t rest = blockIdx.x / p.n_kv_heads;
-    const int chunk = static_cast<int>(rest % p.n_chunks);
-    const int s = static_cast<int>(rest / p.n_chunks);
+    const bool vec = kFull || p.vec;
+    FewWork work;
+    int64_t unit, end;  // this worker's units
+    if (p.workers == 0) {
+        work.heads = 1;
+        work.s = static_cast<int>(blockIdx.x / p.n_kv_heads);
+        work.units = FewUnits(p, work.s);
+        work.before = 0;
+        unit = static_cast<int64_t>(blockIdx.x % p.n_kv_heads) * work.units;
+        end = unit + work.units;
+    } else {
+        if (!FindFewWork(p, blockIdx.x, &work)) return;
+        unit = blockIdx.x * work.share;
+        end = unit + work.share;
+    }
+    const int heads = __builtin_amdgcn_readfirstlane(work.heads);  // of a block
+    const int blocks = p.n_kv_heads / heads;
+    const int along = kWaves / heads;   // waves of a head, taking tiles in turn
+    const int my_head = wave % heads, my_turn = wave / heads;
+    for (bool first = true; unit < end; first = false) {
+    while (work.units == 0 || unit >= (work.before + work.units) * blocks) {
+        work.before += work.units;
+        if (++work.s >= p.batch.n_seqs) return;
+        work.units = FewUnits(p, work.s);
+    }
+    const int s = __builtin_amdgcn_readfirstlane(work.s);
+    const int32_t units = __builtin_amdgcn_readfirstlane(work.units);
+    const int64_t in_seq = unit - work.before * blocks;
+    const int head0 = __builtin_amdgcn_readfirstlane(static_cast<int>(in_seq / units)) * heads;
+    const int kvh = head0 + my_head;
+    const int32_t u0 = __builtin_amdgcn_readfirstlane(static_cast<int>(in_seq % units));
+    const int32_t u1 = __builtin_amdgcn_readfirstlane(
+        end - unit < units - u0 ? u0 + static_cast<int32_t>(end - unit) : units);
+    unit += u1 - u0;
     Seq q;
     if (!LoadSeq(p.batch, s, &q)) return;
     const int rows = q.n * p.group;
-    const int32_t j_begin = chunk * p.chunk;
-    if (rows == 0 || rows > p.few_rows || j_begin >= q.len) return;
-    const int32_t j_end = q.len - j_begin < p.chunk ? q.len : j_begin + p.chunk;
-    const bool split = q.len > p.chunk;
-    const bool vec = kFull || p.vec;
+    const int32_t j_begin = u0 * kFewKeys;
+    const int32_t j_end = u1 < units ? u1 * kFewKeys : q.len;
+    const bool split = u1 - u0 < units;
 
     const FewRows fr{&p.rows,
                      p.batch.table == nullptr ? nullptr : p.batch.table + s * p.batch.table_stride,
@@ -155,10 +181,12 @@ __global__ __launch_bounds__(kThreads) void AttnFew(const RaggedParams p) {
     const CB* kb = static_cast<const CB*>(p.rows.k) + static_cast<int64_t>(kvh) * hd;
     const CB* vb = static_cast<const CB*>(p.rows.v) + static_cast<int64_t>(kvh) * hd;
 
-    // the rows' positions and q operands
+    // the rows' positions and q as it lies in memory; converted when the first
+    // tile's loads are on their way
+    constexpr int NQR = kF32 ? HD / 16 : HD / 32;  // runs of q a lane holds
+    constexpr int NQW = kF32 ? 4 : (sizeof(AB) == 4 ? 8 : 4);
     int32_t pos[NB];
-    float factor[NB];
-    u32x4 qp[NB][kF32 ? HD / 16 : HD / 32][NQ];
+    uint32_t raw[NB][NQR][NQW];
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
         const int m = 16 * nb + i16;
@@ -167,48 +195,13 @@ __global__ __launch_bounds__(kThreads) void AttnFew(const RaggedParams p) {
         pos[nb] = real ? q.len - q.n + i : -1;
         const AB* qr = static_cast<const AB*>(p.q) + static_cast<int64_t>(q.t0 + i) * p.q_row +
                        static_cast<int64_t>(kvh * p.group + (real ? m % p.group : 0)) * hd;
-        factor[nb] = p.factor;
-        if constexpr (kF32) {
 #pragma unroll
-            for (int c = 0; c < HD / 16; ++c) {
-                uint32_t w[4];
+        for (int c = 0; c < NQR; ++c) {
+            if constexpr (kF32) {
                 FewTile<F32, HD, kFull>::template Run<4>(qr + 16 * c + 4 * g4, hd - 16 * c - 4 * g4,
-                                                         vec, w);
-                qp[nb][c][0] = u32x4{w[0], w[1], w[2], w[3]};
-            }
-        } else {
-            uint32_t raw[HD / 32][sizeof(AB) == 4 ? 8 : 4];
-#pragma unroll
-            for (int c = 0; c < HD / 32; ++c) {
-                LoadChunk<A, kFull>(qr + 32 * c + 8 * g4, hd - 32 * c - 8 * g4, vec, raw[c]);
-            }
-            if constexpr (NQ == 1) {
-#pragma unroll
-                for (int c = 0; c < HD / 32; ++c) {
-                    qp[nb][c][0] = u32x4{raw[c][0], raw[c][1], raw[c][2], raw[c][3]};
-                }
+                                                         vec, raw[nb][c]);
             } else {
-                float up = 1.0f;
-                if constexpr (P::kScaleQ) {
-                    float amax = 0.0f;
-#pragma unroll
-                    for (int c = 0; c < HD / 32; ++c) {
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) {
-                            amax = fmaxf(amax, fabsf(__uint_as_float(raw[c][e])));
-                        }
-                    }
-                    const int e = RowExponent(Max32(Max16(amax)));
-                    up = ldexpf(1.0f, e);
-                    factor[nb] = ldexpf(p.factor, -e);
-                }
-#pragma unroll
-                for (int c = 0; c < HD / 32; ++c) {
-                    float x[8];
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) x[e] = __uint_as_float(raw[c][e]) * up;
-                    Split8<M, NQ>(x, qp[nb][c]);
-                }
+                LoadChunk<A, kFull>(qr + 32 * c + 8 * g4, hd - 32 * c - 8 * g4, vec, raw[nb][c]);
             }
         }
     }
@@ -217,15 +210,27 @@ __global__ __launch_bounds__(kThreads) void AttnFew(const RaggedParams p) {
     bool bad = false;
     // 16-position blocks whose rows lie evenly apart: whole pages' parts, or packed
     const bool even = fr.table == nullptr || p.rows.page_shift >= 4;
-    auto block_base = [&](int32_t j, int64_t row) -> int64_t {  // j uniform, j + 15 < end
+    // element offsets of the blocks' first rows; the pages of the tile after the
+    // next are looked up a tile ahead, so that no load waits for its page
+    int32_t page[NBK];
+    auto find = [&](int32_t j) {
+        if (fr.table == nullptr || !even) return;
+#pragma unroll
+        for (int b = 0; b < NBK; ++b) {
+            if (j + 16 * b < j_end) page[b] = ReadIndex(fr.table + ((j + 16 * b) >> p.rows.page_shift));
+        }
+    };
+    auto block_base = [&](int b, int32_t j, int64_t row) -> int64_t {  // j + 15 < end
         if (fr.table == nullptr) return (fr.t0 + j) * row;
-        return PagedRow(p.rows, PageOf(p.rows, fr.table, j, &bad), j);
+        const bool in = page[b] >= 0 && page[b] < p.rows.n_pages;
+        if (!in) bad = true;
+        return PagedRow(p.rows, in ? page[b] : 0, j);
     };
     auto load_k = [&](int32_t j0) {
         if (even && j0 + KT <= j_end) {
 #pragma unroll
             for (int b = 0; b < NBK; ++b) {
-                const CB* base = kb + block_base(j0 + 16 * b, p.rows.k_row);
+                const CB* base = kb + block_base(b, j0 + 16 * b, p.rows.k_row);
                 tile.LoadK(b, base + i16 * static_cast<uint32_t>(p.rows.k_row), g4, hd, vec);
             }
             return;
@@ -241,7 +246,7 @@ __global__ __launch_bounds__(kThreads) void AttnFew(const RaggedParams p) {
         if (even && j0 + KT <= j_end) {
 #pragma unroll
             for (int b = 0; b < NBK; ++b) {
-                const CB* base = vb + block_base(j0 + 16 * b, p.rows.v_row);
+                const CB* base = vb + block_base(b, j0 + 16 * b, p.rows.v_row);
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     tile.LoadV(4 * b + r, base + r * p.rows.v_row +
@@ -258,6 +263,45 @@ __global__ __launch_bounds__(kThreads) void AttnFew(const RaggedParams p) {
         }
     };
 
+    const int32_t step = along * KT;
+    int32_t j0 = j_begin + my_turn * KT;
+    if (j0 < j_end) {
+        find(j0);
+        load_k(j0);
+        load_v(j0);
+        find(j0 + step);
+    }
+
+    float factor[NB];
+    u32x4 qp[NB][NQR][NQ];
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+        factor[nb] = p.factor;
+        float up = 1.0f;
+        if constexpr (!kF32 && P::kScaleQ) {
+            float amax = 0.0f;
+#pragma unroll
+            for (int c = 0; c < NQR; ++c) {
+#pragma unroll
+                for (int e = 0; e < NQW; ++e) amax = fmaxf(amax, fabsf(__uint_as_float(raw[nb][c][e])));
+            }
+            const int e = RowExponent(Max32(Max16(amax)));
+            up = ldexpf(1.0f, e);
+            factor[nb] = ldexpf(p.factor, -e);
+        }
+#pragma unroll
+        for (int c = 0; c < NQR; ++c) {
+            if constexpr (NQ == 1) {
+                qp[nb][c][0] = u32x4{raw[nb][c][0], raw[nb][c][1], raw[nb][c][2], raw[nb][c][3]};
+            } else {
+                float x[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[e] = __uint_as_float(raw[nb][c][e]) * up;
+                Split8<M, NQ>(x, qp[nb][c]);
+            }
+        }
+    }
+
     f32x4 o[NB][NI];
     float m[NB], l[NB];
 #pragma unroll
@@ -270,13 +314,8 @@ __global__ __launch_bounds__(kThreads) void AttnFew(const RaggedParams p) {
     const int32_t first_pos = q.len - q.n;  // the lowest position of a row
     bool special = false;                   // met a non-finite V in a masked tile
 
-    int32_t j0 = j_begin + wave * KT;
-    if (j0 < j_end) {
-        load_k(j0);
-        load_v(j0);
-    }
-    for (; j0 < j_end; j0 += kWaves * KT) {
-        const int32_t jn = j0 + kWaves * KT;
+    for (; j0 < j_end; j0 += step) {
+        const int32_t jn = j0 + step;
         f32x4 sc[NB][NBK];
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
@@ -379,11 +418,59 @@ __global__ __launch_bounds__(kThreads) void AttnFew(const RaggedParams p) {
                 }
             }
         }
-        if (jn < j_end) load_v(jn);
+        if (jn < j_end) {
+            load_v(jn);
+            find(jn + step);
+        }
     }
     if (bad && p.err != nullptr) RaiseFlag(p.err, 1);
 
-    // join the waves: all relative to the largest maximum
+    const int32_t masked_from0 = (first_pos < j_end ? first_pos : j_end) - KT;
+    const int32_t masked_from = masked_from0 > j_begin ? masked_from0 : j_begin;
+    const int place = first ? 0 : 1;
+    if (along == 1) {
+        // the wave has its head's positions to itself
+        const bool any_special = __ballot(special) != 0;
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) {
+            const float lt = Sum32(Sum16(l[nb]));
+            const int row = 16 * nb + i16;
+            if (row >= rows) continue;
+            const int i = row / p.group, h = kvh * p.group + row % p.group;
+            const int64_t at = FewPartial(p, blockIdx.x, place, my_head, row);
+            AB* out = static_cast<AB*>(p.out) + (static_cast<int64_t>(q.t0 + i) * p.n_heads + h) * hd;
+            float* part = p.part_o + at * hd;
+            if (split && g4 == 0) p.part_ml[at] = make_float2(m[nb], lt);
+            const float inv = split ? 1.0f : 1.0f / lt;
+            const int32_t last = pos[nb] < j_end ? pos[nb] : j_end - 1;
+#pragma unroll
+            for (int n = 0; n < Tile::NVR; ++n) {
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const int d0 = 16 * Tile::VE * n + Tile::VE * (4 * g4 + r);
+                    float x[Tile::VE];
+#pragma unroll
+                    for (int e = 0; e < Tile::VE; ++e) x[e] = o[nb][Tile::VE * n + e][r] * inv;
+                    if (any_special) {
+                        for (int e = 0; e < Tile::VE; ++e) {
+                            if (d0 + e < hd) {
+                                x[e] += NonFiniteSum<C>(p.rows, fr.table, fr.t0, vb, masked_from,
+                                                        last, d0 + e);
+                            }
+                        }
+                    }
+#pragma unroll
+                    for (int e = 0; e < Tile::VE; ++e) {
+                        if (kFull || d0 + e < hd) {
+                            if (split) part[d0 + e] = x[e];
+                            else out[d0 + e] = A::Put(x[e]);
+                        }
+                    }
+                }
+            }
+        }
+    } else {
+    // join the waves of a head: all relative to the largest maximum
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
         const float lt = Sum32(Sum16(l[nb]));
@@ -396,9 +483,8 @@ __global__ __launch_bounds__(kThreads) void AttnFew(const RaggedParams p) {
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
         const int row = 16 * nb + i16;
-        float top = sm[0][row];
-#pragma unroll
-        for (int w = 1; w < kWaves; ++w) top = fmaxf(top, sm[w][row]);
+        float top = -INFINITY;
+        for (int w = my_head; w < kWaves; w += heads) top = fmaxf(top, sm[w][row]);
         const float f = __builtin_amdgcn_exp2f(m[nb] - (top == -INFINITY ? 0.0f : top));
 #pragma unroll
         for (int e = 0; e < NI; ++e) {
@@ -410,27 +496,26 @@ __global__ __launch_bounds__(kThreads) void AttnFew(const RaggedParams p) {
         }
     }
     special = __syncthreads_or(special);
-    const int32_t masked_from = (first_pos < j_end ? first_pos : j_end) - KT;
-    for (int u = tid; u < rows * HD; u += kThreads) {
-        const int row = u / HD, d = u % HD;
+    for (int u = tid; u < heads * rows * HD; u += kThreads) {
+        const int d = u % HD, row = u / HD % rows, hb = u / HD / rows;
         if (!kFull && d >= hd) continue;
-        float top = sm[0][row], lt = 0.0f, sum = 0.0f;
-#pragma unroll
-        for (int w = 1; w < kWaves; ++w) top = fmaxf(top, sm[w][row]);
+        float top = -INFINITY, lt = 0.0f, sum = 0.0f;
+        for (int w = hb; w < kWaves; w += heads) top = fmaxf(top, sm[w][row]);
         const float base = top == -INFINITY ? 0.0f : top;
-#pragma unroll
-        for (int w = 0; w < kWaves; ++w) {
+        for (int w = hb; w < kWaves; w += heads) {
             lt += sl[w][row] * __builtin_amdgcn_exp2f(sm[w][row] - base);
             sum += so[w][row][d];
         }
-        const int i = row / p.group, h = kvh * p.group + row % p.group;
+        const int i = row / p.group, h = (head0 + hb) * p.group + row % p.group;
         if (special) {
             const int32_t last = first_pos + i < j_end ? first_pos + i : j_end - 1;
-            sum += NonFiniteSum<C>(p.rows, fr.table, fr.t0, vb,
-                                   masked_from > j_begin ? masked_from : j_begin, last, d);
+            sum += NonFiniteSum<C>(p.rows, fr.table, fr.t0,
+                                   static_cast<const CB*>(p.rows.v) +
+                                       static_cast<int64_t>(head0 + hb) * hd,
+                                   masked_from, last, d);
         }
         if (split) {
-            const int64_t at = FewPartial(p, s, kvh, row) + chunk;
+            const int64_t at = FewPartial(p, blockIdx.x, place, hb, row);
             p.part_o[at * hd + d] = sum;
             if (d == 0) p.part_ml[at] = make_float2(top, lt);
         } else {
@@ -439,17 +524,27 @@ __global__ __launch_bounds__(kThreads) void AttnFew(const RaggedParams p) {
             out[d] = A::Put(sum / lt);
         }
     }
+    __syncthreads();  // the next pair writes over what was read here
+    }
+    }
+}
+
+template <typename A, typename C, int HD, int NB, int kWaves>
+void Start(const RaggedParams& p, dim3 grid, hipStream_t s) {
+    if (p.vec && p.rows.head_dim == HD) {
+        hipLaunchKernelGGL((AttnFew<A, C, HD, NB, kWaves, true>), grid, dim3(kWaves * kWave), 0, s, p);
+    } else {
+        hipLaunchKernelGGL((AttnFew<A, C, HD, NB, kWaves, false>), grid, dim3(kWaves * kWave), 0, s, p);
+    }
 }
 
 template <typename A, typename C, int HD>
 mlk_status Launch(const RaggedParams& p, dim3 grid, hipStream_t s) {
-    const bool full = p.vec && p.rows.head_dim == HD;
-    if (p.few_rows <= 16) {
-        if (full) hipLaunchKernelGGL((AttnFew<A, C, HD, 1, true>), grid, dim3(kThreads), 0, s, p);
-        else hipLaunchKernelGGL((AttnFew<A, C, HD, 1, false>), grid, dim3(kThreads), 0, s, p);
-    } else if constexpr (HD <= 128) {
-        if (full) hipLaunchKernelGGL((AttnFew<A, C, HD, 2, true>), grid, dim3(kThreads), 0, s, p);
-        else hipLaunchKernelGGL((AttnFew<A, C, HD, 2, false>), grid, dim3(kThreads), 0, s, p);
+    if constexpr (HD <= 128) {
+        if (p.few_rows <= 16) Start<A, C, HD, 1, 8>(p, grid, s);
+        else Start<A, C, HD, 2, 4>(p, grid, s);
+    } else {
+        Start<A, C, HD, 1, 4>(p, grid, s);
     }
     return CheckLaunch("AttnFew");
 }
@@ -469,7 +564,8 @@ struct ByDim {
 }  // namespace
 
 mlk_status LaunchFew(const RaggedParams& p, int32_t type, int32_t cache_type, hipStream_t stream) {
-    const int64_t blocks = static_cast<int64_t>(p.batch.n_seqs) * p.n_chunks * p.n_kv_heads;
+    const int64_t blocks = p.workers != 0 ? p.workers
+                                          : static_cast<int64_t>(p.batch.n_seqs) * p.n_kv_heads;
     if (blocks > INT_MAX) {
         return Fail(MLK_ERR_INVALID, "attention: %lld workgroups exceed the grid",
                     static_cast<long long>(blocks));

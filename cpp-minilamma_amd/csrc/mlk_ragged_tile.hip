@@ -26,8 +26,8 @@
 namespace mlk {
 namespace {
 
-constexpr int kThreads = 256;
-constexpr int kRows = 128;
+constexpr int kThreads = 512;
+constexpr int kRows = 256;
 
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) s16x4* LdsS16x4;
@@ -41,7 +41,7 @@ __device__ inline int Swizzle(int r) {
 template <typename C, int HD>
 struct TileShape {
     static constexpr int NK = std::is_same<C, F32>::value ? 3 : 1;
-    static constexpr int KT = NK == 3 || HD == 256 ? 32 : 64;
+    static constexpr int KT = HD != 64 && (NK == 3 || HD == 256) ? 32 : 64;
     static constexpr int NBUF = NK == 3 ? 1 : 2;
     static constexpr int kPlane = KT * HD;             // elements
     static constexpr int NCH = KT * HD / 8 / kThreads;  // chunks a thread stages
@@ -49,7 +49,7 @@ struct TileShape {
 };
 
 template <typename A, typename C, int HD, bool kFull>
-__global__ __launch_bounds__(kThreads) void AttnTile(const RaggedParams p, int n_slots) {
+__global__ __launch_bounds__(kThreads, HD <= 128 ? 2 : 1) void AttnTile(const RaggedParams p, int n_slots) {
     typedef Pieces<A, C> P;
     typedef typename P::M M;
     typedef TileShape<C, HD> T;
@@ -144,50 +144,75 @@ __global__ __launch_bounds__(kThreads) void AttnTile(const RaggedParams p, int n
         }
     }
 
-    // staging: chunk tid + kThreads * i of the tile
+    // staging: chunk tid + kThreads * i of the tile; a wave's 64 chunks are kPer
+    // neighbouring rows
+    constexpr int kChunks = HD / 8, kPer = kWave / kChunks;
     uint32_t gk[NCH][T::NW], gv[NCH][T::NW];
     bool bad = false, special = false;
-    auto load = [&](int32_t j0) {
+    const int my_r = lane / kChunks, my_c = lane % kChunks;
+    auto first_row = [&](int i) { return kPer * wave + kThreads / kChunks * i; };
+    // whole tiles whose kPer rows share a page (or are packed): uniform bases; their
+    // pages are looked up a tile ahead
+    const bool even = table == nullptr || (1 << p.rows.page_shift) >= kPer;
+    int32_t page[NCH] = {};
+    auto find = [&](int32_t j0) {
+        if (table == nullptr || !even || j0 + KT > j_end) return;
 #pragma unroll
-        for (int i = 0; i < NCH; ++i) {
-            const int idx = tid + kThreads * i, r = idx / (HD / 8), c = idx % (HD / 8);
-            const int32_t j = j0 + r < j_end ? j0 + r : j_end - 1;
-            int64_t ko, vo;
-            if (table != nullptr) {
-                ko = vo = PagedRow(p.rows, PageOf(p.rows, table, j, &bad), j);
-            } else {
-                ko = (static_cast<int64_t>(q.t0) + j) * p.rows.k_row;
-                vo = (static_cast<int64_t>(q.t0) + j) * p.rows.v_row;
+        for (int i = 0; i < NCH; ++i) page[i] = ReadIndex(table + ((j0 + first_row(i)) >> p.rows.page_shift));
+    };
+    auto load = [&](int32_t j0, const CB* base, int64_t row, uint32_t (&g)[NCH][T::NW]) {
+        if (even && j0 + KT <= j_end) {
+            const uint32_t mine = static_cast<uint32_t>(my_r) * static_cast<uint32_t>(row) + 8 * my_c;
+#pragma unroll
+            for (int i = 0; i < NCH; ++i) {
+                const int32_t j = j0 + first_row(i);
+                int64_t at = (static_cast<int64_t>(q.t0) + j) * row;
+                if (table != nullptr) {
+                    const bool in = page[i] >= 0 && page[i] < p.rows.n_pages;
+                    bad |= !in;
+                    at = PagedRow(p.rows, in ? page[i] : 0, j);
+                }
+                LoadChunk<C, kFull>(base + at + mine, hd - 8 * my_c, vec, g[i]);
             }
-            LoadChunk<C, kFull>(kb + ko + 8 * c, hd - 8 * c, vec, gk[i]);
-            LoadChunk<C, kFull>(vb + vo + 8 * c, hd - 8 * c, vec, gv[i]);
+            return;
         }
-    };
-    auto put = [&](uint16_t* dst, int r, int c, const uint32_t* g) {
-        const int at = r * HD + ((c ^ Swizzle<HD>(r)) * 8);
-        if constexpr (NK == 1) {
-            *reinterpret_cast<u32x4*>(dst + at) = u32x4{g[0], g[1], g[2], g[3]};
-        } else {
-            float x[8];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] = __uint_as_float(g[e]);
-            u32x4 w[NK];
-            Split8<M, NK>(x, w);
-#pragma unroll
-            for (int n = 0; n < NK; ++n) *reinterpret_cast<u32x4*>(dst + n * T::kPlane + at) = w[n];
-        }
-    };
-    auto store = [&](int32_t j0, int buf) {
-        const bool masked = j0 + KT - 1 > lo || j0 + KT > j_end;
 #pragma unroll
         for (int i = 0; i < NCH; ++i) {
-            const int idx = tid + kThreads * i, r = idx / (HD / 8), c = idx % (HD / 8);
-            put(sk[buf], r, c, gk[i]);
-            if (masked) special |= OnlyFinite<C, T::NW>(gv[i]);
-            put(sv[buf], r, c, gv[i]);
+            const int r = first_row(i) + my_r;
+            const int32_t j = j0 + r < j_end ? j0 + r : j_end - 1;
+            const int64_t at = table != nullptr
+                                   ? PagedRow(p.rows, PageOf(p.rows, table, j, &bad), j)
+                                   : (static_cast<int64_t>(q.t0) + j) * row;
+            LoadChunk<C, kFull>(base + at + 8 * my_c, hd - 8 * my_c, vec, g[i]);
         }
     };
-
+    auto put = [&](uint16_t* dst, const uint32_t (&g)[NCH][T::NW]) {
+#pragma unroll
+        for (int i = 0; i < NCH; ++i) {
+            const int r = first_row(i) + my_r;
+            const int at = r * HD + ((my_c ^ Swizzle<HD>(r)) * 8);
+            if constexpr (NK == 1) {
+                *reinterpret_cast<u32x4*>(dst + at) = u32x4{g[i][0], g[i][1], g[i][2], g[i][3]};
+            } else {
+                float x[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[e] = __uint_as_float(g[i][e]);
+                u32x4 w[NK];
+                Split8<M, NK>(x, w);
+#pragma unroll
+                for (int n = 0; n < NK; ++n) {
+                    *reinterpret_cast<u32x4*>(dst + n * T::kPlane + at) = w[n];
+                }
+            }
+        }
+    };
+    auto put_v = [&](int32_t j0, uint16_t* dst) {
+        if (j0 + KT - 1 > lo || j0 + KT > j_end) {  // some row does not attend to all of it
+#pragma unroll
+            for (int i = 0; i < NCH; ++i) special |= OnlyFinite<C, T::NW>(gv[i]);
+        }
+        put(dst, gv);
+    };
     f32x16 o[ND];
     float mx = -INFINITY, l = 0.0f;  // of the scores times the factor; this lane's part
 #pragma unroll
@@ -196,120 +221,144 @@ __global__ __launch_bounds__(kThreads) void AttnTile(const RaggedParams p, int n
         for (int r = 0; r < 16; ++r) o[d][r] = 0.0f;
     }
 
-    load(j_begin);
-    store(j_begin, 0);
+    find(j_begin);
+    load(j_begin, kb, p.rows.k_row, gk);
+    load(j_begin, vb, p.rows.v_row, gv);
+    find(j_begin + KT);
+    put(sk[0], gk);
+    put_v(j_begin, sv[0]);
     __syncthreads();
-    int buf = 0;
-    for (int32_t j0 = j_begin; j0 < j_end; j0 += KT) {
-        const bool more = j0 + KT < j_end;
-        if (more) load(j0 + KT);
-        if (j0 < wave_hi) {
-            const uint16_t* ks = sk[buf];
-            const uint16_t* vs = sv[buf];
-            f32x16 sc[NKB];
+    // the tile in buffer B; the next one's loads are on their way
+    auto compute = [&](int32_t j0, const uint16_t* ks, const uint16_t* vs) {
+        f32x16 sc[NKB];
+#pragma unroll
+        for (int b = 0; b < NKB; ++b) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) sc[b][r] = 0.0f;
+        }
+#pragma unroll
+        for (int c = 0; c < NS; ++c) {
 #pragma unroll
             for (int b = 0; b < NKB; ++b) {
+                u32x4 kf[NK];
 #pragma unroll
-                for (int r = 0; r < 16; ++r) sc[b][r] = 0.0f;
-            }
+                for (int n = 0; n < NK; ++n) {
+                    kf[n] = *reinterpret_cast<const u32x4*>(
+                        ks + n * T::kPlane + (32 * b + l32) * HD +
+                        (((2 * c + half) ^ Swizzle<HD>(l32)) * 8));
+                }
 #pragma unroll
-            for (int c = 0; c < NS; ++c) {
-#pragma unroll
-                for (int b = 0; b < NKB; ++b) {
-                    u32x4 kf[NK];
+                for (int i = 0; i < NQ; ++i) {
 #pragma unroll
                     for (int n = 0; n < NK; ++n) {
-                        kf[n] = *reinterpret_cast<const u32x4*>(
-                            ks + n * T::kPlane + (32 * b + l32) * HD +
-                            (((2 * c + half) ^ Swizzle<HD>(l32)) * 8));
-                    }
-#pragma unroll
-                    for (int i = 0; i < NQ; ++i) {
-#pragma unroll
-                        for (int n = 0; n < NK; ++n) {
-                            if (i + n < kTerms) sc[b] = M::Mma32(kf[n], qf[c][i], sc[b]);
-                        }
-                    }
-                }
-            }
-            const bool masked = j0 + KT - 1 > wave_lo || j0 + KT > j_end;
-            if (masked) {
-                const int32_t last = pos < j_end ? pos : j_end - 1;
-#pragma unroll
-                for (int b = 0; b < NKB; ++b) {
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) {
-                        const int32_t j = j0 + 32 * b + 8 * (r / 4) + 4 * half + r % 4;
-                        if (j > last) sc[b][r] = -INFINITY;
-                    }
-                }
-            }
-            float top = sc[0][0];
-#pragma unroll
-            for (int b = 0; b < NKB; ++b) {
-#pragma unroll
-                for (int r = 0; r < 16; ++r) top = fmaxf(top, sc[b][r]);
-            }
-            const float mn = fmaxf(mx, Max32(top) * factor);
-            const float base = mn == -INFINITY ? 0.0f : mn;
-            if (__ballot(mn != mx) != 0) {
-                const float alpha = __builtin_amdgcn_exp2f(mx - base);
-                l *= alpha;
-#pragma unroll
-                for (int d = 0; d < ND; ++d) o[d] *= alpha;
-                mx = mn;
-            }
-            const float off = static_cast<float>(P::W) - base;
-            float sum = 0.0f;
-#pragma unroll
-            for (int b = 0; b < NKB; ++b) {
-#pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    sc[b][r] = __builtin_amdgcn_exp2f(fmaf(sc[b][r], factor, off));
-                    sum += sc[b][r];
-                }
-            }
-            l += sum;
-            const int i16 = lane % 16, g2 = (lane / 16) % 2;
-#pragma unroll
-            for (int t = 0; t < KT / 16; ++t) {
-                float w[8];
-#pragma unroll
-                for (int e = 0; e < 8; ++e) w[e] = sc[t / 2][8 * (t % 2) + e];
-                u32x4 wf[NQ];
-                Split8<M, NQ>(w, wf);
-#pragma unroll
-                for (int d = 0; d < ND; ++d) {
-                    u32x4 vf[NK];
-#pragma unroll
-                    for (int n = 0; n < NK; ++n) {
-#pragma unroll
-                        for (int jj = 0; jj < 2; ++jj) {
-                            const int r = 16 * t + 8 * jj + 4 * half + i16 / 4;
-                            const int c = 4 * d + 2 * g2 + (i16 % 4) / 2;
-                            const uint16_t* at = vs + n * T::kPlane + r * HD +
-                                                 ((c ^ Swizzle<HD>(r)) * 8) + 4 * (i16 % 2);
-                            const u32x2 x = __builtin_bit_cast(
-                                u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                                           (LdsS16x4)(const_cast<uint16_t*>(at))));
-                            vf[n][2 * jj] = x[0];
-                            vf[n][2 * jj + 1] = x[1];
-                        }
-                    }
-#pragma unroll
-                    for (int i = 0; i < NQ; ++i) {
-#pragma unroll
-                        for (int n = 0; n < NK; ++n) {
-                            if (i + n < kTerms) o[d] = M::Mma32(vf[n], wf[i], o[d]);
-                        }
+                        if (i + n < kTerms) sc[b] = M::Mma32(kf[n], qf[c][i], sc[b]);
                     }
                 }
             }
         }
+        constexpr int NM = NK == 3 ? 6 : NQ, kSteps = NS * NKB, kDeep = 8 / NK;
+        __builtin_amdgcn_sched_group_barrier(0x100, NK * kDeep, 0);
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i) {
+            __builtin_amdgcn_sched_group_barrier(0x008, NM, 0);
+            if (i + kDeep < kSteps) __builtin_amdgcn_sched_group_barrier(0x100, NK, 0);
+        }
+        if (j0 + KT - 1 > wave_lo || j0 + KT > j_end) {
+            const int32_t last = (pos < j_end ? pos : j_end - 1) - j0 - 4 * half;
+#pragma unroll
+            for (int b = 0; b < NKB; ++b) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    sc[b][r] = 32 * b + 8 * (r / 4) + r % 4 > last ? -INFINITY : sc[b][r];
+                }
+                asm volatile("" : "+v"(sc[b]));  // a branch: else every tile pays for the mask
+            }
+        }
+        float top = sc[0][0];
+#pragma unroll
+        for (int b = 0; b < NKB; ++b) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) top = fmaxf(top, sc[b][r]);
+        }
+        const float mn = fmaxf(mx, Max32(top) * factor);
+        const float base = mn == -INFINITY ? 0.0f : mn;
+        if (__ballot(mn != mx) != 0) {
+            const float alpha = __builtin_amdgcn_exp2f(mx - base);
+            l *= alpha;
+#pragma unroll
+            for (int d = 0; d < ND; ++d) o[d] *= alpha;
+            mx = mn;
+        }
+        const float off = static_cast<float>(P::W) - base;
+        float sum = 0.0f;
+#pragma unroll
+        for (int b = 0; b < NKB; ++b) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                sc[b][r] = __builtin_amdgcn_exp2f(fmaf(sc[b][r], factor, off));
+                sum += sc[b][r];
+            }
+        }
+        l += sum;
+        const int i16 = lane % 16, g2 = (lane / 16) % 2;
+#pragma unroll
+        for (int t = 0; t < KT / 16; ++t) {
+            float w[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) w[e] = sc[t / 2][8 * (t % 2) + e];
+            u32x4 wf[NQ];
+            Split8<M, NQ>(w, wf);
+#pragma unroll
+            for (int d = 0; d < ND; ++d) {
+                u32x4 vf[NK];
+#pragma unroll
+                for (int n = 0; n < NK; ++n) {
+#pragma unroll
+                    for (int jj = 0; jj < 2; ++jj) {
+                        const int r = 16 * t + 8 * jj + 4 * half + i16 / 4;
+                        const int c = 4 * d + 2 * g2 + (i16 % 4) / 2;
+                        const uint16_t* at = vs + n * T::kPlane + r * HD +
+                                             ((c ^ Swizzle<HD>(r)) * 8) + 4 * (i16 % 2);
+                        const u32x2 x = __builtin_bit_cast(
+                            u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                       (LdsS16x4)(const_cast<uint16_t*>(at))));
+                        vf[n][2 * jj] = x[0];
+                        vf[n][2 * jj + 1] = x[1];
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < NQ; ++i) {
+#pragma unroll
+                    for (int n = 0; n < NK; ++n) {
+                        if (i + n < kTerms) o[d] = M::Mma32(vf[n], wf[i], o[d]);
+                    }
+                }
+            }
+        }
+    };
+    auto step = [&](int32_t j0, int buf) {
+        const bool more = j0 + KT < j_end;
+        if (more) {
+            load(j0 + KT, kb, p.rows.k_row, gk);
+            load(j0 + KT, vb, p.rows.v_row, gv);
+            find(j0 + 2 * KT);
+        }
+        if (j0 < wave_hi) compute(j0, sk[buf], sv[buf]);
+        const int other = T::NBUF == 1 ? 0 : buf ^ 1;
         if constexpr (T::NBUF == 1) __syncthreads();
-        if (more) store(j0 + KT, T::NBUF == 1 ? 0 : buf ^ 1);
+        if (more) {
+            put(sk[other], gk);
+            put_v(j0 + KT, sv[other]);
+        }
         __syncthreads();
-        if constexpr (T::NBUF == 2) buf ^= 1;
+    };
+    if constexpr (T::NBUF == 2) {
+        for (int32_t j0 = j_begin; j0 < j_end; j0 += 2 * KT) {
+            step(j0, 0);
+            if (j0 + KT < j_end) step(j0 + KT, 1);
+        }
+    } else {
+        for (int32_t j0 = j_begin; j0 < j_end; j0 += KT) step(j0, 0);
     }
     if (bad && p.err != nullptr) RaiseFlag(p.err, 1);
     special = __syncthreads_or(special);
