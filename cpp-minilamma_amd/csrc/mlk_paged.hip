@@ -9,9 +9,12 @@
 // writes q and the two cache rows once.
 //
 // One workgroup per token: its first threads evaluate the token's angles into
-// shared memory (every head of q and k turns by the same ones), all threads
-// then move units of 8 elements, 16 or 32 bytes a load.  A unit's 4 pairs are
-// neighbours (normal) or two runs of 4, half a head apart (NeoX).
+// shared memory (every head of q and k turns by the same ones), all threads move
+// units of PV pairs.  A unit's elements are one run of 16 bytes (normal pairs: PV
+// neighbouring ones) or two (NeoX: half a head apart), so that every load and
+// store of a wave is contiguous, which the non-temporal stores need: with runs of
+// 32 bytes in two halves they cost 15% instead of gaining 10%.  The first
+// kBatch units' loads are issued before the angles.
 #include "mlk_paged.h"
 
 #include <climits>
@@ -29,9 +32,11 @@ struct AppendArgs {
     void* q_out;
     int64_t k_row, v_row, q_row, q_out_row;
     int32_t n_heads, n_kv_heads;  // n_heads 0: no q
-    int32_t rope;                 // 0: none, 1: normal, 2: NeoX
+    bool rope;
     int32_t* err;
 };
+
+constexpr int kBatch = 3;  // units a thread loads before it rotates the first
 
 // N elements of T from / to memory, through fp32.
 template <typename T, int N>
@@ -40,7 +45,7 @@ __device__ inline void LoadN(const typename T::Bits* p, float* x) {
         x[0] = T::Get(*p);
     } else {
         typedef typename T::Bits Vec __attribute__((ext_vector_type(N)));
-        const Vec v = *reinterpret_cast<const Vec*>(p);
+        const Vec v = __builtin_nontemporal_load(reinterpret_cast<const Vec*>(p));
 #pragma unroll
         for (int i = 0; i < N; ++i) x[i] = T::Get(v[i]);
     }
@@ -54,12 +59,59 @@ __device__ inline void StoreN(typename T::Bits* p, const float* x) {
         Vec v;
 #pragma unroll
         for (int i = 0; i < N; ++i) v[i] = T::Put(x[i]);
-        *reinterpret_cast<Vec*>(p) = v;
+        __builtin_nontemporal_store(v, reinterpret_cast<Vec*>(p));
     }
 }
 
-// PV pairs a unit (4, or 1 for odd sizes and alignments).
-template <typename A, typename C, int PV>
+// One unit in fp32: x[2 i], x[2 i + 1] are pair i.
+template <typename A, int PV, bool kNeox>
+struct Unit {
+    float x[2 * PV];
+    int64_t o;   // element offset of the head in its row
+    int g, to;   // group of pairs in the head; 0: q, 1: k, 2: v, -1: none
+    template <typename T>
+    __device__ void Load(const T* row, int half, int hd) {
+        const T* src = row + o;
+        if constexpr (PV == 1) {
+            const int e1 = kNeox ? g + half : 2 * g + 1;
+            x[0] = A::Get(src[kNeox ? g : 2 * g]);
+            x[1] = e1 < hd ? A::Get(src[e1]) : 0.0f;
+        } else if constexpr (kNeox) {
+            float a[PV], b[PV];
+            LoadN<A, PV>(src + PV * g, a);
+            LoadN<A, PV>(src + PV * g + half, b);
+#pragma unroll
+            for (int i = 0; i < PV; ++i) {
+                x[2 * i] = a[i];
+                x[2 * i + 1] = b[i];
+            }
+        } else {
+            LoadN<A, 2 * PV>(src + 2 * PV * g, x);
+        }
+    }
+    template <typename C, typename T>
+    __device__ void Store(T* row, int half, int hd) const {
+        T* dst = row + o;
+        if constexpr (PV == 1) {
+            const int e1 = kNeox ? g + half : 2 * g + 1;
+            dst[kNeox ? g : 2 * g] = C::Put(x[0]);
+            if (e1 < hd) dst[e1] = C::Put(x[1]);
+        } else if constexpr (kNeox) {
+            float a[PV], b[PV];
+#pragma unroll
+            for (int i = 0; i < PV; ++i) {
+                a[i] = x[2 * i];
+                b[i] = x[2 * i + 1];
+            }
+            StoreN<C, PV>(dst + PV * g, a);
+            StoreN<C, PV>(dst + PV * g + half, b);
+        } else {
+            StoreN<C, 2 * PV>(dst + 2 * PV * g, x);
+        }
+    }
+};
+
+template <typename A, typename C, int PV, bool kNeox>
 __global__ __launch_bounds__(kAppendThreads) void PagedAppend(AppendArgs p, const RopeFreqs f) {
     __shared__ double2 turn[kRopePairs];  // cos, sin of the token's pairs
     const int tid = static_cast<int>(threadIdx.x);
@@ -74,12 +126,6 @@ __global__ __launch_bounds__(kAppendThreads) void PagedAppend(AppendArgs p, cons
     const int32_t page = PageOf(p.rows, p.batch.table + s * p.batch.table_stride, pos, &bad);
     if (bad && tid == 0) RaiseFlag(p.err, 1);
     const int64_t at = PagedRow(p.rows, page, pos);
-    if (p.rope != 0) {
-        for (int i = tid; i < half; i += kAppendThreads) {
-            RopeCosSin(pos, f.inv[i], &turn[i].x, &turn[i].y);
-        }
-        __syncthreads();
-    }
     typedef typename A::Bits AB;
     typedef typename C::Bits CB;
     const AB* rq = static_cast<const AB*>(p.q) + t * p.q_row;
@@ -90,76 +136,63 @@ __global__ __launch_bounds__(kAppendThreads) void PagedAppend(AppendArgs p, cons
     CB* ov = static_cast<CB*>(const_cast<void*>(p.rows.v)) + at;
     const int groups = half / PV;
     const int units = (p.n_heads + 2 * p.n_kv_heads) * groups;
-    for (int u = tid; u < units; u += kAppendThreads) {
-        const int h = u / groups, g = u % groups;
-        const bool is_q = h < p.n_heads, is_v = h >= p.n_heads + p.n_kv_heads;
-        if (!is_q && bad) continue;
-        const int kh = is_v ? h - p.n_heads - p.n_kv_heads : h - p.n_heads;
-        const int64_t o = static_cast<int64_t>(is_q ? h : kh) * hd;
-        const AB* src = (is_q ? rq : is_v ? rv : rk) + o;
-        // the unit's two runs: x0[i] at e0 + i * step, its partner x1[i]
-        const bool apart = p.rope == 2;
-        float x0[PV], x1[PV];
-        int e0, e1;
-        if constexpr (PV == 1) {
-            e0 = apart ? g : 2 * g;
-            e1 = apart ? g + half : 2 * g + 1;
-            x0[0] = A::Get(src[e0]);
-            x1[0] = e1 < hd ? A::Get(src[e1]) : 0.0f;
-        } else {
-            e0 = apart ? PV * g : 2 * PV * g;
-            e1 = apart ? e0 + half : e0 + PV;
-            float a[PV], b[PV];
-            LoadN<A, PV>(src + e0, a);
-            LoadN<A, PV>(src + e1, b);
+    Unit<A, PV, kNeox> u[kBatch];
+    auto load = [&](int first) {
 #pragma unroll
-            for (int i = 0; i < PV; ++i) {
-                x0[i] = apart ? a[i] : (2 * i < PV ? a[2 * i] : b[2 * i - PV]);
-                x1[i] = apart ? b[i] : (2 * i < PV ? a[2 * i + 1] : b[2 * i + 1 - PV]);
-            }
+        for (int b = 0; b < kBatch; ++b) {
+            const int i = first + b * kAppendThreads;
+            u[b].to = -1;
+            if (i >= units) continue;
+            const int h = i / groups;
+            u[b].g = i % groups;
+            u[b].to = h < p.n_heads ? 0 : h < p.n_heads + p.n_kv_heads ? 1 : 2;
+            const int in = u[b].to == 0 ? h
+                           : u[b].to == 1 ? h - p.n_heads : h - p.n_heads - p.n_kv_heads;
+            u[b].o = static_cast<int64_t>(in) * hd;
+            u[b].Load(u[b].to == 0 ? rq : u[b].to == 1 ? rk : rv, half, hd);
         }
-        if (p.rope != 0 && !is_v) {
-#pragma unroll
-            for (int i = 0; i < PV; ++i) {
-                const double2 c = turn[g * PV + i];
-                RopeRotate(x0[i], x1[i], c.x, c.y, &x0[i], &x1[i]);
-            }
+    };
+    load(tid);
+    if (p.rope) {
+        for (int i = tid; i < half; i += kAppendThreads) {
+            RopeCosSin(pos, f.inv[i], &turn[i].x, &turn[i].y);
         }
-        if constexpr (PV == 1) {
-            if (is_q) {
-                oq[o + e0] = A::Put(x0[0]);
-                if (e1 < hd) oq[o + e1] = A::Put(x1[0]);
-            } else {
-                CB* d = (is_v ? ov : ok) + o;
-                d[e0] = C::Put(x0[0]);
-                if (e1 < hd) d[e1] = C::Put(x1[0]);
-            }
-        } else {
-            float a[PV], b[PV];
+        __syncthreads();
+    }
+    for (int first = tid; first < units; first += kBatch * kAppendThreads) {
+        if (first != tid) load(first);
 #pragma unroll
-            for (int i = 0; i < PV; ++i) {
-                a[i] = apart ? x0[i] : (i % 2 ? x1[i / 2] : x0[i / 2]);
-                b[i] = apart ? x1[i] : (i % 2 ? x1[(PV + i) / 2] : x0[(PV + i) / 2]);
+        for (int b = 0; b < kBatch; ++b) {
+            if (u[b].to < 0) continue;
+            if (p.rope && u[b].to != 2) {
+#pragma unroll
+                for (int i = 0; i < PV; ++i) {
+                    const double2 c = turn[u[b].g * PV + i];
+                    RopeRotate(u[b].x[2 * i], u[b].x[2 * i + 1], c.x, c.y, &u[b].x[2 * i],
+                               &u[b].x[2 * i + 1]);
+                }
             }
-            if (is_q) {
-                StoreN<A, PV>(oq + o + e0, a);
-                StoreN<A, PV>(oq + o + e1, b);
-            } else {
-                CB* d = (is_v ? ov : ok) + o;
-                StoreN<C, PV>(d + e0, a);
-                StoreN<C, PV>(d + e1, b);
-            }
+            if (u[b].to == 0) u[b].template Store<A>(oq, half, hd);
+            else if (!bad) u[b].template Store<C>(u[b].to == 1 ? ok : ov, half, hd);
         }
     }
 }
 
+// Pairs of a 16-byte unit.
+template <typename A>
+constexpr int UnitPairs(bool neox) {
+    return (neox ? 16 : 8) / static_cast<int>(sizeof(typename A::Bits));
+}
+
 template <typename A, typename C>
-void LaunchAppend(const AppendArgs& p, const RopeFreqs& f, bool wide, hipStream_t s) {
-    const dim3 grid(static_cast<unsigned>(p.batch.n_tokens));
-    if (wide) {
-        hipLaunchKernelGGL((PagedAppend<A, C, 4>), grid, dim3(kAppendThreads), 0, s, p, f);
+void LaunchAppend(const AppendArgs& p, const RopeFreqs& f, bool neox, bool wide, hipStream_t s) {
+    const dim3 grid(static_cast<unsigned>(p.batch.n_tokens)), block(kAppendThreads);
+    if (neox) {
+        if (wide) hipLaunchKernelGGL((PagedAppend<A, C, UnitPairs<A>(true), true>), grid, block, 0, s, p, f);
+        else hipLaunchKernelGGL((PagedAppend<A, C, 1, true>), grid, block, 0, s, p, f);
     } else {
-        hipLaunchKernelGGL((PagedAppend<A, C, 1>), grid, dim3(kAppendThreads), 0, s, p, f);
+        if (wide) hipLaunchKernelGGL((PagedAppend<A, C, UnitPairs<A>(false), false>), grid, block, 0, s, p, f);
+        else hipLaunchKernelGGL((PagedAppend<A, C, 1, false>), grid, block, 0, s, p, f);
     }
 }
 
@@ -298,7 +331,6 @@ mlk_status mlk_paged_kv_append(const mlk_paged_cache* cache, const mlk_paged_bat
     } else if (q != nullptr) {
         return Fail(MLK_ERR_INVALID, "%s: theta 0 rotates nothing: q must be null", fn);
     }
-    bool wide_q = true;
     if (q != nullptr) {
         st = CheckElements(fn, "q", q, type);
         if (st != MLK_OK) return st;
@@ -318,8 +350,6 @@ mlk_status mlk_paged_kv_append(const mlk_paged_cache* cache, const mlk_paged_bat
         if (q_out == k || q_out == v || q_out == cache->k || q_out == cache->v) {
             return Fail(MLK_ERR_INVALID, "%s: q_out may not alias k, v or the pages", fn);
         }
-        wide_q = q_row_stride % 4 == 0 && q_out_row_stride % 4 == 0 &&
-                 Aligned(q, 4 * TypeBytes(type)) && Aligned(q_out, 4 * TypeBytes(type));
     }
     if (k == cache->k || k == cache->v || v == cache->k || v == cache->v) {
         return Fail(MLK_ERR_INVALID, "%s: k and v may not alias the pages", fn);
@@ -332,29 +362,32 @@ mlk_status mlk_paged_kv_append(const mlk_paged_cache* cache, const mlk_paged_bat
     p.k = k;
     p.v = v;
     p.q = q;
-    p.q_out = q_out;
+    p.q_out = q != nullptr ? q_out : nullptr;
     p.k_row = k_row_stride;
     p.v_row = v_row_stride;
     p.q_row = q != nullptr ? q_row_stride : 0;
     p.q_out_row = q != nullptr ? q_out_row_stride : 0;
     p.n_heads = q != nullptr ? n_heads : 0;
     p.n_kv_heads = KV;
-    p.rope = theta == 0.0f ? 0 : neox ? 2 : 1;
+    p.rope = theta != 0.0f;
     p.err = err;
-    const int ab = TypeBytes(type), cb = TypeBytes(cache->type);
-    const bool wide = hd % 8 == 0 && wide_q && k_row_stride % 4 == 0 && v_row_stride % 4 == 0 &&
-                      cache->page_stride % 4 == 0 && Aligned(k, 4 * ab) && Aligned(v, 4 * ab) &&
-                      Aligned(cache->k, 4 * cb) && Aligned(cache->v, 4 * cb);
-    const RopeFreqs f = p.rope != 0 ? MakeRopeFreqs(theta, hd) : RopeFreqs{};
+    // 16-byte units: `run` neighbouring elements everywhere
+    const int ab = TypeBytes(type), cb = TypeBytes(cache->type), run = 16 / ab;
+    const bool wide = hd % (neox ? 2 * run : run) == 0 && k_row_stride % run == 0 &&
+                      v_row_stride % run == 0 && cache->page_stride % run == 0 &&
+                      p.q_row % run == 0 && p.q_out_row % run == 0 && Aligned(k, 16) &&
+                      Aligned(v, 16) && Aligned(q, 16) && Aligned(p.q_out, 16) &&
+                      Aligned(cache->k, run * cb) && Aligned(cache->v, run * cb);
+    const RopeFreqs f = p.rope ? MakeRopeFreqs(theta, hd) : RopeFreqs{};
     const hipStream_t s = AsStream(stream);
     if (type == MLK_F32) {
-        if (cache->type == MLK_F32) LaunchAppend<F32, F32>(p, f, wide, s);
-        else if (cache->type == MLK_F16) LaunchAppend<F32, F16>(p, f, wide, s);
-        else LaunchAppend<F32, BF16>(p, f, wide, s);
+        if (cache->type == MLK_F32) LaunchAppend<F32, F32>(p, f, neox, wide, s);
+        else if (cache->type == MLK_F16) LaunchAppend<F32, F16>(p, f, neox, wide, s);
+        else LaunchAppend<F32, BF16>(p, f, neox, wide, s);
     } else if (type == MLK_F16) {
-        LaunchAppend<F16, F16>(p, f, wide, s);
+        LaunchAppend<F16, F16>(p, f, neox, wide, s);
     } else {
-        LaunchAppend<BF16, BF16>(p, f, wide, s);
+        LaunchAppend<BF16, BF16>(p, f, neox, wide, s);
     }
     return CheckLaunch("PagedAppend");
 }

@@ -259,6 +259,9 @@ constexpr int kFewHeads = 8;   // most KV heads of its workgroup
 // Waves of a few-row workgroup: 8, or 4 where the registers of 8 would not do.
 inline int FewWaves(int head_dim, int few_rows) { return head_dim <= 128 && few_rows <= 16 ? 8 : 4; }
 mlk_status LaunchFew(const RaggedParams& p, int32_t type, int32_t cache_type, hipStream_t stream);
+// Rows of a tile: 8 waves' 32 each, 4 waves' where a row's results take twice the
+// registers.
+__host__ __device__ constexpr int TileRows(int head_dim) { return head_dim <= 128 ? 256 : 128; }
 mlk_status LaunchTile(const RaggedParams& p, int32_t type, int32_t cache_type, hipStream_t stream);
 
 // f.template Run<A, C>() for the types.

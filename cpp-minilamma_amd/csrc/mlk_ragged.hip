@@ -22,63 +22,20 @@ constexpr int kThreads = 256;
 // (one 8B decode row over 32 chunks: 21 us with one wave walking them all, 5 us).
 constexpr int kAhead = 4;
 
-template <typename A, int L, bool kFew>
-__global__ __launch_bounds__(kThreads) void AttnJoin(const RaggedParams p, int per_row, int per_seq) {
-    constexpr int NG = kThreads / L;
-    __shared__ f32x4 sums[NG][L];
+// Row of `n` parts: the first at partial `base`, the second at `next`, and from
+// there one every `step`.
+struct JoinRow {
+    int64_t base, next, step;
+    int32_t t, h, n;
+};
+
+template <typename A, int L>
+__device__ inline void Join(const RaggedParams& p, const JoinRow& row, int part_of, int per_row,
+                            f32x4 (*sums)[L]) {
     const int lane = static_cast<int>(threadIdx.x) % L, g = static_cast<int>(threadIdx.x) / L;
-    const int rows_here = NG / per_row, part_of = g % per_row;
-    const int hd = p.rows.head_dim;
-    Seq q;
-    int64_t base = 0;              // the first part's partial, the second part's
-    int64_t next = 0, step = 1;    // partial, and from there one to the next
-    int32_t t = 0, h = 0, n = 0;   // n 0: no such row, or one part
-    if constexpr (kFew) {
-        // a workgroup's rows are of one sequence, so its waves count together
-        const int s = static_cast<int>(blockIdx.x / per_seq);
-        const int64_t in_seq =
-            static_cast<int64_t>(blockIdx.x % per_seq) * rows_here + g / per_row;
-        const int32_t units = FewUnits(p, s);
-        if (units == 0 || !LoadSeq(p.batch, s, &q)) return;
-        const int64_t real_rows = static_cast<int64_t>(q.n) * p.group;
-        const int row = static_cast<int>(in_seq % real_rows);
-        const int64_t kvh = in_seq / real_rows;
-        // none of the workgroup's rows is one
-        if (static_cast<int64_t>(blockIdx.x % per_seq) * rows_here >= real_rows * p.n_kv_heads) return;
-        int64_t before = 0;
-        FewWork work;
-        DivideFew(p, p.batch.n_seqs == 1 ? units : CountFewUnits(p, s, &before), &work);
-        if (kvh < p.n_kv_heads) {
-            const int64_t u0 = before * (p.n_kv_heads / work.heads) + kvh / work.heads * units;
-            const int64_t w0 = u0 / work.share, w1 = (u0 + units - 1) / work.share;
-            const int head = static_cast<int>(kvh % work.heads);
-            if (w1 > w0) {
-                t = q.t0 + row / p.group;
-                h = static_cast<int>(kvh) * p.group + row % p.group;
-                n = static_cast<int>(w1 - w0) + 1;
-                base = FewPartial(p, w0, u0 == w0 * work.share ? 0 : 1, head, row);
-                next = FewPartial(p, w0 + 1, 0, head, row);
-                step = 2 * kFewHeads * p.few_rows;
-            }
-        }
-    } else {
-        const int64_t id = static_cast<int64_t>(blockIdx.x) * rows_here + g / per_row;
-        // the wave's first row finds the sequence, its others look on from there
-        t = static_cast<int32_t>(id / p.n_heads);
-        h = static_cast<int32_t>(id % p.n_heads);
-        int s = LastSeq(p.batch, __builtin_amdgcn_readfirstlane(t), [](int32_t a, int) { return a; });
-        while (s + 1 < p.batch.n_seqs && p.batch.start[s + 1] <= t) ++s;
-        if (t < p.batch.n_tokens && LoadSeq(p.batch, s, &q) && t >= q.t0 && t < q.t0 + q.n) {
-            const int32_t pos = q.len - q.n + (t - q.t0);
-            if (static_cast<int64_t>(q.n) * p.group > p.few_rows && pos >= p.chunk) {
-                n = pos / p.chunk + 1;
-                base = TilePartial(p, t, h);
-                next = base + 1;
-            }
-        }
-    }
+    const int hd = p.rows.head_dim, n = row.n;
     const bool wide = hd % 4 == 0;
-    auto part = [&](int c) { return c == 0 ? base : next + (c - 1) * step; };
+    auto part = [&](int c) { return c == 0 ? row.base : row.next + (c - 1) * row.step; };
     auto dims = [&](int c) {
         f32x4 x = {0, 0, 0, 0};
         const float* at = p.part_o + part(c) * hd + 4 * lane;
@@ -120,44 +77,128 @@ __global__ __launch_bounds__(kThreads) void AttnJoin(const RaggedParams p, int p
     for (int c = part_of + per_row * kAhead; c < n; c += per_row) {
         o += dims(c) * __builtin_amdgcn_exp2f(p.part_ml[part(c)].x - m);
     }
-    sums[g][lane] = o;
-    __syncthreads();
+    if (per_row > 1) {
+        sums[g][lane] = o;
+        __syncthreads();
+    }
     if (part_of != 0 || n == 0) return;
     for (int i = 1; i < per_row; ++i) o += sums[g + i][lane];
-    typename A::Bits* out =
-        static_cast<typename A::Bits*>(p.out) + (static_cast<int64_t>(t) * p.n_heads + h) * hd;
+    typename A::Bits* out = static_cast<typename A::Bits*>(p.out) +
+                            (static_cast<int64_t>(row.t) * p.n_heads + row.h) * hd;
+    const float inv = 1.0f / l;
+    if (p.vec) {  // out is 16-byte aligned, head_dim a multiple of 8
+        if (4 * lane < hd) {
+            typedef typename A::Bits Out4 __attribute__((ext_vector_type(4)));
+            *reinterpret_cast<Out4*>(out + 4 * lane) =
+                Out4{A::Put(o[0] * inv), A::Put(o[1] * inv), A::Put(o[2] * inv), A::Put(o[3] * inv)};
+        }
+        return;
+    }
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-        if (4 * lane + e < hd) out[4 * lane + e] = A::Put(o[e] / l);
+        if (4 * lane + e < hd) out[4 * lane + e] = A::Put(o[e] * inv);
     }
 }
 
-// per_seq: rows of a sequence (few-row kernel; 0: the tile kernel's, one after
-// the other), `parts` the most a row can have.
-template <typename A, bool kFew>
-mlk_status LaunchJoin(const RaggedParams& p, int64_t rows, int64_t parts, hipStream_t s) {
-    const int groups = p.rows.head_dim <= 128 ? 8 : 4;
+// Few-row kernel's rows: blockIdx.x = sequence * per_seq + place of its rows.
+template <typename A, int L>
+__global__ __launch_bounds__(kThreads) void JoinFew(const RaggedParams p, int per_row, int per_seq) {
+    constexpr int NG = kThreads / L;
+    __shared__ f32x4 sums[NG][L];
+    const int g = static_cast<int>(threadIdx.x) / L;
+    const int rows_here = NG / per_row;
+    const int s = static_cast<int>(blockIdx.x / per_seq);
+    const int64_t first = static_cast<int64_t>(blockIdx.x % per_seq) * rows_here;
+    const int64_t in_seq = first + g / per_row;
+    const int32_t units = FewUnits(p, s);
+    Seq q;
+    if (units == 0 || !LoadSeq(p.batch, s, &q)) return;
+    const int64_t rows = static_cast<int64_t>(q.n) * p.group;
+    if (first >= rows * p.n_kv_heads) return;  // none of the workgroup's rows is one
+    const int m = static_cast<int>(in_seq % rows);
+    const int64_t kvh = in_seq / rows;
+    int64_t before = 0;
+    FewWork work;
+    DivideFew(p, p.batch.n_seqs == 1 ? units : CountFewUnits(p, s, &before), &work);
+    JoinRow row{};
+    if (kvh < p.n_kv_heads) {
+        const int64_t u0 = before * (p.n_kv_heads / work.heads) + kvh / work.heads * units;
+        const int64_t w0 = u0 / work.share, w1 = (u0 + units - 1) / work.share;
+        const int head = static_cast<int>(kvh % work.heads);
+        if (w1 > w0) {
+            row.t = q.t0 + m / p.group;
+            row.h = static_cast<int>(kvh) * p.group + m % p.group;
+            row.n = static_cast<int>(w1 - w0) + 1;
+            row.base = FewPartial(p, w0, u0 == w0 * work.share ? 0 : 1, head, m);
+            row.next = FewPartial(p, w0 + 1, 0, head, m);
+            row.step = 2 * kFewHeads * p.few_rows;
+        }
+    }
+    Join<A, L>(p, row, g % per_row, per_row, sums);
+}
+
+// Tile kernel's rows: blockIdx.x = token * per_token + place of its heads.
+template <typename A, int L>
+__global__ __launch_bounds__(kThreads) void JoinTile(const RaggedParams p, int per_row,
+                                                     int per_token) {
+    constexpr int NG = kThreads / L;
+    __shared__ f32x4 sums[NG][L];
+    const int g = static_cast<int>(threadIdx.x) / L;
+    const int32_t t = static_cast<int32_t>(blockIdx.x / per_token);
+    const int32_t h = static_cast<int32_t>(blockIdx.x % per_token) * (NG / per_row) + g / per_row;
+    const int s = LastSeq(p.batch, t, [](int32_t a, int) { return a; });
+    Seq q;
+    if (!LoadSeq(p.batch, s, &q) || t < q.t0 || t >= q.t0 + q.n) return;
+    const int32_t pos = q.len - q.n + (t - q.t0);
+    if (static_cast<int64_t>(q.n) * p.group <= p.few_rows || pos < p.chunk) return;
+    JoinRow row{0, 0, 1, t, h, 0};
+    if (h < p.n_heads) {
+        row.base = TilePartial(p, t, h);
+        row.next = row.base + 1;
+        row.n = pos / p.chunk + 1;
+    }
+    Join<A, L>(p, row, g % per_row, per_row, sums);
+}
+
+// A row's parts go over so many groups that each has them on their way at once, up to
+// the workgroup's (a row over more groups only waits for them at the barrier).
+inline int PerRow(int groups, int64_t parts) {
     int per_row = 1;
-    while (per_row < groups && per_row < parts) per_row *= 2;
+    while (per_row < groups && per_row * kAhead < parts) per_row *= 2;
+    return per_row;
+}
+
+template <typename A>
+mlk_status LaunchJoinFew(const RaggedParams& p, int64_t parts, hipStream_t s) {
+    const int groups = p.rows.head_dim <= 128 ? 8 : 4, per_row = PerRow(groups, parts);
+    const int64_t rows = static_cast<int64_t>(p.n_kv_heads) * p.few_rows;
     const int64_t per_seq = (rows * per_row + groups - 1) / groups;
-    const int64_t blocks = kFew ? per_seq * p.batch.n_seqs : per_seq;
+    const int64_t blocks = per_seq * p.batch.n_seqs;
     if (blocks > 0x7FFFFFFF) return Fail(MLK_ERR_INVALID, "attention: too many rows to join");
     const dim3 grid(static_cast<unsigned>(blocks));
     const int n = static_cast<int>(per_seq);
     if (groups == 8) {
-        hipLaunchKernelGGL((AttnJoin<A, 32, kFew>), grid, dim3(kThreads), 0, s, p, per_row, n);
+        hipLaunchKernelGGL((JoinFew<A, 32>), grid, dim3(kThreads), 0, s, p, per_row, n);
     } else {
-        hipLaunchKernelGGL((AttnJoin<A, 64, kFew>), grid, dim3(kThreads), 0, s, p, per_row, n);
+        hipLaunchKernelGGL((JoinFew<A, 64>), grid, dim3(kThreads), 0, s, p, per_row, n);
     }
-    return CheckLaunch("AttnJoin");
+    return CheckLaunch("JoinFew");
 }
 
-template <bool kFew>
-mlk_status LaunchJoin(const RaggedParams& p, int32_t type, int64_t rows, int64_t parts,
-                      hipStream_t s) {
-    if (type == MLK_F32) return LaunchJoin<F32, kFew>(p, rows, parts, s);
-    if (type == MLK_F16) return LaunchJoin<F16, kFew>(p, rows, parts, s);
-    return LaunchJoin<BF16, kFew>(p, rows, parts, s);
+template <typename A>
+mlk_status LaunchJoinTile(const RaggedParams& p, hipStream_t s) {
+    const int groups = p.rows.head_dim <= 128 ? 8 : 4, per_row = PerRow(groups, p.n_chunks);
+    const int heads = groups / per_row;
+    const int per_token = (p.n_heads + heads - 1) / heads;
+    const int64_t blocks = static_cast<int64_t>(p.batch.n_tokens) * per_token;
+    if (blocks > 0x7FFFFFFF) return Fail(MLK_ERR_INVALID, "attention: too many rows to join");
+    const dim3 grid(static_cast<unsigned>(blocks));
+    if (groups == 8) {
+        hipLaunchKernelGGL((JoinTile<A, 32>), grid, dim3(kThreads), 0, s, p, per_row, per_token);
+    } else {
+        hipLaunchKernelGGL((JoinTile<A, 64>), grid, dim3(kThreads), 0, s, p, per_row, per_token);
+    }
+    return CheckLaunch("JoinTile");
 }
 
 struct Plan {
@@ -199,8 +240,8 @@ Plan MakePlan(int64_t n_seqs, int64_t n_tokens, int64_t max_new, int64_t max_len
         }
     }
     if (plan.tile) {
-        const int64_t base = (n_tokens * group / 128 + 1) * n_kv_heads;
-        int64_t n = (2 * cus + base - 1) / base;
+        const int64_t base = (n_tokens * group / TileRows(head_dim) + 1) * n_kv_heads;
+        int64_t n = (cus + base - 1) / base;  // a tile per compute unit at a time
         const int64_t longest = (max_len + kTileLeast - 1) / kTileLeast;
         if (n > longest) n = longest;
         plan.chunk = ((max_len + n - 1) / n + kTileLeast - 1) / kTileLeast * kTileLeast;
@@ -268,8 +309,10 @@ mlk_status Attend(const AttendArgs& a) {
         if (st != MLK_OK) return st;
         if (p.workers > 0) {
             const int64_t pairs = static_cast<int64_t>(b.n_seqs) * a.n_kv_heads;
-            st = LaunchJoin<true>(p, a.type, static_cast<int64_t>(a.n_kv_heads) * p.few_rows,
-                                  (p.workers + pairs - 1) / pairs + 1, a.stream);
+            const int64_t parts = (p.workers + pairs - 1) / pairs + 1;
+            st = a.type == MLK_F32   ? LaunchJoinFew<F32>(p, parts, a.stream)
+                 : a.type == MLK_F16 ? LaunchJoinFew<F16>(p, parts, a.stream)
+                                     : LaunchJoinFew<BF16>(p, parts, a.stream);
             if (st != MLK_OK) return st;
         }
     }
@@ -280,8 +323,9 @@ mlk_status Attend(const AttendArgs& a) {
         mlk_status st = LaunchTile(p, a.type, a.cache_type, a.stream);
         if (st != MLK_OK) return st;
         if (p.n_chunks > 1) {
-            return LaunchJoin<false>(p, a.type, static_cast<int64_t>(b.n_tokens) * a.n_heads,
-                                     p.n_chunks, a.stream);
+            return a.type == MLK_F32   ? LaunchJoinTile<F32>(p, a.stream)
+                   : a.type == MLK_F16 ? LaunchJoinTile<F16>(p, a.stream)
+                                       : LaunchJoinTile<BF16>(p, a.stream);
         }
     }
     return MLK_OK;

@@ -26,9 +26,6 @@
 namespace mlk {
 namespace {
 
-constexpr int kThreads = 512;
-constexpr int kRows = 256;
-
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) s16x4* LdsS16x4;
 
@@ -40,6 +37,7 @@ __device__ inline int Swizzle(int r) {
 
 template <typename C, int HD>
 struct TileShape {
+    static constexpr int kThreads = TileRows(HD) / 32 * kWave;
     static constexpr int NK = std::is_same<C, F32>::value ? 3 : 1;
     static constexpr int KT = HD != 64 && (NK == 3 || HD == 256) ? 32 : 64;
     static constexpr int NBUF = NK == 3 ? 1 : 2;
@@ -49,12 +47,13 @@ struct TileShape {
 };
 
 template <typename A, typename C, int HD, bool kFull>
-__global__ __launch_bounds__(kThreads, HD <= 128 ? 2 : 1) void AttnTile(const RaggedParams p, int n_slots) {
+__global__ __launch_bounds__((TileShape<C, HD>::kThreads), HD <= 128 ? 2 : 1) void AttnTile(const RaggedParams p, int n_slots) {
     typedef Pieces<A, C> P;
     typedef typename P::M M;
     typedef TileShape<C, HD> T;
     typedef typename C::Bits CB;
     typedef typename A::Bits AB;
+    constexpr int kThreads = T::kThreads, kRows = TileRows(HD);
     constexpr int NQ = P::NQ, NK = T::NK, KT = T::KT, NKB = KT / 32, NCH = T::NCH;
     constexpr int ND = HD / 32, NS = HD / 16;
     constexpr int kTerms = NQ > NK ? NQ : NK;  // products of pieces i, j: i + j < kTerms
@@ -290,16 +289,16 @@ __global__ __launch_bounds__(kThreads, HD <= 128 ? 2 : 1) void AttnTile(const Ra
             mx = mn;
         }
         const float off = static_cast<float>(P::W) - base;
-        float sum = 0.0f;
+        float sum[4] = {0, 0, 0, 0};
 #pragma unroll
         for (int b = 0; b < NKB; ++b) {
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
                 sc[b][r] = __builtin_amdgcn_exp2f(fmaf(sc[b][r], factor, off));
-                sum += sc[b][r];
+                sum[r % 4] += sc[b][r];
             }
         }
-        l += sum;
+        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
         const int i16 = lane % 16, g2 = (lane / 16) % 2;
 #pragma unroll
         for (int t = 0; t < KT / 16; ++t) {
@@ -419,6 +418,7 @@ __global__ __launch_bounds__(kThreads, HD <= 128 ? 2 : 1) void AttnTile(const Ra
 
 template <typename A, typename C, int HD>
 mlk_status Launch(const RaggedParams& p, dim3 grid, int n_slots, hipStream_t s) {
+    constexpr int kThreads = TileShape<C, HD>::kThreads;
     if (p.vec && p.rows.head_dim == HD) {
         hipLaunchKernelGGL((AttnTile<A, C, HD, true>), grid, dim3(kThreads), 0, s, p, n_slots);
     } else {
@@ -440,16 +440,17 @@ struct ByDim {
     }
 };
 
-// Row tiles of a batch: sequence s owns the slots from start[s] * group / kRows
+// Row tiles of a batch: sequence s owns the slots from start[s] * group / rows
 // + s on, at least as many as it has tiles, whatever the lengths.
-int64_t TileSlots(int64_t n_seqs, int64_t n_tokens, int32_t group) {
-    return n_tokens * group / kRows + n_seqs;
+int64_t TileSlots(int64_t n_seqs, int64_t n_tokens, int32_t group, int rows) {
+    return n_tokens * group / rows + n_seqs;
 }
 
 }  // namespace
 
 mlk_status LaunchTile(const RaggedParams& p, int32_t type, int32_t cache_type, hipStream_t stream) {
-    const int64_t slots = TileSlots(p.batch.n_seqs, p.batch.n_tokens, p.group);
+    const int64_t slots = TileSlots(p.batch.n_seqs, p.batch.n_tokens, p.group,
+                                    TileRows(p.rows.head_dim));
     const int64_t blocks = slots * p.n_chunks * p.n_kv_heads;
     if (blocks > INT_MAX) {
         return Fail(MLK_ERR_INVALID, "attention: %lld workgroups exceed the grid",
