@@ -289,11 +289,15 @@ struct FewWork {
     int32_t s, units;
 };
 
+// (A short sequence counts kFewRun units, what it costs; those past its length
+// hold nothing.)
+constexpr int kFewRun = 8;
 __device__ inline int32_t FewUnits(const RaggedParams& p, int s) {
     Seq q;
     if (s >= p.batch.n_seqs || !LoadSeq(p.batch, s, &q)) return 0;
     if (q.n == 0 || static_cast<int64_t>(q.n) * p.group > p.few_rows) return 0;
-    return (q.len + kFewKeys - 1) / kFewKeys;
+    const int32_t units = (q.len + kFewKeys - 1) / kFewKeys;
+    return units > kFewRun ? units : kFewRun;
 }
 
 // Units of all sequences, and of those before sequence `upto` (a whole wave;
@@ -318,7 +322,6 @@ __device__ inline int64_t CountFewUnits(const RaggedParams& p, int upto, int64_t
 // the same positions (whole rows of the cache, read once and together) where
 // that leaves every worker kFewRun units or more; else fewer heads and more
 // waves per head, down to one head's positions spread over all waves.
-constexpr int kFewRun = 8;
 __device__ inline void DivideFew(const RaggedParams& p, int64_t total, FewWork* w) {
     int heads = p.few_heads;
     while (heads > 1 && total * (p.n_kv_heads / heads) < static_cast<int64_t>(p.workers) * kFewRun) {
@@ -377,27 +380,41 @@ __device__ inline int64_t TilePartial(const RaggedParams& p, int32_t t, int h) {
     return (static_cast<int64_t>(t) * p.n_heads + h) * p.n_chunks;
 }
 
-// One K or V row chunk of 8 elements at p (nullptr: zeros), the first `left` of
-// them real, as raw bits.
-template <typename C, bool kFull>
-__device__ inline void LoadChunk(const typename C::Bits* p, int left, bool vec, uint32_t* o) {
-    constexpr int NW = sizeof(typename C::Bits) == 4 ? 8 : 4;
-    if (kFull || (vec && left >= 8)) {
+// How rows lie.  kFull: head_dim is the instance's and rows are 16-byte aligned.
+// kPadded: aligned, head_dim a smaller multiple of 8; runs past it read the row's
+// first elements instead (K's meet q's zeros, V's results are not kept).  kScalar:
+// anything else, element by element.
+enum Lie { kScalar = 0, kPadded = 1, kFull = 2 };
+inline Lie LieOf(const RaggedParams& p, int head_dim) {
+    return !p.vec ? kScalar : p.rows.head_dim == head_dim ? kFull : kPadded;
+}
+
+// Elements d .. d + N - 1 of a K, V or q row, as raw bits; kOnce: no other workgroup
+// reads them (a non-temporal load); kZero: zeros past hd.
+template <typename C, int N, Lie kLie, bool kOnce, bool kZero = false>
+__device__ inline void LoadRun(const typename C::Bits* row, int d, int hd, uint32_t* o) {
+    constexpr int W = N * static_cast<int>(sizeof(typename C::Bits)) / 4;
+    if constexpr (kLie == kScalar) {
 #pragma unroll
-        for (int i = 0; i < NW / 4; ++i) {
-            const u32x4 v = reinterpret_cast<const u32x4*>(p)[i];
+        for (int i = 0; i < W; ++i) o[i] = 0;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) o[4 * i + e] = v[e];
+        for (int i = 0; i < N; ++i) {
+            if (d + i < hd) {
+                if constexpr (sizeof(typename C::Bits) == 4) o[i] = __float_as_uint(row[d + i]);
+                else o[i / 2] |= static_cast<uint32_t>(row[d + i]) << (16 * (i % 2));
+            }
         }
-        return;
-    }
-    for (int i = 0; i < NW; ++i) o[i] = 0;
-    if (vec) return;  // head_dim % 8 == 0: nothing here
+    } else {
+        const bool in = kLie == kFull || d < hd;
+        const typename C::Bits* p = row + (in ? d : 0);
+        constexpr int V = W < 4 ? W : 4;
+        typedef uint32_t Vec __attribute__((ext_vector_type(V)));
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        if (i < left) {
-            if constexpr (NW == 8) o[i] = __float_as_uint(p[i]);
-            else o[i / 2] |= static_cast<uint32_t>(p[i]) << (16 * (i % 2));
+        for (int i = 0; i < W / V; ++i) {
+            const Vec v = kOnce ? __builtin_nontemporal_load(reinterpret_cast<const Vec*>(p) + i)
+                                : reinterpret_cast<const Vec*>(p)[i];
+#pragma unroll
+            for (int e = 0; e < V; ++e) o[V * i + e] = kZero && !in ? 0u : v[e];
         }
     }
 }

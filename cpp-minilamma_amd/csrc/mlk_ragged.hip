@@ -123,7 +123,8 @@ __global__ __launch_bounds__(kThreads) void JoinFew(const RaggedParams p, int pe
     JoinRow row{};
     if (kvh < p.n_kv_heads) {
         const int64_t u0 = before * (p.n_kv_heads / work.heads) + kvh / work.heads * units;
-        const int64_t w0 = u0 / work.share, w1 = (u0 + units - 1) / work.share;
+        const int32_t held = (q.len + kFewKeys - 1) / kFewKeys;  // units with positions
+        const int64_t w0 = u0 / work.share, w1 = (u0 + held - 1) / work.share;
         const int head = static_cast<int>(kvh % work.heads);
         if (w1 > w0) {
             row.t = q.t0 + m / p.group;
@@ -215,7 +216,12 @@ int64_t PlanBytes(const Plan& plan, int32_t hd) {
 }
 
 constexpr int64_t kFewUnsplit = 512;   // longest sequences that are not split
-constexpr int64_t kTileLeast = 512;    // positions of a tile row's least chunk
+constexpr int64_t kTileLeast = 256;    // positions of a tile row's least chunk
+constexpr int64_t kTileMost = 64;      // most chunks of a tile row
+constexpr int64_t kTileFixed = 300;    // what a tile's start and end cost, in positions
+constexpr int64_t kTileJoin = 300;     // what the join costs
+
+int64_t RoundUp(int64_t a, int64_t to) { return (a + to - 1) / to * to; }
 
 Plan MakePlan(int64_t n_seqs, int64_t n_tokens, int64_t max_new, int64_t max_len, int32_t n_heads,
               int32_t n_kv_heads, int32_t head_dim, bool packed) {
@@ -230,7 +236,7 @@ Plan MakePlan(int64_t n_seqs, int64_t n_tokens, int64_t max_new, int64_t max_len
         const int64_t limit = plan.tile ? 16 : most;
         plan.few_rows = max_rows < limit ? max_rows : limit;
         if (max_len > kFewUnsplit) {
-            const int64_t units = n_seqs * n_kv_heads * ((max_len + kFewKeys - 1) / kFewKeys);
+            const int64_t units = n_seqs * n_kv_heads * ((max_len + kFewKeys - 1) / kFewKeys + kFewRun);
             // 8 waves per compute unit: two such workgroups' loads get in each other's
             // way (64 bf16 decode rows of the 8B heads: 189 us, with twice as many 213)
             plan.few_workers = cus * 8 / FewWaves(head_dim, static_cast<int32_t>(plan.few_rows));
@@ -240,11 +246,28 @@ Plan MakePlan(int64_t n_seqs, int64_t n_tokens, int64_t max_new, int64_t max_len
         }
     }
     if (plan.tile) {
-        const int64_t base = (n_tokens * group / TileRows(head_dim) + 1) * n_kv_heads;
-        int64_t n = (cus + base - 1) / base;  // a tile per compute unit at a time
-        const int64_t longest = (max_len + kTileLeast - 1) / kTileLeast;
-        if (n > longest) n = longest;
-        plan.chunk = ((max_len + n - 1) / n + kTileLeast - 1) / kTileLeast * kTileLeast;
+        // Positions split into n chunks where that shortens the call: a compute unit has
+        // one tile at a time, so rounds(n) * (chunk + kTileFixed), and the join if any
+        // (1023 bf16 tokens after 3000 beside 31 decode rows: n = 1 252 us, 2 171, 3 210;
+        // 3 x 448 fp16 tokens after 2800: n = 2 206, 3 172; 2500 packed fp32 tokens in 9
+        // prompts: n = 1 120, 2 160; all of the 8B heads).
+        // The tiles are estimated: in a mixed batch all sequences but one bring one token,
+        // in others each but one has half a tile more than its rows fill.
+        const bool mixed = plan.few_rows > 0;
+        const int64_t rows = (n_tokens - (mixed ? n_seqs - 1 : 0)) * group;
+        const int64_t each = TileRows(head_dim);
+        const int64_t tiles =
+            ((rows + each - 1) / each + (mixed ? 0 : (n_seqs - 1) / 2)) * n_kv_heads;
+        int64_t best = INT64_MAX;
+        for (int64_t n = 1; n <= kTileMost && (n == 1 || (n - 1) * kTileLeast < max_len); ++n) {
+            const int64_t chunk = RoundUp((max_len + n - 1) / n, kTileLeast);
+            const int64_t cost = ((tiles < 1 ? 1 : tiles) * n + cus - 1) / cus * (chunk + kTileFixed) +
+                                 (n > 1 ? kTileJoin : 0);
+            if (cost < best) {
+                best = cost;
+                plan.chunk = chunk;
+            }
+        }
         plan.n_chunks = (max_len + plan.chunk - 1) / plan.chunk;
         if (plan.n_chunks > 1) plan.tile_partials = n_tokens * n_heads * plan.n_chunks;
     }

@@ -37,7 +37,7 @@ __device__ inline uint32_t HighHalves(uint32_t a, uint32_t b) {
 }
 
 // K and V operands of one tile in registers, and their loads.
-template <typename C, int HD, bool kFull>
+template <typename C, int HD, Lie kLie>
 struct FewTile {
     static constexpr bool kF32 = std::is_same<C, F32>::value;
     static constexpr int KT = kF32 ? 16 : 32;        // positions
@@ -52,44 +52,17 @@ struct FewTile {
     uint32_t v[NKEY][NVW];
 
     // K row at `row`, this lane's dims: 16-bit 32 c + 8 g .. + 7, fp32 16 c + 4 g .. + 3
-    __device__ void LoadK(int b, const B* row, int g, int hd, bool vec) {
+    __device__ void LoadK(int b, const B* row, int g, int hd) {
         constexpr int N = kF32 ? 4 : 8, S = 4 * N;
 #pragma unroll
-        for (int c = 0; c < HD / S; ++c) Run<N>(row + S * c + N * g, hd - S * c - N * g, vec, &k[b][4 * c]);
+        for (int c = 0; c < HD / S; ++c) LoadRun<C, N, kLie, true>(row, S * c + N * g, hd, &k[b][4 * c]);
     }
     // V row at `row`, dims 16 VE n + VE (l % 16) .. + VE - 1
-    __device__ void LoadV(int j, const B* row, int i16, int hd, bool vec) {
+    __device__ void LoadV(int j, const B* row, int i16, int hd) {
         constexpr int W = VE * sizeof(B) / 4;
 #pragma unroll
         for (int n = 0; n < NVR; ++n) {
-            Run<VE>(row + 16 * VE * n + VE * i16, hd - 16 * VE * n - VE * i16, vec, &v[j][W * n]);
-        }
-    }
-    // N elements at p, `left` of them real
-    template <int N>
-    static __device__ void Run(const B* p, int left, bool vec, uint32_t* o) {
-        constexpr int W = N * sizeof(B) / 4;
-        if (kFull || (vec && left >= N)) {
-            if constexpr (W == 4) {
-                const u32x4 x = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p));
-#pragma unroll
-                for (int i = 0; i < 4; ++i) o[i] = x[i];
-            } else {
-                const u32x2 x = __builtin_nontemporal_load(reinterpret_cast<const u32x2*>(p));
-                o[0] = x[0];
-                o[1] = x[1];
-            }
-            return;
-        }
-#pragma unroll
-        for (int i = 0; i < W; ++i) o[i] = 0;
-        if (vec) return;  // head_dim is a multiple of 8: nothing real here
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-            if (i < left) {
-                if constexpr (kF32) o[i] = __float_as_uint(p[i]);
-                else o[i / 2] |= static_cast<uint32_t>(p[i]) << (16 * (i % 2));
-            }
+            LoadRun<C, VE, kLie, true>(row, 16 * VE * n + VE * i16, hd, &v[j][W * n]);
         }
     }
 };
@@ -113,12 +86,12 @@ __device__ inline void RowOffsets(const FewRows& r, int32_t j, int64_t* ko, int6
     }
 }
 
-template <typename A, typename C, int HD, int NB, int kWaves, bool kFull>
+template <typename A, typename C, int HD, int NB, int kWaves, Lie kLie>
 __global__ __launch_bounds__(kWaves * kWave) void AttnFew(const RaggedParams p) {
     constexpr int kThreads = kWaves * kWave;
     typedef Pieces<A, C> P;
     typedef typename P::M M;
-    typedef FewTile<C, HD, kFull> Tile;
+    typedef FewTile<C, HD, kLie> Tile;
     typedef typename C::Bits CB;
     typedef typename A::Bits AB;
     constexpr bool kF32 = Tile::kF32;
@@ -132,9 +105,8 @@ __global__ __launch_bounds__(kWaves * kWave) void AttnFew(const RaggedParams p) 
     const int tid = static_cast<int>(threadIdx.x), lane = tid % kWave;
     const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
     const int i16 = lane % 16, g4 = lane / 16;
-    const int hd = kFull ? HD : p.rows.head_dim;
+    const int hd = kLie == kFull ? HD : p.rows.head_dim;
     if (blockIdx.x == 0) CheckSeqs(p.batch, p.err);
-    const bool vec = kFull || p.vec;
     FewWork work;
     int64_t unit, end;  // this worker's units
     if (p.workers == 0) {
@@ -168,12 +140,14 @@ __global__ __launch_bounds__(kWaves * kWave) void AttnFew(const RaggedParams p) 
     const int32_t u1 = __builtin_amdgcn_readfirstlane(
         end - unit < units - u0 ? u0 + static_cast<int32_t>(end - unit) : units);
     unit += u1 - u0;
-    Seq q;
-    if (!LoadSeq(p.batch, s, &q)) return;
+    Seq loaded;
+    if (!LoadSeq(p.batch, s, &loaded)) return;
+    const Seq q = loaded;
     const int rows = q.n * p.group;
     const int32_t j_begin = u0 * kFewKeys;
-    const int32_t j_end = u1 < units ? u1 * kFewKeys : q.len;
-    const bool split = u1 - u0 < units;
+    if (j_begin >= q.len) continue;
+    const int32_t j_end = q.len - j_begin > (u1 - u0) * kFewKeys ? u1 * kFewKeys : q.len;
+    const bool split = u0 != 0 || j_end < q.len;
 
     const FewRows fr{&p.rows,
                      p.batch.table == nullptr ? nullptr : p.batch.table + s * p.batch.table_stride,
@@ -198,10 +172,9 @@ __global__ __launch_bounds__(kWaves * kWave) void AttnFew(const RaggedParams p) 
 #pragma unroll
         for (int c = 0; c < NQR; ++c) {
             if constexpr (kF32) {
-                FewTile<F32, HD, kFull>::template Run<4>(qr + 16 * c + 4 * g4, hd - 16 * c - 4 * g4,
-                                                         vec, raw[nb][c]);
+                LoadRun<F32, 4, kLie, false, true>(qr, 16 * c + 4 * g4, hd, raw[nb][c]);
             } else {
-                LoadChunk<A, kFull>(qr + 32 * c + 8 * g4, hd - 32 * c - 8 * g4, vec, raw[nb][c]);
+                LoadRun<A, 8, kLie, false, true>(qr, 32 * c + 8 * g4, hd, raw[nb][c]);
             }
         }
     }
@@ -210,28 +183,50 @@ __global__ __launch_bounds__(kWaves * kWave) void AttnFew(const RaggedParams p) 
     bool bad = false;
     // 16-position blocks whose rows lie evenly apart: whole pages' parts, or packed
     const bool even = fr.table == nullptr || p.rows.page_shift >= 4;
+    // else, pages of 4 positions or more: a lane's K row and its 4 V rows of a block
+    // have a page each
+    const bool lanes = !even && p.rows.page_shift >= 2;
     // element offsets of the blocks' first rows; the pages of the tile after the
     // next are looked up a tile ahead, so that no load waits for its page
-    int32_t page[NBK];
-    auto find = [&](int32_t j) {
-        if (fr.table == nullptr || !even) return;
-#pragma unroll
-        for (int b = 0; b < NBK; ++b) {
-            if (j + 16 * b < j_end) page[b] = ReadIndex(fr.table + ((j + 16 * b) >> p.rows.page_shift));
+    // (scalars: as arrays they stayed in scratch memory, decode of 64 rows 189 -> 233 us)
+    int32_t page0 = 0, page1 = 0, page_k0 = 0, page_k1 = 0, page_v0 = 0, page_v1 = 0;
+    const int shift = p.rows.page_shift;
+    auto find = [&](int32_t j) __attribute__((always_inline)) {
+        if (fr.table == nullptr) return;
+        if (even) {
+            if (j < j_end) page0 = ReadIndex(fr.table + (j >> shift));
+            if (NBK > 1 && j + 16 < j_end) page1 = ReadIndex(fr.table + ((j + 16) >> shift));
+        } else if (lanes && j + KT <= j_end) {
+            page_k0 = ReadIndex(fr.table + ((j + i16) >> shift));
+            page_v0 = ReadIndex(fr.table + ((j + 4 * g4) >> shift));
+            if (NBK > 1) {
+                page_k1 = ReadIndex(fr.table + ((j + 16 + i16) >> shift));
+                page_v1 = ReadIndex(fr.table + ((j + 16 + 4 * g4) >> shift));
+            }
         }
     };
-    auto block_base = [&](int b, int32_t j, int64_t row) -> int64_t {  // j + 15 < end
-        if (fr.table == nullptr) return (fr.t0 + j) * row;
-        const bool in = page[b] >= 0 && page[b] < p.rows.n_pages;
+    auto lane_row = [&](int32_t pg, int32_t j) __attribute__((always_inline)) -> int64_t {
+        const bool in = pg >= 0 && pg < p.rows.n_pages;
         if (!in) bad = true;
-        return PagedRow(p.rows, in ? page[b] : 0, j);
+        return PagedRow(p.rows, in ? pg : 0, j);
     };
-    auto load_k = [&](int32_t j0) {
+    auto block_base = [&](int b, int32_t j, int64_t row) __attribute__((always_inline)) -> int64_t {
+        if (fr.table == nullptr) return (fr.t0 + j) * row;  // j + 15 < end
+        return lane_row(b == 0 ? page0 : page1, j);
+    };
+    auto load_k = [&](int32_t j0) __attribute__((always_inline)) {
         if (even && j0 + KT <= j_end) {
 #pragma unroll
             for (int b = 0; b < NBK; ++b) {
                 const CB* base = kb + block_base(b, j0 + 16 * b, p.rows.k_row);
-                tile.LoadK(b, base + i16 * static_cast<uint32_t>(p.rows.k_row), g4, hd, vec);
+                tile.LoadK(b, base + i16 * static_cast<uint32_t>(p.rows.k_row), g4, hd);
+            }
+            return;
+        }
+        if (lanes && j0 + KT <= j_end) {
+#pragma unroll
+            for (int b = 0; b < NBK; ++b) {
+                tile.LoadK(b, kb + lane_row(b == 0 ? page_k0 : page_k1, j0 + 16 * b + i16), g4, hd);
             }
             return;
         }
@@ -239,10 +234,10 @@ __global__ __launch_bounds__(kWaves * kWave) void AttnFew(const RaggedParams p) 
         for (int b = 0; b < NBK; ++b) {
             int64_t ko, vo;
             RowOffsets(fr, j0 + 16 * b + i16, &ko, &vo, &bad);
-            tile.LoadK(b, kb + ko, g4, hd, vec);
+            tile.LoadK(b, kb + ko, g4, hd);
         }
     };
-    auto load_v = [&](int32_t j0) {
+    auto load_v = [&](int32_t j0) __attribute__((always_inline)) {
         if (even && j0 + KT <= j_end) {
 #pragma unroll
             for (int b = 0; b < NBK; ++b) {
@@ -250,8 +245,17 @@ __global__ __launch_bounds__(kWaves * kWave) void AttnFew(const RaggedParams p) 
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     tile.LoadV(4 * b + r, base + r * p.rows.v_row +
-                               (4 * g4) * static_cast<uint32_t>(p.rows.v_row), i16, hd, vec);
+                               (4 * g4) * static_cast<uint32_t>(p.rows.v_row), i16, hd);
                 }
+            }
+            return;
+        }
+        if (lanes && j0 + KT <= j_end) {
+#pragma unroll
+            for (int b = 0; b < NBK; ++b) {
+                const CB* base = vb + lane_row(b == 0 ? page_v0 : page_v1, j0 + 16 * b + 4 * g4);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) tile.LoadV(4 * b + r, base + r * p.rows.v_row, i16, hd);
             }
             return;
         }
@@ -259,7 +263,7 @@ __global__ __launch_bounds__(kWaves * kWave) void AttnFew(const RaggedParams p) 
         for (int j = 0; j < Tile::NKEY; ++j) {
             int64_t ko, vo;
             RowOffsets(fr, j0 + 16 * (j / 4) + 4 * g4 + j % 4, &ko, &vo, &bad);
-            tile.LoadV(j, vb + vo, i16, hd, vec);
+            tile.LoadV(j, vb + vo, i16, hd);
         }
     };
 
@@ -461,7 +465,7 @@ __global__ __launch_bounds__(kWaves * kWave) void AttnFew(const RaggedParams p) 
                     }
 #pragma unroll
                     for (int e = 0; e < Tile::VE; ++e) {
-                        if (kFull || d0 + e < hd) {
+                        if (kLie == kFull || d0 + e < hd) {
                             if (split) part[d0 + e] = x[e];
                             else out[d0 + e] = A::Put(x[e]);
                         }
@@ -498,7 +502,7 @@ __global__ __launch_bounds__(kWaves * kWave) void AttnFew(const RaggedParams p) 
     special = __syncthreads_or(special);
     for (int u = tid; u < heads * rows * HD; u += kThreads) {
         const int d = u % HD, row = u / HD % rows, hb = u / HD / rows;
-        if (!kFull && d >= hd) continue;
+        if (kLie != kFull && d >= hd) continue;
         float top = -INFINITY, lt = 0.0f, sum = 0.0f;
         for (int w = hb; w < kWaves; w += heads) top = fmaxf(top, sm[w][row]);
         const float base = top == -INFINITY ? 0.0f : top;
@@ -531,10 +535,11 @@ __global__ __launch_bounds__(kWaves * kWave) void AttnFew(const RaggedParams p) 
 
 template <typename A, typename C, int HD, int NB, int kWaves>
 void Start(const RaggedParams& p, dim3 grid, hipStream_t s) {
-    if (p.vec && p.rows.head_dim == HD) {
-        hipLaunchKernelGGL((AttnFew<A, C, HD, NB, kWaves, true>), grid, dim3(kWaves * kWave), 0, s, p);
-    } else {
-        hipLaunchKernelGGL((AttnFew<A, C, HD, NB, kWaves, false>), grid, dim3(kWaves * kWave), 0, s, p);
+    const dim3 block(kWaves * kWave);
+    switch (LieOf(p, HD)) {
+        case kFull: hipLaunchKernelGGL((AttnFew<A, C, HD, NB, kWaves, kFull>), grid, block, 0, s, p); break;
+        case kPadded: hipLaunchKernelGGL((AttnFew<A, C, HD, NB, kWaves, kPadded>), grid, block, 0, s, p); break;
+        default: hipLaunchKernelGGL((AttnFew<A, C, HD, NB, kWaves, kScalar>), grid, block, 0, s, p); break;
     }
 }
 

@@ -35,22 +35,22 @@ __device__ inline int Swizzle(int r) {
     return HD == 64 ? (((r >> 1) & 1) << 2) | ((r >> 2) & 3) : ((r & 3) << 2) | ((r >> 2) & 3);
 }
 
-template <typename C, int HD>
+template <typename A, typename C, int HD>
 struct TileShape {
     static constexpr int kThreads = TileRows(HD) / 32 * kWave;
     static constexpr int NK = std::is_same<C, F32>::value ? 3 : 1;
-    static constexpr int KT = HD != 64 && (NK == 3 || HD == 256) ? 32 : 64;
+    static constexpr int KT = HD != 64 && (NK == 3 || HD == 256 || Pieces<A, C>::NQ == 3) ? 32 : 64;
     static constexpr int NBUF = NK == 3 ? 1 : 2;
     static constexpr int kPlane = KT * HD;             // elements
     static constexpr int NCH = KT * HD / 8 / kThreads;  // chunks a thread stages
     static constexpr int NW = NK == 3 ? 8 : 4;         // dwords a chunk has in memory
 };
 
-template <typename A, typename C, int HD, bool kFull>
-__global__ __launch_bounds__((TileShape<C, HD>::kThreads), HD <= 128 ? 2 : 1) void AttnTile(const RaggedParams p, int n_slots) {
+template <typename A, typename C, int HD, Lie kLie>
+__global__ __launch_bounds__((TileShape<A, C, HD>::kThreads), HD <= 128 ? 2 : 1) void AttnTile(const RaggedParams p, int n_slots) {
     typedef Pieces<A, C> P;
     typedef typename P::M M;
-    typedef TileShape<C, HD> T;
+    typedef TileShape<A, C, HD> T;
     typedef typename C::Bits CB;
     typedef typename A::Bits AB;
     constexpr int kThreads = T::kThreads, kRows = TileRows(HD);
@@ -63,8 +63,7 @@ __global__ __launch_bounds__((TileShape<C, HD>::kThreads), HD <= 128 ? 2 : 1) vo
     const int tid = static_cast<int>(threadIdx.x), lane = tid % kWave;
     const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
     const int l32 = lane % 32, half = lane / 32;
-    const int hd = kFull ? HD : p.rows.head_dim;
-    const bool vec = kFull || p.vec;
+    const int hd = kLie == kFull ? HD : p.rows.head_dim;
     if (blockIdx.x == 0) CheckSeqs(p.batch, p.err);
 
     const int kvh = static_cast<int>(blockIdx.x % p.n_kv_heads);
@@ -115,7 +114,7 @@ __global__ __launch_bounds__((TileShape<C, HD>::kThreads), HD <= 128 ? 2 : 1) vo
         uint32_t raw[NS][sizeof(AB) == 4 ? 8 : 4];
 #pragma unroll
         for (int c = 0; c < NS; ++c) {
-            LoadChunk<A, kFull>(qr + 16 * c + 8 * half, hd - 16 * c - 8 * half, vec, raw[c]);
+            LoadRun<A, 8, kLie, false, true>(qr, 16 * c + 8 * half, hd, raw[c]);
         }
         if constexpr (NQ == 1) {
 #pragma unroll
@@ -161,7 +160,7 @@ __global__ __launch_bounds__((TileShape<C, HD>::kThreads), HD <= 128 ? 2 : 1) vo
     };
     auto load = [&](int32_t j0, const CB* base, int64_t row, uint32_t (&g)[NCH][T::NW]) {
         if (even && j0 + KT <= j_end) {
-            const uint32_t mine = static_cast<uint32_t>(my_r) * static_cast<uint32_t>(row) + 8 * my_c;
+            const uint32_t mine = static_cast<uint32_t>(my_r) * static_cast<uint32_t>(row);
 #pragma unroll
             for (int i = 0; i < NCH; ++i) {
                 const int32_t j = j0 + first_row(i);
@@ -171,7 +170,7 @@ __global__ __launch_bounds__((TileShape<C, HD>::kThreads), HD <= 128 ? 2 : 1) vo
                     bad |= !in;
                     at = PagedRow(p.rows, in ? page[i] : 0, j);
                 }
-                LoadChunk<C, kFull>(base + at + mine, hd - 8 * my_c, vec, g[i]);
+                LoadRun<C, 8, kLie, false>(base + at + mine, 8 * my_c, hd, g[i]);
             }
             return;
         }
@@ -182,7 +181,7 @@ __global__ __launch_bounds__((TileShape<C, HD>::kThreads), HD <= 128 ? 2 : 1) vo
             const int64_t at = table != nullptr
                                    ? PagedRow(p.rows, PageOf(p.rows, table, j, &bad), j)
                                    : (static_cast<int64_t>(q.t0) + j) * row;
-            LoadChunk<C, kFull>(base + at + 8 * my_c, hd - 8 * my_c, vec, g[i]);
+            LoadRun<C, 8, kLie, false>(base + at, 8 * my_c, hd, g[i]);
         }
     };
     auto put = [&](uint16_t* dst, const uint32_t (&g)[NCH][T::NW]) {
@@ -390,7 +389,7 @@ __global__ __launch_bounds__((TileShape<C, HD>::kThreads), HD <= 128 ? 2 : 1) vo
                 }
             }
             if (split) {
-                if constexpr (kFull) {
+                if constexpr (kLie == kFull) {
                     *reinterpret_cast<f32x4*>(part + dim) = f32x4{x[0], x[1], x[2], x[3]};
                 } else {
 #pragma unroll
@@ -398,9 +397,9 @@ __global__ __launch_bounds__((TileShape<C, HD>::kThreads), HD <= 128 ? 2 : 1) vo
                         if (dim + e < hd) part[dim + e] = x[e];
                     }
                 }
-            } else if constexpr (kFull && sizeof(AB) == 4) {
+            } else if constexpr (kLie == kFull && sizeof(AB) == 4) {
                 *reinterpret_cast<f32x4*>(out + dim) = f32x4{x[0], x[1], x[2], x[3]};
-            } else if constexpr (kFull) {
+            } else if constexpr (kLie == kFull) {
                 *reinterpret_cast<u32x2*>(out + dim) =
                     u32x2{static_cast<uint32_t>(A::Put(x[0])) |
                               (static_cast<uint32_t>(A::Put(x[1])) << 16),
@@ -418,11 +417,12 @@ __global__ __launch_bounds__((TileShape<C, HD>::kThreads), HD <= 128 ? 2 : 1) vo
 
 template <typename A, typename C, int HD>
 mlk_status Launch(const RaggedParams& p, dim3 grid, int n_slots, hipStream_t s) {
-    constexpr int kThreads = TileShape<C, HD>::kThreads;
-    if (p.vec && p.rows.head_dim == HD) {
-        hipLaunchKernelGGL((AttnTile<A, C, HD, true>), grid, dim3(kThreads), 0, s, p, n_slots);
-    } else {
-        hipLaunchKernelGGL((AttnTile<A, C, HD, false>), grid, dim3(kThreads), 0, s, p, n_slots);
+    constexpr int kThreads = TileShape<A, C, HD>::kThreads;
+    const dim3 block(kThreads);
+    switch (LieOf(p, HD)) {
+        case kFull: hipLaunchKernelGGL((AttnTile<A, C, HD, kFull>), grid, block, 0, s, p, n_slots); break;
+        case kPadded: hipLaunchKernelGGL((AttnTile<A, C, HD, kPadded>), grid, block, 0, s, p, n_slots); break;
+        default: hipLaunchKernelGGL((AttnTile<A, C, HD, kScalar>), grid, block, 0, s, p, n_slots); break;
     }
     return CheckLaunch("AttnTile");
 }
