@@ -66,6 +66,10 @@ __device__ inline int LastSeq(const Ragged& r, int64_t x, F f) {
 
 // ------------------------------------------------------------ host checks
 
+// Bounds that keep grids below 2^32 threads and the offsets of a few rows, from
+// one of them on, below 2^32 elements.
+constexpr int64_t kMaxSeqs = 1 << 20, kMaxTokens = 1 << 23, kMaxRow = 1 << 27;
+
 struct PagedArgs {
     Ragged batch;
     RowsAt rows;

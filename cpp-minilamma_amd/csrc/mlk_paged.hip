@@ -225,6 +225,13 @@ mlk_status CheckHeads(const char* fn, int32_t n_heads, int32_t n_kv_heads, int32
     return MLK_OK;
 }
 
+static mlk_status CheckCounts(const char* fn, int64_t n_seqs, int64_t n_tokens) {
+    if (n_seqs < 0 || n_seqs > kMaxSeqs || n_tokens < 0 || n_tokens > kMaxTokens) {
+        return Fail(MLK_ERR_INVALID, "%s: n_seqs must be in 0..2^20 and n_tokens in 0..2^23", fn);
+    }
+    return MLK_OK;
+}
+
 mlk_status CheckPaged(const char* fn, const mlk_paged_cache* cache, const mlk_paged_batch* batch,
                       int32_t type, PagedArgs* args) {
     if (cache == nullptr || batch == nullptr) {
@@ -260,12 +267,8 @@ mlk_status CheckPaged(const char* fn, const mlk_paged_cache* cache, const mlk_pa
     st = CheckElements(fn, "v pages", c.v, c.type);
     if (st != MLK_OK) return st;
     if (c.k == c.v) return Fail(MLK_ERR_INVALID, "%s: k and v pages must be distinct", fn);
-    if (b.n_seqs < 0 || b.n_seqs > (1 << 24)) {
-        return Fail(MLK_ERR_INVALID, "%s: n_seqs must be in 0..2^24", fn);
-    }
-    if (b.n_tokens < 0 || b.n_tokens > (1 << 28)) {
-        return Fail(MLK_ERR_INVALID, "%s: n_tokens must be in 0..2^28", fn);
-    }
+    st = CheckCounts(fn, b.n_seqs, b.n_tokens);
+    if (st != MLK_OK) return st;
     int shift = 0;
     while ((1 << shift) < c.page_size) ++shift;
     *args = {};
@@ -453,9 +456,11 @@ mlk_status mlk_attention_packed(int32_t type, const void* q, int64_t q_row_strid
     if (out == q || out == k || out == v) {
         return Fail(MLK_ERR_INVALID, "%s: out may not alias q, k or v", fn);
     }
-    if (n_seqs < 0 || n_seqs > (1 << 24) || n_tokens < 0 || n_tokens > (1 << 28)) {
-        return Fail(MLK_ERR_INVALID, "%s: n_seqs must be in 0..2^24 and n_tokens in 0..2^28", fn);
+    if (k_row_stride > kMaxRow || v_row_stride > kMaxRow) {
+        return Fail(MLK_ERR_INVALID, "%s: k and v row strides must be at most 2^27 elements", fn);
     }
+    st = CheckCounts(fn, n_seqs, n_tokens);
+    if (st != MLK_OK) return st;
     if (workspace != nullptr && !Aligned(workspace, 16)) {
         return Fail(MLK_ERR_INVALID, "%s: workspace must be 16-byte aligned", fn);
     }

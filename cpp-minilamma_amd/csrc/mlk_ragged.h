@@ -258,6 +258,10 @@ constexpr int kFewHeads = 8;   // most KV heads of its workgroup
 // Launches on `stream`; type and cache_type choose the instance.
 // Waves of a few-row workgroup: 8, or 4 where the registers of 8 would not do.
 inline int FewWaves(int head_dim, int few_rows) { return head_dim <= 128 && few_rows <= 16 ? 8 : 4; }
+// Most workgroups of a launch (512 threads each, below 2^32 in all).
+constexpr int64_t kMaxBlocks = 1 << 22;
+int64_t FewBlocks(const RaggedParams& p);
+int64_t TileBlocks(const RaggedParams& p);
 mlk_status LaunchFew(const RaggedParams& p, int32_t type, int32_t cache_type, hipStream_t stream);
 // Rows of a tile: 8 waves' 32 each, 4 waves' where a row's results take twice the
 // registers.
@@ -344,7 +348,7 @@ __device__ inline bool FindFewWork(const RaggedParams& p, int64_t worker, FewWor
     }
     int64_t before = 0, total = 0;
     if (p.batch.n_seqs > kWave) total = CountFewUnits(p, 0, &before);
-    for (int s0 = 0;; s0 += kWave) {
+    for (int s0 = 0; s0 < p.batch.n_seqs; s0 += kWave) {
         const int32_t mine = FewUnits(p, s0 + lane);
         int64_t sum = mine;  // of lanes 0 .. lane
         for (int off = 1; off < kWave; off *= 2) {
@@ -368,6 +372,7 @@ __device__ inline bool FindFewWork(const RaggedParams& p, int64_t worker, FewWor
         }
         before += here;
     }
+    return false;
 }
 
 // Where the partial of row m lies: few-row kernel, by worker, place in its range

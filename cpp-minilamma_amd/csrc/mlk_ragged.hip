@@ -169,38 +169,45 @@ inline int PerRow(int groups, int64_t parts) {
     return per_row;
 }
 
-template <typename A>
-mlk_status LaunchJoinFew(const RaggedParams& p, int64_t parts, hipStream_t s) {
-    const int groups = p.rows.head_dim <= 128 ? 8 : 4, per_row = PerRow(groups, parts);
+inline int JoinGroups(const RaggedParams& p) { return p.rows.head_dim <= 128 ? 8 : 4; }
+inline int JoinFewPerRow(const RaggedParams& p) {
+    const int64_t pairs = static_cast<int64_t>(p.batch.n_seqs) * p.n_kv_heads;
+    return PerRow(JoinGroups(p), (p.workers + pairs - 1) / pairs + 1);
+}
+inline int64_t JoinFewPerSeq(const RaggedParams& p) {
     const int64_t rows = static_cast<int64_t>(p.n_kv_heads) * p.few_rows;
-    const int64_t per_seq = (rows * per_row + groups - 1) / groups;
-    const int64_t blocks = per_seq * p.batch.n_seqs;
-    if (blocks > 0x7FFFFFFF) return Fail(MLK_ERR_INVALID, "attention: too many rows to join");
-    const dim3 grid(static_cast<unsigned>(blocks));
-    const int n = static_cast<int>(per_seq);
-    if (groups == 8) {
-        hipLaunchKernelGGL((JoinFew<A, 32>), grid, dim3(kThreads), 0, s, p, per_row, n);
-    } else {
-        hipLaunchKernelGGL((JoinFew<A, 64>), grid, dim3(kThreads), 0, s, p, per_row, n);
-    }
+    return (rows * JoinFewPerRow(p) + JoinGroups(p) - 1) / JoinGroups(p);
+}
+inline int64_t JoinFewBlocks(const RaggedParams& p) { return JoinFewPerSeq(p) * p.batch.n_seqs; }
+inline int64_t JoinTilePerToken(const RaggedParams& p) {
+    const int heads = JoinGroups(p) / PerRow(JoinGroups(p), p.n_chunks);
+    return (p.n_heads + heads - 1) / heads;
+}
+inline int64_t JoinTileBlocks(const RaggedParams& p) {
+    return JoinTilePerToken(p) * p.batch.n_tokens;
+}
+
+template <typename A>
+mlk_status LaunchJoinFew(const RaggedParams& p, hipStream_t s) {
+    const dim3 grid(static_cast<unsigned>(JoinFewBlocks(p))), block(kThreads);
+    const int per_row = JoinFewPerRow(p), n = static_cast<int>(JoinFewPerSeq(p));
+    if (JoinGroups(p) == 8) hipLaunchKernelGGL((JoinFew<A, 32>), grid, block, 0, s, p, per_row, n);
+    else hipLaunchKernelGGL((JoinFew<A, 64>), grid, block, 0, s, p, per_row, n);
     return CheckLaunch("JoinFew");
 }
 
 template <typename A>
 mlk_status LaunchJoinTile(const RaggedParams& p, hipStream_t s) {
-    const int groups = p.rows.head_dim <= 128 ? 8 : 4, per_row = PerRow(groups, p.n_chunks);
-    const int heads = groups / per_row;
-    const int per_token = (p.n_heads + heads - 1) / heads;
-    const int64_t blocks = static_cast<int64_t>(p.batch.n_tokens) * per_token;
-    if (blocks > 0x7FFFFFFF) return Fail(MLK_ERR_INVALID, "attention: too many rows to join");
-    const dim3 grid(static_cast<unsigned>(blocks));
-    if (groups == 8) {
-        hipLaunchKernelGGL((JoinTile<A, 32>), grid, dim3(kThreads), 0, s, p, per_row, per_token);
-    } else {
-        hipLaunchKernelGGL((JoinTile<A, 64>), grid, dim3(kThreads), 0, s, p, per_row, per_token);
-    }
+    const dim3 grid(static_cast<unsigned>(JoinTileBlocks(p))), block(kThreads);
+    const int per_row = PerRow(JoinGroups(p), p.n_chunks);
+    const int n = static_cast<int>(JoinTilePerToken(p));
+    if (JoinGroups(p) == 8) hipLaunchKernelGGL((JoinTile<A, 32>), grid, block, 0, s, p, per_row, n);
+    else hipLaunchKernelGGL((JoinTile<A, 64>), grid, block, 0, s, p, per_row, n);
     return CheckLaunch("JoinTile");
 }
+
+int64_t Larger(int64_t a, int64_t b) { return a > b ? a : b; }
+int64_t RoundUp(int64_t a, int64_t to) { return (a + to - 1) / to * to; }
 
 struct Plan {
     int64_t few_rows = 0, few_workers = 0, few_partials = 0;
@@ -209,7 +216,7 @@ struct Plan {
 };
 
 int64_t PartBytes(int64_t partials, int32_t hd) {
-    return (partials * (4 * hd + 8) + 255) / 256 * 256;
+    return RoundUp(RoundUp(partials * 4 * hd, 16) + partials * 8, 256);
 }
 int64_t PlanBytes(const Plan& plan, int32_t hd) {
     return PartBytes(plan.few_partials, hd) + PartBytes(plan.tile_partials, hd);
@@ -220,8 +227,6 @@ constexpr int64_t kTileLeast = 256;    // positions of a tile row's least chunk
 constexpr int64_t kTileMost = 64;      // most chunks of a tile row
 constexpr int64_t kTileFixed = 300;    // what a tile's start and end cost, in positions
 constexpr int64_t kTileJoin = 300;     // what the join costs
-
-int64_t RoundUp(int64_t a, int64_t to) { return (a + to - 1) / to * to; }
 
 Plan MakePlan(int64_t n_seqs, int64_t n_tokens, int64_t max_new, int64_t max_len, int32_t n_heads,
               int32_t n_kv_heads, int32_t head_dim, bool packed) {
@@ -282,9 +287,10 @@ int64_t AttendWorkspace(int64_t n_seqs, int64_t n_tokens, int64_t max_new, int64
                         int32_t n_heads, int32_t n_kv_heads, int32_t head_dim, bool packed) {
     if (n_seqs <= 0 || n_tokens <= 0 || max_new <= 0 || max_len <= 0 || n_heads <= 0 ||
         n_kv_heads <= 0 || n_heads % n_kv_heads != 0 || n_heads > 65536 || head_dim <= 0 ||
-        head_dim > 256 || n_seqs > (1 << 24) || n_tokens > (1 << 28) || max_len > (1 << 30)) {
+        head_dim > 256 || n_seqs > kMaxSeqs || n_tokens > kMaxTokens || max_len > (1 << 30)) {
         return 0;
     }
+    if (packed && max_len > n_tokens) max_len = n_tokens;
     if (max_new > max_len) max_new = max_len;
     if (max_new > n_tokens) max_new = n_tokens;
     return PlanBytes(
@@ -318,38 +324,49 @@ mlk_status Attend(const AttendArgs& a) {
     p.few_rows = static_cast<int32_t>(plan.few_rows);
     p.err = a.err;
     char* ws = static_cast<char*>(a.workspace);
-    auto place = [&](int64_t partials) {
-        p.part_o = reinterpret_cast<float*>(ws);
-        p.part_ml = reinterpret_cast<float2*>(ws + partials * 4 * hd);
+    auto place = [&](int64_t partials, RaggedParams* to) {
+        to->part_o = reinterpret_cast<float*>(ws);
+        to->part_ml = reinterpret_cast<float2*>(ws + RoundUp(partials * 4 * hd, 16));
         ws += PartBytes(partials, hd);
     };
+    RaggedParams few = p, tile = p;
+    int64_t blocks = 0;
     if (plan.few_rows > 0) {
-        p.workers = static_cast<int32_t>(plan.few_workers);
-        p.few_heads = FewWaves(hd, p.few_rows);
-        while (a.n_kv_heads % p.few_heads != 0) p.few_heads /= 2;
-        if (p.workers > 0) place(plan.few_partials);
-        mlk_status st = LaunchFew(p, a.type, a.cache_type, a.stream);
-        if (st != MLK_OK) return st;
-        if (p.workers > 0) {
-            const int64_t pairs = static_cast<int64_t>(b.n_seqs) * a.n_kv_heads;
-            const int64_t parts = (p.workers + pairs - 1) / pairs + 1;
-            st = a.type == MLK_F32   ? LaunchJoinFew<F32>(p, parts, a.stream)
-                 : a.type == MLK_F16 ? LaunchJoinFew<F16>(p, parts, a.stream)
-                                     : LaunchJoinFew<BF16>(p, parts, a.stream);
-            if (st != MLK_OK) return st;
-        }
+        few.workers = static_cast<int32_t>(plan.few_workers);
+        few.few_heads = FewWaves(hd, few.few_rows);
+        while (a.n_kv_heads % few.few_heads != 0) few.few_heads /= 2;
+        if (few.workers > 0) place(plan.few_partials, &few);
+        blocks = FewBlocks(few);
+        if (few.workers > 0) blocks = Larger(blocks, JoinFewBlocks(few));
     }
     if (plan.tile) {
-        p.chunk = static_cast<int32_t>(plan.chunk);
-        p.n_chunks = static_cast<int32_t>(plan.n_chunks);
-        if (p.n_chunks > 1) place(plan.tile_partials);
-        mlk_status st = LaunchTile(p, a.type, a.cache_type, a.stream);
-        if (st != MLK_OK) return st;
-        if (p.n_chunks > 1) {
-            return a.type == MLK_F32   ? LaunchJoinTile<F32>(p, a.stream)
-                   : a.type == MLK_F16 ? LaunchJoinTile<F16>(p, a.stream)
-                                       : LaunchJoinTile<BF16>(p, a.stream);
+        tile.chunk = static_cast<int32_t>(plan.chunk);
+        tile.n_chunks = static_cast<int32_t>(plan.n_chunks);
+        if (tile.n_chunks > 1) place(plan.tile_partials, &tile);
+        blocks = Larger(blocks, TileBlocks(tile));
+        if (tile.n_chunks > 1) blocks = Larger(blocks, JoinTileBlocks(tile));
+    }
+    if (blocks > kMaxBlocks) {
+        return Fail(MLK_ERR_INVALID, "attention: %lld workgroups exceed a launch's 2^22",
+                    static_cast<long long>(blocks));
+    }
+    if (plan.few_rows > 0) {
+        mlk_status st = LaunchFew(few, a.type, a.cache_type, a.stream);
+        if (st == MLK_OK && few.workers > 0) {
+            st = a.type == MLK_F32   ? LaunchJoinFew<F32>(few, a.stream)
+                 : a.type == MLK_F16 ? LaunchJoinFew<F16>(few, a.stream)
+                                     : LaunchJoinFew<BF16>(few, a.stream);
         }
+        if (st != MLK_OK) return st;
+    }
+    if (plan.tile) {
+        mlk_status st = LaunchTile(tile, a.type, a.cache_type, a.stream);
+        if (st == MLK_OK && tile.n_chunks > 1) {
+            st = a.type == MLK_F32   ? LaunchJoinTile<F32>(tile, a.stream)
+                 : a.type == MLK_F16 ? LaunchJoinTile<F16>(tile, a.stream)
+                                     : LaunchJoinTile<BF16>(tile, a.stream);
+        }
+        return st;
     }
     return MLK_OK;
 }

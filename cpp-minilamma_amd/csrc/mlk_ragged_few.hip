@@ -24,8 +24,6 @@
 // keeps one tile (16 KB at head_dim 128) in flight through its arithmetic.
 #include "mlk_ragged.h"
 
-#include <climits>
-
 namespace mlk {
 namespace {
 
@@ -568,14 +566,13 @@ struct ByDim {
 
 }  // namespace
 
+int64_t FewBlocks(const RaggedParams& p) {
+    return p.workers != 0 ? p.workers : static_cast<int64_t>(p.batch.n_seqs) * p.n_kv_heads;
+}
+
 mlk_status LaunchFew(const RaggedParams& p, int32_t type, int32_t cache_type, hipStream_t stream) {
-    const int64_t blocks = p.workers != 0 ? p.workers
-                                          : static_cast<int64_t>(p.batch.n_seqs) * p.n_kv_heads;
-    if (blocks > INT_MAX) {
-        return Fail(MLK_ERR_INVALID, "attention: %lld workgroups exceed the grid",
-                    static_cast<long long>(blocks));
-    }
-    return ByType(type, cache_type, ByDim{p, dim3(static_cast<unsigned>(blocks)), stream});
+    const dim3 grid(static_cast<unsigned>(FewBlocks(p)));
+    return ByType(type, cache_type, ByDim{p, grid, stream});
 }
 
 }  // namespace mlk

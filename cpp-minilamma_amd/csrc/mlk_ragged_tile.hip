@@ -21,8 +21,6 @@
 // once.
 #include "mlk_ragged.h"
 
-#include <climits>
-
 namespace mlk {
 namespace {
 
@@ -100,7 +98,8 @@ __global__ __launch_bounds__((TileShape<A, C, HD>::kThreads), HD <= 128 ? 2 : 1)
     const int32_t tok = real ? static_cast<int32_t>(m / group) : 0;
     const int h = kvh * group + (real ? static_cast<int>(m % group) : 0);
     const int32_t pos = real ? first + tok : -1;
-    // positions the wave's rows attend to: some row all below wave_lo, none from wave_hi
+    // positions that all rows of the wave attend to: up to wave_lo; that any does: below
+    // wave_hi
     const int64_t w0 = m0 + 32 * wave;
     const int32_t wave_lo = w0 <= m_last ? first + static_cast<int32_t>(w0 / group) : -1;
     const int64_t w1 = w0 + 31 < m_last ? w0 + 31 : m_last;
@@ -448,16 +447,16 @@ int64_t TileSlots(int64_t n_seqs, int64_t n_tokens, int32_t group, int rows) {
 
 }  // namespace
 
+int64_t TileBlocks(const RaggedParams& p) {
+    return TileSlots(p.batch.n_seqs, p.batch.n_tokens, p.group, TileRows(p.rows.head_dim)) *
+           p.n_chunks * p.n_kv_heads;
+}
+
 mlk_status LaunchTile(const RaggedParams& p, int32_t type, int32_t cache_type, hipStream_t stream) {
     const int64_t slots = TileSlots(p.batch.n_seqs, p.batch.n_tokens, p.group,
                                     TileRows(p.rows.head_dim));
-    const int64_t blocks = slots * p.n_chunks * p.n_kv_heads;
-    if (blocks > INT_MAX) {
-        return Fail(MLK_ERR_INVALID, "attention: %lld workgroups exceed the grid",
-                    static_cast<long long>(blocks));
-    }
-    return ByType(type, cache_type, ByDim{p, dim3(static_cast<unsigned>(blocks)),
-                                          static_cast<int>(slots), stream});
+    const dim3 grid(static_cast<unsigned>(TileBlocks(p)));
+    return ByType(type, cache_type, ByDim{p, grid, static_cast<int>(slots), stream});
 }
 
 }  // namespace mlk

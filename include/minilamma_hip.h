@@ -364,7 +364,8 @@ typedef struct {
  * replays with new values within the host's bounds: n_tokens token rows exist
  * (rows behind token_start[n_seqs] are neither read nor written), no sequence
  * brings over max_new_tokens, none is longer than max_seq_len
- * (<= table_stride * page_size).  A sequence outside these bounds, or with more
+ * (<= table_stride * page_size; n_seqs up to 2^20, n_tokens up to 2^23).  A
+ * sequence outside these bounds, or with more
  * new tokens than its length, raises *err (NULL: no report; the caller clears
  * it) and gets nothing written. */
 typedef struct {
@@ -403,18 +404,20 @@ mlk_status mlk_paged_kv_append(const mlk_paged_cache* cache, const mlk_paged_bat
  * both in one batch.  q rows and out (dense [n_tokens, n_heads, head_dim]) are
  * of `type`; out must not overlap q or the pages.  head_dim 1..256.  Scores,
  * statistics and sums are fp32.  With fp32 activations q and w enter the
- * products in enough 16-bit pieces that each product is within 2^-20 of
- * itself; with 16-bit ones w is rounded to that type.  What a token does not
+ * products in enough 16-bit pieces that each product is within 2^-20 of itself
+ * (over an fp16 cache, for values 2^17 below their row's largest, within 2^-38 of
+ * that one); with 16-bit ones w is rounded to that type.  What a token does not
  * attend to (later positions, the rest of the last page) never changes its
  * result, whatever bits lie there; a token that attends to a non-finite value
- * gets non-finite results.  A page index outside [0, n_pages) raises *err and
+ * gets non-finite results (of 16-bit activations: an infinity in V as such).  A page index outside [0, n_pages) raises *err and
  * page 0 is read in its place.
  *
  * workspace: optional scratch (16-byte aligned,
  * mlk_attention_paged_workspace_bytes(); it may differ between calls, its
- * content does not matter).  With it few rows over long sequences split their
- * positions over workgroups, the partial sums joined in a fixed order; without
- * it (NULL or smaller) the call is correct, only slower.
+ * content does not matter, and calls that may overlap need one each).  With it
+ * few rows over long sequences split their positions over workgroups, the partial
+ * sums joined in a fixed order; without it (NULL or smaller) the call is correct,
+ * only slower.
  */
 mlk_status mlk_attention_paged(const mlk_paged_cache* cache, const mlk_paged_batch* batch,
                                int32_t type, const void* q, int64_t q_row_stride, void* out,
@@ -432,7 +435,8 @@ int64_t mlk_attention_paged_workspace_bytes(int64_t n_seqs, int64_t n_tokens,
  * non-decreasing; empty sequences are allowed), and each row attends to its
  * own sequence's rows up to itself, as mlk_attention_paged does over pages, with
  * the same semantics and precision.  q, k, v (rows q_row_stride, k_row_stride,
- * v_row_stride elements apart: slices of one fused projection are fine) and out
+ * v_row_stride elements apart, k's and v's at most 2^27: slices of one fused
+ * projection are fine) and out
  * (dense) are of `type`.  Rows behind seq_start[n_seqs] are neither read nor
  * written; n_tokens and max_seq_len bound them on the host; a sequence outside
  * the bounds raises *err and gets nothing written.  workspace: as above

@@ -633,3 +633,88 @@ def test_cache_beyond_32_bit_offsets(mlk, paged):
                                    default_scale(hd))
             vsum = np.repeat(np.abs(v64[:n]).sum(0), H, axis=0)
             assert_close(got[i], o, pav, d, n, vsum, act, f"row {i}")
+
+
+# ------------------------------------------------------------------ many sequences, odd tables
+
+@pytest.mark.parametrize("act,ct", PAIRS)
+def test_more_sequences_than_a_wave(mlk, paged, act, ct):
+    """150 sequences: decode steps, a mixed batch with empty ones, and packed
+    prompts; some of them longer than what is left unsplit."""
+    H, KV, hd = 8, 2, 64
+    rng = np.random.default_rng(11)
+    lens = rng.integers(1, 90, 150)
+    lens[[3, 64, 149]] = 1200, 700, 2001
+    for counts in (np.ones(150, int), np.where(np.arange(150) % 7 == 2, 0, 1)):
+        counts = counts.copy()
+        if counts.sum() < 150:
+            counts[[3, 77, 149]] = 9, 21, 300
+        lens = np.maximum(lens, counts)
+        batch = Batch(counts, lens, 16, spare=1, seed=3)
+        cache = Cache(mlk, paged, batch, KV, hd, ct, rng)
+        q = to_type(rng.standard_normal((batch.T, H, hd)), act)
+        got = run_paged(mlk, paged, batch, cache, q, H, act)
+        some = set(rng.integers(0, sum(counts), 60)) | {0, 3, 4, 20, 64, sum(counts) - 1}
+        check_paged(batch, cache, q, got, H, act, rows=some)
+    if act == ct:
+        batch = Batch(np.minimum(lens, 90), None)
+        qkv = [to_type(rng.standard_normal((batch.T, n, hd)), act) for n in (H, KV, KV)]
+        got = run_packed(mlk, paged, batch, *qkv, H, KV, hd, act)
+        check_packed(batch, *qkv, got, H, KV, hd, act, rows=set(rng.integers(0, batch.T, 60)))
+
+
+@pytest.mark.parametrize("act,ct", PAIRS)
+@pytest.mark.parametrize("page", [2, 4, 8, 32])
+@pytest.mark.parametrize("heads", [(8, 2, 64), (8, 8, 128), (4, 1, 160), (4, 2, 72)], ids=str)
+def test_page_sizes(mlk, paged, heads, page, act, ct):
+    H, KV, hd = heads
+    rng = np.random.default_rng(page)
+    for counts, lens in (([1, 1, 1], [777, 64, 33]), ([40, 1], [700, 130])):
+        batch = Batch(counts, lens, page, seed=page)
+        cache = Cache(mlk, paged, batch, KV, hd, ct, rng)
+        q = to_type(rng.standard_normal((batch.T, H, hd)), act)
+        got = run_paged(mlk, paged, batch, cache, q, H, act)
+        check_paged(batch, cache, q, got, H, act, rows=set(range(0, batch.T, 5)) | {batch.T - 1})
+
+
+@pytest.mark.parametrize("act,ct", [("f32", "f16"), ("bf16", "bf16")])
+def test_shared_pages_dirty_workspace_and_no_flag(mlk, paged, act, ct):
+    """Two sequences on the same first pages; a workspace full of NaN bits, used
+    by two calls of different sizes; err not given."""
+    H, KV, hd, page = 8, 2, 128, 16
+    rng = np.random.default_rng(12)
+    batch = Batch([1, 1], [1000, 900], page)
+    shared = 800 // page
+    batch.table[1, :shared] = batch.table[0, :shared]
+    cache = Cache(mlk, paged, batch, KV, hd, ct, rng)
+    dev = batch.device(mlk, paged)
+    need = paged.attention_workspace_bytes(cache.handle, dev, H, act)
+    assert need > 0
+    ws = mlk.DeviceBuffer.from_array(np.full(need, 0xFF, np.uint8))
+    q = to_type(rng.standard_normal((2, H, hd)), act)
+    for b in (batch, Batch([1], [600], page)):
+        b.table, b.n_pages, b.width = batch.table, batch.n_pages, batch.width
+        d = b.device(mlk, paged)
+        out = mlk.DeviceBuffer.from_array(np.full((b.T, H, hd), 7, NP[act]))
+        paged.attention(cache.handle, d, mlk.DeviceBuffer.from_array(q[:b.T].copy()), out, H, act,
+                        workspace=ws)
+        mlk.synchronize()
+        cache.batch = b
+        check_paged(b, cache, q[:b.T], out.download(), H, act)
+
+
+def test_split_results_do_not_depend_on_the_bounds(mlk, paged):
+    """Host bounds far above the lengths: the same values to rounding, with the
+    workspace such bounds ask for."""
+    H, KV, hd = 32, 8, 128
+    rng = np.random.default_rng(13)
+    for counts, lens in (([1, 1], [900, 40]), ([70], [800])):
+        batch = Batch(counts, lens, 16)
+        cache = Cache(mlk, paged, batch, KV, hd, "f16", rng)
+        batch.table = np.pad(batch.table, ((0, 0), (0, 2000)), constant_values=-1)
+        batch.width = batch.table.shape[1]
+        q = rng.standard_normal((batch.T, H, hd)).astype(np.float32)
+        for bounds in ((None, None), (batch.T, 30000)):
+            dev = batch.device(mlk, paged, *bounds)
+            got = run_paged(mlk, paged, batch, cache, q, H, "f32", dev=dev)
+            check_paged(batch, cache, q, got, H, "f32", rows=set(range(0, batch.T, 9)))

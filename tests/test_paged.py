@@ -118,7 +118,12 @@ def test_packed_refusals(mlk, paged):
             (dict(scale=-1.0), "scale"), (dict(n_seqs=-1), "n_seqs"),
             (dict(n_tokens=2 ** 28 + 1), "n_tokens"), (dict(seq_start=None), "seq_start"),
             (dict(max_seq_len=0), "max_seq_len"),
+            (dict(k_row_stride=2 ** 27 + 1), "2\\^27"), (dict(v_row_stride=2 ** 27 + 1), "2\\^27"),
+            (dict(n_seqs=2 ** 20, n_tokens=2 ** 20, n_heads=65536, n_kv_heads=65536),
+             "workgroups exceed"),
             (dict(workspace=8, workspace_bytes=8), "16-byte aligned")]:
+        if "n_kv_heads" in kw:
+            kw = dict(kw, k_row_stride=65536 * 8, v_row_stride=65536 * 8)
         with pytest.raises(mlk.MlkError, match=text):
             paged.attention_packed(**{**ok, **kw})
 
@@ -130,6 +135,19 @@ def test_empty_calls_do_nothing(mlk, paged):
         paged.kv_append(cache, batch, 3 * FAKE, 4 * FAKE, "f16")
         paged.attention_packed("f32", FAKE, 2 * FAKE, 3 * FAKE, None, kw.get("n_seqs", 2),
                                kw.get("n_tokens", 4), 5, 4, 2, 8, 5 * FAKE)
+
+
+def test_workspace_bytes_of_bad_and_of_large_bounds(mlk, paged):
+    size = mlk.lib.mlk_attention_paged_workspace_bytes
+    for bad in ((0, 1, 1, 1, 4, 2, 8), (1, 0, 1, 1, 4, 2, 8), (1, 1, 0, 1, 4, 2, 8),
+                (1, 1, 1, 0, 4, 2, 8), (1, 1, 1, 1, 5, 2, 8), (1, 1, 1, 1, 4, 0, 8),
+                (1, 1, 1, 1, 4, 2, 257), (2 ** 21, 1, 1, 1, 4, 2, 8)):
+        assert size(*bad) == 0
+    assert size(1, 1, 1, 100, 32, 8, 128) == 0  # short: nothing is split
+    assert 0 < size(64, 64, 1, 131072, 32, 8, 128) < 2 ** 28
+    assert size(1, 2 ** 23, 2 ** 23, 2 ** 30, 32, 8, 128) < 2 ** 34
+    packed = mlk.lib.mlk_attention_packed_workspace_bytes
+    assert packed(3, 100, 2 ** 30, 32, 8, 128) == packed(3, 100, 100, 32, 8, 128)
 
 
 def test_unknown_types_through_the_c_abi(mlk):
