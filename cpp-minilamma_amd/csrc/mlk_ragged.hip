@@ -171,7 +171,8 @@ inline int PerRow(int groups, int64_t parts) {
 
 inline int JoinGroups(const RaggedParams& p) { return p.rows.head_dim <= 128 ? 8 : 4; }
 inline int JoinFewPerRow(const RaggedParams& p) {
-    const int64_t pairs = static_cast<int64_t>(p.batch.n_seqs) * p.n_kv_heads;
+    // parts of a row where the sequences are alike and few_heads heads go together
+    const int64_t pairs = static_cast<int64_t>(p.batch.n_seqs) * p.n_kv_heads / p.few_heads;
     return PerRow(JoinGroups(p), (p.workers + pairs - 1) / pairs + 1);
 }
 inline int64_t JoinFewPerSeq(const RaggedParams& p) {
