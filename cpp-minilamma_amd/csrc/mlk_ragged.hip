@@ -15,11 +15,11 @@ namespace {
 
 constexpr int kThreads = 256;
 
-// out = sum_c 2^(m_c - m) o_c / sum_c 2^(m_c - m) l_c over a row's n chunks.  A
-// group of L lanes (4 dims each) takes every `per_row`-th chunk of a row, the
+// out = sum_c 2^(m_c - m) o_c / sum_c 2^(m_c - m) l_c over a row's n parts.  A
+// group of L lanes (4 dims each) takes every `per_row`-th part of a row, the
 // groups' sums are added in order.  What costs is latency, not bytes: the first
-// kAhead chunks of each group are on their way before the maxima are looked at
-// (one 8B decode row over 32 chunks: 21 us with one wave walking them all, 5 us).
+// kAhead parts of each group are on their way before the maxima are looked at
+// (one 8B decode row over 32 parts: 21 us with one wave walking them all, 6 us).
 constexpr int kAhead = 4;
 
 // Row of `n` parts: the first at partial `base`, the second at `next`, and from
