@@ -30,7 +30,7 @@
 // are non-temporal, no other workgroup reads those rows.  Pages are looked up a
 // tile ahead by scalar loads, which do not queue behind the rows.
 //
-// 64 sequences of 8B heads, bf16, 1.10 GB of K and V: 191 us with the join, 5.8
+// 64 sequences of 8B heads, bf16, 1.10 GB of K and V: 190 us with the join, 5.8
 // TB/s; of the time before, waves on neighbouring heads instead of one head 7 us,
 // non-temporal loads 12, scalar look-ups 5.  4 sequences of 70B heads, fp32 over
 // fp16, 0.79 GB: 146 us, 5.4 TB/s.  A kernel that only reads reached 5.0 to 7.0 TB/s,

@@ -21,7 +21,7 @@
 // K's reads (16 rows of one chunk) and V's (4 rows of 64 bytes) meet each bank
 // once (counted: no conflicts).
 //
-// 9001 packed bf16 tokens of 70B heads: 567 GFLOP in 653 us, 0.87 PFLOP/s where
+// 9001 packed bf16 tokens of 70B heads: 567 GFLOP in 648 us, 0.88 PFLOP/s where
 // an 8192^3 bf16 product reaches 1.32.  2500 packed fp32 tokens of 8B heads: 6
 // products for each of 11.9 GFLOP, 120 us, 0.6 PFLOP/s.  256 rows share a tile's
 // loads: with 128 these took 674 and 144 us.  Counted with 128 rows on the packed
