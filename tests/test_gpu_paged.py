@@ -718,3 +718,53 @@ def test_split_results_do_not_depend_on_the_bounds(mlk, paged):
             dev = batch.device(mlk, paged, *bounds)
             got = run_paged(mlk, paged, batch, cache, q, H, "f32", dev=dev)
             check_paged(batch, cache, q, got, H, "f32", rows=set(range(0, batch.T, 9)))
+
+
+@pytest.mark.parametrize("act,ct", PAIRS)
+@pytest.mark.parametrize("heads", [(8, 2, 64), (8, 8, 128), (4, 1, 160)], ids=str)
+def test_more_sequences_than_workgroups(mlk, paged, heads, act, ct):
+    """700 sequences, few of them long enough to be split, some without a new
+    token: those that lie across two workgroups' shares are joined, and only
+    those; the same again without a workspace."""
+    H, KV, hd = heads
+    rng = np.random.default_rng(21)
+    lens = [int(n) for n in rng.integers(1, 41, 700)]
+    for s in range(13, 700, 60):
+        lens[s] = int(rng.integers(600, 1500))
+    counts = [0 if s % 9 == 4 else 1 for s in range(700)]
+    batch = Batch(counts, lens, 16, 2)
+    cache = Cache(mlk, paged, batch, KV, hd, ct, rng)
+    q = to_type(rng.standard_normal((batch.T, H, hd)), act)
+    rows = {t for t, s, p in batch.rows() if lens[s] > 500 or s % 17 == 0}
+    for ws in (True, False):
+        got = run_paged(mlk, paged, batch, cache, q, H, act, workspace=ws)
+        check_paged(batch, cache, q, got, H, act, rows=rows)
+        g = values(got[:sum(counts)], act)
+        assert np.isfinite(g).all() and (g != 7).any(axis=(1, 2)).all()
+
+
+def test_thousands_of_sequences(mlk, paged):
+    """5000 sequences of 0, 1 or 2 new tokens, one of 40: each token's place in
+    its own sequence's pages, and packed attention within its own sequence."""
+    H, KV, hd = 4, 1, 16
+    rng = np.random.default_rng(22)
+    counts = [int(n) for n in rng.integers(0, 3, 5000)]
+    counts[4321] = 40
+    batch = Batch(counts, [n + s % 3 + 1 for s, n in enumerate(counts)], 2, 3)
+    cache = Cache(mlk, paged, batch, KV, hd, "f32", rng, fill=False)
+    q, k, v = (rng.standard_normal((batch.T, n, hd)).astype(np.float32) for n in (H, KV, KV))
+    err = mlk.DeviceBuffer.from_array(np.zeros(1, np.int32))
+    paged.kv_append(cache.handle, batch.device(mlk, paged), mlk.DeviceBuffer.from_array(k),
+                    mlk.DeviceBuffer.from_array(v), "f32", theta=0.0, err=err)
+    mlk.synchronize()
+    assert err.download()[0] == 0
+    for t, s, p in batch.rows():
+        cache.pages(0)[batch.table[s, p // 2], p % 2] = k[t]
+        cache.pages(1)[batch.table[s, p // 2], p % 2] = v[t]
+    assert (cache.k.download().view(np.uint8) == cache.host[0].view(np.uint8)).all()
+    assert (cache.v.download().view(np.uint8) == cache.host[1].view(np.uint8)).all()
+    packed = Batch(counts, None, spare=3)
+    got = run_packed(mlk, paged, packed, q, k, v, H, KV, hd, "f32")
+    at = int(packed.start[4321])
+    check_packed(packed, q, k, v, got, H, KV, hd, "f32",
+                 rows=set(range(0, sum(counts), 23)) | set(range(at, at + 42)))
