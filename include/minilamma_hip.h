@@ -409,8 +409,9 @@ mlk_status mlk_paged_kv_append(const mlk_paged_cache* cache, const mlk_paged_bat
  * that one); with 16-bit ones w is rounded to that type.  What a token does not
  * attend to (later positions, the rest of the last page) never changes its
  * result, whatever bits lie there; a token that attends to a non-finite value
- * gets non-finite results (of 16-bit activations: an infinity in V as such).  A
- * page index outside [0, n_pages) raises *err and page 0 is read in its place.
+ * gets non-finite results (of 16-bit activations: an infinity in V as such, and
+ * a position whose score comes out as -infinity may count as weight 0 instead).
+ * A page index outside [0, n_pages) raises *err and page 0 is read in its place.
  *
  * workspace: optional scratch (16-byte aligned,
  * mlk_attention_paged_workspace_bytes(); it may differ between calls, its
