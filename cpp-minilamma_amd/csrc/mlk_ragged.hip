@@ -295,8 +295,17 @@ Plan MakePlan(int64_t n_seqs, int64_t n_tokens, int64_t max_new, int64_t max_len
         const int64_t each = TileRows(head_dim);
         const int64_t tiles =
             ((rows + each - 1) / each + (mixed ? 0 : (n_seqs - 1) / 2)) * n_kv_heads;
+        RaggedParams grid{};  // what a launch's size follows from
+        grid.batch.n_seqs = static_cast<int32_t>(n_seqs);
+        grid.batch.n_tokens = static_cast<int32_t>(n_tokens);
+        grid.rows.head_dim = head_dim;
+        grid.n_heads = n_heads;
+        grid.n_kv_heads = n_kv_heads;
+        grid.group = static_cast<int32_t>(group);
         int64_t best = INT64_MAX;
         for (int64_t n = 1; n <= kTileMost && (n == 1 || (n - 1) * kTileLeast < max_len); ++n) {
+            grid.n_chunks = static_cast<int32_t>(n);
+            if (n > 1 && (TileBlocks(grid) > kMaxBlocks || JoinTileBlocks(grid) > kMaxBlocks)) break;
             const int64_t chunk = RoundUp((max_len + n - 1) / n, kTileLeast);
             const int64_t cost = ((tiles < 1 ? 1 : tiles) * n + cus - 1) / cus * (chunk + kTileFixed) +
                                  (n > 1 ? kTileJoin : 0);

@@ -364,10 +364,11 @@ typedef struct {
  * replays with new values within the host's bounds: n_tokens token rows exist
  * (rows behind token_start[n_seqs] are neither read nor written), no sequence
  * brings over max_new_tokens, none is longer than max_seq_len
- * (<= table_stride * page_size; n_seqs up to 2^20, n_tokens up to 2^23).  A
- * sequence outside these bounds, or with more
- * new tokens than its length, raises *err (NULL: no report; the caller clears
- * it) and gets nothing written. */
+ * (<= table_stride * page_size; n_seqs up to 2^20, n_tokens up to 2^23; an
+ * attention call over 2^22 workgroups, of the order of n_seqs * n_kv_heads, is
+ * refused).  A sequence outside these bounds, or with more new tokens than its
+ * length, raises *err (NULL: no report; the caller clears it) and gets nothing
+ * written. */
 typedef struct {
     const int32_t* token_start;  /* device [n_seqs + 1] */
     const int32_t* seq_len;      /* device [n_seqs] */

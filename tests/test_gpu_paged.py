@@ -768,3 +768,21 @@ def test_thousands_of_sequences(mlk, paged):
     at = int(packed.start[4321])
     check_packed(packed, q, k, v, got, H, KV, hd, "f32",
                  rows=set(range(0, sum(counts), 23)) | set(range(at, at + 42)))
+
+
+def test_mixed_batch_of_very_many_sequences(mlk, paged):
+    """70000 decode tokens on two shared pages and a chunk of 40 beside them,
+    under a bound of 8192 positions: too many row tiles for as many parts as the
+    chunk alone would be split into."""
+    H, KV, hd = 8, 8, 8
+    rng = np.random.default_rng(23)
+    lens = [int(n) for n in rng.integers(1, 6, 70000)] + [700]
+    batch = Batch([1] * 70000 + [40], lens, 8192)
+    batch.n_pages = 2
+    batch.table[:, 0] = np.arange(len(lens)) % 2
+    cache = Cache(mlk, paged, batch, KV, hd, "bf16", rng)
+    q = to_type(rng.standard_normal((batch.T, H, hd)), "bf16")
+    got = run_paged(mlk, paged, batch, cache, q, H, "bf16",
+                    dev=batch.device(mlk, paged, None, 8192))
+    check_paged(batch, cache, q, got, H, "bf16",
+                rows=set(range(0, 70000, 997)) | set(range(69995, 70040, 3)))

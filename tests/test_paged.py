@@ -168,3 +168,12 @@ def test_index_arithmetic_on_the_host(tmp_path):
                     os.path.join(ROOT, "tests", "cpp", "paged_index.cc"), "-o", exe], check=True)
     out = subprocess.run([exe], capture_output=True, text=True, timeout=120)
     assert out.returncode == 0, out.stdout + out.stderr
+
+
+def test_many_sequences_are_not_split_beyond_a_launch(mlk, paged):
+    """300000 decode tokens and a chunk of 100 at 8 KV heads: 300000 + 100 * 8 /
+    256 row tiles and more, times 8, are under 2^22 workgroups and twice that is
+    not, so the tile kernel's positions are not split; the few-row partials alone
+    remain (2 parts of 512 workgroups at most, 8 heads, 16 rows)."""
+    size = mlk.lib.mlk_attention_paged_workspace_bytes
+    assert 0 < size(300000, 300100, 100, 8192, 64, 8, 128) <= 2 * 512 * 8 * 16 * (128 * 4 + 8) + 512
