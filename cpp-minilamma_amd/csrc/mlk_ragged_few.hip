@@ -322,7 +322,7 @@ __global__ __launch_bounds__(kWaves * kWave) void AttnFew(const RaggedParams p) 
         float m[NB], l[NB];
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
-            m[nb] = -INFINITY;  // of the scores times the factor
+            m[nb] = -INFINITY;  // of the scores before the factor
             l[nb] = 0.0f;       // this lane's part of the sum
 #pragma unroll
             for (int e = 0; e < NI; ++e) o[nb][e] = f32x4{0, 0, 0, 0};
@@ -371,7 +371,7 @@ __global__ __launch_bounds__(kWaves * kWave) void AttnFew(const RaggedParams p) 
                 for (int b = 0; b < NBK; ++b) {
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
-                        float x = sc[nb][b][r] * factor[nb];
+                        float x = sc[nb][b][r];
                         const int32_t j = j0 + 16 * b + 4 * g4 + r;
                         if (masked && (j > pos[nb] || j >= j_end)) x = -INFINITY;
                         w[nb][4 * b + r] = x;
@@ -382,16 +382,17 @@ __global__ __launch_bounds__(kWaves * kWave) void AttnFew(const RaggedParams p) 
                 const float mn = fmaxf(m[nb], top);
                 const float base = mn == -INFINITY ? 0.0f : mn;
                 if (__ballot(mn != m[nb]) != 0) {
-                    const float alpha = __builtin_amdgcn_exp2f(m[nb] - base);
+                    const float alpha = __builtin_amdgcn_exp2f((m[nb] - base) * factor[nb]);
                     l[nb] *= alpha;
 #pragma unroll
                     for (int e = 0; e < NI; ++e) o[nb][e] *= alpha;
                     m[nb] = mn;
                 }
+                // the difference first: the largest weight is 2^kW however large the scores are
                 float sum = 0.0f;
 #pragma unroll
                 for (int i = 0; i < 4 * NBK; ++i) {
-                    w[nb][i] = __builtin_amdgcn_exp2f(w[nb][i] - (base - kW));
+                    w[nb][i] = __builtin_amdgcn_exp2f(fmaf(w[nb][i] - base, factor[nb], kW));
                     sum += w[nb][i];
                 }
                 l[nb] += sum;
@@ -440,6 +441,8 @@ __global__ __launch_bounds__(kWaves * kWave) void AttnFew(const RaggedParams p) 
             }
         }
         if (bad && p.err != nullptr) RaiseFlag(p.err, 1);
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) m[nb] *= factor[nb];  // as the joins take it
 
         const int32_t masked_from0 = (first_pos < j_end ? first_pos : j_end) - KT;
         const int32_t masked_from = masked_from0 > j_begin ? masked_from0 : j_begin;

@@ -42,6 +42,8 @@ __device__ inline int Swizzle(int r) {
     return HD == 64 ? (((r >> 1) & 1) << 2) | ((r >> 2) & 3) : ((r & 3) << 2) | ((r >> 2) & 3);
 }
 
+constexpr float kLarge = 4096.0f;  // of a score times the factor
+
 template <typename A, typename C, int HD>
 struct TileShape {
     static constexpr int kThreads = TileRows(HD) / 32 * kWave;
@@ -220,7 +222,7 @@ __global__ __launch_bounds__((TileShape<A, C, HD>::kThreads), HD <= 128 ? 2 : 1)
         put(dst, gv);
     };
     f32x16 o[ND];
-    float mx = -INFINITY, l = 0.0f;  // of the scores times the factor; this lane's part
+    float mx = -INFINITY, l = 0.0f;  // of the scores before the factor; this lane's part
 #pragma unroll
     for (int d = 0; d < ND; ++d) {
 #pragma unroll
@@ -286,16 +288,30 @@ __global__ __launch_bounds__((TileShape<A, C, HD>::kThreads), HD <= 128 ? 2 : 1)
 #pragma unroll
             for (int r = 0; r < 16; ++r) top = fmaxf(top, sc[b][r]);
         }
-        const float mn = fmaxf(mx, Max32(top) * factor);
-        const float base = mn == -INFINITY ? 0.0f : mn;
+        const float mn = fmaxf(mx, Max32(top));
+        const float from = mn == -INFINITY ? 0.0f : mn;
         if (__ballot(mn != mx) != 0) {
-            const float alpha = __builtin_amdgcn_exp2f(mx - base);
+            const float alpha = __builtin_amdgcn_exp2f((mx - from) * factor);
             l *= alpha;
 #pragma unroll
             for (int d = 0; d < ND; ++d) o[d] *= alpha;
             mx = mn;
         }
-        const float off = static_cast<float>(P::W) - base;
+        // The weights' exponents are (score - maximum) * factor + W.  With the maximum in
+        // the addend that is one instruction a score, off by the addend's rounding: up
+        // to kLarge at most 2^-11, like the score's own.  Beyond it the difference is taken
+        // first: the largest weight is 2^W however large the scores are.
+        const float base = from * factor;
+        float off = static_cast<float>(P::W) - base;
+        if (__ballot(fabsf(base) > kLarge) != 0) {
+            off = static_cast<float>(P::W);
+#pragma unroll
+            for (int b = 0; b < NKB; ++b) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) sc[b][r] -= from;
+                asm volatile("" : "+v"(sc[b]));  // a branch, as above
+            }
+        }
         float sum[4] = {0, 0, 0, 0};
 #pragma unroll
         for (int b = 0; b < NKB; ++b) {
@@ -374,7 +390,7 @@ __global__ __launch_bounds__((TileShape<A, C, HD>::kThreads), HD <= 128 ? 2 : 1)
     const int32_t masked_from = (lo < j_end ? lo : j_end) - KT;
     const bool split = pos >= p.chunk;
     const int64_t at = split ? TilePartial(p, q.t0 + tok, h) + chunk : 0;
-    if (split && half == 0) p.part_ml[at] = make_float2(mx, l);
+    if (split && half == 0) p.part_ml[at] = make_float2(mx * factor, l);
     const float inv = split ? 1.0f : 1.0f / l;
     AB* out = static_cast<AB*>(p.out) + (static_cast<int64_t>(q.t0 + tok) * p.n_heads + h) * hd;
     float* part = p.part_o + at * hd;

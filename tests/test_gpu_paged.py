@@ -786,3 +786,48 @@ def test_mixed_batch_of_very_many_sequences(mlk, paged):
                     dev=batch.device(mlk, paged, None, 8192))
     check_paged(batch, cache, q, got, H, "bf16",
                 rows=set(range(0, 70000, 997)) | set(range(69995, 70040, 3)))
+
+
+# ------------------------------------------------------------------ large scores
+
+PLANS = {  # new tokens, lengths, workspace: which kernel, positions split or not
+    "few": ([1, 3], [300, 90], False),
+    "few split": ([1, 1, 1], [3000, 700, 20], True),
+    "tile": ([40], [190], False),
+    "tile split": ([40], [3000], True),
+    "both": ([40, 1, 1], [1200, 900, 30], True),
+}
+
+
+@pytest.mark.parametrize("act,ct", PAIRS)
+@pytest.mark.parametrize("name", list(PLANS))
+@pytest.mark.parametrize("hd,scale", [(128, None), (128, 1.0), (64, None)])
+def test_large_finite_scores(mlk, paged, hd, scale, name, act, ct):
+    """Every key alike but one per KV head, which all of q prefers by far: a token
+    before it gets the mean of V so far, the others its V row.  Equal keys give
+    bit-equal scores and the others differ by far more than a score's rounding, so
+    the error of a score, however large the scores are, is no part of the bound."""
+    H, KV = 8, 2
+    counts, lens, ws = PLANS[name]
+    rng = np.random.default_rng(31)
+    batch = Batch(counts, lens, 16, seed=2)
+    for x in (1448, 1700, 2222, 4000) if "f16" in (act, ct) else (17000, 20000, 50000, 1000000):
+        cache = Cache(mlk, paged, batch, KV, hd, ct, rng)
+        for s, n in enumerate(lens):
+            pg, r = batch.slots(s, n)
+            cache.pages(0)[pg, r] = to_type(np.float32([-x]), ct)[0]
+            for g, j in ((0, n - 1 - counts[s] // 2), (1, n // 3)):
+                cache.pages(0)[pg[j], r[j], g] = to_type(np.float32([x]), ct)[0]
+        cache.upload(mlk)
+        cache.handle = paged.PagedCache(cache.k, cache.v, ct, batch.n_pages, batch.page, KV, hd)
+        q = to_type(np.full((batch.T, H, hd), x, np.float32), act)
+        got = run_paged(mlk, paged, batch, cache, q, H, act, scale=scale, workspace=ws)
+        q64 = values(q, act).astype(np.float64)
+        for t, s, p in batch.rows():
+            if t % 3 and p + 1 < lens[s]:
+                continue
+            k, v = (a[:p + 1] for a in cache.gathered(s, lens[s]))
+            out, pav, _ = exact_rows(q64[t], k, v, scale or default_scale(hd))
+            vsum = np.repeat(np.abs(v).sum(0), H // KV, axis=0)
+            assert_close(values(got[t], act), out, pav, 0.0, p + 1, vsum, act,
+                         f"{x}: token {t} (sequence {s}, position {p})")
