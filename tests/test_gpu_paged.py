@@ -831,3 +831,97 @@ def test_large_finite_scores(mlk, paged, hd, scale, name, act, ct):
             vsum = np.repeat(np.abs(v).sum(0), H // KV, axis=0)
             assert_close(values(got[t], act), out, pav, 0.0, p + 1, vsum, act,
                          f"{x}: token {t} (sequence {s}, position {p})")
+
+
+# ------------------------------------------------------------------ wrong values where positions are split
+
+SPLITS = {  # H, KV, hd, page, new tokens, lengths, sequences that a wrong value is put into
+    "few, page 2": (8, 2, 64, 2, [1, 1, 1, 1], [3000, 700, 20, 900], [0, 1, 2]),
+    "few, page 8": (8, 2, 64, 8, [3, 1, 2, 1], [3000, 700, 20, 900], [0, 2]),
+    "few, page 16": (8, 2, 128, 16, [1, 1, 2], [2000, 1500, 1300], [1]),
+    "few, a wave a head": (16, 8, 64, 16, [1] * 40, [1700] * 40, [0, 17, 39]),
+    "few, by worker": (8, 8, 64, 16, [0 if s % 9 == 4 else 1 for s in range(700)],
+                       [1200 if s % 60 == 13 else 1 + s % 40 for s in range(700)], [13, 73, 300]),
+    "tile": (8, 2, 64, 16, [40, 60], [3000, 1500], [0, 1]),
+    "tile, page 2": (8, 2, 128, 2, [70, 0, 9], [2000, 30, 600], [0]),
+    "both": (8, 2, 64, 16, [40, 1, 1, 0, 1], [2500, 1500, 30, 20, 1100], [0, 1]),
+}
+
+
+@pytest.mark.parametrize("act,ct", [("f32", "f32"), ("f32", "f16"), ("bf16", "bf16")])
+@pytest.mark.parametrize("name", list(SPLITS))
+def test_bad_pages_and_sequences_where_positions_are_split(mlk, paged, name, act, ct):
+    """Page indexes outside the cache and sequences outside the bounds, through
+    every form of the page look-up, the division of work and the joins: the flag,
+    nothing written for a refused sequence, the others as ever."""
+    H, KV, hd, page, counts, lens, where = SPLITS[name]
+    rng = np.random.default_rng(41)
+    batch = Batch(counts, lens, page, spare=2, seed=5)
+    cache = Cache(mlk, paged, batch, KV, hd, ct, rng)
+    q = to_type(rng.standard_normal((batch.T, H, hd)), act)
+    good_table, good_lens = batch.table.copy(), list(batch.lens)
+    rows = list(batch.rows())
+    for wrong in where:
+        n = lens[wrong]
+        for what in ("first page", "middle page", "last page", "too long", "more than its length"):
+            batch.table, batch.lens = good_table.copy(), list(good_lens)
+            if what == "too long":
+                batch.lens[wrong] = max(lens) + 1
+            elif what == "more than its length":
+                batch.lens[wrong] = counts[wrong] - 1
+            else:
+                at = {"first page": 0, "middle page": (n - 1) // page // 2,
+                      "last page": (n - 1) // page}[what]
+                batch.table[wrong, at] = -7 if wrong % 2 else batch.n_pages
+            dev = batch.device(mlk, paged, max(counts), max(lens))
+            batch.table, batch.lens = good_table, good_lens
+            need = paged.attention_workspace_bytes(cache.handle, dev, H, act)
+            assert need > 0
+            ws = mlk.DeviceBuffer.from_array(np.full(need, 0xFF, np.uint8))
+            out = mlk.DeviceBuffer.from_array(np.full((batch.T, H, hd), 7, NP[act]))
+            err = mlk.DeviceBuffer.from_array(np.zeros(1, np.int32))
+            paged.attention(cache.handle, dev, mlk.DeviceBuffer.from_array(q), out, H, act,
+                            workspace=ws, err=err)
+            mlk.synchronize()
+            # (pages of a sequence without a new token are not looked at)
+            assert (err.download()[0] != 0) == (counts[wrong] > 0 or "page" not in what), what
+            got = out.download()
+            if "page" not in what:
+                assert (got[[t for t, s, p in rows if s == wrong]] == 7).all(), what
+            others = [t for t, s, p in rows if s != wrong]
+            assert (got[others] != 7).any(axis=(1, 2)).all(), what
+            check_paged(batch, cache, q, got, H, act, rows=set(others[::1 + len(others) // 9]))
+
+
+@pytest.mark.parametrize("act,ct", PAIRS)
+@pytest.mark.parametrize("name", ["few, page 8", "few, a wave a head", "tile", "tile, page 2", "both"])
+def test_non_finite_values_where_positions_are_split(mlk, paged, name, act, ct):
+    """A non-finite V or K, met in a fully or partly masked tile of one part of a
+    row: the rows that attend to it non-finite in its dims, all others as without."""
+    H, KV, hd, page, counts, lens, _ = SPLITS[name]
+    rng = np.random.default_rng(43)
+    counts = [3] * len(counts) if name == "few, a wave a head" else counts
+    batch = Batch(counts, lens, page, seed=6)
+    cache = Cache(mlk, paged, batch, KV, hd, ct, rng)
+    q = to_type(rng.standard_normal((batch.T, H, hd)), act)
+    good = [a.copy() for a in cache.host]
+    n, c = lens[0], counts[0]
+    pg, r = batch.slots(0, n)
+    for pos in (n - 2, n - c // 2 - 1, n - c - 1, n // 2, 257, 0):
+        for which, value in ((1, np.inf), (1, -np.inf), (1, np.nan), (0, np.nan)):
+            dims = slice(hd // 2, hd // 2 + 3) if which else slice(0, hd)
+            cache.host = [a.copy() for a in good]
+            cache.pages(which)[pg[pos], r[pos], 1, dims] = to_type(np.float32([value]), ct)[0]
+            cache.upload(mlk)
+            cache.handle = paged.PagedCache(cache.k, cache.v, ct, batch.n_pages, batch.page, KV, hd)
+            got = run_paged(mlk, paged, batch, cache, q, H, act)
+            what = f"position {pos}, {'KV'[which]} {value}"
+            g = values(got, act).reshape(batch.T, KV, H // KV, hd)
+            first = n - c  # token row t of sequence 0 is at position first + t
+            sees = [t for t in range(c) if first + t >= pos]
+            assert not np.isfinite(g[sees, 1][..., dims]).any(), what
+            g = g.copy()
+            g[sees, 1, :, dims] = 0
+            assert np.isfinite(g).all(), what
+            others = [t for t, s, p in batch.rows() if s != 0 or p < pos]
+            check_paged(batch, cache, q, got, H, act, rows=set(others[-7:] + others[:2]))
