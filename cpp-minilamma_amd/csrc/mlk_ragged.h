@@ -239,6 +239,8 @@ struct RaggedParams {
     // few-row kernel: workgroups (0: one per sequence and KV head), and the most KV
     // heads a workgroup's waves may take side by side
     int32_t workers, few_heads;
+    // sequences or row tiles that earlier launches of the call have taken
+    int64_t taken;
     // partial results (maximum and sum of a row's part, then its weighted rows)
     // where a row has more than one part
     float2* part_ml;
@@ -258,9 +260,9 @@ constexpr int kFewHeads = 8;   // most KV heads of its workgroup
 // Launches on `stream`; type and cache_type choose the instance.
 // Waves of a few-row workgroup: 8, or 4 where the registers of 8 would not do.
 inline int FewWaves(int head_dim, int few_rows) { return head_dim <= 128 && few_rows <= 16 ? 8 : 4; }
-// Most workgroups of a launch (512 threads each, below 2^32 in all).
-constexpr int64_t kMaxBlocks = 1 << 22;
-int64_t FewBlocks(const RaggedParams& p);
+// Most workgroups of a launch (512 threads each, below 2^32 in all), and of a call:
+// what is not split goes over as many launches as it takes.
+constexpr int64_t kMaxBlocks = 1 << 22, kMaxCallBlocks = int64_t{1} << 35;
 int64_t TileBlocks(const RaggedParams& p);
 mlk_status LaunchFew(const RaggedParams& p, int32_t type, int32_t cache_type, hipStream_t stream);
 // Rows of a tile: 8 waves' 32 each, 4 waves' where a row's results take twice the

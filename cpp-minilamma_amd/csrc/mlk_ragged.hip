@@ -376,19 +376,19 @@ mlk_status Attend(const AttendArgs& a) {
         few.workers = static_cast<int32_t>(plan.few_workers);
         few.few_heads = FewWaves(hd, few.few_rows);
         while (a.n_kv_heads % few.few_heads != 0) few.few_heads /= 2;
+        if (few.workers > 0 && JoinFewBlocks(few) > kMaxBlocks) few.workers = 0;  // thousands of heads: no split
         if (few.workers > 0) place(plan.few_partials, &few);
-        blocks = FewBlocks(few);
-        if (few.workers > 0) blocks = Larger(blocks, JoinFewBlocks(few));
+        blocks = static_cast<int64_t>(b.n_seqs) * a.n_kv_heads;
     }
     if (plan.tile) {
         tile.chunk = static_cast<int32_t>(plan.chunk);
         tile.n_chunks = static_cast<int32_t>(plan.n_chunks);
         if (tile.n_chunks > 1) place(plan.tile_partials, &tile);
-        blocks = Larger(blocks, TileBlocks(tile));
-        if (tile.n_chunks > 1) blocks = Larger(blocks, JoinTileBlocks(tile));
+        blocks = Larger(blocks, TileBlocks(tile) / tile.n_chunks);
     }
-    if (blocks > kMaxBlocks) {
-        return Fail(MLK_ERR_INVALID, "attention: %lld workgroups exceed a launch's 2^22",
+    // (depends neither on the lengths nor on the workspace)
+    if (blocks > kMaxCallBlocks) {
+        return Fail(MLK_ERR_INVALID, "attention: %lld workgroups exceed a call's 2^35",
                     static_cast<long long>(blocks));
     }
     if (plan.few_rows > 0) {

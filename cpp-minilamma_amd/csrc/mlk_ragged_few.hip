@@ -118,12 +118,12 @@ __global__ __launch_bounds__(kWaves * kWave) void AttnFew(const RaggedParams p) 
     const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
     const int i16 = lane % 16, g4 = lane / 16;
     const int hd = kLie == kFull ? HD : p.rows.head_dim;
-    if (blockIdx.x == 0) CheckSeqs(p.batch, p.err);
+    if (blockIdx.x == 0 && p.taken == 0) CheckSeqs(p.batch, p.err);
     FewWork work;
     int64_t unit, end;  // this worker's units
     if (p.workers == 0) {
         work.heads = 1;
-        work.s = static_cast<int>(blockIdx.x / p.n_kv_heads);
+        work.s = static_cast<int>(p.taken + blockIdx.x / p.n_kv_heads);
         work.units = FewUnits(p, work.s);
         work.before = 0;
         unit = static_cast<int64_t>(blockIdx.x % p.n_kv_heads) * work.units;
@@ -583,13 +583,19 @@ struct ByDim {
 
 }  // namespace
 
-int64_t FewBlocks(const RaggedParams& p) {
-    return p.workers != 0 ? p.workers : static_cast<int64_t>(p.batch.n_seqs) * p.n_kv_heads;
-}
-
 mlk_status LaunchFew(const RaggedParams& p, int32_t type, int32_t cache_type, hipStream_t stream) {
-    const dim3 grid(static_cast<unsigned>(FewBlocks(p)));
-    return ByType(type, cache_type, ByDim{p, grid, stream});
+    if (p.workers != 0) {
+        return ByType(type, cache_type, ByDim{p, dim3(static_cast<unsigned>(p.workers)), stream});
+    }
+    RaggedParams part = p;
+    const int64_t most = kMaxBlocks / p.n_kv_heads;  // sequences of a launch
+    mlk_status st = MLK_OK;
+    for (part.taken = 0; part.taken < p.batch.n_seqs && st == MLK_OK; part.taken += most) {
+        const int64_t left = p.batch.n_seqs - part.taken;
+        const dim3 grid(static_cast<unsigned>((left < most ? left : most) * p.n_kv_heads));
+        st = ByType(type, cache_type, ByDim{part, grid, stream});
+    }
+    return st;
 }
 
 }  // namespace mlk

@@ -56,7 +56,7 @@ struct TileShape {
 };
 
 template <typename A, typename C, int HD, Lie kLie>
-__global__ __launch_bounds__((TileShape<A, C, HD>::kThreads), HD <= 128 ? 2 : 1) void AttnTile(const RaggedParams p, int n_slots) {
+__global__ __launch_bounds__((TileShape<A, C, HD>::kThreads), HD <= 128 ? 2 : 1) void AttnTile(const RaggedParams p, int64_t n_slots) {
     typedef Pieces<A, C> P;
     typedef typename P::M M;
     typedef TileShape<A, C, HD> T;
@@ -73,13 +73,13 @@ __global__ __launch_bounds__((TileShape<A, C, HD>::kThreads), HD <= 128 ? 2 : 1)
     const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
     const int l32 = lane % 32, half = lane / 32;
     const int hd = kLie == kFull ? HD : p.rows.head_dim;
-    if (blockIdx.x == 0) CheckSeqs(p.batch, p.err);
+    if (blockIdx.x == 0 && p.taken == 0) CheckSeqs(p.batch, p.err);
 
     const int kvh = static_cast<int>(blockIdx.x % p.n_kv_heads);
     const int64_t rest = blockIdx.x / p.n_kv_heads;
     const int chunk = static_cast<int>(rest % p.n_chunks);
     // the longest prefixes first
-    const int64_t slot = n_slots - 1 - rest / p.n_chunks;
+    const int64_t slot = n_slots - 1 - p.taken - rest / p.n_chunks;
     const int group = p.group;
     auto first_slot = [group](int32_t start, int s) {
         return static_cast<int64_t>(start) * group / kRows + s;
@@ -440,7 +440,7 @@ __global__ __launch_bounds__((TileShape<A, C, HD>::kThreads), HD <= 128 ? 2 : 1)
 }
 
 template <typename A, typename C, int HD>
-mlk_status Launch(const RaggedParams& p, dim3 grid, int n_slots, hipStream_t s) {
+mlk_status Launch(const RaggedParams& p, dim3 grid, int64_t n_slots, hipStream_t s) {
     constexpr int kThreads = TileShape<A, C, HD>::kThreads;
     const dim3 block(kThreads);
     switch (LieOf(p, HD)) {
@@ -454,7 +454,7 @@ mlk_status Launch(const RaggedParams& p, dim3 grid, int n_slots, hipStream_t s) 
 struct ByDim {
     const RaggedParams& p;
     dim3 grid;
-    int n_slots;
+    int64_t n_slots;
     hipStream_t stream;
     template <typename A, typename C>
     mlk_status Run() const {
@@ -480,8 +480,16 @@ int64_t TileBlocks(const RaggedParams& p) {
 mlk_status LaunchTile(const RaggedParams& p, int32_t type, int32_t cache_type, hipStream_t stream) {
     const int64_t slots = TileSlots(p.batch.n_seqs, p.batch.n_tokens, p.group,
                                     TileRows(p.rows.head_dim));
-    const dim3 grid(static_cast<unsigned>(TileBlocks(p)));
-    return ByType(type, cache_type, ByDim{p, grid, static_cast<int>(slots), stream});
+    RaggedParams part = p;
+    const int64_t per_slot = static_cast<int64_t>(p.n_chunks) * p.n_kv_heads;
+    const int64_t most = kMaxBlocks / per_slot;  // row tiles of a launch
+    mlk_status st = MLK_OK;
+    for (part.taken = 0; part.taken < slots && st == MLK_OK; part.taken += most) {
+        const int64_t here = slots - part.taken < most ? slots - part.taken : most;
+        const dim3 grid(static_cast<unsigned>(here * per_slot));
+        st = ByType(type, cache_type, ByDim{part, grid, slots, stream});
+    }
+    return st;
 }
 
 }  // namespace mlk

@@ -365,8 +365,10 @@ typedef struct {
  * (rows behind token_start[n_seqs] are neither read nor written), no sequence
  * brings over max_new_tokens, none is longer than max_seq_len
  * (<= table_stride * page_size; n_seqs up to 2^20, n_tokens up to 2^23; an
- * attention call over 2^22 workgroups, of the order of n_seqs * n_kv_heads, is
- * refused).  A sequence outside these bounds, or with more new tokens than its
+ * attention call of over 2^35 workgroups is refused, whatever its lengths and
+ * workspace: n_seqs * n_kv_heads, or, where some sequence may bring more than 32
+ * (new token, query head of a KV head) rows, 16 past head_dim 128, n_kv_heads for
+ * every 256 rows, 128 past head_dim 128, and every sequence).  A sequence outside these bounds, or with more new tokens than its
  * length, raises *err (NULL: no report; the caller clears it) and gets nothing
  * written. */
 typedef struct {

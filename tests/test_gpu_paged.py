@@ -925,3 +925,35 @@ def test_non_finite_values_where_positions_are_split(mlk, paged, name, act, ct):
             assert np.isfinite(g).all(), what
             others = [t for t, s, p in batch.rows() if s != 0 or p < pos]
             check_paged(batch, cache, q, got, H, act, rows=set(others[-7:] + others[:2]))
+
+
+# ------------------------------------------------------------------ more workgroups than a launch takes
+
+@pytest.mark.parametrize("chunk,max_len,workspace", [(1, 512, True), (1, 513, True), (1, 513, False),
+                                                     (40, 512, True), (40, 513, False)])
+def test_more_workgroups_than_a_launch(mlk, paged, chunk, max_len, workspace):
+    """600000 sequences at 8 KV heads, 4.8 million (sequence, head) pairs, on two
+    shared pages: run whether the lengths' bound lets them be split or not, with and
+    without a workspace, with one token each and beside a chunk."""
+    H, KV, hd, n = 8, 8, 8, 600000
+    rng = np.random.default_rng(51)
+    lens = rng.integers(1, 6, n)
+    counts = np.ones(n, int)
+    lens[n // 2], counts[n // 2] = 500, chunk
+    batch = Batch([1], [1024], 1024)
+    batch.counts, batch.lens = counts.tolist(), lens.tolist()
+    batch.start = np.concatenate([[0], np.cumsum(counts)]).astype(np.int32)
+    batch.T, batch.n_pages = int(batch.start[-1]), 2
+    batch.table = (np.arange(n) % 2).astype(np.int32).reshape(n, 1)
+    cache = Cache(mlk, paged, batch, KV, hd, "bf16", rng, fill=False)
+    for i in range(2):
+        cache.host[i] = to_type(rng.standard_normal(cache.host[i].shape), "bf16")
+    cache.upload(mlk)
+    cache.handle = paged.PagedCache(cache.k, cache.v, "bf16", 2, 1024, KV, hd)
+    q = to_type(rng.standard_normal((batch.T, H, hd)), "bf16")
+    got = run_paged(mlk, paged, batch, cache, q, H, "bf16", workspace=workspace,
+                    dev=batch.device(mlk, paged, chunk, max_len))
+    assert (got != 7).any(axis=(1, 2)).all()
+    at = int(batch.start[n // 2])
+    check_paged(batch, cache, q, got, H, "bf16",
+                rows=set(range(0, n, 4999)) | set(range(524280, 524296)) | {at, batch.T - 1})
