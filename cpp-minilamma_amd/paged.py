@@ -12,7 +12,8 @@ A step of a server:
     attention(cache, batch, q_rot, out, H, "f32", workspace=ws)
 
 Types are "f32", "f16" or "bf16"; buffers are DeviceBuffers or device
-addresses.  include/minilamma_hip.h documents layouts and semantics.
+addresses (a workspace's address needs workspace_bytes).
+include/minilamma_hip.h documents layouts and semantics.
 """
 from __future__ import annotations
 
@@ -148,4 +149,8 @@ def _scale(scale, head_dim):
 def _ws_bytes(workspace, nbytes):
     if nbytes is not None:
         return nbytes
-    return getattr(workspace, "nbytes", 0) if workspace is not None else 0
+    if not _p(workspace):
+        return 0
+    if not hasattr(workspace, "nbytes"):
+        raise ValueError("a workspace given as an address needs workspace_bytes")
+    return workspace.nbytes

@@ -177,3 +177,31 @@ def test_many_sequences_are_not_split_beyond_a_launch(mlk, paged):
     remain (2 parts of 512 workgroups at most, 8 heads, 16 rows)."""
     size = mlk.lib.mlk_attention_paged_workspace_bytes
     assert 0 < size(300000, 300100, 100, 8192, 64, 8, 128) <= 2 * 512 * 8 * 16 * (128 * 4 + 8) + 512
+
+
+def test_bounds_on_counts_are_those_documented(mlk, paged):
+    """One more than 2^23 tokens or 2^20 sequences, through every entry."""
+    for kw in (dict(n_tokens=2 ** 23 + 1), dict(n_seqs=2 ** 20 + 1)):
+        cache, batch = make(paged, **kw)
+        with pytest.raises(mlk.MlkError, match="n_seqs must be"):
+            paged.attention(cache, batch, 3 * FAKE, 4 * FAKE, 4, "f16")
+        with pytest.raises(mlk.MlkError, match="n_seqs must be"):
+            paged.kv_append(cache, batch, 3 * FAKE, 4 * FAKE, "f16")
+        with pytest.raises(mlk.MlkError, match="n_seqs must be"):
+            paged.attention_packed("f16", FAKE, 2 * FAKE, 3 * FAKE, 4 * FAKE, kw.get("n_seqs", 1),
+                                   kw.get("n_tokens", 1), 5, 4, 2, 8, 5 * FAKE)
+
+
+def test_a_workspace_address_needs_its_size(mlk, paged):
+    """A workspace given as an address has no size of its own: without
+    workspace_bytes it would go unused."""
+    cache, batch = make(paged, n_seqs=0)
+    for kw in (dict(workspace=16 * FAKE), dict(workspace=16 * FAKE, workspace_bytes=None)):
+        with pytest.raises(ValueError, match="workspace_bytes"):
+            paged.attention(cache, batch, 3 * FAKE, 4 * FAKE, 4, "f16", **kw)
+        with pytest.raises(ValueError, match="workspace_bytes"):
+            paged.attention_packed("f16", FAKE, 2 * FAKE, 3 * FAKE, 4 * FAKE, 0, 1, 5, 4, 2, 8,
+                                   5 * FAKE, **kw)
+    paged.attention(cache, batch, 3 * FAKE, 4 * FAKE, 4, "f16", workspace=16 * FAKE,
+                    workspace_bytes=0)
+    paged.attention(cache, batch, 3 * FAKE, 4 * FAKE, 4, "f16")
