@@ -12,7 +12,12 @@
 //   bf16 K, V: 3 bf16 pieces, exact (8 + 8 + 8 bits).
 //   fp32 K, V: 3 x 3 bf16 pieces, the 6 products above 2^-21 of q k (the three
 //     dropped ones are below 2^-20).
-// 16-bit q needs no split; its w is rounded to q's type (fp16: scaled as above).
+// 16-bit q needs no split.  Its w (fp16: scaled as above) is two pieces of its type in
+// the few-row kernel, within 2^-15 of it (fp16 2^-20): bound by bytes, that costs
+// nothing there (64 bf16 decode rows of the 8B heads 190 us either way).  In the tile
+// kernel w is rounded to q's type: the second piece's products would take 657 to 836 us
+// (9001 packed bf16 tokens of the 70B heads), and over values of either sign the
+// weights' roundings add about a quarter to the error of the result's own.
 #pragma once
 
 #include "mlk_paged.h"
@@ -54,7 +59,7 @@ struct MmaBf {
         } else {
 #pragma unroll
             for (int i = 0; i < N; ++i) {
-                o[i] = PackBf(a, b);
+                o[i] = i + 1 < N ? PackBf(a, b) : Round2(a, b);
                 if (i + 1 < N) {
                     a -= __uint_as_float(__float_as_uint(a) & 0xFFFF0000u);
                     b -= __uint_as_float(__float_as_uint(b) & 0xFFFF0000u);
@@ -92,38 +97,39 @@ struct MmaF16 {
     }
 };
 
-// How activations of type A meet a cache of type C: NQ pieces of q and w, NK of
-// K and V; W: w's scale, a power of two; kScaleQ: q scaled per row.
+// How activations of type A meet a cache of type C: NQ pieces of q (and of w in the
+// tile kernel), NK of K and V, NW of w in the few-row kernel; W: w's scale, a power
+// of two; kScaleQ: q scaled per row.
 template <typename A, typename C>
 struct Pieces;
 template <>
 struct Pieces<BF16, BF16> {
     typedef MmaBf M;
-    static constexpr int NQ = 1, NK = 1, W = 0;
+    static constexpr int NQ = 1, NK = 1, NW = 2, W = 0;
     static constexpr bool kScaleQ = false;
 };
 template <>
 struct Pieces<F16, F16> {
     typedef MmaF16 M;
-    static constexpr int NQ = 1, NK = 1, W = 14;
+    static constexpr int NQ = 1, NK = 1, NW = 2, W = 14;
     static constexpr bool kScaleQ = false;
 };
 template <>
 struct Pieces<F32, F16> {
     typedef MmaF16 M;
-    static constexpr int NQ = 2, NK = 1, W = 14;
+    static constexpr int NQ = 2, NK = 1, NW = 2, W = 14;
     static constexpr bool kScaleQ = true;
 };
 template <>
 struct Pieces<F32, BF16> {
     typedef MmaBf M;
-    static constexpr int NQ = 3, NK = 1, W = 0;
+    static constexpr int NQ = 3, NK = 1, NW = 3, W = 0;
     static constexpr bool kScaleQ = false;
 };
 template <>
 struct Pieces<F32, F32> {
     typedef MmaBf M;
-    static constexpr int NQ = 3, NK = 3, W = 0;
+    static constexpr int NQ = 3, NK = 3, NW = 3, W = 0;
     static constexpr bool kScaleQ = false;
 };
 

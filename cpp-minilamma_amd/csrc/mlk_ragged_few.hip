@@ -41,11 +41,21 @@
 namespace mlk {
 namespace {
 
+typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+
 __device__ inline uint32_t LowHalves(uint32_t a, uint32_t b) {
     return __builtin_amdgcn_perm(b, a, 0x05040100u);
 }
 __device__ inline uint32_t HighHalves(uint32_t a, uint32_t b) {
     return __builtin_amdgcn_perm(b, a, 0x07060302u);
+}
+
+// Per half: the larger of x and min(y, least).
+__device__ inline uint32_t AtLeast(uint32_t x, uint32_t y, uint16_t least) {
+    const u16x2 a = __builtin_bit_cast(u16x2, x), b = __builtin_bit_cast(u16x2, y);
+    const u16x2 c = {least, least};
+    return __builtin_bit_cast(uint32_t,
+                              __builtin_elementwise_max(a, __builtin_elementwise_min(b, c)));
 }
 
 // K and V operands of one tile in registers, and their loads.
@@ -108,7 +118,7 @@ __global__ __launch_bounds__(kWaves * kWave) void AttnFew(const RaggedParams p) 
     typedef typename A::Bits AB;
     constexpr bool kF32 = Tile::kF32;
     constexpr int KT = Tile::KT, NBK = Tile::NBK, NI = HD / 16;
-    constexpr int NQ = kF32 ? 1 : P::NQ;
+    constexpr int NQ = kF32 ? 1 : P::NQ, NW = P::NW;
     constexpr float kW = kF32 ? 0.0f : static_cast<float>(P::W);
     constexpr int kOLd = HD + 4;  // row stride of a wave's results in shared memory
     __shared__ float so[kWaves][16 * NB][kOLd];
@@ -417,9 +427,20 @@ __global__ __launch_bounds__(kWaves * kWave) void AttnFew(const RaggedParams p) 
                     }
                 }
             } else {
-                u32x4 wp[NB][NQ];
+                u32x4 wp[NB][NW];
 #pragma unroll
-                for (int nb = 0; nb < NB; ++nb) Split8<M, NQ>(w[nb], wp[nb]);
+                for (int nb = 0; nb < NB; ++nb) {
+                    Split8<M, NW>(w[nb], wp[nb]);
+                    if constexpr (sizeof(AB) == 2) {
+                        // no second piece 0 beside a first that is not: an infinity in V
+                        // stays one (0 * inf is NaN)
+                        constexpr uint16_t kLeast = C::kType == MLK_F16 ? 0x0001 : 0x0080;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            wp[nb][1][i] = AtLeast(wp[nb][1][i], wp[nb][0][i], kLeast);
+                        }
+                    }
+                }
 #pragma unroll
                 for (int e = 0; e < NI; ++e) {
                     u32x4 a;  // the e-th dim of each of the lane's positions
@@ -431,7 +452,7 @@ __global__ __launch_bounds__(kWaves * kWave) void AttnFew(const RaggedParams p) 
 #pragma unroll
                     for (int nb = 0; nb < NB; ++nb) {
 #pragma unroll
-                        for (int n = 0; n < NQ; ++n) o[nb][e] = M::Mma16(a, wp[nb][n], o[nb][e]);
+                        for (int n = 0; n < NW; ++n) o[nb][e] = M::Mma16(a, wp[nb][n], o[nb][e]);
                     }
                 }
             }

@@ -409,7 +409,10 @@ mlk_status mlk_paged_kv_append(const mlk_paged_cache* cache, const mlk_paged_bat
  * statistics and sums are fp32.  With fp32 activations q and w enter the
  * products in enough 16-bit pieces that each product is within 2^-20 of itself
  * (over an fp16 cache, for values 2^17 below their row's largest, within 2^-38 of
- * that one); with 16-bit ones w is rounded to that type.  What a token does not
+ * that one).  With 16-bit ones q is exact; w is two pieces of that type, within
+ * 2^-15 of it (fp16: 2^-20, or 2^-37 of the row's largest), for sequences of up to
+ * 32 (new token, query head of a KV head) rows, 16 past head_dim 128 and where a
+ * call has longer chunks too, and otherwise may be rounded to that type.  What a token does not
  * attend to (later positions, the rest of the last page) never changes its
  * result, whatever bits lie there; a token that attends to a non-finite value
  * gets non-finite results (of 16-bit activations: an infinity in V as such, and

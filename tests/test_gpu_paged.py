@@ -957,3 +957,74 @@ def test_more_workgroups_than_a_launch(mlk, paged, chunk, max_len, workspace):
     at = int(batch.start[n // 2])
     check_paged(batch, cache, q, got, H, "bf16",
                 rows=set(range(0, n, 4999)) | set(range(524280, 524296)) | {at, batch.T - 1})
+
+
+# ------------------------------------------------------------------ few rows: weights of 16-bit activations
+
+FEW = {  # new tokens, lengths, workspace; 8 KV heads over many sequences: a wave to a head
+    "one": ([1, 2, 1], [24, 300, 33], 2, False),
+    "split": ([1, 1, 2], [40, 2000, 700], 2, True),
+    "a wave a head": ([1] * 40, [700] * 40, 8, True),
+}
+
+
+@pytest.mark.parametrize("act", ["f16", "bf16"])
+@pytest.mark.parametrize("name", list(FEW))
+@pytest.mark.parametrize("hd", [64, 128])
+def test_few_rows_keep_the_weights_of_16_bit_activations(mlk, paged, hd, name, act):
+    """Scores that are exact (whole numbers times a power of two), so that what is
+    left is the weights' precision: two pieces, 2^-15 of a weight (bf16), 2^-20 and
+    2^-37 of the largest (fp16), not one rounding to the type (2^-9, 2^-12).  The
+    rest as in paged_cases.py: exp, sum and division (n + 54) u, the result's own
+    rounding."""
+    counts, lens, KV, ws = FEW[name]
+    H = 2 * KV
+    rng = np.random.default_rng(61)
+    batch = Batch(counts, lens, 16, seed=8)
+    cache = Cache(mlk, paged, batch, KV, hd, act, rng)
+    for s, n in enumerate(lens):
+        pg, r = batch.slots(s, n)
+        cache.pages(0)[pg, r] = to_type(rng.integers(-1, 2, (n, KV, hd)), act)
+    cache.upload(mlk)
+    cache.handle = paged.PagedCache(cache.k, cache.v, act, batch.n_pages, batch.page, KV, hd)
+    q = to_type(rng.choice([-1.0, 1.0], (batch.T, H, hd)), act)
+    got = values(run_paged(mlk, paged, batch, cache, q, H, act, scale=1 / 16, workspace=ws), act)
+    e, least = (2.0 ** -15, 0.0) if act == "bf16" else (2.0 ** -20, 2.0 ** -37)
+    half, tiny = 2.0 ** -8 if act == "bf16" else 2.0 ** -11, 2.0 ** -25 if act == "f16" else 0.0
+    for t, s, p in batch.rows():
+        if t % 5 and s < len(lens) - 1:
+            continue
+        k, v = (a[:p + 1] for a in cache.gathered(s, lens[s]))
+        out, pav, _ = exact_rows(values(q[t], act).astype(np.float64), k, v, 1 / 16)
+        vsum = np.repeat(np.abs(v).sum(0), H // KV, axis=0)
+        bound = ((p + 55) * 2.0 ** -24 + e) * pav + least * vsum
+        bound = bound + half * (np.abs(out) + bound) + tiny
+        err = np.abs(got[t].astype(np.float64) - out)
+        assert (err <= bound).all(), (f"token {t}: {int((err > bound).sum())} of {err.size}, "
+                                      f"{float((err / bound).max()):.2f} of the bound")
+
+
+@pytest.mark.parametrize("act", ["f16", "bf16"])
+@pytest.mark.parametrize("name", list(FEW))
+@pytest.mark.parametrize("value", [np.inf, -np.inf])
+@pytest.mark.parametrize("equal", [False, True])
+def test_few_rows_keep_an_infinity(mlk, paged, equal, value, name, act):
+    """An infinity in V in a tile that every row attends to, of 16-bit activations:
+    itself, also where the weights are powers of two."""
+    counts, lens, KV, ws = FEW[name]
+    H, hd = 2 * KV, 64
+    rng = np.random.default_rng(62)
+    batch = Batch(counts, lens, 16, seed=9)
+    cache = Cache(mlk, paged, batch, KV, hd, act, rng)
+    pg, r = batch.slots(1, lens[1])
+    for pos in (3, lens[1] // 2):
+        cache.pages(1)[pg[pos], r[pos], 1, 7 + pos % 2] = to_type(np.float32([value]), act)[0]
+    cache.upload(mlk)
+    cache.handle = paged.PagedCache(cache.k, cache.v, act, batch.n_pages, batch.page, KV, hd)
+    q = to_type(rng.standard_normal((batch.T, H, hd)) * (0 if equal else 1), act)
+    got = values(run_paged(mlk, paged, batch, cache, q, H, act, workspace=ws), act)
+    rows = slice(int(batch.start[1]), int(batch.start[2]))
+    hit = np.zeros(got.shape, bool)
+    for pos in (3, lens[1] // 2):
+        hit[rows, 2:4, 7 + pos % 2] = True
+    assert (got[hit] == value).all() and np.isfinite(got[~hit]).all()
