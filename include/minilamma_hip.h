@@ -364,13 +364,16 @@ typedef struct {
  * replays with new values within the host's bounds: n_tokens token rows exist
  * (rows behind token_start[n_seqs] are neither read nor written), no sequence
  * brings over max_new_tokens, none is longer than max_seq_len
- * (<= table_stride * page_size; n_seqs up to 2^20, n_tokens up to 2^23; an
- * attention call of over 2^35 workgroups is refused, whatever its lengths and
- * workspace: n_seqs * n_kv_heads, or, where some sequence may bring more than 32
- * (new token, query head of a KV head) rows, 16 past head_dim 128, n_kv_heads for
- * every 256 rows, 128 past head_dim 128, and every sequence).  A sequence outside these bounds, or with more new tokens than its
- * length, raises *err (NULL: no report; the caller clears it) and gets nothing
- * written. */
+ * (<= table_stride * page_size; n_seqs up to 2^20, n_tokens up to 2^23).  How an
+ * attention call divides its work follows from these bounds too: bounds far above
+ * what comes cost time, results are right with any.  A call of over 2^35
+ * workgroups is refused, whatever its lengths and workspace: n_seqs * n_kv_heads,
+ * or, where some sequence may bring more than 32 (new token, query head of a KV
+ * head) rows (16 past head_dim 128), n_kv_heads for every sequence and every 256
+ * (128) such rows.  A sequence outside these bounds, or with more new tokens than
+ * its length, raises *err (NULL: no report; the caller clears it) and gets nothing
+ * written.  Where token_start decreases, *err is raised and what the other
+ * sequences get is not defined (their rows alone are written). */
 typedef struct {
     const int32_t* token_start;  /* device [n_seqs + 1] */
     const int32_t* seq_len;      /* device [n_seqs] */
@@ -384,9 +387,9 @@ typedef struct {
  * where q is not NULL, q (n_heads * head_dim elements a row) rotated into q_out
  * (of the same type; q_out == q with equal strides rotates in place, otherwise
  * the two do not overlap).  The rotation is mlk_rope_f32's: angles, cos and sin
- * in float64, each result rounded once to the type it is stored in.  theta == 0:
- * k is stored as it is, and q must be NULL.  k and v are only read.  Every
- * position written belongs to one sequence of the batch (pages shared between
+ * in float64, each result rounded to float and, where it is stored in 16 bits,
+ * from there to that type.  theta == 0: k is stored as it is, and q must be NULL.
+ * k and v are only read.  Every position written belongs to one sequence of the batch (pages shared between
  * sequences may be read by mlk_attention_paged, not appended to).  A page index
  * outside [0, n_pages) raises *err and its row is not written.  head_dim 1..256,
  * even where theta != 0.
@@ -412,12 +415,15 @@ mlk_status mlk_paged_kv_append(const mlk_paged_cache* cache, const mlk_paged_bat
  * that one).  With 16-bit ones q is exact; w is two pieces of that type, within
  * 2^-15 of it (fp16: 2^-20, or 2^-37 of the row's largest), for sequences of up to
  * 32 (new token, query head of a KV head) rows, 16 past head_dim 128 and where a
- * call has longer chunks too, and otherwise may be rounded to that type.  What a token does not
- * attend to (later positions, the rest of the last page) never changes its
- * result, whatever bits lie there; a token that attends to a non-finite value
- * gets non-finite results (of 16-bit activations: an infinity in V as such, and
- * a position whose score comes out as -infinity may count as weight 0 instead).
- * A page index outside [0, n_pages) raises *err and page 0 is read in its place.
+ * call has longer chunks too, and otherwise may be rounded to that type.  What a
+ * token does not attend to (later positions, the rest of the last page) never
+ * changes its result, whatever bits lie there.  A token that attends to a non-finite element
+ * of V gets a non-finite result in that dim (an infinity as itself or, with fp32
+ * activations or where the position's weight comes out as 0, NaN).  A score that
+ * comes out as -infinity is weight 0; +infinity or NaN makes all of that head's
+ * results NaN, as do scores that are all -infinity.  Scores, and the sums of |V|
+ * over the positions, have to stay within fp32's range.  A page index outside
+ * [0, n_pages) raises *err and page 0 is read in its place.
  *
  * workspace: optional scratch (16-byte aligned,
  * mlk_attention_paged_workspace_bytes(); it may differ between calls, its
@@ -441,7 +447,7 @@ int64_t mlk_attention_paged_workspace_bytes(int64_t n_seqs, int64_t n_tokens,
  * token rows seq_start[s] .. seq_start[s + 1] - 1 (device [n_seqs + 1],
  * non-decreasing; empty sequences are allowed), and each row attends to its
  * own sequence's rows up to itself, as mlk_attention_paged does over pages, with
- * the same semantics and precision.  q, k, v (rows q_row_stride, k_row_stride,
+ * the same semantics and precision (seq_start decreasing: as token_start there).  q, k, v (rows q_row_stride, k_row_stride,
  * v_row_stride elements apart, k's and v's at most 2^27: slices of one fused
  * projection are fine) and out
  * (dense) are of `type`.  Rows behind seq_start[n_seqs] are neither read nor

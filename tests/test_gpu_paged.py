@@ -1028,3 +1028,45 @@ def test_few_rows_keep_an_infinity(mlk, paged, equal, value, name, act):
     for pos in (3, lens[1] // 2):
         hit[rows, 2:4, 7 + pos % 2] = True
     assert (got[hit] == value).all() and np.isfinite(got[~hit]).all()
+
+
+@pytest.mark.parametrize("act,ct", [("f16", "f16"), ("bf16", "bf16")])
+@pytest.mark.parametrize("name", list(PLANS))
+def test_infinite_scores(mlk, paged, name, act, ct):
+    """A score of -infinity is weight 0, one of +infinity makes the head's results
+    NaN; of the KV head and the tokens that meet it, no others."""
+    H, KV, hd = 8, 2, 128
+    counts, lens, ws = PLANS[name]
+    rng = np.random.default_rng(71)
+    batch = Batch(counts, lens, 16, seed=4)
+    cache = Cache(mlk, paged, batch, KV, hd, ct, rng)
+    x = rng.standard_normal((batch.T, H, hd))
+    x[..., 5] = 1.0
+    q = to_type(x, act)
+    q64 = values(q, act).astype(np.float64)
+    n, c = lens[0], counts[0]
+    pg, r = batch.slots(0, n)
+    good = [a.copy() for a in cache.host]
+    for pos in (n - c // 2 - 1, n // 3):
+        for value in (-np.inf, np.inf):
+            cache.host = [a.copy() for a in good]
+            cache.pages(0)[pg[pos], r[pos], 1, 5] = to_type(np.float32([value]), ct)[0]
+            cache.upload(mlk)
+            cache.handle = paged.PagedCache(cache.k, cache.v, ct, batch.n_pages, batch.page, KV, hd)
+            got = run_paged(mlk, paged, batch, cache, q, H, act, workspace=ws)
+            g = values(got, act).reshape(batch.T, KV, H // KV, hd)
+            sees = [t for t, s, p in batch.rows() if s == 0 and p >= pos]
+            others = [t for t, s, p in batch.rows() if s != 0 or p < pos]
+            check_paged(batch, cache, q, got, H, act, rows=set(others[-5:]))
+            assert np.isfinite(g[:, 0]).all() and np.isfinite(g[others]).all()
+            if value > 0:
+                assert np.isnan(g[sees, 1]).all()
+                continue
+            k, v = cache.gathered(0, n)
+            for t in sees[::1 + len(sees) // 6]:
+                keep = np.delete(np.arange(n - c + t + 1), pos)
+                kk, vv = k[keep][:, 1:], v[keep][:, 1:]
+                out, pav, d = exact_rows(q64[t, H // 2:], kk, vv, default_scale(hd))
+                vsum = np.repeat(np.abs(vv).sum(0), H // KV, axis=0)
+                assert_close(values(got[t, H // 2:], act), out, pav, d, len(keep), vsum, act,
+                             f"token {t} without position {pos}")
