@@ -17,7 +17,7 @@
 // kBatch units' loads are issued before the angles.
 //
 // 4096 fp32 tokens of 8B heads into an fp16 cache (185 MB) take 34 us, 8191 bf16
-// tokens of 70B heads (336 MB) 62 us: 5.4 TB/s, where torch's 4 GiB copy reaches
+// tokens of 70B heads (336 MB) 61 us: 5.5 TB/s, where torch's 4 GiB copy reaches
 // 4.8.  64 decode tokens take 6 us, a launch.
 #include "mlk_paged.h"
 

@@ -105,9 +105,9 @@ __device__ inline void Join(const RaggedParams& p, const JoinRow& row, int part_
 // sequences than workers, a worker, standing for the one (sequence, block of heads)
 // that it is the second to hold a part of: others have no parts to join, and looking
 // for each sequence's share is work for all the sequences before it.  (The whole call,
-// 8B heads, bf16, by sequence and by worker: 16384 sequences of lengths to 1024 21.3
-// and 6.7 ms, 1024 of them 0.50 and 0.45; 64 of lengths to 8192 190 and 194 us, one
-// of 8191 in fp32 27 and 39.)
+// 8B heads, bf16, by sequence and by worker: 16384 sequences of lengths to 1024 21.5
+// and 6.7 ms, 1024 of them 0.50 and 0.46; 64 of lengths to 8192 191 and 195 us, one
+// of 8191 in fp32 27 and 38.)
 template <typename A, int L, bool kByWorker>
 __global__ __launch_bounds__(kThreads) void JoinFew(const RaggedParams p, int per_row,
                                                     int per_place) {

@@ -33,9 +33,10 @@
 // 64 sequences of 8B heads, bf16, 1.10 GB of K and V: 190 us with the join, 5.8
 // TB/s; of the time before, waves on neighbouring heads instead of one head 7 us,
 // non-temporal loads 12, scalar look-ups 5.  4 sequences of 70B heads, fp32 over
-// fp16, 0.79 GB: 146 us, 5.4 TB/s.  A kernel that only reads reached 5.0 to 7.0 TB/s,
+// fp16, 0.79 GB: 146 us, 5.4 TB/s.  A kernel that only reads reached 5.0 to 7.5 TB/s,
 // by its access pattern.  A single fp32 sequence (67 MB, 26 us) is far from its
 // bytes: length, page, row and join each wait for the one before.
+// Instances: head_dim 64, 128 and 256; another runs on the next one, padded.
 #include "mlk_ragged.h"
 
 namespace mlk {

@@ -21,13 +21,14 @@
 // K's reads (16 rows of one chunk) and V's (4 rows of 64 bytes) meet each bank
 // once (counted: no conflicts).
 //
-// 9001 packed bf16 tokens of 70B heads: 567 GFLOP in 648 us, 0.88 PFLOP/s where
-// an 8192^3 bf16 product reaches 1.32.  2500 packed fp32 tokens of 8B heads: 6
-// products for each of 11.9 GFLOP, 120 us, 0.6 PFLOP/s.  256 rows share a tile's
-// loads: with 128 these took 674 and 144 us.  Counted with 128 rows on the packed
-// bf16 call, the matrix units were busy 37 % of the cycles and the vector units
-// active 44 %, and taking work out shortened it by 13 % (loads) and 8 %
-// (exponentials): no one resource is full, the two kinds of phase overlap partly.
+// 9001 packed bf16 tokens of 70B heads: 567 GFLOP in 643 us, 0.88 PFLOP/s where
+// an 8192^3 bf16 product reaches 1.35.  2500 packed fp32 tokens of 8B heads: 6
+// products for each of 11.9 GFLOP, 119 us, 0.6 PFLOP/s.  256 rows share a tile's
+// loads: with 128 these took 674 and 144 us.  Counted on the packed bf16 call, the
+// matrix units are busy 37 % of the cycles and vector instructions issue in 43 %:
+// no one resource is full, the two kinds of phase overlap partly.
+// Instances: head_dim 64, 128 and 256; another runs on the next one, padded, at that
+// one's cost (4096 packed bf16 tokens of 8 heads: 80 in 90 us, 128 in 83).
 #include "mlk_ragged.h"
 
 namespace mlk {
