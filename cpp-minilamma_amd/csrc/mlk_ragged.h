@@ -154,6 +154,13 @@ __device__ inline int RowExponent(float amax) {
     return s < 100 ? s : 100;
 }
 
+// The scores' factor for a row scaled by 2^e, kept a normal number: 0 or infinity times
+// a difference of infinity or 0 would be NaN.  Below the least one every weight is 1
+// (scores are below 2^40 in size), above the largest only the maximum's is not 0.
+__device__ inline float RowFactor(float factor, int e) {
+    return fminf(fmaxf(ldexpf(factor, -e), 0x1p-126f), 0x1.fffffep127f);
+}
+
 // Maximum / sum over the lanes l, l ^ 32 (every lane gets it).
 __device__ inline float Max32(float v) {
     const u32x2 r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false,

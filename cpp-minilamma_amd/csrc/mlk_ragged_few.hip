@@ -314,7 +314,7 @@ __global__ __launch_bounds__(kWaves * kWave) void AttnFew(const RaggedParams p) 
                 }
                 const int e = RowExponent(Max32(Max16(amax)));
                 up = ldexpf(1.0f, e);
-                factor[nb] = ldexpf(p.factor, -e);
+                factor[nb] = RowFactor(p.factor, e);
             }
 #pragma unroll
             for (int c = 0; c < NQR; ++c) {

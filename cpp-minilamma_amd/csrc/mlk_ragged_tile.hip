@@ -141,7 +141,7 @@ __global__ __launch_bounds__((TileShape<A, C, HD>::kThreads), HD <= 128 ? 2 : 1)
                 }
                 const int e = RowExponent(Max32(amax));
                 up = ldexpf(1.0f, e);
-                factor = ldexpf(p.factor, -e);
+                factor = RowFactor(p.factor, e);
             }
 #pragma unroll
             for (int c = 0; c < NS; ++c) {

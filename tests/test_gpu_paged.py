@@ -1070,3 +1070,26 @@ def test_infinite_scores(mlk, paged, name, act, ct):
                 vsum = np.repeat(np.abs(vv).sum(0), H // KV, axis=0)
                 assert_close(values(got[t, H // 2:], act), out, pav, d, len(keep), vsum, act,
                              f"token {t} without position {pos}")
+
+
+@pytest.mark.parametrize("act,ct", PAIRS)
+@pytest.mark.parametrize("name", list(PLANS))
+def test_tiny_rows_and_a_tiny_scale(mlk, paged, name, act, ct):
+    """Scores that are nothing beside 1: the mean of V, whatever power of two a row
+    of q is scaled by on the way (1e-27 is 2^-90, the scale 2^-66).  |score| <= 64 x
+    1e-27 x 10 x 1e-20, so its part of the bound is 0."""
+    H, KV, hd = 8, 2, 64
+    counts, lens, ws = PLANS[name]
+    rng = np.random.default_rng(81)
+    batch = Batch(counts, lens, 16, seed=4)
+    cache = Cache(mlk, paged, batch, KV, hd, ct, rng)
+    size = 1e-7 if act == "f16" else 1e-27
+    q = to_type(rng.uniform(0.5, 1, (batch.T, H, hd)) * size, act)
+    got = run_paged(mlk, paged, batch, cache, q, H, act, scale=1e-20, workspace=ws)
+    for t, s, p in batch.rows():
+        if t % 7 and p + 1 < lens[s]:
+            continue
+        k, v = (a[:p + 1] for a in cache.gathered(s, lens[s]))
+        out, pav, _ = exact_rows(np.zeros((H, hd)), k, v, 1.0)
+        vsum = np.repeat(np.abs(v).sum(0), H // KV, axis=0)
+        assert_close(values(got[t], act), out, pav, 0.0, p + 1, vsum, act, f"token {t}, position {p}")
