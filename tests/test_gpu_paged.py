@@ -1093,3 +1093,27 @@ def test_tiny_rows_and_a_tiny_scale(mlk, paged, name, act, ct):
         out, pav, _ = exact_rows(np.zeros((H, hd)), k, v, 1.0)
         vsum = np.repeat(np.abs(v).sum(0), H // KV, axis=0)
         assert_close(values(got[t], act), out, pav, 0.0, p + 1, vsum, act, f"token {t}, position {p}")
+
+
+def test_thousands_of_kv_heads_are_left_unsplit(mlk, paged):
+    """256 sequences at 8192 KV heads under bounds that ask for a split whose join
+    would take 2^23 workgroups: the call runs without it."""
+    H = KV = 8192
+    hd, n = 2, 256
+    rng = np.random.default_rng(91)
+    lens = rng.integers(32, 700, n)
+    counts = np.ones(n, int)
+    counts[100] = 32
+    batch = Batch(counts.tolist(), lens.tolist(), 1024)
+    batch.n_pages = 2
+    batch.table = (np.arange(n) % 2).astype(np.int32).reshape(n, 1)
+    cache = Cache(mlk, paged, batch, KV, hd, "f16", rng, fill=False)
+    for i in range(2):
+        cache.host[i] = to_type(rng.standard_normal(cache.host[i].shape), "f16")
+    cache.upload(mlk)
+    cache.handle = paged.PagedCache(cache.k, cache.v, "f16", 2, 1024, KV, hd)
+    q = to_type(rng.standard_normal((batch.T, H, hd)), "f16")
+    got = run_paged(mlk, paged, batch, cache, q, H, "f16")
+    assert (got != 7).any(axis=2).all()
+    at = int(batch.start[100])
+    check_paged(batch, cache, q, got, H, "f16", rows={0, at + 3, at + 31, batch.T - 1})
