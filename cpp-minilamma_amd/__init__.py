@@ -163,7 +163,15 @@ def exported_symbols():
                                        "mlk_paged_kv_append", "mlk_attention_paged",
                                        "mlk_attention_paged_workspace_bytes",
                                        "mlk_attention_packed",
-                                       "mlk_attention_packed_workspace_bytes"])
+                                       "mlk_attention_packed_workspace_bytes",
+                                       "mlk_paged_plan", "mlk_paged_release",
+                                       "mlk_paged_plan_workspace_bytes",
+                                       "mlk_attention_paged_scored",
+                                       "mlk_attention_paged_scored_workspace_bytes",
+                                       "mlk_attention_packed_scored",
+                                       "mlk_attention_packed_scored_workspace_bytes",
+                                       # and in sampling.py
+                                       "mlk_sample", "mlk_sample_workspace_bytes"])
 
 
 # ------------------------------------------------------------------ runtime

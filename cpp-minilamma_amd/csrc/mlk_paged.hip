@@ -303,6 +303,103 @@ mlk_status CheckPaged(const char* fn, const mlk_paged_cache* cache, const mlk_pa
     return MLK_OK;
 }
 
+namespace {
+
+// Score functions and masks of an attention call; they are read while out is written.
+mlk_status CheckScores(const char* fn, const mlk_attention_scores* scores, const void* out, Scores* to) {
+    if (scores == nullptr) return Fail(MLK_ERR_INVALID, "%s: scores must not be null", fn);
+    if (!std::isfinite(scores->softcap) || scores->softcap < 0.0f) {
+        return Fail(MLK_ERR_INVALID, "%s: softcap must be finite and not negative", fn);
+    }
+    if (scores->window < 0) return Fail(MLK_ERR_INVALID, "%s: window must not be negative", fn);
+    const void* ptrs[3] = {scores->slopes, scores->prefix_len, scores->first};
+    for (const void* p : ptrs) {
+        if (!Aligned(p, 4)) return Fail(MLK_ERR_INVALID, "%s: slopes, prefix_len and first must be 4-byte aligned", fn);
+        if (p != nullptr && p == out) return Fail(MLK_ERR_INVALID, "%s: out may not alias slopes, prefix_len or first", fn);
+    }
+    // (a window of over 2^30 positions, the longest sequence, limits nothing)
+    *to = {scores->slopes, scores->prefix_len, scores->first, scores->softcap,
+           scores->window > (1 << 30) ? 0 : static_cast<int32_t>(scores->window)};
+    return MLK_OK;
+}
+
+// The arguments of an attention call over pages, checked (batch.n_seqs 0: nothing to do).
+mlk_status PagedCall(const char* fn, const mlk_paged_cache* cache, const mlk_paged_batch* batch,
+                     int32_t type, const void* q, int64_t q_row_stride, void* out,
+                     int32_t n_heads, float scale, void* workspace, size_t workspace_bytes,
+                     int32_t* err, void* stream, AttendArgs* to) {
+    PagedArgs a;
+    mlk_status st = CheckPaged(fn, cache, batch, type, &a);
+    if (st != MLK_OK) return st;
+    st = CheckHeads(fn, n_heads, cache->n_kv_heads, cache->head_dim, scale);
+    if (st != MLK_OK) return st;
+    st = CheckElements(fn, "q", q, type);
+    if (st != MLK_OK) return st;
+    st = CheckElements(fn, "out", out, type);
+    if (st != MLK_OK) return st;
+    if (q_row_stride < static_cast<int64_t>(n_heads) * cache->head_dim) {
+        return Fail(MLK_ERR_INVALID, "%s: q_row_stride must be at least n_heads * head_dim", fn);
+    }
+    if (out == q || out == cache->k || out == cache->v) {
+        return Fail(MLK_ERR_INVALID, "%s: out may not alias q or the pages", fn);
+    }
+    if (workspace != nullptr && !Aligned(workspace, 16)) {
+        return Fail(MLK_ERR_INVALID, "%s: workspace must be 16-byte aligned", fn);
+    }
+    *to = {a.batch, a.rows, type, cache->type, q, q_row_stride, out, n_heads, cache->n_kv_heads,
+           scale, workspace, workspace == nullptr ? 0 : workspace_bytes, err, AsStream(stream), {}};
+    return MLK_OK;
+}
+
+// The same over packed rows.
+mlk_status PackedCall(const char* fn, int32_t type, const void* q, int64_t q_row_stride,
+                      const void* k, int64_t k_row_stride, const void* v, int64_t v_row_stride,
+                      const int32_t* seq_start, int64_t n_seqs, int64_t n_tokens,
+                      int64_t max_seq_len, int32_t n_heads, int32_t n_kv_heads, int32_t head_dim,
+                      float scale, void* out, void* workspace, size_t workspace_bytes,
+                      int32_t* err, void* stream, AttendArgs* to) {
+    if (!KnownType(type)) return Fail(MLK_ERR_INVALID, "%s: unknown element type", fn);
+    mlk_status st = CheckHeads(fn, n_heads, n_kv_heads, head_dim, scale);
+    if (st != MLK_OK) return st;
+    const char* names[4] = {"q", "k", "v", "out"};
+    const void* ptrs[4] = {q, k, v, out};
+    for (int i = 0; i < 4; ++i) {
+        st = CheckElements(fn, names[i], ptrs[i], type);
+        if (st != MLK_OK) return st;
+    }
+    const int64_t slot = static_cast<int64_t>(n_kv_heads) * head_dim;
+    if (q_row_stride < static_cast<int64_t>(n_heads) * head_dim || k_row_stride < slot ||
+        v_row_stride < slot) {
+        return Fail(MLK_ERR_INVALID, "%s: row strides must be at least heads * head_dim", fn);
+    }
+    if (out == q || out == k || out == v) {
+        return Fail(MLK_ERR_INVALID, "%s: out may not alias q, k or v", fn);
+    }
+    if (k_row_stride > kMaxRow || v_row_stride > kMaxRow) {
+        return Fail(MLK_ERR_INVALID, "%s: k and v row strides must be at most 2^27 elements", fn);
+    }
+    st = CheckCounts(fn, n_seqs, n_tokens);
+    if (st != MLK_OK) return st;
+    if (workspace != nullptr && !Aligned(workspace, 16)) {
+        return Fail(MLK_ERR_INVALID, "%s: workspace must be 16-byte aligned", fn);
+    }
+    *to = {};
+    if (n_seqs == 0 || n_tokens == 0) return MLK_OK;
+    if (seq_start == nullptr || !Aligned(seq_start, 4)) {
+        return Fail(MLK_ERR_INVALID, "%s: seq_start must be a 4-byte aligned device array", fn);
+    }
+    if (max_seq_len < 1) return Fail(MLK_ERR_INVALID, "%s: max_seq_len must be positive", fn);
+    const int32_t T = static_cast<int32_t>(n_tokens);
+    const int32_t most = max_seq_len < n_tokens ? static_cast<int32_t>(max_seq_len) : T;
+    const Ragged b{seq_start, nullptr, nullptr, 0, static_cast<int32_t>(n_seqs), T, most, most};
+    const RowsAt r{k, v, 0, k_row_stride, v_row_stride, 0, 0, head_dim};
+    *to = {b, r, type, type, q, q_row_stride, out, n_heads, n_kv_heads, scale, workspace,
+           workspace == nullptr ? 0 : workspace_bytes, err, AsStream(stream), {}};
+    return MLK_OK;
+}
+
+}  // namespace
+
 }  // namespace mlk
 
 using namespace mlk;
@@ -403,29 +500,23 @@ mlk_status mlk_attention_paged(const mlk_paged_cache* cache, const mlk_paged_bat
                                int32_t type, const void* q, int64_t q_row_stride, void* out,
                                int32_t n_heads, float scale, void* workspace,
                                size_t workspace_bytes, int32_t* err, void* stream) {
-    const char* fn = "mlk_attention_paged";
-    PagedArgs a;
-    mlk_status st = CheckPaged(fn, cache, batch, type, &a);
-    if (st != MLK_OK) return st;
-    st = CheckHeads(fn, n_heads, cache->n_kv_heads, cache->head_dim, scale);
-    if (st != MLK_OK) return st;
-    st = CheckElements(fn, "q", q, type);
-    if (st != MLK_OK) return st;
-    st = CheckElements(fn, "out", out, type);
-    if (st != MLK_OK) return st;
-    if (q_row_stride < static_cast<int64_t>(n_heads) * cache->head_dim) {
-        return Fail(MLK_ERR_INVALID, "%s: q_row_stride must be at least n_heads * head_dim", fn);
-    }
-    if (out == q || out == cache->k || out == cache->v) {
-        return Fail(MLK_ERR_INVALID, "%s: out may not alias q or the pages", fn);
-    }
-    if (workspace != nullptr && !Aligned(workspace, 16)) {
-        return Fail(MLK_ERR_INVALID, "%s: workspace must be 16-byte aligned", fn);
-    }
-    if (a.batch.n_seqs == 0) return MLK_OK;
-    return Attend({a.batch, a.rows, type, cache->type, q, q_row_stride, out, n_heads,
-                   cache->n_kv_heads, scale, workspace, workspace == nullptr ? 0 : workspace_bytes,
-                   err, AsStream(stream)});
+    AttendArgs a;
+    const mlk_status st = PagedCall("mlk_attention_paged", cache, batch, type, q, q_row_stride, out,
+                                    n_heads, scale, workspace, workspace_bytes, err, stream, &a);
+    return st != MLK_OK || a.batch.n_seqs == 0 ? st : Attend(a);
+}
+
+mlk_status mlk_attention_paged_scored(const mlk_paged_cache* cache, const mlk_paged_batch* batch,
+                                      const mlk_attention_scores* scores, int32_t type,
+                                      const void* q, int64_t q_row_stride, void* out,
+                                      int32_t n_heads, float scale, void* workspace,
+                                      size_t workspace_bytes, int32_t* err, void* stream) {
+    const char* fn = "mlk_attention_paged_scored";
+    AttendArgs a;
+    mlk_status st = PagedCall(fn, cache, batch, type, q, q_row_stride, out, n_heads, scale,
+                              workspace, workspace_bytes, err, stream, &a);
+    if (st == MLK_OK) st = CheckScores(fn, scores, out, &a.scores);
+    return st != MLK_OK || a.batch.n_seqs == 0 ? st : AttendScored(a);
 }
 
 int64_t mlk_attention_paged_workspace_bytes(int64_t n_seqs, int64_t n_tokens,
@@ -442,43 +533,46 @@ mlk_status mlk_attention_packed(int32_t type, const void* q, int64_t q_row_strid
                                 int64_t max_seq_len, int32_t n_heads, int32_t n_kv_heads,
                                 int32_t head_dim, float scale, void* out, void* workspace,
                                 size_t workspace_bytes, int32_t* err, void* stream) {
-    const char* fn = "mlk_attention_packed";
-    if (!KnownType(type)) return Fail(MLK_ERR_INVALID, "%s: unknown element type", fn);
-    mlk_status st = CheckHeads(fn, n_heads, n_kv_heads, head_dim, scale);
-    if (st != MLK_OK) return st;
-    const char* names[4] = {"q", "k", "v", "out"};
-    const void* ptrs[4] = {q, k, v, out};
-    for (int i = 0; i < 4; ++i) {
-        st = CheckElements(fn, names[i], ptrs[i], type);
-        if (st != MLK_OK) return st;
-    }
-    const int64_t slot = static_cast<int64_t>(n_kv_heads) * head_dim;
-    if (q_row_stride < static_cast<int64_t>(n_heads) * head_dim || k_row_stride < slot ||
-        v_row_stride < slot) {
-        return Fail(MLK_ERR_INVALID, "%s: row strides must be at least heads * head_dim", fn);
-    }
-    if (out == q || out == k || out == v) {
-        return Fail(MLK_ERR_INVALID, "%s: out may not alias q, k or v", fn);
-    }
-    if (k_row_stride > kMaxRow || v_row_stride > kMaxRow) {
-        return Fail(MLK_ERR_INVALID, "%s: k and v row strides must be at most 2^27 elements", fn);
-    }
-    st = CheckCounts(fn, n_seqs, n_tokens);
-    if (st != MLK_OK) return st;
-    if (workspace != nullptr && !Aligned(workspace, 16)) {
-        return Fail(MLK_ERR_INVALID, "%s: workspace must be 16-byte aligned", fn);
-    }
-    if (n_seqs == 0 || n_tokens == 0) return MLK_OK;
-    if (seq_start == nullptr || !Aligned(seq_start, 4)) {
-        return Fail(MLK_ERR_INVALID, "%s: seq_start must be a 4-byte aligned device array", fn);
-    }
-    if (max_seq_len < 1) return Fail(MLK_ERR_INVALID, "%s: max_seq_len must be positive", fn);
-    const int32_t T = static_cast<int32_t>(n_tokens);
-    const int32_t most = max_seq_len < n_tokens ? static_cast<int32_t>(max_seq_len) : T;
-    const Ragged b{seq_start, nullptr, nullptr, 0, static_cast<int32_t>(n_seqs), T, most, most};
-    const RowsAt r{k, v, 0, k_row_stride, v_row_stride, 0, 0, head_dim};
-    return Attend({b, r, type, type, q, q_row_stride, out, n_heads, n_kv_heads, scale, workspace,
-                   workspace == nullptr ? 0 : workspace_bytes, err, AsStream(stream)});
+    AttendArgs a;
+    const mlk_status st = PackedCall("mlk_attention_packed", type, q, q_row_stride, k, k_row_stride,
+                                     v, v_row_stride, seq_start, n_seqs, n_tokens, max_seq_len,
+                                     n_heads, n_kv_heads, head_dim, scale, out, workspace,
+                                     workspace_bytes, err, stream, &a);
+    return st != MLK_OK || a.batch.n_seqs == 0 ? st : Attend(a);
+}
+
+mlk_status mlk_attention_packed_scored(int32_t type, const mlk_attention_scores* scores,
+                                       const void* q, int64_t q_row_stride, const void* k,
+                                       int64_t k_row_stride, const void* v, int64_t v_row_stride,
+                                       const int32_t* seq_start, int64_t n_seqs, int64_t n_tokens,
+                                       int64_t max_seq_len, int32_t n_heads, int32_t n_kv_heads,
+                                       int32_t head_dim, float scale, void* out, void* workspace,
+                                       size_t workspace_bytes, int32_t* err, void* stream) {
+    const char* fn = "mlk_attention_packed_scored";
+    AttendArgs a;
+    mlk_status st = PackedCall(fn, type, q, q_row_stride, k, k_row_stride, v, v_row_stride,
+                               seq_start, n_seqs, n_tokens, max_seq_len, n_heads, n_kv_heads,
+                               head_dim, scale, out, workspace, workspace_bytes, err, stream, &a);
+    if (st == MLK_OK) st = CheckScores(fn, scores, out, &a.scores);
+    return st != MLK_OK || a.batch.n_seqs == 0 ? st : AttendScored(a);
+}
+
+int64_t mlk_attention_paged_scored_workspace_bytes(int64_t n_seqs, int64_t n_tokens,
+                                                   int64_t max_new_tokens, int64_t max_seq_len,
+                                                   int32_t n_heads, int32_t n_kv_heads,
+                                                   int32_t head_dim, int64_t window) {
+    (void)window;
+    return AttendWorkspace(n_seqs, n_tokens, max_new_tokens, max_seq_len, n_heads, n_kv_heads,
+                           head_dim, false);
+}
+
+int64_t mlk_attention_packed_scored_workspace_bytes(int64_t n_seqs, int64_t n_tokens,
+                                                    int64_t max_seq_len, int32_t n_heads,
+                                                    int32_t n_kv_heads, int32_t head_dim,
+                                                    int64_t window) {
+    (void)window;
+    return AttendWorkspace(n_seqs, n_tokens, max_seq_len, max_seq_len, n_heads, n_kv_heads,
+                           head_dim, true);
 }
 
 int64_t mlk_attention_packed_workspace_bytes(int64_t n_seqs, int64_t n_tokens,

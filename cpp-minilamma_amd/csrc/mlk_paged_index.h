@@ -51,6 +51,33 @@ MLK_HD inline bool LoadSeq(const Ragged& r, int s, Seq* q) {
     return n <= r.max_new && len >= n && len <= r.max_len;
 }
 
+// Score functions and masks (mlk_attention_scores); all zero: plain causal attention.
+struct Scores {
+    const float* slopes;          // [n_heads] or nullptr
+    const int32_t *prefix, *first;  // [n_seqs], [n_tokens] or nullptr
+    float softcap;
+    int32_t window;               // 0: none
+};
+
+// The positions that token row t, at position pos of sequence s of length len, sees:
+// lo .. hi, none where lo > hi.
+struct Seen {
+    int32_t lo, hi;
+};
+MLK_HD inline Seen SeenBy(const Scores& m, int s, int32_t t, int32_t pos, int32_t len) {
+    Seen v{0, pos};
+    if (m.window > 0 && pos - m.window + 1 > 0) v.lo = pos - m.window + 1;
+    if (m.first != nullptr) {
+        const int32_t f = ReadIndex(m.first + t);
+        if (f > v.lo) v.lo = f;
+    }
+    if (m.prefix != nullptr) {
+        const int32_t n = ReadIndex(m.prefix + s), last = (n < len ? n : len) - 1;
+        if (last > v.hi) v.hi = last;
+    }
+    return v;
+}
+
 // Where K and V rows lie: position j's row of KV head g starts at element
 //   paged:  page * page_stride + (j % page_size) * k_row + g * head_dim
 //   packed: (t0 + j) * k_row + g * head_dim      (v_row for V)

@@ -465,6 +465,164 @@ int64_t mlk_attention_packed_workspace_bytes(int64_t n_seqs, int64_t n_tokens,
                                              int64_t max_seq_len, int32_t n_heads,
                                              int32_t n_kv_heads, int32_t head_dim);
 
+/* ------------------------------------------------ pages of a step
+ * Which pages and rows a step's new tokens get, on the device: a server's step
+ * needs no host between the choice of its tokens and the next append.  No
+ * counterpart in the reference (one sequence, one contiguous cache). */
+
+/* The pages of n_seqs sequences: sequence s holds seq_len[s] positions in its
+ * first ceil(seq_len[s] / page_size) pages of page_table's row s, and
+ * free_pages[0 .. *n_free - 1] are the pages that no sequence holds, a stack
+ * whose top is the last.  All four are device arrays that the calls below
+ * change in place; seq_len and page_table are those of mlk_paged_batch.
+ * page_size is a power of two, n_pages at most 2^30, n_seqs at most 2^20. */
+typedef struct {
+    int32_t* page_table;  /* device [n_seqs, table_stride] */
+    int32_t* seq_len;     /* device [n_seqs] */
+    int32_t* free_pages;  /* device [n_pages] */
+    int32_t* n_free;      /* device [1] */
+    int64_t n_seqs, table_stride, n_pages;
+    int32_t page_size;
+} mlk_paged_pool;
+
+/*
+ * Takes in new_tokens[s] (device [n_seqs], 0 is allowed) new tokens of each
+ * sequence, for a step of at most n_tokens: pops the pages that they start,
+ * enters them in the table, adds the tokens to seq_len, and writes
+ *   token_start [n_seqs + 1]   the sequences' token rows, as mlk_paged_batch
+ *                              and mlk_attention_packed take them;
+ *   positions   [n_tokens]     each token row's position in its sequence,
+ *   token_seq   [n_tokens]     its sequence,
+ *   slots       [n_tokens]     its cache row, page * page_size + position %
+ *                              page_size (-1: page outside [0, n_pages))
+ * (the last three may be NULL; rows behind the last token are left as they
+ * are).  With need_s the pages that sequence s starts, it is taken in where it
+ * starts none or need_0 + .. + need_s <= *n_free, and new_tokens[0] + .. +
+ * new_tokens[s] <= n_tokens: first come, first served, no sequence overtakes one
+ * that had to wait for pages.  One that is not taken in brings no token rows
+ * (token_start[s + 1] == token_start[s]) and keeps what it has.  Pages are
+ * popped in the order of the sequences and their positions.  A sequence with a
+ * negative length or count, or one that would come to more than max_seq_len
+ * (<= table_stride * page_size, at most 2^30) asks for nothing and raises *err
+ * (NULL: no report; the caller clears it), as does a page outside [0, n_pages)
+ * or *n_free outside 0 .. n_pages (then the nearest of the two counts).
+ * n_tokens at most 2^23.  The outputs do not overlap each other nor the pool.
+ * workspace: mlk_paged_plan_workspace_bytes(), 16-byte aligned; its content does
+ * not matter, and calls that may overlap need one each.
+ */
+mlk_status mlk_paged_plan(const mlk_paged_pool* pool, const int32_t* new_tokens, int64_t n_tokens,
+                          int64_t max_seq_len, int32_t* token_start, int32_t* positions,
+                          int32_t* token_seq, int64_t* slots, void* workspace,
+                          size_t workspace_bytes, int32_t* err, void* stream);
+
+/*
+ * Cuts each sequence s back to its first keep[s] positions (device [n_seqs];
+ * 0: it has ended; negative: it stays as it is): seq_len[s] becomes keep[s],
+ * the pages past ceil(keep[s] / page_size) go back on the stack, and their
+ * table entries become -1.  They are pushed so that the first page of the first
+ * sequence ends on top: a plan that is cut back whole leaves the stack as it
+ * was.  keep[s] over seq_len[s], or a length outside 0 .. table_stride *
+ * page_size, leaves the sequence as it is and raises *err.  Pages that do not
+ * fit the stack (the same page held twice) are dropped and raise *err.
+ * Pages that sequences share are not counted: a shared page is given back by
+ * one of them alone.  workspace as above.
+ */
+mlk_status mlk_paged_release(const mlk_paged_pool* pool, const int32_t* keep, void* workspace,
+                             size_t workspace_bytes, int32_t* err, void* stream);
+/* Bytes of the workspace of both (0 on bad input). */
+int64_t mlk_paged_plan_workspace_bytes(int64_t n_seqs);
+
+/* ------------------------------------------- score functions and masks */
+
+/* What a score goes through between q . k and the softmax, and which positions
+ * a token sees.  Token row t at position p of sequence s, head i, position j:
+ *   x = scale (q . k_j)
+ *   x = softcap tanh(x / softcap)        (softcap > 0; 0: as it is)
+ *   x = x - slopes[i] |p - j|            (slopes != NULL)
+ *   j is seen where  max(first[t], p - window + 1) <= j <= max(p, prefix_len[s] - 1)
+ * first NULL: from 0 on; window 0: no limit; prefix_len NULL: causal.  A prefix
+ * is what all of its own tokens see whole (an instruction, an image's tokens);
+ * it ends where the sequence does if it is given as longer.  first holds, for
+ * documents side by side in one sequence, where each token's own begins; it may
+ * lie behind the token's last position: a token that sees nothing gets zeros. */
+typedef struct {
+    float softcap;              /* finite, >= 0 */
+    const float* slopes;        /* device [n_heads] or NULL */
+    int64_t window;             /* >= 0 */
+    const int32_t* prefix_len;  /* device [n_seqs] or NULL */
+    const int32_t* first;       /* device [n_tokens] or NULL */
+} mlk_attention_scores;
+
+/* mlk_attention_paged and mlk_attention_packed with scores and masks of this
+ * kind: the same arguments, semantics and precision (x / softcap, tanh and the
+ * bias in fp32), positions that no token of a sequence sees by its window are
+ * not read.  The new tokens of a prefix see later ones of it, so those have to
+ * be in the cache too (mlk_paged_kv_append puts all there first). */
+mlk_status mlk_attention_paged_scored(const mlk_paged_cache* cache, const mlk_paged_batch* batch,
+                                      const mlk_attention_scores* scores, int32_t type,
+                                      const void* q, int64_t q_row_stride, void* out,
+                                      int32_t n_heads, float scale, void* workspace,
+                                      size_t workspace_bytes, int32_t* err, void* stream);
+mlk_status mlk_attention_packed_scored(int32_t type, const mlk_attention_scores* scores,
+                                       const void* q, int64_t q_row_stride, const void* k,
+                                       int64_t k_row_stride, const void* v, int64_t v_row_stride,
+                                       const int32_t* seq_start, int64_t n_seqs, int64_t n_tokens,
+                                       int64_t max_seq_len, int32_t n_heads, int32_t n_kv_heads,
+                                       int32_t head_dim, float scale, void* out, void* workspace,
+                                       size_t workspace_bytes, int32_t* err, void* stream);
+/* Bytes of their optional workspaces; window as in mlk_attention_scores. */
+int64_t mlk_attention_paged_scored_workspace_bytes(int64_t n_seqs, int64_t n_tokens,
+                                                   int64_t max_new_tokens, int64_t max_seq_len,
+                                                   int32_t n_heads, int32_t n_kv_heads,
+                                                   int32_t head_dim, int64_t window);
+int64_t mlk_attention_packed_scored_workspace_bytes(int64_t n_seqs, int64_t n_tokens,
+                                                    int64_t max_seq_len, int32_t n_heads,
+                                                    int32_t n_kv_heads, int32_t head_dim,
+                                                    int64_t window);
+
+/* ------------------------------------------------------------ sampling */
+
+/* How each row's token is chosen: device arrays [n_rows], or NULL for the value
+ * that leaves all as it is. */
+typedef struct {
+    const float* temperature;  /* NULL: 1.  0: the largest logit */
+    const int32_t* top_k;      /* NULL, or <= 0 in a row: all */
+    const float* top_p;        /* NULL, or >= 1 in a row: all */
+    const float* min_p;        /* NULL, or <= 0 in a row: all */
+} mlk_sampling;
+
+/*
+ * The next token of each row of logits (n_rows of `vocab` elements of `type`,
+ * row_stride elements apart) from the caller's uniform numbers in [0, 1).  With
+ * the row's logits in descending order (the lower index first where they are
+ * equal), x_1 .. x_vocab, w_i = exp((x_i - x_1) / temperature) and C_n = w_1 +
+ * .. + w_n, the tokens kept are the first
+ *   n = max(1, min(n_k, n_p, n_m)):   n_k = top_k,
+ *   n_p = the least with C_(n_p) >= top_p C_(n_k),   n_m = how many w_i >= min_p
+ * and the token is the first of them with C_i > uniform C_n; prob (NULL: not
+ * wanted) is its share w_i / C_n.  uniform = 0 chooses the largest logit, as does
+ * temperature 0 (uniform is then not looked at).  A logit of -infinity is never
+ * chosen; logits of +infinity share all the weight.  Weights below 2^-44 (30
+ * temperatures below the largest) may count as 0; temperatures below 2^-14 count
+ * as 2^-14, logits of over 2^26 temperatures in size as that.
+ * The weights are added as whole numbers: a row's token depends on
+ * neither the other rows nor how the work is divided, run for run.
+ * A row that has a NaN, or only -infinities, or a setting that is a NaN, a negative
+ * temperature or a uniform outside [0, 1), gets token -1 and prob 0 and raises *err
+ * (NULL: no report; the caller clears it).  vocab at most 2^20, n_rows at most 2^20.
+ * tokens and prob do not overlap the inputs.  workspace:
+ * mlk_sample_workspace_bytes(), 16-byte aligned; its content does not matter, and
+ * calls that may overlap need one each.
+ * No counterpart in the reference on the device (its sampler reads the logits
+ * on the host, src/sampler.cc).
+ */
+mlk_status mlk_sample(int32_t type, const void* logits, int64_t row_stride, int64_t n_rows,
+                      int64_t vocab, const mlk_sampling* how, const float* uniform,
+                      int32_t* tokens, float* prob, void* workspace, size_t workspace_bytes,
+                      int32_t* err, void* stream);
+/* Bytes of that workspace on the current device (0 on bad input). */
+int64_t mlk_sample_workspace_bytes(int32_t type, int64_t n_rows, int64_t vocab);
+
 /* ------------------------------------------------------ batched forward
  * One transformer layer over a batch of tokens: the reference's
  * ForwardLayerDevice (src/forward.cc:337-384) for all tokens at once, i.e.
