@@ -33,9 +33,12 @@
 namespace mlk {
 namespace {
 
-constexpr int kThreads = 512, kWaves = kThreads / kWave;
-constexpr int kBins = 512;      // of a histogram, a power of two
-constexpr int kSort = 2048;     // elements gathered and sorted at once
+constexpr int kThreads = 512, kWaves = kThreads / kWave;  // first pass
+constexpr int kChooseThreads = 1024, kChooseWaves = kChooseThreads / kWave;
+constexpr int kBins = 1024;     // of a histogram, a power of two
+constexpr int kPerUnit = 32;    // bins of a temperature
+constexpr int kList = 4096;     // elements gathered at once
+constexpr int kChunk = 4096;    // segments looked at at once
 constexpr int kMaxParts = 48;   // workgroups of a row
 constexpr int64_t kMaxVocab = 1 << 20, kMaxRows = 1 << 20;
 constexpr double kOne = 0x1p42;  // a weight of 1
@@ -87,25 +90,24 @@ __device__ inline How HowOf(const SampleArgs& a, int64_t row) {
     h.bad = !(h.t >= 0.0f) || !(h.u >= 0.0f && h.u < 1.0f) || h.p != h.p || h.m != h.m;
     if (h.k <= 0 || h.k >= a.vocab) h.k = 0;
     const float t = fmaxf(h.t, 0x1p-14f);
-    h.c = 16.0 / static_cast<double>(t);
-    h.limit = fminf(t * 0x1p25f, 0x1.fffffep127f);
+    h.c = kPerUnit / static_cast<double>(t);
+    h.limit = fminf(t * 0x1p24f, 0x1.fffffep127f);
     return h;
 }
 
 // Bin of a logit (at most 2^29 in size by the limit) and its place f in it.
 __device__ inline int32_t BinOf(const How& h, float x, double* f) {
-    const double v = fminf(fmaxf(x, -h.limit), h.limit);
+    const double v = __builtin_amdgcn_fmed3f(x, -h.limit, h.limit);
     constexpr double kRound = 0x1.8p52;
     const double t = fma(v, h.c, kRound);
     *f = fma(v, h.c, -(t - kRound));
     return static_cast<int32_t>(__double2loint(t));
 }
 
-// exp(f / 16) 2^42 as a whole number.
+// exp(f / kPerUnit) 2^42 as a whole number.
 __device__ inline uint64_t Weight(double f) {
-    constexpr double z = 1.0 / 16;
-    double e = z * z * z * z * z * z / 720 * kOne;
-    e = fma(e, f, z * z * z * z * z / 120 * kOne);
+    constexpr double z = 1.0 / kPerUnit;
+    double e = z * z * z * z * z / 120 * kOne;
     e = fma(e, f, z * z * z * z / 24 * kOne);
     e = fma(e, f, z * z * z / 6 * kOne);
     e = fma(e, f, z * z / 2 * kOne);
@@ -212,12 +214,14 @@ __global__ __launch_bounds__(kThreads) void SampleBins(const SampleArgs p) {
     uint64_t best = ~uint64_t{0};
     float* largest = p.largest + row * p.segments;
 
-    for (int32_t b = b0 + wave * kAhead; b < b1; b += kWaves * kAhead) {
+    // neighbouring blocks for each wave, the same number or one less
+    const int32_t w0 = b0 + (b1 - b0) * wave / kWaves, w1 = b0 + (b1 - b0) * (wave + 1) / kWaves;
+    for (int32_t b = w0; b < w1; b += kAhead) {
         u32x4 raw[kAhead];
 #pragma unroll
         for (int a = 0; a < kAhead; ++a) {
             const int32_t unit = (b + a) * kWave + lane;
-            raw[a] = r.Load(unit, b + a < b1 && unit < units);
+            raw[a] = r.Load(unit, b + a < w1 && unit < units);
         }
         float v[kAhead][E];
 #pragma unroll
@@ -235,7 +239,7 @@ __global__ __launch_bounds__(kThreads) void SampleBins(const SampleArgs p) {
                 m = fmaxf(m, v[a][e]);
             }
             m = Max8(m);
-            if (b + a < b1 && lane % kSegment == 0) {
+            if (b + a < w1 && lane % kSegment == 0) {
                 const int32_t seg = ((b + a) * kWave + lane) / kSegment;
                 if (seg < p.segments) largest[seg] = m;
             }
@@ -338,7 +342,7 @@ __device__ inline V ScanBlock(V v, V* scratch, V* total) {
     __syncthreads();
     V before = 0, all = 0;
 #pragma unroll
-    for (int i = 0; i < kWaves; ++i) {
+    for (int i = 0; i < kChooseWaves; ++i) {
         if (i == wave) before = all;
         all += scratch[i];
     }
@@ -347,17 +351,32 @@ __device__ inline V ScanBlock(V v, V* scratch, V* total) {
 }
 
 struct Choice {
-    uint64_t sorted[kSort];
-    double edge[kBins];  // exp(-i / 16): a bin's middle, of the largest bin's
-    double sum[kBins];   // of the weights up to and with bin i
-    uint64_t bin[kBins];  // masses or counts of the bins; of a search's digits
-    uint32_t number[kBins];  // a search's counts
-    int32_t segment[kWaves][kWave];  // those a wave is to look through
+    uint64_t list[kList];  // keys of gathered elements
+    uint64_t bin[kBins];   // masses or counts of the bins; of a search's ranges
+    double edge[kBins];    // exp(-i / kPerUnit): a bin's middle, of the largest bin's
+    double sum[kBins];     // of the weights up to and with bin i
+    uint16_t segment[kChunk];
+    uint64_t few[kWave];
+    uint64_t scan_u[kChooseWaves], scan_v[kChooseWaves];
+    double scan_d[kChooseWaves];
     int32_t tops[kMaxParts];  // the parts' largest bins, INT32_MIN: none
-    uint64_t scan_u[kWaves];
-    double scan_d[kWaves];
-    uint32_t at, n;  // a place looked for; elements gathered
+    int32_t found[2];
+    uint32_t n_list, n_segments, n_few;
     uint64_t word[3];
+};
+
+enum Bound { kCount, kReach, kPass };  // count >= bound, sum >= bound, sum > bound
+
+// The first place in a bin's order that meets a bound: its key, the sum before it and its
+// own weight (whole numbers).
+struct Place {
+    uint64_t key, before, own;
+};
+
+// Bins lo .. hi.
+struct Span {
+    int lo, hi;
+    __device__ bool Has(int b) const { return b >= lo && b <= hi; }
 };
 
 template <typename T>
@@ -368,320 +387,323 @@ struct Chooser {
     RowUnits<T> r;
     const float* largest;
     int32_t top;
-    uint64_t limit;  // keys past it are cut off (a top-k too large to be sorted)
+    uint64_t limit;  // keys past it are cut off by top-k
 
     __device__ int Tid() const { return static_cast<int>(threadIdx.x); }
+    __device__ int Lane() const { return Tid() % kWave; }
+    __device__ int Wave() const { return __builtin_amdgcn_readfirstlane(Tid() / kWave); }
+    __device__ int BinOfKey(uint64_t key, double* f) const {
+        return top - BinOf(h, Logit(static_cast<uint32_t>(key >> 32)), f);
+    }
+    __device__ double WeightOf(float x) const {
+        double f;
+        const int32_t b = top - BinOf(h, x, &f);
+        return static_cast<double>(Weight(f)) * s.edge[b];
+    }
+    __device__ double Below(int bin) const { return bin > 0 ? s.sum[bin - 1] : 0.0; }
 
-    // First i < n with ok(i) (n: none), monotone or not; every thread gets it.
-    template <typename F>
-    __device__ int First(int n, const F& ok) {
-        __syncthreads();
-        if (Tid() == 0) s.at = static_cast<uint32_t>(n);
-        __syncthreads();
-        for (int i = Tid(); i < n; i += kThreads) {
-            if (ok(i)) {
-                atomicMin(&s.at, static_cast<uint32_t>(i));
-                break;
-            }
-        }
-        __syncthreads();
-        return static_cast<int>(s.at);
+    // Logits no smaller (larger) than any of bin `bin`, to within a thousandth of a bin and a
+    // rounding.
+    __device__ float Lowest(int bin) const {
+        const double b = static_cast<double>(top) - bin;
+        if (!(h.c > 0.0) || b <= -0x1p28) return -0x1.fffffep127f;
+        const double x = (b - 0.501) / h.c;
+        return static_cast<float>(x - fabs(x) * 0x1p-23);
+    }
+    __device__ float Highest(int bin) const {
+        const double b = static_cast<double>(top) - bin;
+        if (!(h.c > 0.0) || bin == 0 || b >= 0x1p28) return INFINITY;
+        const double x = (b + 0.501) / h.c;
+        return static_cast<float>(x + fabs(x) * 0x1p-23);
     }
 
-    // f(whether it is one, bin below the largest, place in it, logit, index) over the elements of
-    // bins lo .. hi: of each 128 bytes whose largest is no lower than those.  Whole waves
-    // call f.  A wave looks at 64 segments at a time and has all that it needs of
-    // them on their way before it takes the first.
-    template <typename F>
-    __device__ void Visit(int lo, int hi, const F& f) {
-        constexpr int E = RowUnits<T>::E, kRounds = kWave / (kWave / kSegment);
-        const int lane = Tid() % kWave, wave = Tid() / kWave;
-        const int32_t units = r.Units(), segments = (units + kSegment - 1) / kSegment;
-        const bool cut = limit != ~uint64_t{0};
-        int32_t* mine = s.segment[wave];
-        float next = wave * kWave + lane < segments ? largest[wave * kWave + lane] : -INFINITY;
-        for (int32_t s0 = wave * kWave; s0 < segments; s0 += kThreads) {
-            const float m = next;
-            const int32_t then = s0 + kThreads + lane;
-            next = then < segments ? largest[then] : -INFINITY;
-            double place;
-            const bool hit = m > -INFINITY && top - BinOf(h, m, &place) <= hi;
+    // The segments c0 .. c0 + kChunk - 1 whose largest is at least `low` into s.segment; how many.
+    __device__ int Segments(int32_t c0, int32_t segments, float low) {
+        __syncthreads();
+        if (Tid() == 0) s.n_segments = 0;
+        __syncthreads();
+        float m[kChunk / kChooseThreads];
+#pragma unroll
+        for (int i = 0; i < kChunk / kChooseThreads; ++i) {
+            const int32_t seg = c0 + i * kChooseThreads + Tid();
+            m[i] = seg < segments ? largest[seg] : -INFINITY;
+        }
+#pragma unroll
+        for (int i = 0; i < kChunk / kChooseThreads; ++i) {
+            const bool hit = m[i] >= low;
             const uint64_t mask = __ballot(hit);
-            const int n = __popcll(mask);
-            if (n == 0) continue;
-            if (hit) mine[__popcll(mask & ((uint64_t{1} << lane) - 1))] = s0 + lane;
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-            u32x4 raw[kRounds];
-            int32_t unit[kRounds];
+            if (mask == 0) continue;
+            uint32_t at = 0;
+            if (Lane() == 0) at = atomicAdd(&s.n_segments, static_cast<uint32_t>(__popcll(mask)));
+            at = __builtin_amdgcn_readfirstlane(at) + __popcll(mask & ((uint64_t{1} << Lane()) - 1));
+            if (hit) s.segment[at] = static_cast<uint16_t>(i * kChooseThreads + Tid());
+        }
+        __syncthreads();
+        return static_cast<int>(s.n_segments);
+    }
+
+    // f(there, raw unit, its number) over the units of the row that have elements of at least
+    // `low` near; 8 lanes a segment, kRounds of them on their way at once.  Whole waves call f.
+    static constexpr int kRounds = 32 / RowUnits<T>::E;
+    template <typename F>
+    __device__ void Units(float low, const F& f) {
+        constexpr int kGroups = kWave / kSegment;
+        const int32_t units = r.Units(), segments = (units + kSegment - 1) / kSegment;
+        for (int32_t c0 = 0; c0 < segments; c0 += kChunk) {
+            const int n = Segments(c0, segments, low);
+            for (int g = Wave() * kGroups; g < n; g += kChooseWaves * kGroups * kRounds) {
+                u32x4 raw[kRounds];
+                int32_t unit[kRounds];
 #pragma unroll
-            for (int i = 0; i < kRounds; ++i) {
-                const int j = i * (kWave / kSegment) + lane / kSegment;
-                unit[i] = (j < n ? mine[j] : 0) * kSegment + lane % kSegment;
-                raw[i] = r.Load(unit[i], j < n && unit[i] < units);
+                for (int i = 0; i < kRounds; ++i) {
+                    const int j = g + i * kChooseWaves * kGroups + Lane() / kSegment;
+                    unit[i] = j < n ? (c0 + s.segment[j]) * kSegment + Lane() % kSegment : units;
+                    raw[i] = r.Load(unit[i], unit[i] < units);
+                }
+                f(raw, unit);
             }
+        }
+    }
+
+    // The elements of two spans of bins (and a few of their neighbours) into s.list; how many
+    // there are (of more than kList, not all are there).
+    __device__ int Gather(const Span& a, const Span& b) {
+        constexpr int E = RowUnits<T>::E;
+        const float al = Lowest(a.hi), ah = Highest(a.lo), bl = Lowest(b.hi), bh = Highest(b.lo);
+        __syncthreads();
+        if (Tid() == 0) s.n_list = 0;  // (a barrier follows in Units)
+        Units(fminf(al, bl), [&](const u32x4 (&raw)[kRounds], const int32_t (&unit)[kRounds]) {
+            uint32_t hits = 0;
 #pragma unroll
             for (int i = 0; i < kRounds; ++i) {
-                if (i * (kWave / kSegment) >= n) break;
 #pragma unroll
                 for (int e = 0; e < E; ++e) {
                     const float x = r.Get(raw[i], e);
-                    const int32_t b = top - BinOf(h, x, &place);
-                    const int32_t index = r.Index(unit[i], e);
-                    bool in = x > -INFINITY && b >= lo && b <= hi;
-                    if (cut) in = in && Key(x, index) <= limit;
-                    f(in, b, place, x, index);
+                    const bool in = (x >= al && x <= ah) || (x >= bl && x <= bh);
+                    hits |= in ? 1u << (i * E + e) : 0u;
                 }
             }
+            if (__ballot(hits != 0) == 0) return;
+            // places for the wave's hits: one addition for all
+            const uint32_t mine = __popc(hits);
+            uint32_t upto = mine;
+#pragma unroll
+            for (int off = 1; off < kWave; off *= 2) {
+                const uint32_t o = __shfl_up(upto, off, kWave);
+                if (Lane() >= off) upto += o;
+            }
+            uint32_t at = 0;
+            if (Lane() == kWave - 1) at = atomicAdd(&s.n_list, upto);
+            at = __builtin_amdgcn_readlane(at, kWave - 1) + upto - mine;
+#pragma unroll
+            for (int i = 0; i < kRounds; ++i) {
+#pragma unroll
+                for (int e = 0; e < E; ++e) {
+                    if (hits >> (i * E + e) & 1) {
+                        if (at < kList) s.list[at] = Key(r.Get(raw[i], e), r.Index(unit[i], e));
+                        ++at;
+                    }
+                }
+            }
+        });
+        __syncthreads();
+        return static_cast<int>(s.n_list);
+    }
+
+    // f(bin, place in it, key) over the row's elements of a span of bins, up to the limit; for
+    // rows whose elements do not fit the list.
+    template <typename F>
+    __device__ void Visit(const Span& span, const F& f) {
+        constexpr int kEach = kSegment * RowUnits<T>::E;  // elements of a segment
+        const float low = Lowest(span.hi), high = Highest(span.lo);
+        const int32_t segments = (r.Units() + kSegment - 1) / kSegment;
+        for (int32_t c0 = 0; c0 < segments; c0 += kChunk) {
+            const int n = Segments(c0, segments, low);
+            for (int j = Tid(); j < n * kEach; j += kChooseThreads) {
+                const int32_t i = r.Index((c0 + s.segment[j / kEach]) * kSegment, j % kEach);
+                if (i < 0 || i >= r.vocab) continue;
+                const float x = T::Get(r.x[i]);
+                if (!(x >= low && x <= high)) continue;
+                double place;
+                const uint64_t key = Key(x, i);
+                const int b = BinOfKey(key, &place);
+                if (span.Has(b) && key <= limit) f(b, place, key);
+            }
+        }
+        __syncthreads();
+    }
+    // The same over the first n of s.list.
+    template <typename F>
+    __device__ void InList(int n, const Span& span, const F& f) {
+        for (int i = Tid(); i < n; i += kChooseThreads) {
+            const uint64_t key = s.list[i];
+            double place;
+            const int b = BinOfKey(key, &place);
+            if (span.Has(b) && key <= limit) f(b, place, key);
+        }
+        __syncthreads();
+    }
+
+    // Least and largest over the workgroup.
+    __device__ void MinMax(uint64_t* lo, uint64_t* hi) {
+#pragma unroll
+        for (int off = kWave / 2; off > 0; off /= 2) {
+            const uint64_t a = __shfl_xor(static_cast<ull>(*lo), off, kWave), b = __shfl_xor(static_cast<ull>(*hi), off, kWave);
+            *lo = a < *lo ? a : *lo;
+            *hi = b > *hi ? b : *hi;
+        }
+        __syncthreads();
+        if (Lane() == 0) {
+            s.scan_u[Wave()] = *lo;
+            s.scan_v[Wave()] = *hi;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < kChooseWaves; ++i) {
+            *lo = s.scan_u[i] < *lo ? s.scan_u[i] : *lo;
+            *hi = s.scan_v[i] > *hi ? s.scan_v[i] : *hi;
         }
     }
 
-    // Which of 512 equal ranges of its bin an element lies in, from the largest down.
-    static __device__ int RangeOf(double place) {
-        const int i = static_cast<int>((0.5 - place) * kBins);
-        return i < 0 ? 0 : i < kBins ? i : kBins - 1;
-    }
-
-    // The elements of bins lo .. hi (range >= 0: of that range of them) into s.sorted; how many
-    // there are (of more than kSort, not all are there).
-    __device__ int Gather(int lo, int hi, int range = -1) {
-        __syncthreads();
-        if (Tid() == 0) s.n = 0;
-        __syncthreads();
-        const int lane = Tid() % kWave;
-        Visit(lo, hi, [&](bool in, int32_t, double place, float x, int32_t i) {
-            if (range >= 0) in = in && RangeOf(place) == range;
-            const uint64_t mask = __ballot(in);
-            if (mask == 0) return;
-            uint32_t at = 0;
-            if (lane == 0) at = atomicAdd(&s.n, static_cast<uint32_t>(__popcll(mask)));
-            at = __builtin_amdgcn_readfirstlane(at) + __popcll(mask & ((uint64_t{1} << lane) - 1));
-            if (in && at < kSort) s.sorted[at] = Key(x, i);
-        });
-        __syncthreads();
-        return static_cast<int>(s.n);
-    }
-
-    // Bin `bin` by its ranges: the one where the sum of whole weights first reaches (kReach)
-    // or passes `bound`; *before: the sum before it.
-    __device__ int RangeWhere(int bin, bool reach, uint64_t bound, uint64_t* before) {
-        __syncthreads();
-        s.bin[Tid()] = 0;
-        __syncthreads();
-        Visit(bin, bin, [&](bool in, int32_t, double place, float, int32_t) {
-            if (in) atomicAdd(reinterpret_cast<ull*>(&s.bin[RangeOf(place)]), static_cast<ull>(Weight(place)));
-        });
-        __syncthreads();
+    // A step of a search: s.bin holds what lies in kBins ranges of the order (what: counts or
+    // sums); the first range where the bound is met after `before`, or the last that holds
+    // any.  *before: with what lies before that range.
+    __device__ int Narrow(Bound what, uint64_t bound, uint64_t* before) {
         uint64_t all;
-        const uint64_t mine = s.bin[Tid()], sum = ScanBlock(mine, s.scan_u, &all);
-        if (bound >= all) bound = reach ? all : all - 1;
-        __syncthreads();
-        if ((reach ? sum >= bound : sum > bound) && (reach ? sum - mine < bound : sum - mine <= bound)) {
-            s.at = static_cast<uint32_t>(Tid());
+        const uint64_t mine = s.bin[Tid()], sum = *before + ScanBlock(mine, s.scan_u, &all);
+        all += *before;
+        // (a bound past the end: the last place)
+        if (what == kPass ? bound >= all : bound > all) bound = what == kPass ? all - 1 : all;
+        const bool ok = what == kPass ? sum > bound && sum - mine <= bound : sum >= bound && sum - mine < bound;
+        if (ok) {
+            s.found[0] = Tid();
             s.word[0] = sum - mine;
         }
         __syncthreads();
         *before = s.word[0];
-        return static_cast<int>(s.at);
+        const int at = s.found[0];
+        __syncthreads();
+        return at;
     }
 
-    // s.sorted[0 .. n - 1] in order, n <= kSort.
-    __device__ void Sort(int n) {
-        int size = 2;
-        while (size < n) size *= 2;
-        for (int i = Tid() + n; i < size; i += kThreads) s.sorted[i] = ~uint64_t{0};
-        for (int k = 2; k <= size; k *= 2) {
-            for (int j = k / 2; j > 0; j /= 2) {
-                __syncthreads();
-                for (int i = Tid(); i < size / 2; i += kThreads) {
-                    const int a = 2 * i - (i & (j - 1)), b = a + j;
-                    const uint64_t x = s.sorted[a], y = s.sorted[b];
-                    if ((x > y) == ((a & k) == 0)) {
-                        s.sorted[a] = y;
-                        s.sorted[b] = x;
-                    }
-                }
-            }
-        }
-        __syncthreads();
-    }
-
-    __device__ double WeightOf(uint64_t key) const {
-        double f;
-        const int32_t b = top - BinOf(h, Logit(static_cast<uint32_t>(key >> 32)), &f);
-        return b < 0 || b >= kBins ? 0.0 : static_cast<double>(Weight(f)) * s.edge[b];
-    }
-
-    // Sums up to each of the sorted elements a thread holds: 4 neighbours.
-    static constexpr int kEach = kSort / kThreads;
-    __device__ void SumSorted(int n, double base, double (&w)[kEach], double (&c)[kEach]) {
-        double mine = 0, all;
-#pragma unroll
-        for (int i = 0; i < kEach; ++i) {
-            const int at = Tid() * kEach + i;
-            w[i] = at < n ? WeightOf(s.sorted[at]) : 0.0;
-            mine += w[i];
-        }
-        double before = base + (ScanBlock(mine, s.scan_d, &all) - mine);
-#pragma unroll
-        for (int i = 0; i < kEach; ++i) {
-            before += w[i];
-            c[i] = before;
-        }
-    }
-    // First of the n sorted elements with ok(sum, weight); n if none.
-    template <typename F>
-    __device__ int FirstSorted(int n, const double (&w)[kEach], const double (&c)[kEach], const F& ok) {
-        __syncthreads();
-        if (Tid() == 0) s.at = static_cast<uint32_t>(n);
-        __syncthreads();
-#pragma unroll
-        for (int i = kEach - 1; i >= 0; --i) {
-            const int at = Tid() * kEach + i;
-            if (at < n && ok(c[i], w[i])) atomicMin(&s.at, static_cast<uint32_t>(at));
-        }
-        __syncthreads();
-        return static_cast<int>(s.at);
-    }
-    // Sum up to sorted element i.
-    __device__ double SumAt(int i, const double (&c)[kEach]) {
-        __syncthreads();
-#pragma unroll
-        for (int e = 0; e < kEach; ++e) {
-            if (Tid() * kEach + e == i) s.scan_d[0] = c[e];
-        }
-        __syncthreads();
-        const double v = s.scan_d[0];
-        __syncthreads();
-        return v;
-    }
-
-    // By digits of the keys of one bin's elements, pass by pass over the row: the first with
-    // count >= bound (kCount), sum >= bound or sum > bound (whole numbers, of this bin's
-    // middle).  Its key; *before and *own: the sum before it and its own weight.
-    enum Bound { kCount, kReach, kPass };
-    __device__ uint64_t Search(int bin, Bound what, uint64_t bound, uint64_t* before, uint64_t* own) {
-        uint64_t high = 0, n0 = 0, m0 = 0;
-        constexpr int kDigit = 9, kShifts = 8;  // 64 bits: 1 and 7 times 9
-        for (int d = kShifts - 1; d >= 0; --d) {
-            const int shift = d * kDigit;
+    // The first place of bin `bin`, all of whose elements are in the list of n, to meet the
+    // bound: ranges of the keys that are left, 1024 of them at a time, until a wave holds them.
+    __device__ Place Select(int n, int bin, Bound what, uint64_t bound) {
+        const Span span{bin, bin};
+        uint64_t lo = 0, hi = ~uint64_t{0}, before = 0;
+        for (;;) {
+            uint64_t least = ~uint64_t{0}, most = 0;
+            if (Tid() == 0) s.n_few = 0;
             __syncthreads();
-            for (int i = Tid(); i < kBins; i += kThreads) {
-                s.bin[i] = 0;
-                s.number[i] = 0;
-            }
-            __syncthreads();
-            Visit(bin, bin, [&](bool in, int32_t, double f, float x, int32_t i) {
-                const uint64_t key = Key(x, i);
-                // (the first digit has one bit, the key's highest)
-                if (!in || (d < kShifts - 1 && key >> (shift + kDigit) != high)) return;
-                const int at = static_cast<int>(key >> shift) & (kBins - 1);
-                atomicAdd(&s.number[at], 1u);
-                atomicAdd(reinterpret_cast<ull*>(&s.bin[at]), static_cast<ull>(Weight(f)));
+            InList(n, span, [&](int, double, uint64_t key) {
+                if (key < lo || key > hi) return;
+                least = key < least ? key : least;
+                most = key > most ? key : most;
+                const uint32_t at = atomicAdd(&s.n_few, 1u);
+                if (at < kWave) s.few[at] = key;
             });
+            if (s.n_few <= kWave) break;
+            MinMax(&least, &most);
+            int shift = 0;
+            while ((most - least) >> shift >= kBins) ++shift;
+            s.bin[Tid()] = 0;
             __syncthreads();
-            uint64_t sums = 0, counts = 0, all;
-            const uint64_t my_m = s.bin[Tid()], my_n = s.number[Tid()];
-            sums = m0 + ScanBlock(my_m, s.scan_u, &all);
-            counts = n0 + ScanBlock(my_n, s.scan_u, &all);
-            const bool ok = my_n != 0 && (what == kCount ? counts >= bound : what == kReach ? sums >= bound : sums > bound);
-            __syncthreads();
-            if (Tid() == 0) s.at = kBins;
-            __syncthreads();
-            if (ok) atomicMin(&s.at, static_cast<uint32_t>(Tid()));
-            __syncthreads();
-            if (s.at == kBins) {  // none: the last element
-                if (Tid() == 0) s.at = 0;
-                __syncthreads();
-                if (my_n != 0) atomicMax(&s.at, static_cast<uint32_t>(Tid()));
-                __syncthreads();
-            }
-            const uint32_t at = s.at;
-            if (static_cast<uint32_t>(Tid()) == at) {
-                s.word[0] = sums - my_m;
-                s.word[1] = counts - my_n;
-                s.word[2] = my_m;
-            }
-            __syncthreads();
-            high = (high << kDigit) | at;
-            m0 = s.word[0];
-            n0 = s.word[1];
-            *own = s.word[2];
+            InList(n, span, [&](int, double place, uint64_t key) {
+                if (key < lo || key > hi) return;
+                atomicAdd(reinterpret_cast<ull*>(&s.bin[(key - least) >> shift]),
+                          static_cast<ull>(what == kCount ? 1 : Weight(place)));
+            });
+            const uint64_t at = Narrow(what, bound, &before);
+            lo = least + (at << shift);
+            hi = lo + ((uint64_t{1} << shift) - 1);
         }
-        *before = m0;
+        // one wave: every lane an element, its place by comparison with all others
+        if (Tid() < kWave) {
+            const int m = static_cast<int>(s.n_few);
+            const bool real = Tid() < m;
+            const uint64_t key = real ? s.few[Tid()] : ~uint64_t{0};
+            double place;
+            BinOfKey(real ? key : s.few[0], &place);
+            const uint64_t own = Weight(place), one = what == kCount ? 1 : own;
+            s.bin[Tid()] = one;
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            uint64_t sum = before;
+#pragma unroll 8
+            for (int i = 0; i < m; ++i) sum += s.few[i] <= key ? s.bin[i] : 0;
+            const bool ok = real && (what == kPass ? sum > bound : sum >= bound);
+            // the first that is ok; none: the last of all
+            uint64_t best = __ballot(ok) != 0 ? (ok ? key : ~uint64_t{0}) : (real ? ~key : ~uint64_t{0});
+#pragma unroll
+            for (int off = kWave / 2; off > 0; off /= 2) {
+                const uint64_t o = __shfl_xor(static_cast<ull>(best), off, kWave);
+                best = o < best ? o : best;
+            }
+            if (__ballot(ok) == 0) best = ~best;
+            if (real && key == best) {
+                s.word[0] = key;
+                s.word[1] = sum - one;
+                s.word[2] = own;
+            }
+        }
         __syncthreads();
-        return high;
+        const Place at{s.word[0], s.word[1], s.word[2]};
+        __syncthreads();
+        return at;
+    }
+
+    // The same for a bin of more elements than the list holds (nearly equal logits): by the
+    // digits of their keys, pass by pass over the row.
+    __device__ Place Search(int bin, Bound what, uint64_t bound) {
+        uint64_t high = 0, before = 0;
+        constexpr int kDigit = 10;
+        for (int shift = 60; shift >= 0; shift -= kDigit) {
+            __syncthreads();
+            s.bin[Tid()] = 0;
+            Visit({bin, bin}, [&](int, double place, uint64_t key) {
+                if (shift < 60 && key >> (shift + kDigit) != high) return;
+                atomicAdd(reinterpret_cast<ull*>(&s.bin[(key >> shift) & (kBins - 1)]),
+                          static_cast<ull>(what == kCount ? 1 : Weight(place)));
+            });
+            high = (high << kDigit) | static_cast<uint64_t>(Narrow(what, bound, &before));
+        }
+        double place;
+        BinOfKey(high, &place);
+        return {high, before, Weight(place)};
+    }
+
+    // A bound on the sum over all as one on whole weights within bin `bin`.
+    __device__ uint64_t InBin(double bound, int bin, bool reach) const {
+        const double in = (bound - Below(bin)) / s.edge[bin];
+        if (reach) return in > 1.0 ? static_cast<uint64_t>(ceil(in)) : 1;
+        return in > 0.0 ? static_cast<uint64_t>(in) : 0;
     }
 
     // Sums over the bins from their masses.
     __device__ void SumBins() {
         double all;
+        __syncthreads();
         const double mine = static_cast<double>(s.bin[Tid()]) * s.edge[Tid()];
-        const double c = ScanBlock(mine, s.scan_d, &all);
-        s.sum[Tid()] = c;
+        s.sum[Tid()] = ScanBlock(mine, s.scan_d, &all);
         __syncthreads();
     }
-    __device__ double Below(int bin) const { return bin > 0 ? s.sum[bin - 1] : 0.0; }
-
-    // The element of bins up to `last` where the sum passes `bound`.
-    struct Found {
-        uint64_t key;
-        double own;
-    };
-    __device__ Found Pass(double bound, int last) {
-        int bin = First(last + 1, [&](int i) { return s.sum[i] > bound; });
-        // (rounding: not above the last; and one that has elements)
-        if (bin > last) bin = last;
-        if (Below(bin) == s.sum[bin]) bin = First(last + 1, [&](int i) { return s.sum[i] == s.sum[last]; });
-        const double base = Below(bin);
-        const double in = (bound - base) / s.edge[bin];  // in whole weights of the bin
-        const uint64_t whole = in > 0.0 ? static_cast<uint64_t>(in) : 0;
-        double from = base;
-        int n = Gather(bin, bin);
-        if (n > kSort) n = GatherRange(bin, false, whole, &from);
-        if (n <= kSort) {
-            Sort(n);
-            double w[kEach], c[kEach];
-            SumSorted(n, from, w, c);
-            int at = FirstSorted(n, w, c, [&](double sum, double) { return sum > bound; });
-            at = at < n ? at : n - 1;
-            return {s.sorted[at], WeightOf(s.sorted[at])};
+    // First bins up to `last` whose sum is past (reach: at least) each bound; `last` if none.
+    __device__ void FirstBins(int last, bool reach, double x, double y, int* at_x, int* at_y) {
+        if (Tid() < 2) s.found[Tid()] = last;
+        __syncthreads();
+        const double sum = s.sum[Tid()], before = Below(Tid());
+        if (Tid() < last) {
+            if (reach ? sum >= x && (Tid() == 0 || before < x) : sum > x && (Tid() == 0 || before <= x)) s.found[0] = Tid();
+            if (reach ? sum >= y && (Tid() == 0 || before < y) : sum > y && (Tid() == 0 || before <= y)) s.found[1] = Tid();
         }
-        uint64_t before, own;
-        const uint64_t key = Search(bin, kPass, whole, &before, &own);
-        return {key, static_cast<double>(own) * s.edge[bin]};
-    }
-
-    // The least sum up to an element of bin `bin` that reaches `bound`.
-    __device__ double Reach(double bound, int bin) {
-        const double base = Below(bin);
-        const double in = ceil((bound - base) / s.edge[bin]);
-        const uint64_t whole = in > 1.0 ? static_cast<uint64_t>(in) : 1;
-        double from = base;
-        int n = Gather(bin, bin);
-        if (n > kSort) n = GatherRange(bin, true, whole, &from);
-        if (n <= kSort) {
-            Sort(n);
-            double w[kEach], c[kEach];
-            SumSorted(n, from, w, c);
-            const int at = FirstSorted(n, w, c, [&](double sum, double) { return sum >= bound; });
-            return SumAt(at < n ? at : n - 1, c);
-        }
-        uint64_t before, own;
-        Search(bin, kReach, whole, &before, &own);
-        return base + static_cast<double>(before + own) * s.edge[bin];
-    }
-
-    // The range of a bin in which a bound lies, gathered; *from: the sum before it.
-    __device__ int GatherRange(int bin, bool reach, uint64_t whole, double* from) {
-        uint64_t before;
-        const int range = RangeWhere(bin, reach, whole, &before);
-        *from += static_cast<double>(before) * s.edge[bin];
-        return Gather(bin, bin, range);
+        __syncthreads();
+        *at_x = s.found[0];
+        *at_y = s.found[1];
+        __syncthreads();
     }
 };
 
 template <typename T>
-__global__ __launch_bounds__(kThreads) void SampleChoose(const SampleArgs p) {
+__global__ __launch_bounds__(kChooseThreads) void SampleChoose(const SampleArgs p) {
     __shared__ Choice s;
     const int tid = static_cast<int>(threadIdx.x);
     const int64_t row = blockIdx.x;
@@ -699,7 +721,6 @@ __global__ __launch_bounds__(kThreads) void SampleChoose(const SampleArgs p) {
             if (tid == 0) s.tops[i] = part.flags & kSome ? part.top : INT32_MIN;
         }
     }
-    __syncthreads();
     if (h.bad || !(flags & kSome) || (flags & kNan)) {
         if (tid == 0) {
             p.tokens[row] = -1;
@@ -715,128 +736,160 @@ __global__ __launch_bounds__(kThreads) void SampleChoose(const SampleArgs p) {
         }
         return;
     }
+    __syncthreads();
     Chooser<T> ch{p, h, s, RowUnits<T>(p, row), p.largest + row * p.segments, top, ~uint64_t{0}};
-    static_assert(kBins == kThreads, "a thread a bin");
+    static_assert(kBins == kChooseThreads, "a thread a bin");
     uint64_t mine = 0;
 #pragma unroll 8
     for (int i = 0; i < p.parts; ++i) {
         const int32_t at = s.tops[i] == INT32_MIN ? -1 : s.tops[i] - (top - tid);  // this thread's bin in the part
         if (at >= 0) mine += reinterpret_cast<const uint64_t*>(parts + i * kPartBytes + sizeof(Part))[at];
     }
-    s.edge[tid] = exp(tid * (-1.0 / 16));
-    s.bin[tid] = mine;
-    __syncthreads();
-    int k = h.k, last = kBins - 1;
-    bool in_list = false;  // all that can be chosen is to be sorted
-    if (k != 0) {
-        uint64_t all;
-        const uint64_t upto = ScanBlock(mine, s.scan_u, &all);
-        s.bin[tid] = upto;
-        __syncthreads();
-        if (all <= static_cast<uint64_t>(k)) k = 0;  // the others weigh nothing
-        else last = ch.First(kBins, [&](int i) { return s.bin[i] >= static_cast<uint64_t>(k); });
-        const uint64_t n = s.bin[last], before = last > 0 ? s.bin[last - 1] : 0;
-        in_list = n <= kSort;
-        __syncthreads();
-        if (!in_list) {
-            if (k != 0) {
-                uint64_t sum, own;
-                ch.limit = ch.Search(last, Chooser<T>::kCount, k - before, &sum, &own);
+    s.edge[tid] = exp(tid * (-1.0 / kPerUnit));
+    // Three places are looked for in turn, each where its cut is asked for: the top-k's, the
+    // top-p's (with the sum that min-p leaves) and the token's.  The row is gathered once for
+    // the first two as a rule, or once for the last two.
+    enum { kTopK, kTopP, kToken };
+    int last = kBins - 1;       // no element of a later bin can be chosen
+    int n = -1;                 // elements of the list, where it has all that is needed
+    const double u = h.u;
+    double kept = 0.0, least = 0.0, reach = 0.0;
+    bool by_p = h.p < 1.0f, by_m = h.m > 0.0f;
+    Span m{0, 0}, drawn{0, 0};
+    int p_bin = 0;
+#pragma unroll 1
+    for (int what = h.k != 0 ? kTopK : kTopP; what <= kToken; ++what) {
+        Span a, b;      // bins to gather, if there is no list
+        bool look = true, cuts = false;
+        int bin;
+        uint64_t bound;
+        if (what == kTopK) {
+            uint64_t all;
+            const uint64_t upto = ScanBlock(mine, s.scan_u, &all), k = static_cast<uint64_t>(h.k);
+            cuts = all > k;  // else what is beyond the bins weighs nothing
+            if (cuts ? upto >= k && upto - mine < k : tid == kBins - 1) {
+                s.found[0] = tid;
+                s.word[0] = upto;
+                s.word[1] = upto - mine;
             }
-            // the masses of what is left
+            __syncthreads();
+            last = bin = s.found[0];
+            const uint64_t held = s.word[0];
+            bound = k - s.word[1];
+            __syncthreads();
+            a = b = {held <= kList ? 0 : last, last};
+            look = cuts;
+        } else if (what == kTopP) {
+            if (h.k == 0) s.bin[tid] = mine;
+            ch.SumBins();
+            kept = s.sum[last];
+            double low = kept;  // what is kept will weigh low .. kept
+            if (by_p) {
+                int same;
+                reach = static_cast<double>(h.p) * kept;
+                ch.FirstBins(last, true, reach, reach, &p_bin, &same);
+            }
+            if (by_m) {
+                float x = -INFINITY;  // the largest logit
+                const int segments = (ch.r.Units() + kSegment - 1) / kSegment;
+                for (int i = tid; i < segments; i += kChooseThreads) x = fmaxf(x, ch.largest[i]);
+                x = BlockMax<kChooseWaves>(x, reinterpret_cast<float*>(s.scan_u));
+                __syncthreads();
+                least = fmin(static_cast<double>(h.m), 1.0) * ch.WeightOf(x);  // its equals are kept
+                const double where = -static_cast<double>(kPerUnit) * log(least / kOne);
+                m.hi = where >= kBins ? kBins - 1 : static_cast<int>(where + 0.51);
+                m.lo = m.hi > 1 ? m.hi - 2 : 0;
+                // whichever cut lies in earlier bins is the one
+                if (m.lo > last || (by_p && m.lo > p_bin)) by_m = false;
+                else if (by_p && m.hi < p_bin) by_p = false;
+                if (m.hi > last) m.hi = last;
+            }
+            a = {0, -1};
+            if (by_p) {
+                a = {p_bin, p_bin};
+                last = p_bin;
+                kept = s.sum[p_bin];
+                low = ch.Below(p_bin);
+            }
+            if (by_m) {
+                a = {by_p && p_bin < m.lo ? p_bin : m.lo, by_p && p_bin > m.hi ? p_bin : m.hi};
+                if (m.hi < last) last = m.hi;
+                if (s.sum[m.hi] < kept) kept = s.sum[m.hi];
+                if (ch.Below(m.lo) < low) low = ch.Below(m.lo);
+            }
+            ch.FirstBins(last, false, u * low, u * kept, &drawn.lo, &drawn.hi);
+            b = drawn;
+            if (a.lo > a.hi) a = b;
+            bin = p_bin;
+            bound = by_p ? ch.InBin(reach, p_bin, true) : 0;
+            look = by_p;
+        } else {
+            int same;
+            const double x = u * kept;
+            ch.FirstBins(last, false, x, x, &bin, &same);
+            bin = bin < drawn.lo ? drawn.lo : bin > drawn.hi ? drawn.hi : bin;  // (sums' roundings)
+            bound = ch.InBin(x, bin, false);
+            a = b = {bin, bin};
+        }
+        bool whole = true;  // the list serves the places looked for later too
+        for (int tries = 0; n < 0 && tries < 2; ++tries) {
+            n = ch.Gather(a, b);
+            if (n > kList) n = -1;
+            whole = tries == 0 && !(what == kTopK && a.lo != 0);
+            a = b = {bin, bin};
+        }
+        if (what == kTopP && by_m) {
+            uint64_t sum[3] = {0, 0, 0};
+            auto add = [&](int at, double place, uint64_t) {
+                const uint64_t w = Weight(place);
+                if (static_cast<double>(w) * s.edge[at] < least) return;
+#pragma unroll
+                for (int i = 0; i < 3; ++i) sum[i] += at - m.lo == i ? w : 0;
+            };
+            if (n >= 0 && whole) ch.InList(n, m, add);
+            else ch.Visit(m, add);
+            double upto = ch.Below(m.lo);
+#pragma unroll
+            for (int i = 0; i < 3; ++i) {
+                uint64_t all;
+                ScanBlock(sum[i], s.scan_u, &all);
+                if (m.lo + i <= m.hi) upto += static_cast<double>(all) * s.edge[m.lo + i];
+            }
+            kept = upto;
+        }
+        if (look) {
+            constexpr Bound kBounds[3] = {kCount, kReach, kPass};
+            const Bound meets = kBounds[what];
+            const Place at = n >= 0 ? ch.Select(n, bin, meets, bound) : ch.Search(bin, meets, bound);
+            if (what == kTopK) {
+                ch.limit = at.key;
+            } else if (what == kTopP) {
+                const double upto = ch.Below(bin) + static_cast<double>(at.before + at.own) * s.edge[bin];
+                if (!by_m || upto < kept) kept = upto;
+            } else if (tid == 0) {
+                p.tokens[row] = static_cast<int32_t>(at.key);
+                if (p.prob != nullptr) p.prob[row] = static_cast<float>(static_cast<double>(at.own) * s.edge[bin] / kept);
+            }
+        }
+        if (what == kTopK) {  // the masses of what is left
             s.bin[tid] = 0;
             __syncthreads();
-            ch.Visit(0, last, [&](bool in, int32_t b, double f, float, int32_t) {
-                if (in) atomicAdd(reinterpret_cast<ull*>(&s.bin[b]), static_cast<ull>(Weight(f)));
-            });
-            __syncthreads();
+            auto add = [&](int at, double place, uint64_t) {
+                atomicAdd(reinterpret_cast<ull*>(&s.bin[at]), static_cast<ull>(Weight(place)));
+            };
+            if (n >= 0 && whole) ch.InList(n, {0, last}, add);
+            else ch.Visit({0, last}, add);
         }
-    }
-    double least = 0.0;  // a weight's, by min_p
-    if (h.m > 0.0f) {
-        // the largest weight: that of the row's first, at the largest bin's place
-        float m = -INFINITY;
-        const int segments = (ch.r.Units() + kSegment - 1) / kSegment;
-        for (int i = tid; i < segments; i += kThreads) m = fmaxf(m, ch.largest[i]);
-        __syncthreads();
-        m = BlockMax<kWaves>(m, reinterpret_cast<float*>(s.scan_u));
-        const double w = ch.WeightOf(Key(m, 0));
-        least = fmin(static_cast<double>(h.m), 1.0) * w;  // the first at least, and its equals
-    }
-    double bound;
-    if (!in_list) {
-        ch.SumBins();
-        double kept = s.sum[last];
-        if (h.p < 1.0f) {
-            const double reach = static_cast<double>(h.p) * kept;
-            const int bin = ch.First(last, [&](int i) { return s.sum[i] >= reach; });
-            kept = ch.Reach(reach, bin);
-            last = bin;
-        }
-        if (h.m > 0.0f) {
-            // the bins that least lies in or beside
-            const double where = -16.0 * log(least / kOne);
-            int hi = where >= kBins ? kBins - 1 : static_cast<int>(where + 0.51);
-            const int lo = hi > 1 ? hi - 2 : 0;
-            if (lo <= last) {
-                hi = hi < last ? hi : last;
-                uint64_t sum[3] = {0, 0, 0};
-                ch.Visit(lo, hi, [&](bool in, int32_t b, double f, float, int32_t) {
-                    if (!in) return;
-                    const uint64_t w = Weight(f);
-                    if (static_cast<double>(w) * s.edge[b] < least) return;
-#pragma unroll
-                    for (int i = 0; i < 3; ++i) sum[i] += b - lo == i ? w : 0;
-                });
-                double upto = ch.Below(lo);
-                for (int i = 0; i < 3; ++i) {
-                    uint64_t all;
-                    ScanBlock(sum[i], s.scan_u, &all);
-                    if (lo + i <= hi) upto += static_cast<double>(all) * s.edge[lo + i];
-                }
-                if (upto < kept) kept = upto;
-                if (hi < last) last = hi;
-                __syncthreads();
-            }
-        }
-        bound = static_cast<double>(h.u) * kept;
-        const auto found = ch.Pass(bound, last);
-        if (tid == 0) {
-            p.tokens[row] = static_cast<int32_t>(found.key);
-            if (p.prob != nullptr) p.prob[row] = static_cast<float>(found.own / kept);
-        }
-        return;
-    }
-    const int n = ch.Gather(0, last);
-    ch.Sort(n);
-    double w[Chooser<T>::kEach], c[Chooser<T>::kEach];
-    ch.SumSorted(n, 0.0, w, c);
-    int kept = k != 0 && k < n ? k : n;
-    if (h.p < 1.0f) {
-        const double reach = static_cast<double>(h.p) * ch.SumAt(kept - 1, c);
-        const int at = ch.FirstSorted(kept, w, c, [&](double sum, double) { return sum >= reach; });
-        kept = at < kept ? at + 1 : kept;
-    }
-    if (h.m > 0.0f) {
-        const int at = ch.FirstSorted(kept, w, c, [&](double, double weight) { return weight < least; });
-        kept = at < 1 ? 1 : at;
-    }
-    const double whole = ch.SumAt(kept - 1, c);
-    bound = static_cast<double>(h.u) * whole;
-    int at = ch.FirstSorted(kept, w, c, [&](double sum, double) { return sum > bound; });
-    at = at < kept ? at : kept - 1;
-    if (tid == 0) {
-        p.tokens[row] = static_cast<int32_t>(s.sorted[at]);
-        if (p.prob != nullptr) p.prob[row] = static_cast<float>(ch.WeightOf(s.sorted[at]) / whole);
+        if (!whole) n = -1;
     }
 }
 
-// Workgroups of the first pass a row: as many as fill the device at 3 a compute unit,
-// with 2 blocks of 64 loads at least for each wave.
+// Workgroups of the first pass a row: as many as fill the device at 2 a compute unit,
+// with kAhead blocks of 64 loads at least for each wave.
 int Parts(int64_t n_rows, int64_t vocab, int bytes) {
     const int64_t blocks = (vocab * bytes + 1023) / 1024;
-    int64_t parts = (static_cast<int64_t>(ComputeUnits()) * 3 + n_rows - 1) / n_rows;
-    const int64_t most = blocks / (2 * kWaves);  // 2 blocks a wave
+    int64_t parts = (static_cast<int64_t>(ComputeUnits()) * 2 + n_rows - 1) / n_rows;
+    const int64_t most = blocks / (kAhead * kWaves);
     if (parts > most) parts = most;
     if (parts > kMaxParts) parts = kMaxParts;
     return static_cast<int>(parts < 1 ? 1 : parts);
@@ -848,7 +901,7 @@ int64_t Segments(int64_t vocab, int bytes) {  // one more where the row is not a
 template <typename T>
 void Launch(const SampleArgs& p, int64_t n_rows, hipStream_t s) {
     hipLaunchKernelGGL(SampleBins<T>, dim3(static_cast<unsigned>(n_rows * p.parts)), dim3(kThreads), 0, s, p);
-    hipLaunchKernelGGL(SampleChoose<T>, dim3(static_cast<unsigned>(n_rows)), dim3(kThreads), 0, s, p);
+    hipLaunchKernelGGL(SampleChoose<T>, dim3(static_cast<unsigned>(n_rows)), dim3(kChooseThreads), 0, s, p);
 }
 
 }  // namespace

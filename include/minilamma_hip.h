@@ -604,7 +604,7 @@ typedef struct {
  * temperature 0 (uniform is then not looked at).  A logit of -infinity is never
  * chosen; logits of +infinity share all the weight.  Weights below 2^-44 (30
  * temperatures below the largest) may count as 0; temperatures below 2^-14 count
- * as 2^-14, logits of over 2^25 temperatures in size as that.
+ * as 2^-14, logits of over 2^24 temperatures in size as that.
  * The weights are added as whole numbers: a row's token depends on
  * neither the other rows nor how the work is divided, run for run.
  * A row that has a NaN, or only -infinities, or a setting that is a NaN, a negative
