@@ -54,9 +54,22 @@ struct Part {
     int32_t top;     // its largest bin
     uint32_t flags;  // kSome, kNan
     uint64_t best;   // temperature 0: the order's first
+    float largest;   // logit
+    int32_t unused[3];
 };
 constexpr uint32_t kSome = 1, kNan = 2;
 constexpr int64_t kPartBytes = sizeof(Part) + kBins * 8;
+
+// What the second pass leaves of a row for the two that follow, then the kBins masses (or
+// counts) of its bins, then kList keys.
+struct RowState {
+    int32_t top;     // its largest bin
+    float largest;   // logit
+    float al, ah, bl, bh;  // logits to gather: al .. ah and bl .. bh
+    uint32_t live;   // 0: its token is chosen
+    uint32_t n;      // how many were gathered
+};
+constexpr int64_t kStateBytes = sizeof(RowState) + kBins * 8 + kList * 8;
 
 struct SampleArgs {
     const void* x;
@@ -67,6 +80,7 @@ struct SampleArgs {
     int32_t* tokens;
     float* prob;
     char* part;      // [rows][parts] of kPartBytes
+    char* state;     // [rows] of kStateBytes
     float* largest;  // [rows][segments]
     int32_t* err;
 };
@@ -127,6 +141,8 @@ __device__ inline float Logit(uint32_t key) {
 __device__ inline uint64_t Key(float x, int32_t i) {
     return (static_cast<uint64_t>(Descending(x)) << 32) | static_cast<uint32_t>(i);
 }
+
+constexpr uint64_t kNoKey = ~uint64_t{0}, kLastKey = kNoKey - 1;  // past every element's
 
 // A row as units of 16 bytes from the last 16-byte boundary at or before it.
 template <typename T>
@@ -195,6 +211,7 @@ __global__ __launch_bounds__(kThreads) void SampleBins(const SampleArgs p) {
     __shared__ int32_t tops[kWaves];
     __shared__ uint32_t flags_of[kWaves];
     __shared__ uint64_t best_of[kWaves];
+    __shared__ float largest_of[kWaves];
     const int tid = static_cast<int>(threadIdx.x), lane = tid % kWave;
     const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
     const int64_t row = blockIdx.x / p.parts;
@@ -301,17 +318,20 @@ __global__ __launch_bounds__(kThreads) void SampleBins(const SampleArgs p) {
         tops[wave] = top;
         flags_of[wave] = (some ? kSome : 0) | (nan ? kNan : 0);
         best_of[wave] = best;
+        largest_of[wave] = so_far;
     }
     __syncthreads();
     uint32_t flags = 0;
     int32_t all_top = INT32_MIN;
+    float most = -INFINITY;
     for (int w = 0; w < kWaves; ++w) {
         flags |= flags_of[w];
         if ((flags_of[w] & kSome) && tops[w] > all_top) all_top = tops[w];
         if (best_of[w] < best) best = best_of[w];
+        most = fmaxf(most, largest_of[w]);
     }
     Part* out = reinterpret_cast<Part*>(p.part + blockIdx.x * kPartBytes);
-    if (tid == 0) *out = {all_top, flags, best};
+    if (tid == 0) *out = {all_top, flags, best, most, {}};
     if (h.t == 0.0f || !(flags & kSome)) return;
     uint64_t* bins = reinterpret_cast<uint64_t*>(out + 1);
     for (int i = tid; i < kBins; i += kThreads) {
@@ -359,7 +379,6 @@ struct Choice {
     uint64_t few[kWave];
     uint64_t scan_u[kChooseWaves], scan_v[kChooseWaves];
     double scan_d[kChooseWaves];
-    int32_t tops[kMaxParts];  // the parts' largest bins, INT32_MIN: none
     int32_t found[2];
     uint32_t n_list, n_segments, n_few;
     uint64_t word[3];
@@ -442,78 +461,21 @@ struct Chooser {
         return static_cast<int>(s.n_segments);
     }
 
-    // f(there, raw unit, its number) over the units of the row that have elements of at least
-    // `low` near; 8 lanes a segment, kRounds of them on their way at once.  Whole waves call f.
-    static constexpr int kRounds = 32 / RowUnits<T>::E;
-    template <typename F>
-    __device__ void Units(float low, const F& f) {
-        constexpr int kGroups = kWave / kSegment;
-        const int32_t units = r.Units(), segments = (units + kSegment - 1) / kSegment;
-        for (int32_t c0 = 0; c0 < segments; c0 += kChunk) {
-            const int n = Segments(c0, segments, low);
-            for (int g = Wave() * kGroups; g < n; g += kChooseWaves * kGroups * kRounds) {
-                u32x4 raw[kRounds];
-                int32_t unit[kRounds];
-#pragma unroll
-                for (int i = 0; i < kRounds; ++i) {
-                    const int j = g + i * kChooseWaves * kGroups + Lane() / kSegment;
-                    unit[i] = j < n ? (c0 + s.segment[j]) * kSegment + Lane() % kSegment : units;
-                    raw[i] = r.Load(unit[i], unit[i] < units);
-                }
-                f(raw, unit);
-            }
-        }
-    }
-
-    // The elements of two spans of bins (and a few of their neighbours) into s.list; how many
-    // there are (of more than kList, not all are there).
-    __device__ int Gather(const Span& a, const Span& b) {
-        constexpr int E = RowUnits<T>::E;
-        const float al = Lowest(a.hi), ah = Highest(a.lo), bl = Lowest(b.hi), bh = Highest(b.lo);
-        __syncthreads();
-        if (Tid() == 0) s.n_list = 0;  // (a barrier follows in Units)
-        Units(fminf(al, bl), [&](const u32x4 (&raw)[kRounds], const int32_t (&unit)[kRounds]) {
-            uint32_t hits = 0;
-#pragma unroll
-            for (int i = 0; i < kRounds; ++i) {
-#pragma unroll
-                for (int e = 0; e < E; ++e) {
-                    const float x = r.Get(raw[i], e);
-                    const bool in = (x >= al && x <= ah) || (x >= bl && x <= bh);
-                    hits |= in ? 1u << (i * E + e) : 0u;
-                }
-            }
-            if (__ballot(hits != 0) == 0) return;
-            // places for the wave's hits: one addition for all
-            const uint32_t mine = __popc(hits);
-            uint32_t upto = mine;
-#pragma unroll
-            for (int off = 1; off < kWave; off *= 2) {
-                const uint32_t o = __shfl_up(upto, off, kWave);
-                if (Lane() >= off) upto += o;
-            }
-            uint32_t at = 0;
-            if (Lane() == kWave - 1) at = atomicAdd(&s.n_list, upto);
-            at = __builtin_amdgcn_readlane(at, kWave - 1) + upto - mine;
-#pragma unroll
-            for (int i = 0; i < kRounds; ++i) {
-#pragma unroll
-                for (int e = 0; e < E; ++e) {
-                    if (hits >> (i * E + e) & 1) {
-                        if (at < kList) s.list[at] = Key(r.Get(raw[i], e), r.Index(unit[i], e));
-                        ++at;
-                    }
-                }
-            }
+    // The elements of a bin (and a few of its neighbours) into s.list; how many there are (of
+    // more than kList, not all are there).
+    __device__ int Gather(int bin) {
+        if (Tid() == 0) s.n_list = 0;  // (a barrier follows in Segments)
+        Near({bin, bin}, [&](float x, int32_t i) {
+            const uint32_t at = atomicAdd(&s.n_list, 1u);
+            if (at < kList) s.list[at] = Key(x, i);
         });
-        __syncthreads();
         return static_cast<int>(s.n_list);
     }
 
-    // f(bin, place in it, key) over the row's elements of a span of bins, up to the limit; for
-    // rows whose elements do not fit the list.
+    // f(logit, index) over the row's elements near a span of bins: of each 128 bytes whose
+    // largest is no lower than those.
     template <typename F>
-    __device__ void Visit(const Span& span, const F& f) {
+    __device__ void Near(const Span& span, const F& f) {
         constexpr int kEach = kSegment * RowUnits<T>::E;  // elements of a segment
         const float low = Lowest(span.hi), high = Highest(span.lo);
         const int32_t segments = (r.Units() + kSegment - 1) / kSegment;
@@ -521,16 +483,21 @@ struct Chooser {
             const int n = Segments(c0, segments, low);
             for (int j = Tid(); j < n * kEach; j += kChooseThreads) {
                 const int32_t i = r.Index((c0 + s.segment[j / kEach]) * kSegment, j % kEach);
-                if (i < 0 || i >= r.vocab) continue;
-                const float x = T::Get(r.x[i]);
-                if (!(x >= low && x <= high)) continue;
-                double place;
-                const uint64_t key = Key(x, i);
-                const int b = BinOfKey(key, &place);
-                if (span.Has(b) && key <= limit) f(b, place, key);
+                const float x = i >= 0 && i < r.vocab ? T::Get(r.x[i]) : -INFINITY;
+                if (x >= low && x <= high) f(x, i);
             }
         }
         __syncthreads();
+    }
+    // f(bin, place in it, key) over the row's elements of a span of bins, up to the limit.
+    template <typename F>
+    __device__ void Visit(const Span& span, const F& f) {
+        Near(span, [&](float x, int32_t i) {
+            double place;
+            const uint64_t key = Key(x, i);
+            const int b = BinOfKey(key, &place);
+            if (span.Has(b) && key <= limit) f(b, place, key);
+        });
     }
     // The same over the first n of s.list.
     template <typename F>
@@ -586,36 +553,68 @@ struct Chooser {
         return at;
     }
 
+    // Which of kBins equal ranges of its bin an element lies in, from the largest down.
+    static __device__ int RangeOf(double place) {
+        const int i = static_cast<int>((0.5 - place) * kBins);
+        return i < 0 ? 0 : i < kBins ? i : kBins - 1;
+    }
+    // s.few[0 .. 63] of the list's elements of bin `bin` with ok(place, key), and their number;
+    // s.bin, of ranges, gets what each element weighs there.
+    template <typename F, typename R>
+    __device__ void Few(int n, int bin, Bound what, const F& ok, const R& range) {
+        if (Tid() == 0) s.n_few = 0;
+        s.bin[Tid()] = 0;
+        __syncthreads();
+        for (int i0 = 0; i0 < n; i0 += kChooseThreads) {
+            const uint64_t key = i0 + Tid() < n ? s.list[i0 + Tid()] : kNoKey;
+            double place;
+            const bool in = BinOfKey(key, &place) == bin && i0 + Tid() < n && key <= limit && ok(place, key);
+            const uint64_t mask = __ballot(in);
+            if (mask == 0) continue;
+            uint32_t at = 0;
+            if (Lane() == 0) at = atomicAdd(&s.n_few, static_cast<uint32_t>(__popcll(mask)));
+            at = __builtin_amdgcn_readfirstlane(at) + __popcll(mask & ((uint64_t{1} << Lane()) - 1));
+            if (in && at < kWave) s.few[at] = key;
+            if (in) {
+                atomicAdd(reinterpret_cast<ull*>(&s.bin[range(place, key)]),
+                          static_cast<ull>(what == kCount ? 1 : Weight(place)));
+            }
+        }
+        __syncthreads();
+    }
+
     // The first place of bin `bin`, all of whose elements are in the list of n, to meet the
-    // bound: ranges of the keys that are left, 1024 of them at a time, until a wave holds them.
+    // bound: first by equal ranges of the bin, then (equal logits) by ranges of the keys that
+    // are left, until a wave holds them.
     __device__ Place Select(int n, int bin, Bound what, uint64_t bound) {
-        const Span span{bin, bin};
-        uint64_t lo = 0, hi = ~uint64_t{0}, before = 0;
+        uint64_t lo = 0, hi = ~uint64_t{0}, before = 0, base = 0;
+        int range = -1, shift = -1;  // shift -1: ranges by place
         for (;;) {
+            Few(n, bin, what,
+                [&](double place, uint64_t key) {
+                    return key >= lo && key <= hi && (range < 0 || RangeOf(place) == range);
+                },
+                [&](double place, uint64_t key) {
+                    return shift < 0 ? RangeOf(place) : static_cast<int>((key - base) >> shift);
+                });
+            if (s.n_few <= kWave) break;
+            const int at = Narrow(what, bound, &before);
+            if (shift < 0) {
+                range = at;
+            } else {
+                lo = base + (static_cast<uint64_t>(at) << shift);
+                hi = lo + ((uint64_t{1} << shift) - 1);
+            }
+            // how far apart the keys of that range are
             uint64_t least = ~uint64_t{0}, most = 0;
-            if (Tid() == 0) s.n_few = 0;
-            __syncthreads();
-            InList(n, span, [&](int, double, uint64_t key) {
-                if (key < lo || key > hi) return;
+            InList(n, {bin, bin}, [&](int, double place, uint64_t key) {
+                if (key < lo || key > hi || RangeOf(place) != range) return;
                 least = key < least ? key : least;
                 most = key > most ? key : most;
-                const uint32_t at = atomicAdd(&s.n_few, 1u);
-                if (at < kWave) s.few[at] = key;
             });
-            if (s.n_few <= kWave) break;
             MinMax(&least, &most);
-            int shift = 0;
-            while ((most - least) >> shift >= kBins) ++shift;
-            s.bin[Tid()] = 0;
-            __syncthreads();
-            InList(n, span, [&](int, double place, uint64_t key) {
-                if (key < lo || key > hi) return;
-                atomicAdd(reinterpret_cast<ull*>(&s.bin[(key - least) >> shift]),
-                          static_cast<ull>(what == kCount ? 1 : Weight(place)));
-            });
-            const uint64_t at = Narrow(what, bound, &before);
-            lo = least + (at << shift);
-            hi = lo + ((uint64_t{1} << shift) - 1);
+            base = least;
+            for (shift = 0; (most - least) >> shift >= kBins;) ++shift;
         }
         // one wave: every lane an element, its place by comparison with all others
         if (Tid() < kWave) {
@@ -702,61 +701,126 @@ struct Chooser {
     }
 };
 
-template <typename T>
+// The passes after the first.  kCuts: which logits to gather; kFinish: the choice from what was
+// gathered; kSmall: the choice from a row that the list holds whole, without any of the others.
+enum Pass { kCuts, kFinish, kSmall };
+
+template <typename T, Pass kPass_>
 __global__ __launch_bounds__(kChooseThreads) void SampleChoose(const SampleArgs p) {
     __shared__ Choice s;
     const int tid = static_cast<int>(threadIdx.x);
     const int64_t row = blockIdx.x;
     const How h = HowOf(p, row);
-    const char* parts = p.part + row * p.parts * kPartBytes;
+    const RowUnits<T> units(p, row);
+    RowState* state = reinterpret_cast<RowState*>(p.state + row * kStateBytes);
+    uint64_t* state_bin = reinterpret_cast<uint64_t*>(state + 1);
+    uint64_t* state_list = state_bin + kBins;
     uint32_t flags = 0;
     int32_t top = INT32_MIN;
-    uint64_t best = ~uint64_t{0};
-    if (!h.bad) {
-        for (int i = 0; i < p.parts; ++i) {
-            const Part part = *reinterpret_cast<const Part*>(parts + i * kPartBytes);
-            flags |= part.flags;
-            if ((part.flags & kSome) && part.top > top) top = part.top;
-            if (part.best < best) best = part.best;
-            if (tid == 0) s.tops[i] = part.flags & kSome ? part.top : INT32_MIN;
-        }
-    }
-    if (h.bad || !(flags & kSome) || (flags & kNan)) {
-        if (tid == 0) {
-            p.tokens[row] = -1;
-            if (p.prob != nullptr) p.prob[row] = 0.0f;
-            RaiseFlag(p.err, 1);
-        }
-        return;
-    }
-    if (h.t == 0.0f) {
-        if (tid == 0) {
-            p.tokens[row] = static_cast<int32_t>(best);
-            if (p.prob != nullptr) p.prob[row] = 1.0f;
-        }
-        return;
-    }
-    __syncthreads();
-    Chooser<T> ch{p, h, s, RowUnits<T>(p, row), p.largest + row * p.segments, top, ~uint64_t{0}};
-    static_assert(kBins == kChooseThreads, "a thread a bin");
-    uint64_t mine = 0;
+    uint64_t best = ~uint64_t{0}, mine = 0;
+    float largest = -INFINITY;
+    if constexpr (kPass_ == kFinish) {
+        if (state->live == 0) return;
+        top = state->top;
+        largest = state->largest;
+        mine = state_bin[tid];
+    } else if constexpr (kPass_ == kCuts) {
+        // lane i of each wave: part i
+        const char* parts = p.part + row * p.parts * kPartBytes;
+        static_assert(kMaxParts <= kWave, "a lane a part");
+        const int lane = tid % kWave;
+        if (!h.bad) {
+            Part part{INT32_MIN, 0, ~uint64_t{0}, -INFINITY, {}};
+            if (lane < p.parts) part = *reinterpret_cast<const Part*>(parts + lane * kPartBytes);
+            flags = (__ballot(part.flags & kSome) != 0 ? kSome : 0) | (__ballot(part.flags & kNan) != 0 ? kNan : 0);
+            if (!(part.flags & kSome)) part.top = INT32_MIN;
+            top = part.top;
+            best = part.best;
+            largest = part.largest;
+#pragma unroll
+            for (int off = kWave / 2; off > 0; off /= 2) {
+                const int32_t t = __shfl_xor(top, off, kWave);
+                top = t > top ? t : top;
+                const uint64_t o = __shfl_xor(static_cast<ull>(best), off, kWave);
+                best = o < best ? o : best;
+                largest = fmaxf(largest, __shfl_xor(largest, off, kWave));
+            }
+            if (h.t != 0.0f && flags == kSome) {
 #pragma unroll 8
-    for (int i = 0; i < p.parts; ++i) {
-        const int32_t at = s.tops[i] == INT32_MIN ? -1 : s.tops[i] - (top - tid);  // this thread's bin in the part
-        if (at >= 0) mine += reinterpret_cast<const uint64_t*>(parts + i * kPartBytes + sizeof(Part))[at];
+                for (int i = 0; i < p.parts; ++i) {
+                    // this thread's bin in part i
+                    const int32_t part_top = __builtin_amdgcn_readlane(part.top, i), at = part_top - (top - tid);
+                    const bool in = part_top != INT32_MIN && at >= 0;
+                    const uint64_t m = reinterpret_cast<const uint64_t*>(parts + i * kPartBytes + sizeof(Part))[in ? at : 0];
+                    mine += in ? m : 0;
+                }
+            }
+        }
+    } else {
+        // a thread has up to kEach elements
+        constexpr int kEach = kList / kChooseThreads;
+        float x[kEach];
+        bool nan = false;
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) {
+            const int32_t at = tid + i * kChooseThreads;
+            x[i] = at < p.vocab ? T::Get(units.x[at]) : -INFINITY;
+            nan |= x[i] != x[i];
+            largest = fmaxf(largest, x[i]);
+            if (at < p.vocab) s.list[at] = x[i] > -INFINITY ? Key(x[i], at) : kNoKey;
+            if (x[i] > -INFINITY) best = Key(x[i], at) < best ? Key(x[i], at) : best;
+        }
+        s.bin[tid] = 0;
+        if (tid == 0) s.word[0] = ~uint64_t{0};
+        largest = BlockMax<kChooseWaves>(largest, reinterpret_cast<float*>(s.scan_u));
+        flags = (largest > -INFINITY ? kSome : 0) | (__syncthreads_or(nan) ? kNan : 0);
+        if (h.t == 0.0f) {
+            atomicMin(reinterpret_cast<ull*>(&s.word[0]), static_cast<ull>(best));
+            __syncthreads();
+            best = s.word[0];
+        } else if (!h.bad) {
+            double f;
+            top = BinOf(h, largest, &f);
+#pragma unroll
+            for (int i = 0; i < kEach; ++i) {
+                const int32_t b = top - BinOf(h, x[i], &f);
+                if (x[i] > -INFINITY && b < kBins) {
+                    atomicAdd(reinterpret_cast<ull*>(&s.bin[b]), static_cast<ull>(h.k != 0 ? 1 : Weight(f)));
+                }
+            }
+            __syncthreads();
+            mine = s.bin[tid];
+            __syncthreads();
+        }
     }
+    if constexpr (kPass_ != kFinish) {
+        const bool none = h.bad || flags != kSome;
+        if (kPass_ == kCuts && tid == 0) state->live = none || h.t == 0.0f ? 0 : 1;
+        if (none || h.t == 0.0f) {
+            if (tid == 0) {
+                p.tokens[row] = none ? -1 : static_cast<int32_t>(best);
+                if (p.prob != nullptr) p.prob[row] = none ? 0.0f : 1.0f;
+                if (none) RaiseFlag(p.err, 1);
+            }
+            return;
+        }
+    }
+    if constexpr (kPass_ == kCuts) state_bin[tid] = mine;
+    Chooser<T> ch{p, h, s, units, p.largest + row * p.segments, top, kLastKey};
+    static_assert(kBins == kChooseThreads, "a thread a bin");
     s.edge[tid] = exp(tid * (-1.0 / kPerUnit));
     // Three places are looked for in turn, each where its cut is asked for: the top-k's, the
     // top-p's (with the sum that min-p leaves) and the token's.  The row is gathered once for
     // the first two as a rule, or once for the last two.
     enum { kTopK, kTopP, kToken };
     int last = kBins - 1;       // no element of a later bin can be chosen
-    int n = -1;                 // elements of the list, where it has all that is needed
+    int n = kPass_ == kSmall ? p.vocab : -1;  // elements of the list, where it has all that is needed
     const double u = h.u;
     double kept = 0.0, least = 0.0, reach = 0.0;
     bool by_p = h.p < 1.0f, by_m = h.m > 0.0f;
     Span m{0, 0}, drawn{0, 0};
     int p_bin = 0;
+    bool first = true;
 #pragma unroll 1
     for (int what = h.k != 0 ? kTopK : kTopP; what <= kToken; ++what) {
         Span a, b;      // bins to gather, if there is no list
@@ -790,12 +854,7 @@ __global__ __launch_bounds__(kChooseThreads) void SampleChoose(const SampleArgs 
                 ch.FirstBins(last, true, reach, reach, &p_bin, &same);
             }
             if (by_m) {
-                float x = -INFINITY;  // the largest logit
-                const int segments = (ch.r.Units() + kSegment - 1) / kSegment;
-                for (int i = tid; i < segments; i += kChooseThreads) x = fmaxf(x, ch.largest[i]);
-                x = BlockMax<kChooseWaves>(x, reinterpret_cast<float*>(s.scan_u));
-                __syncthreads();
-                least = fmin(static_cast<double>(h.m), 1.0) * ch.WeightOf(x);  // its equals are kept
+                least = fmin(static_cast<double>(h.m), 1.0) * ch.WeightOf(largest);  // its equals are kept
                 const double where = -static_cast<double>(kPerUnit) * log(least / kOne);
                 m.hi = where >= kBins ? kBins - 1 : static_cast<int>(where + 0.51);
                 m.lo = m.hi > 1 ? m.hi - 2 : 0;
@@ -832,11 +891,22 @@ __global__ __launch_bounds__(kChooseThreads) void SampleChoose(const SampleArgs 
             a = b = {bin, bin};
         }
         bool whole = true;  // the list serves the places looked for later too
-        for (int tries = 0; n < 0 && tries < 2; ++tries) {
-            n = ch.Gather(a, b);
+        if constexpr (kPass_ == kCuts) {
+            if (tid == 0) *state = {top, largest, ch.Lowest(a.hi), ch.Highest(a.lo), ch.Lowest(b.hi), ch.Highest(b.lo), 1, 0};
+            return;
+        }
+        if (kPass_ == kFinish && first) {  // what was gathered for this
+            first = false;
+            n = static_cast<int>(state->n);
+            for (int i = tid; i < n && i < kList; i += kChooseThreads) s.list[i] = state_list[i];
+            __syncthreads();
             if (n > kList) n = -1;
-            whole = tries == 0 && !(what == kTopK && a.lo != 0);
-            a = b = {bin, bin};
+            whole = !(what == kTopK && a.lo != 0);
+        }
+        if (n < 0 && look) {
+            n = ch.Gather(bin);
+            if (n > kList) n = -1;
+            whole = false;
         }
         if (what == kTopP && by_m) {
             uint64_t sum[3] = {0, 0, 0};
@@ -846,7 +916,7 @@ __global__ __launch_bounds__(kChooseThreads) void SampleChoose(const SampleArgs 
 #pragma unroll
                 for (int i = 0; i < 3; ++i) sum[i] += at - m.lo == i ? w : 0;
             };
-            if (n >= 0 && whole) ch.InList(n, m, add);
+            if (kPass_ == kSmall || (n >= 0 && whole)) ch.InList(n, m, add);
             else ch.Visit(m, add);
             double upto = ch.Below(m.lo);
 #pragma unroll
@@ -860,7 +930,7 @@ __global__ __launch_bounds__(kChooseThreads) void SampleChoose(const SampleArgs 
         if (look) {
             constexpr Bound kBounds[3] = {kCount, kReach, kPass};
             const Bound meets = kBounds[what];
-            const Place at = n >= 0 ? ch.Select(n, bin, meets, bound) : ch.Search(bin, meets, bound);
+            const Place at = kPass_ == kSmall || n >= 0 ? ch.Select(n, bin, meets, bound) : ch.Search(bin, meets, bound);
             if (what == kTopK) {
                 ch.limit = at.key;
             } else if (what == kTopP) {
@@ -877,10 +947,84 @@ __global__ __launch_bounds__(kChooseThreads) void SampleChoose(const SampleArgs 
             auto add = [&](int at, double place, uint64_t) {
                 atomicAdd(reinterpret_cast<ull*>(&s.bin[at]), static_cast<ull>(Weight(place)));
             };
-            if (n >= 0 && whole) ch.InList(n, {0, last}, add);
+            if (kPass_ == kSmall || (n >= 0 && whole)) ch.InList(n, {0, last}, add);
             else ch.Visit({0, last}, add);
         }
         if (!whole) n = -1;
+    }
+}
+
+// Between kCuts and kFinish: the row's logits in the two spans found, in any order, 8 lanes to
+// each 128 bytes whose largest is no lower; a wave has what it needs of 64 segments on its
+// way before it looks at the first.
+constexpr int kGatherThreads = 256;
+template <typename T>
+__global__ __launch_bounds__(kGatherThreads) void SampleGather(const SampleArgs p, int parts) {
+    constexpr int E = RowUnits<T>::E, kGroups = kWave / kSegment, kRounds = 32 / E;
+    __shared__ int32_t hits_of[kGatherThreads / kWave][kWave];
+    const int lane = static_cast<int>(threadIdx.x) % kWave;
+    const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / kWave);
+    const int64_t row = blockIdx.x / parts;
+    const int part = static_cast<int>(blockIdx.x % parts);
+    RowState* state = reinterpret_cast<RowState*>(p.state + row * kStateBytes);
+    if (state->live == 0) return;
+    uint64_t* list = reinterpret_cast<uint64_t*>(state + 1) + kBins;
+    const float al = state->al, ah = state->ah, bl = state->bl, bh = state->bh, low = fminf(al, bl);
+    const float* largest = p.largest + row * p.segments;
+    const RowUnits<T> r(p, row);
+    const int32_t units = r.Units(), segments = (units + kSegment - 1) / kSegment;
+    int32_t* hit_segment = hits_of[wave];
+    const int32_t step = parts * kGatherThreads;
+    int32_t s0 = (part * (kGatherThreads / kWave) + wave) * kWave;
+    float next = s0 + lane < segments ? largest[s0 + lane] : -INFINITY;
+    for (; s0 < segments; s0 += step) {
+        const bool hit = next >= low;
+        next = s0 + step + lane < segments ? largest[s0 + step + lane] : -INFINITY;
+        const uint64_t mask = __ballot(hit);
+        const int n = __popcll(mask);
+        if (hit) hit_segment[__popcll(mask & ((uint64_t{1} << lane) - 1))] = s0 + lane;
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        for (int g = 0; g < n; g += kGroups * kRounds) {
+            u32x4 raw[kRounds];
+            int32_t unit[kRounds];
+#pragma unroll
+            for (int i = 0; i < kRounds; ++i) {
+                const int j = g + i * kGroups + lane / kSegment;
+                unit[i] = j < n ? hit_segment[j] * kSegment + lane % kSegment : units;
+                raw[i] = r.Load(unit[i], unit[i] < units);
+            }
+            uint32_t hits = 0;
+#pragma unroll
+            for (int i = 0; i < kRounds; ++i) {
+#pragma unroll
+                for (int e = 0; e < E; ++e) {
+                    const float x = r.Get(raw[i], e);
+                    const bool in = (x >= al && x <= ah) || (x >= bl && x <= bh);
+                    hits |= in ? 1u << (i * E + e) : 0u;
+                }
+            }
+            // places for the wave's hits: one addition for all
+            const uint32_t mine = __popc(hits);
+            uint32_t upto = mine;
+#pragma unroll
+            for (int off = 1; off < kWave; off *= 2) {
+                const uint32_t o = __shfl_up(upto, off, kWave);
+                if (lane >= off) upto += o;
+            }
+            uint32_t at = 0;
+            if (lane == kWave - 1 && upto != 0) at = atomicAdd(&state->n, upto);
+            at = __builtin_amdgcn_readlane(at, kWave - 1) + upto - mine;
+#pragma unroll
+            for (int i = 0; i < kRounds; ++i) {
+#pragma unroll
+                for (int e = 0; e < E; ++e) {
+                    if (hits >> (i * E + e) & 1) {
+                        if (at < kList) list[at] = Key(r.Get(raw[i], e), r.Index(unit[i], e));
+                        ++at;
+                    }
+                }
+            }
+        }
     }
 }
 
@@ -894,14 +1038,58 @@ int Parts(int64_t n_rows, int64_t vocab, int bytes) {
     if (parts > kMaxParts) parts = kMaxParts;
     return static_cast<int>(parts < 1 ? 1 : parts);
 }
+// Workgroups of the gather a row: 4 a compute unit, 64 segments a wave at least.
+int GatherParts(int64_t n_rows, int64_t vocab, int bytes) {
+    int64_t parts = (static_cast<int64_t>(ComputeUnits()) * 4 + n_rows - 1) / n_rows;
+    const int64_t most = (vocab * bytes / 128 + kGatherThreads - 1) / kGatherThreads;
+    if (parts > most) parts = most;
+    return static_cast<int>(parts < 1 ? 1 : parts);
+}
 int64_t Segments(int64_t vocab, int bytes) {  // one more where the row is not aligned
     return (vocab * bytes + 127) / 128 + 1;
 }
 
+// Rows that one round of launches takes, which is what the workspace is for.
+constexpr int64_t kRowsAtOnce = 1024;
+
+int64_t RowBytes(int parts, int64_t vocab, int bytes) {
+    return kStateBytes + parts * kPartBytes + (4 * Segments(vocab, bytes) + 15) / 16 * 16;
+}
+
 template <typename T>
-void Launch(const SampleArgs& p, int64_t n_rows, hipStream_t s) {
-    hipLaunchKernelGGL(SampleBins<T>, dim3(static_cast<unsigned>(n_rows * p.parts)), dim3(kThreads), 0, s, p);
-    hipLaunchKernelGGL(SampleChoose<T>, dim3(static_cast<unsigned>(n_rows)), dim3(kChooseThreads), 0, s, p);
+mlk_status Launch(SampleArgs p, int64_t n_rows, char* workspace, hipStream_t s) {
+    constexpr int kBytes = sizeof(typename T::Bits);
+    const dim3 block(kChooseThreads);
+    const int64_t most = p.vocab <= kList ? n_rows : kRowsAtOnce;
+    for (int64_t from = 0; from < n_rows; from += most) {
+        const int64_t rows = n_rows - from < most ? n_rows - from : most;
+        const dim3 grid(static_cast<unsigned>(rows));
+        if (p.vocab <= kList) {
+            hipLaunchKernelGGL((SampleChoose<T, kSmall>), grid, block, 0, s, p);
+        } else {
+            p.parts = Parts(rows, p.vocab, kBytes);
+            p.segments = static_cast<int32_t>((Segments(p.vocab, kBytes) + 3) / 4 * 4);
+            p.state = workspace;
+            p.part = p.state + rows * kStateBytes;
+            p.largest = reinterpret_cast<float*>(p.part + rows * p.parts * kPartBytes);
+            hipLaunchKernelGGL(SampleBins<T>, dim3(static_cast<unsigned>(rows * p.parts)), dim3(kThreads), 0, s, p);
+            hipLaunchKernelGGL((SampleChoose<T, kCuts>), grid, block, 0, s, p);
+            const int parts = GatherParts(rows, p.vocab, kBytes);
+            hipLaunchKernelGGL(SampleGather<T>, dim3(static_cast<unsigned>(rows * parts)), dim3(kGatherThreads), 0, s, p, parts);
+            hipLaunchKernelGGL((SampleChoose<T, kFinish>), grid, block, 0, s, p);
+        }
+        const mlk_status st = CheckLaunch("SampleChoose");
+        if (st != MLK_OK) return st;
+        p.x = static_cast<const typename T::Bits*>(p.x) + rows * p.row;
+        p.u += rows;
+        p.tokens += rows;
+        if (p.prob != nullptr) p.prob += rows;
+        if (p.how.temperature != nullptr) p.how.temperature += rows;
+        if (p.how.top_k != nullptr) p.how.top_k += rows;
+        if (p.how.top_p != nullptr) p.how.top_p += rows;
+        if (p.how.min_p != nullptr) p.how.min_p += rows;
+    }
+    return MLK_OK;
 }
 
 }  // namespace
@@ -916,8 +1104,16 @@ int64_t mlk_sample_workspace_bytes(int32_t type, int64_t n_rows, int64_t vocab) 
         n_rows > kMaxRows || vocab <= 0 || vocab > kMaxVocab) {
         return 0;
     }
+    if (vocab <= kList) return 16;
     const int bytes = TypeBytes(type);
-    return n_rows * (Parts(n_rows, vocab, bytes) * kPartBytes + 4 * Segments(vocab, bytes)) + 16;
+    const int64_t rows = n_rows < kRowsAtOnce ? n_rows : kRowsAtOnce;
+    int64_t most = rows * RowBytes(Parts(rows, vocab, bytes), vocab, bytes);
+    const int64_t left = n_rows % kRowsAtOnce;  // a last round of few rows has more parts each
+    if (n_rows > kRowsAtOnce && left != 0) {
+        const int64_t last = left * RowBytes(Parts(left, vocab, bytes), vocab, bytes);
+        if (last > most) most = last;
+    }
+    return most;
 }
 
 mlk_status mlk_sample(int32_t type, const void* logits, int64_t row_stride, int64_t n_rows,
@@ -970,15 +1166,11 @@ mlk_status mlk_sample(int32_t type, const void* logits, int64_t row_stride, int6
     p.tokens = tokens;
     p.prob = prob;
     p.err = err;
-    p.parts = Parts(n_rows, vocab, bytes);
-    p.segments = static_cast<int32_t>(Segments(vocab, bytes));
-    p.part = static_cast<char*>(workspace);
-    p.largest = reinterpret_cast<float*>(p.part + n_rows * p.parts * kPartBytes);
+    char* ws = static_cast<char*>(workspace);
     const hipStream_t s = AsStream(stream);
-    if (type == MLK_F32) Launch<F32>(p, n_rows, s);
-    else if (type == MLK_F16) Launch<F16>(p, n_rows, s);
-    else Launch<BF16>(p, n_rows, s);
-    return CheckLaunch("SampleChoose");
+    if (type == MLK_F32) return Launch<F32>(p, n_rows, ws, s);
+    if (type == MLK_F16) return Launch<F16>(p, n_rows, ws, s);
+    return Launch<BF16>(p, n_rows, ws, s);
 }
 
 }  // extern "C"
