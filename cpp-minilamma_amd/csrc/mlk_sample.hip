@@ -34,11 +34,12 @@ namespace mlk {
 namespace {
 
 constexpr int kThreads = 512, kWaves = kThreads / kWave;  // first pass
-constexpr int kChooseThreads = 1024, kChooseWaves = kChooseThreads / kWave;
+constexpr int kChooseThreads = 256, kChooseWaves = kChooseThreads / kWave;  // the later ones
 constexpr int kBins = 1024;     // of a histogram, a power of two
 constexpr int kPerUnit = 32;    // bins of a temperature
 constexpr int kList = 4096;     // elements gathered at once
-constexpr int kChunk = 4096;    // segments looked at at once
+constexpr int kChunk = 1024;    // segments looked at at once
+constexpr int kEach = kBins / kChooseThreads;  // neighbouring bins a thread has
 constexpr int kMaxParts = 48;   // workgroups of a row
 constexpr int64_t kMaxVocab = 1 << 20, kMaxRows = 1 << 20;
 constexpr double kOne = 0x1p42;  // a weight of 1
@@ -372,13 +373,13 @@ __device__ inline V ScanBlock(V v, V* scratch, V* total) {
 
 struct Choice {
     uint64_t list[kList];  // keys of gathered elements
+    uint32_t code[kList];  // their bins, and where in them: CodeOf
     uint64_t bin[kBins];   // masses or counts of the bins; of a search's ranges
-    double edge[kBins];    // exp(-i / kPerUnit): a bin's middle, of the largest bin's
-    double sum[kBins];     // of the weights up to and with bin i
+    uint64_t sum[kBins];   // of the weights up to and with bin i, of the largest bin's middle
     uint16_t segment[kChunk];
     uint64_t few[kWave];
+    double edge[2 * kPerUnit];  // exp(-i / kPerUnit), and exp(-i)
     uint64_t scan_u[kChooseWaves], scan_v[kChooseWaves];
-    double scan_d[kChooseWaves];
     int32_t found[2];
     uint32_t n_list, n_segments, n_few;
     uint64_t word[3];
@@ -414,12 +415,36 @@ struct Chooser {
     __device__ int BinOfKey(uint64_t key, double* f) const {
         return top - BinOf(h, Logit(static_cast<uint32_t>(key >> 32)), f);
     }
+    // A bin's middle, of the largest bin's: exp(-bin / kPerUnit), as a product of two.
+    static_assert(kBins == kPerUnit * kPerUnit, "two tables of kPerUnit");
+    __device__ double Edge(int bin) const { return s.edge[bin % kPerUnit] * s.edge[kPerUnit + bin / kPerUnit]; }
+    __device__ void MakeEdges() {  // (a barrier follows)
+        if (Tid() < 2 * kPerUnit) s.edge[Tid()] = exp(Tid() < kPerUnit ? Tid() * (-1.0 / kPerUnit) : static_cast<double>(kPerUnit - Tid()));
+    }
     __device__ double WeightOf(float x) const {
         double f;
         const int32_t b = top - BinOf(h, x, &f);
-        return static_cast<double>(Weight(f)) * s.edge[b];
+        return static_cast<double>(Weight(f)) * Edge(b);
     }
-    __device__ double Below(int bin) const { return bin > 0 ? s.sum[bin - 1] : 0.0; }
+    // Which of kBins equal ranges of its bin an element lies in, from the largest down.
+    static __device__ int RangeOf(double place) {
+        const int i = static_cast<int>((0.5 - place) * kBins);
+        return i < 0 ? 0 : i < kBins ? i : kBins - 1;
+    }
+    __device__ uint32_t CodeOf(uint64_t key) const {
+        double place;
+        const int b = BinOfKey(key, &place);
+        return key <= kLastKey && b >= 0 && b < kBins ? static_cast<uint32_t>(b * kBins + RangeOf(place)) : ~0u;
+    }
+    __device__ void PutInList(int at, uint64_t key) {
+        s.list[at] = key;
+        s.code[at] = CodeOf(key);
+    }
+    __device__ uint64_t Below(int bin) const { return bin > 0 ? s.sum[bin - 1] : 0; }
+    // Whole weights of a bin as those of the largest bin's middle.
+    __device__ uint64_t Scaled(uint64_t w, int bin) {
+        return static_cast<uint64_t>(rint(static_cast<double>(w) * Edge(bin)));
+    }
 
     // Logits no smaller (larger) than any of bin `bin`, to within a thousandth of a bin and a
     // rounding.
@@ -467,7 +492,7 @@ struct Chooser {
         if (Tid() == 0) s.n_list = 0;  // (a barrier follows in Segments)
         Near({bin, bin}, [&](float x, int32_t i) {
             const uint32_t at = atomicAdd(&s.n_list, 1u);
-            if (at < kList) s.list[at] = Key(x, i);
+            if (at < kList) PutInList(static_cast<int>(at), Key(x, i));
         });
         return static_cast<int>(s.n_list);
     }
@@ -481,6 +506,7 @@ struct Chooser {
         const int32_t segments = (r.Units() + kSegment - 1) / kSegment;
         for (int32_t c0 = 0; c0 < segments; c0 += kChunk) {
             const int n = Segments(c0, segments, low);
+#pragma unroll 1
             for (int j = Tid(); j < n * kEach; j += kChooseThreads) {
                 const int32_t i = r.Index((c0 + s.segment[j / kEach]) * kSegment, j % kEach);
                 const float x = i >= 0 && i < r.vocab ? T::Get(r.x[i]) : -INFINITY;
@@ -499,14 +525,17 @@ struct Chooser {
             if (span.Has(b) && key <= limit) f(b, place, key);
         });
     }
-    // The same over the first n of s.list.
+    // The same over the first n of s.list; f(bin, place, key, code).
     template <typename F>
     __device__ void InList(int n, const Span& span, const F& f) {
+#pragma unroll 2
         for (int i = Tid(); i < n; i += kChooseThreads) {
+            const uint32_t code = s.code[i];
+            if (!span.Has(static_cast<int>(code / kBins))) continue;
             const uint64_t key = s.list[i];
             double place;
             const int b = BinOfKey(key, &place);
-            if (span.Has(b) && key <= limit) f(b, place, key);
+            if (key <= limit) f(b, place, key, code);
         }
         __syncthreads();
     }
@@ -532,90 +561,91 @@ struct Chooser {
         }
     }
 
-    // A step of a search: s.bin holds what lies in kBins ranges of the order (what: counts or
-    // sums); the first range where the bound is met after `before`, or the last that holds
-    // any.  *before: with what lies before that range.
-    __device__ int Narrow(Bound what, uint64_t bound, uint64_t* before) {
-        uint64_t all;
-        const uint64_t mine = s.bin[Tid()], sum = *before + ScanBlock(mine, s.scan_u, &all);
+    __device__ void ClearBins() {
+        for (int i = Tid(); i < kBins; i += kChooseThreads) s.bin[i] = 0;
+    }
+    __device__ void AddTo(int range, uint64_t w) {
+        atomicAdd(reinterpret_cast<ull*>(&s.bin[range]), static_cast<ull>(w));
+    }
+    // A step of a search: s.bin holds what lies in kBins ranges of the order (counts or
+    // sums); the first range where the bound is met after *before, or the last that holds
+    // any.  *before: with what lies before that range; *held: what it holds.
+    __device__ int Narrow(Bound what, uint64_t bound, uint64_t* before, uint64_t* held) {
+        uint64_t w[kEach], mine = 0, all;
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) {
+            w[i] = s.bin[Tid() * kEach + i];
+            mine += w[i];
+        }
+        uint64_t sum = *before + ScanBlock(mine, s.scan_u, &all) - mine;
         all += *before;
         // (a bound past the end: the last place)
         if (what == kPass ? bound >= all : bound > all) bound = what == kPass ? all - 1 : all;
-        const bool ok = what == kPass ? sum > bound && sum - mine <= bound : sum >= bound && sum - mine < bound;
-        if (ok) {
-            s.found[0] = Tid();
-            s.word[0] = sum - mine;
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) {
+            const uint64_t upto = sum + w[i];
+            if (what == kPass ? upto > bound && sum <= bound : upto >= bound && sum < bound) {
+                s.found[0] = Tid() * kEach + i;
+                s.word[0] = sum;
+                s.word[1] = w[i];
+            }
+            sum = upto;
         }
         __syncthreads();
         *before = s.word[0];
+        *held = s.word[1];
         const int at = s.found[0];
         __syncthreads();
         return at;
     }
 
-    // Which of kBins equal ranges of its bin an element lies in, from the largest down.
-    static __device__ int RangeOf(double place) {
-        const int i = static_cast<int>((0.5 - place) * kBins);
-        return i < 0 ? 0 : i < kBins ? i : kBins - 1;
-    }
-    // s.few[0 .. 63] of the list's elements of bin `bin` with ok(place, key), and their number;
-    // s.bin, of ranges, gets what each element weighs there.
-    template <typename F, typename R>
-    __device__ void Few(int n, int bin, Bound what, const F& ok, const R& range) {
-        if (Tid() == 0) s.n_few = 0;
-        s.bin[Tid()] = 0;
-        __syncthreads();
-        for (int i0 = 0; i0 < n; i0 += kChooseThreads) {
-            const uint64_t key = i0 + Tid() < n ? s.list[i0 + Tid()] : kNoKey;
-            double place;
-            const bool in = BinOfKey(key, &place) == bin && i0 + Tid() < n && key <= limit && ok(place, key);
-            const uint64_t mask = __ballot(in);
-            if (mask == 0) continue;
-            uint32_t at = 0;
-            if (Lane() == 0) at = atomicAdd(&s.n_few, static_cast<uint32_t>(__popcll(mask)));
-            at = __builtin_amdgcn_readfirstlane(at) + __popcll(mask & ((uint64_t{1} << Lane()) - 1));
-            if (in && at < kWave) s.few[at] = key;
-            if (in) {
-                atomicAdd(reinterpret_cast<ull*>(&s.bin[range(place, key)]),
-                          static_cast<ull>(what == kCount ? 1 : Weight(place)));
-            }
-        }
-        __syncthreads();
-    }
-
     // The first place of bin `bin`, all of whose elements are in the list of n, to meet the
-    // bound: first by equal ranges of the bin, then (equal logits) by ranges of the keys that
-    // are left, until a wave holds them.
+    // bound: by equal ranges of the bin, then (equal logits) by ranges of the keys that are
+    // left, until a wave holds them.
     __device__ Place Select(int n, int bin, Bound what, uint64_t bound) {
-        uint64_t lo = 0, hi = ~uint64_t{0}, before = 0, base = 0;
-        int range = -1, shift = -1;  // shift -1: ranges by place
-        for (;;) {
-            Few(n, bin, what,
-                [&](double place, uint64_t key) {
-                    return key >= lo && key <= hi && (range < 0 || RangeOf(place) == range);
-                },
-                [&](double place, uint64_t key) {
-                    return shift < 0 ? RangeOf(place) : static_cast<int>((key - base) >> shift);
+        const Span span{bin, bin};
+        uint64_t lo = 0, hi = kLastKey, before = 0;
+        int range = -1;   // of the bin, once it is known
+        uint64_t left = static_cast<uint64_t>(n);  // no fewer than are left
+        auto has = [&](uint64_t key, uint32_t code) {
+            return range < 0 || (static_cast<int>(code % kBins) == range && key >= lo && key <= hi);
+        };
+        while (left > kWave) {
+            uint64_t base = 0, held;
+            int shift = 0;
+            if (range >= 0) {  // how far apart the keys are
+                uint64_t least = kNoKey, most = 0;
+                InList(n, span, [&](int, double, uint64_t key, uint32_t code) {
+                    if (!has(key, code)) return;
+                    least = key < least ? key : least;
+                    most = key > most ? key : most;
                 });
-            if (s.n_few <= kWave) break;
-            const int at = Narrow(what, bound, &before);
-            if (shift < 0) {
+                MinMax(&least, &most);
+                base = least;
+                while ((most - least) >> shift >= kBins) ++shift;
+            }
+            ClearBins();
+            __syncthreads();
+            InList(n, span, [&](int, double place, uint64_t key, uint32_t code) {
+                if (!has(key, code)) return;
+                AddTo(range >= 0 ? static_cast<int>((key - base) >> shift) : static_cast<int>(code % kBins),
+                      what == kCount ? 1 : Weight(place));
+            });
+            const int at = Narrow(what, bound, &before, &held);
+            if (range < 0) {
                 range = at;
             } else {
                 lo = base + (static_cast<uint64_t>(at) << shift);
                 hi = lo + ((uint64_t{1} << shift) - 1);
             }
-            // how far apart the keys of that range are
-            uint64_t least = ~uint64_t{0}, most = 0;
-            InList(n, {bin, bin}, [&](int, double place, uint64_t key) {
-                if (key < lo || key > hi || RangeOf(place) != range) return;
-                least = key < least ? key : least;
-                most = key > most ? key : most;
-            });
-            MinMax(&least, &most);
-            base = least;
-            for (shift = 0; (most - least) >> shift >= kBins;) ++shift;
+            // a weight is at least exp(-1 / 64), 0.9845
+            left = what == kCount ? held : static_cast<uint64_t>(static_cast<double>(held) * (1 / (0.984 * kOne)));
         }
+        if (Tid() == 0) s.n_few = 0;
+        __syncthreads();
+        InList(n, span, [&](int, double, uint64_t key, uint32_t code) {
+            if (has(key, code)) s.few[atomicAdd(&s.n_few, 1u)] = key;
+        });
         // one wave: every lane an element, its place by comparison with all others
         if (Tid() < kWave) {
             const int m = static_cast<int>(s.n_few);
@@ -624,10 +654,10 @@ struct Chooser {
             double place;
             BinOfKey(real ? key : s.few[0], &place);
             const uint64_t own = Weight(place), one = what == kCount ? 1 : own;
-            s.bin[Tid()] = one;
+            s.bin[Tid()] = one;  // (this wave alone is here)
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
             uint64_t sum = before;
-#pragma unroll 8
+#pragma unroll 4
             for (int i = 0; i < m; ++i) sum += s.few[i] <= key ? s.bin[i] : 0;
             const bool ok = real && (what == kPass ? sum > bound : sum >= bound);
             // the first that is ok; none: the last of all
@@ -653,17 +683,16 @@ struct Chooser {
     // The same for a bin of more elements than the list holds (nearly equal logits): by the
     // digits of their keys, pass by pass over the row.
     __device__ Place Search(int bin, Bound what, uint64_t bound) {
-        uint64_t high = 0, before = 0;
+        uint64_t high = 0, before = 0, held;
         constexpr int kDigit = 10;
         for (int shift = 60; shift >= 0; shift -= kDigit) {
             __syncthreads();
-            s.bin[Tid()] = 0;
+            ClearBins();
             Visit({bin, bin}, [&](int, double place, uint64_t key) {
                 if (shift < 60 && key >> (shift + kDigit) != high) return;
-                atomicAdd(reinterpret_cast<ull*>(&s.bin[(key >> shift) & (kBins - 1)]),
-                          static_cast<ull>(what == kCount ? 1 : Weight(place)));
+                AddTo(static_cast<int>(key >> shift) & (kBins - 1), what == kCount ? 1 : Weight(place));
             });
-            high = (high << kDigit) | static_cast<uint64_t>(Narrow(what, bound, &before));
+            high = (high << kDigit) | static_cast<uint64_t>(Narrow(what, bound, &before, &held));
         }
         double place;
         BinOfKey(high, &place);
@@ -671,35 +700,48 @@ struct Chooser {
     }
 
     // A bound on the sum over all as one on whole weights within bin `bin`.
-    __device__ uint64_t InBin(double bound, int bin, bool reach) const {
-        const double in = (bound - Below(bin)) / s.edge[bin];
-        if (reach) return in > 1.0 ? static_cast<uint64_t>(ceil(in)) : 1;
-        return in > 0.0 ? static_cast<uint64_t>(in) : 0;
+    __device__ uint64_t InBin(uint64_t bound, int bin, bool reach) const {
+        const uint64_t below = Below(bin);
+        const double in = bound > below ? static_cast<double>(bound - below) / Edge(bin) : 0.0;
+        return static_cast<uint64_t>(reach ? ceil(in) : in);
     }
 
     // Sums over the bins from their masses.
     __device__ void SumBins() {
-        double all;
+        uint64_t w[kEach], mine = 0, all;
         __syncthreads();
-        const double mine = static_cast<double>(s.bin[Tid()]) * s.edge[Tid()];
-        s.sum[Tid()] = ScanBlock(mine, s.scan_d, &all);
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) {
+            w[i] = Scaled(s.bin[Tid() * kEach + i], Tid() * kEach + i);
+            mine += w[i];
+        }
+        uint64_t sum = ScanBlock(mine, s.scan_u, &all) - mine;
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) {
+            sum += w[i];
+            s.sum[Tid() * kEach + i] = sum;
+        }
         __syncthreads();
     }
     // First bins up to `last` whose sum is past (reach: at least) each bound; `last` if none.
-    __device__ void FirstBins(int last, bool reach, double x, double y, int* at_x, int* at_y) {
+    __device__ Span FirstBins(int last, bool reach, uint64_t x, uint64_t y) {
         if (Tid() < 2) s.found[Tid()] = last;
         __syncthreads();
-        const double sum = s.sum[Tid()], before = Below(Tid());
-        if (Tid() < last) {
-            if (reach ? sum >= x && (Tid() == 0 || before < x) : sum > x && (Tid() == 0 || before <= x)) s.found[0] = Tid();
-            if (reach ? sum >= y && (Tid() == 0 || before < y) : sum > y && (Tid() == 0 || before <= y)) s.found[1] = Tid();
+        for (int i = Tid(); i < last; i += kChooseThreads) {
+            const uint64_t sum = s.sum[i], before = Below(i);
+            if (reach ? sum >= x && before < x : sum > x && (i == 0 || before <= x)) s.found[0] = i;
+            if (reach ? sum >= y && before < y : sum > y && (i == 0 || before <= y)) s.found[1] = i;
         }
         __syncthreads();
-        *at_x = s.found[0];
-        *at_y = s.found[1];
+        const Span at{s.found[0], s.found[1]};
         __syncthreads();
+        return at;
     }
 };
+
+__device__ inline uint64_t Share(double u, uint64_t sum) {
+    return static_cast<uint64_t>(u * static_cast<double>(sum));
+}
 
 // The passes after the first.  kCuts: which logits to gather; kFinish: the choice from what was
 // gathered; kSmall: the choice from a row that the list holds whole, without any of the others.
@@ -717,13 +759,15 @@ __global__ __launch_bounds__(kChooseThreads) void SampleChoose(const SampleArgs 
     uint64_t* state_list = state_bin + kBins;
     uint32_t flags = 0;
     int32_t top = INT32_MIN;
-    uint64_t best = ~uint64_t{0}, mine = 0;
+    uint64_t best = kNoKey;
     float largest = -INFINITY;
     if constexpr (kPass_ == kFinish) {
-        if (state->live == 0) return;
-        top = state->top;
-        largest = state->largest;
-        mine = state_bin[tid];
+        const RowState at = *state;
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) s.bin[tid + i * kChooseThreads] = state_bin[tid + i * kChooseThreads];
+        if (at.live == 0) return;
+        top = at.top;
+        largest = at.largest;
     } else if constexpr (kPass_ == kCuts) {
         // lane i of each wave: part i
         const char* parts = p.part + row * p.parts * kPartBytes;
@@ -746,32 +790,41 @@ __global__ __launch_bounds__(kChooseThreads) void SampleChoose(const SampleArgs 
                 largest = fmaxf(largest, __shfl_xor(largest, off, kWave));
             }
             if (h.t != 0.0f && flags == kSome) {
+                // the first bin in each part: as far below the part's largest as s.few says
+                if (tid < p.parts) s.few[tid] = static_cast<uint32_t>(part.top == INT32_MIN || part.top - top < -kBins ? -kBins : part.top - top);
+                __syncthreads();
+                uint64_t sum[kEach] = {};
 #pragma unroll 8
                 for (int i = 0; i < p.parts; ++i) {
-                    // this thread's bin in part i
-                    const int32_t part_top = __builtin_amdgcn_readlane(part.top, i), at = part_top - (top - tid);
-                    const bool in = part_top != INT32_MIN && at >= 0;
-                    const uint64_t m = reinterpret_cast<const uint64_t*>(parts + i * kPartBytes + sizeof(Part))[in ? at : 0];
-                    mine += in ? m : 0;
+                    const uint64_t* bins = reinterpret_cast<const uint64_t*>(parts + i * kPartBytes + sizeof(Part));
+                    const int32_t from = static_cast<int32_t>(s.few[i]) + tid;
+#pragma unroll
+                    for (int e = 0; e < kEach; ++e) {
+                        const int32_t at = from + e * kChooseThreads;
+                        const uint64_t m = bins[at >= 0 ? at : 0];
+                        sum[e] += at >= 0 ? m : 0;
+                    }
+                }
+#pragma unroll
+                for (int e = 0; e < kEach; ++e) {
+                    s.bin[tid + e * kChooseThreads] = sum[e];
+                    state_bin[tid + e * kChooseThreads] = sum[e];
                 }
             }
         }
     } else {
-        // a thread has up to kEach elements
-        constexpr int kEach = kList / kChooseThreads;
-        float x[kEach];
         bool nan = false;
-#pragma unroll
-        for (int i = 0; i < kEach; ++i) {
-            const int32_t at = tid + i * kChooseThreads;
-            x[i] = at < p.vocab ? T::Get(units.x[at]) : -INFINITY;
-            nan |= x[i] != x[i];
-            largest = fmaxf(largest, x[i]);
-            if (at < p.vocab) s.list[at] = x[i] > -INFINITY ? Key(x[i], at) : kNoKey;
-            if (x[i] > -INFINITY) best = Key(x[i], at) < best ? Key(x[i], at) : best;
+#pragma unroll 4
+        for (int i = tid; i < p.vocab; i += kChooseThreads) {
+            const float x = T::Get(units.x[i]);
+            const uint64_t key = x > -INFINITY ? Key(x, i) : kNoKey;
+            nan |= x != x;
+            largest = fmaxf(largest, x);
+            s.list[i] = key;
+            best = key < best ? key : best;
         }
-        s.bin[tid] = 0;
-        if (tid == 0) s.word[0] = ~uint64_t{0};
+        for (int i = tid; i < kBins; i += kChooseThreads) s.bin[i] = 0;
+        if (tid == 0) s.word[0] = kNoKey;
         largest = BlockMax<kChooseWaves>(largest, reinterpret_cast<float*>(s.scan_u));
         flags = (largest > -INFINITY ? kSome : 0) | (__syncthreads_or(nan) ? kNan : 0);
         if (h.t == 0.0f) {
@@ -781,16 +834,6 @@ __global__ __launch_bounds__(kChooseThreads) void SampleChoose(const SampleArgs 
         } else if (!h.bad) {
             double f;
             top = BinOf(h, largest, &f);
-#pragma unroll
-            for (int i = 0; i < kEach; ++i) {
-                const int32_t b = top - BinOf(h, x[i], &f);
-                if (x[i] > -INFINITY && b < kBins) {
-                    atomicAdd(reinterpret_cast<ull*>(&s.bin[b]), static_cast<ull>(h.k != 0 ? 1 : Weight(f)));
-                }
-            }
-            __syncthreads();
-            mine = s.bin[tid];
-            __syncthreads();
         }
     }
     if constexpr (kPass_ != kFinish) {
@@ -805,10 +848,18 @@ __global__ __launch_bounds__(kChooseThreads) void SampleChoose(const SampleArgs 
             return;
         }
     }
-    if constexpr (kPass_ == kCuts) state_bin[tid] = mine;
     Chooser<T> ch{p, h, s, units, p.largest + row * p.segments, top, kLastKey};
-    static_assert(kBins == kChooseThreads, "a thread a bin");
-    s.edge[tid] = exp(tid * (-1.0 / kPerUnit));
+    ch.MakeEdges();
+    if constexpr (kPass_ == kSmall) {
+        for (int i = tid; i < p.vocab; i += kChooseThreads) {
+            const uint64_t key = s.list[i];
+            s.code[i] = ch.CodeOf(key);
+            double place;
+            const int b = ch.BinOfKey(key, &place);
+            if (s.code[i] != ~0u) ch.AddTo(b, h.k != 0 ? 1 : Weight(place));
+        }
+    }
+    __syncthreads();
     // Three places are looked for in turn, each where its cut is asked for: the top-k's, the
     // top-p's (with the sum that min-p leaves) and the token's.  The row is gathered once for
     // the first two as a rule, or once for the last two.
@@ -816,9 +867,10 @@ __global__ __launch_bounds__(kChooseThreads) void SampleChoose(const SampleArgs 
     int last = kBins - 1;       // no element of a later bin can be chosen
     int n = kPass_ == kSmall ? p.vocab : -1;  // elements of the list, where it has all that is needed
     const double u = h.u;
-    double kept = 0.0, least = 0.0, reach = 0.0;
+    uint64_t kept = 0, reach = 0;
+    double least = 0.0;
     bool by_p = h.p < 1.0f, by_m = h.m > 0.0f;
-    Span m{0, 0}, drawn{0, 0};
+    Span m{0, 0};
     int p_bin = 0;
     bool first = true;
 #pragma unroll 1
@@ -828,30 +880,24 @@ __global__ __launch_bounds__(kChooseThreads) void SampleChoose(const SampleArgs 
         int bin;
         uint64_t bound;
         if (what == kTopK) {
-            uint64_t all;
-            const uint64_t upto = ScanBlock(mine, s.scan_u, &all), k = static_cast<uint64_t>(h.k);
-            cuts = all > k;  // else what is beyond the bins weighs nothing
-            if (cuts ? upto >= k && upto - mine < k : tid == kBins - 1) {
-                s.found[0] = tid;
-                s.word[0] = upto;
-                s.word[1] = upto - mine;
-            }
-            __syncthreads();
-            last = bin = s.found[0];
-            const uint64_t held = s.word[0];
-            bound = k - s.word[1];
-            __syncthreads();
+            // (where no more than k have a bin, those beyond weigh nothing)
+            uint64_t before = 0, held;
+            const uint64_t k = static_cast<uint64_t>(h.k);
+            last = bin = ch.Narrow(kCount, k, &before, &held);
+            held += before;
+            cuts = held >= k;
+            if (!cuts) last = kBins - 1;
+            bound = k - before;
             a = b = {held <= kList ? 0 : last, last};
             look = cuts;
         } else if (what == kTopP) {
-            if (h.k == 0) s.bin[tid] = mine;
             ch.SumBins();
             kept = s.sum[last];
-            double low = kept;  // what is kept will weigh low .. kept
+            uint64_t low = kept;  // what is kept will weigh low .. kept
             if (by_p) {
-                int same;
-                reach = static_cast<double>(h.p) * kept;
-                ch.FirstBins(last, true, reach, reach, &p_bin, &same);
+                const double x = ceil(static_cast<double>(h.p) * static_cast<double>(kept));
+                reach = x > 1.0 ? static_cast<uint64_t>(x) : 1;
+                p_bin = ch.FirstBins(last, true, reach, reach).lo;
             }
             if (by_m) {
                 least = fmin(static_cast<double>(h.m), 1.0) * ch.WeightOf(largest);  // its equals are kept
@@ -876,17 +922,14 @@ __global__ __launch_bounds__(kChooseThreads) void SampleChoose(const SampleArgs 
                 if (s.sum[m.hi] < kept) kept = s.sum[m.hi];
                 if (ch.Below(m.lo) < low) low = ch.Below(m.lo);
             }
-            ch.FirstBins(last, false, u * low, u * kept, &drawn.lo, &drawn.hi);
-            b = drawn;
+            b = ch.FirstBins(last, false, Share(u, low), Share(u, kept));
             if (a.lo > a.hi) a = b;
             bin = p_bin;
             bound = by_p ? ch.InBin(reach, p_bin, true) : 0;
             look = by_p;
         } else {
-            int same;
-            const double x = u * kept;
-            ch.FirstBins(last, false, x, x, &bin, &same);
-            bin = bin < drawn.lo ? drawn.lo : bin > drawn.hi ? drawn.hi : bin;  // (sums' roundings)
+            const uint64_t x = Share(u, kept);
+            bin = ch.FirstBins(last, false, x, x).lo;
             bound = ch.InBin(x, bin, false);
             a = b = {bin, bin};
         }
@@ -898,7 +941,8 @@ __global__ __launch_bounds__(kChooseThreads) void SampleChoose(const SampleArgs 
         if (kPass_ == kFinish && first) {  // what was gathered for this
             first = false;
             n = static_cast<int>(state->n);
-            for (int i = tid; i < n && i < kList; i += kChooseThreads) s.list[i] = state_list[i];
+#pragma unroll 4
+            for (int i = tid; i < (n < kList ? n : kList); i += kChooseThreads) ch.PutInList(i, state_list[i]);
             __syncthreads();
             if (n > kList) n = -1;
             whole = !(what == kTopK && a.lo != 0);
@@ -910,22 +954,21 @@ __global__ __launch_bounds__(kChooseThreads) void SampleChoose(const SampleArgs 
         }
         if (what == kTopP && by_m) {
             uint64_t sum[3] = {0, 0, 0};
-            auto add = [&](int at, double place, uint64_t) {
+            const double e[3] = {ch.Edge(m.lo), ch.Edge(m.lo < m.hi ? m.lo + 1 : m.lo), ch.Edge(m.hi)};
+            auto add = [&](int at, double place, uint64_t, uint32_t) {
                 const uint64_t w = Weight(place);
-                if (static_cast<double>(w) * s.edge[at] < least) return;
 #pragma unroll
-                for (int i = 0; i < 3; ++i) sum[i] += at - m.lo == i ? w : 0;
+                for (int i = 0; i < 3; ++i) sum[i] += at - m.lo == i && static_cast<double>(w) * e[i] >= least ? w : 0;
             };
             if (kPass_ == kSmall || (n >= 0 && whole)) ch.InList(n, m, add);
-            else ch.Visit(m, add);
-            double upto = ch.Below(m.lo);
+            else ch.Visit(m, [&](int at, double place, uint64_t key) { add(at, place, key, 0); });
+            kept = ch.Below(m.lo);
 #pragma unroll
             for (int i = 0; i < 3; ++i) {
                 uint64_t all;
                 ScanBlock(sum[i], s.scan_u, &all);
-                if (m.lo + i <= m.hi) upto += static_cast<double>(all) * s.edge[m.lo + i];
+                if (m.lo + i <= m.hi) kept += ch.Scaled(all, m.lo + i);
             }
-            kept = upto;
         }
         if (look) {
             constexpr Bound kBounds[3] = {kCount, kReach, kPass};
@@ -934,98 +977,110 @@ __global__ __launch_bounds__(kChooseThreads) void SampleChoose(const SampleArgs 
             if (what == kTopK) {
                 ch.limit = at.key;
             } else if (what == kTopP) {
-                const double upto = ch.Below(bin) + static_cast<double>(at.before + at.own) * s.edge[bin];
+                const uint64_t upto = ch.Below(bin) + ch.Scaled(at.before + at.own, bin);
                 if (!by_m || upto < kept) kept = upto;
             } else if (tid == 0) {
                 p.tokens[row] = static_cast<int32_t>(at.key);
-                if (p.prob != nullptr) p.prob[row] = static_cast<float>(static_cast<double>(at.own) * s.edge[bin] / kept);
+                if (p.prob != nullptr) p.prob[row] = static_cast<float>(static_cast<double>(at.own) * ch.Edge(bin) / static_cast<double>(kept));
             }
         }
         if (what == kTopK) {  // the masses of what is left
-            s.bin[tid] = 0;
+            ch.ClearBins();
             __syncthreads();
-            auto add = [&](int at, double place, uint64_t) {
-                atomicAdd(reinterpret_cast<ull*>(&s.bin[at]), static_cast<ull>(Weight(place)));
-            };
+            auto add = [&](int at, double place, uint64_t, uint32_t) { ch.AddTo(at, Weight(place)); };
             if (kPass_ == kSmall || (n >= 0 && whole)) ch.InList(n, {0, last}, add);
-            else ch.Visit({0, last}, add);
+            else ch.Visit({0, last}, [&](int at, double place, uint64_t key) { add(at, place, key, 0); });
         }
         if (!whole) n = -1;
     }
 }
 
 // Between kCuts and kFinish: the row's logits in the two spans found, in any order, 8 lanes to
-// each 128 bytes whose largest is no lower; a wave has what it needs of 64 segments on its
-// way before it looks at the first.
+// each 128 bytes whose largest is no lower.  A wave looks at 64 kLook segments.
 constexpr int kGatherThreads = 256;
-template <typename T>
+template <typename T, int kLook>
 __global__ __launch_bounds__(kGatherThreads) void SampleGather(const SampleArgs p, int parts) {
     constexpr int E = RowUnits<T>::E, kGroups = kWave / kSegment, kRounds = 32 / E;
-    __shared__ int32_t hits_of[kGatherThreads / kWave][kWave];
+    __shared__ uint64_t found[kList];  // (of more the row's list is of no use)
+    __shared__ int32_t hits_of[kGatherThreads / kWave][kLook * kWave];
+    __shared__ uint32_t n_found, base;
     const int lane = static_cast<int>(threadIdx.x) % kWave;
     const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / kWave);
     const int64_t row = blockIdx.x / parts;
     const int part = static_cast<int>(blockIdx.x % parts);
     RowState* state = reinterpret_cast<RowState*>(p.state + row * kStateBytes);
-    if (state->live == 0) return;
     uint64_t* list = reinterpret_cast<uint64_t*>(state + 1) + kBins;
-    const float al = state->al, ah = state->ah, bl = state->bl, bh = state->bh, low = fminf(al, bl);
     const float* largest = p.largest + row * p.segments;
     const RowUnits<T> r(p, row);
     const int32_t units = r.Units(), segments = (units + kSegment - 1) / kSegment;
     int32_t* hit_segment = hits_of[wave];
-    const int32_t step = parts * kGatherThreads;
-    int32_t s0 = (part * (kGatherThreads / kWave) + wave) * kWave;
-    float next = s0 + lane < segments ? largest[s0 + lane] : -INFINITY;
-    for (; s0 < segments; s0 += step) {
-        const bool hit = next >= low;
-        next = s0 + step + lane < segments ? largest[s0 + step + lane] : -INFINITY;
+    const int32_t s0 = (part * (kGatherThreads / kWave) + wave) * kLook * kWave + lane;
+    float m[kLook];
+#pragma unroll
+    for (int l = 0; l < kLook; ++l) m[l] = s0 + l * kWave < segments ? largest[s0 + l * kWave] : -INFINITY;
+    const RowState at = *state;
+    if (at.live == 0) return;
+    if (threadIdx.x == 0) n_found = 0;
+    __syncthreads();
+    const float al = at.al, ah = at.ah, bl = at.bl, bh = at.bh, low = fminf(al, bl);
+    int n = 0;
+#pragma unroll
+    for (int l = 0; l < kLook; ++l) {
+        const bool hit = m[l] >= low;
         const uint64_t mask = __ballot(hit);
-        const int n = __popcll(mask);
-        if (hit) hit_segment[__popcll(mask & ((uint64_t{1} << lane) - 1))] = s0 + lane;
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        for (int g = 0; g < n; g += kGroups * kRounds) {
-            u32x4 raw[kRounds];
-            int32_t unit[kRounds];
+        if (hit) hit_segment[n + __popcll(mask & ((uint64_t{1} << lane) - 1))] = s0 + l * kWave;
+        n += __popcll(mask);
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    for (int g = 0; g < n; g += kGroups * kRounds) {
+        u32x4 raw[kRounds];
+        int32_t unit[kRounds];
 #pragma unroll
-            for (int i = 0; i < kRounds; ++i) {
-                const int j = g + i * kGroups + lane / kSegment;
-                unit[i] = j < n ? hit_segment[j] * kSegment + lane % kSegment : units;
-                raw[i] = r.Load(unit[i], unit[i] < units);
+        for (int i = 0; i < kRounds; ++i) {
+            const int j = g + i * kGroups + lane / kSegment;
+            unit[i] = j < n ? hit_segment[j] * kSegment + lane % kSegment : units;
+            raw[i] = r.Load(unit[i], unit[i] < units);
+        }
+        uint32_t hits = 0;
+#pragma unroll
+        for (int i = 0; i < kRounds; ++i) {
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                const float x = r.Get(raw[i], e);
+                const bool in = (x >= al && x <= ah) || (x >= bl && x <= bh);
+                hits |= in ? 1u << (i * E + e) : 0u;
             }
-            uint32_t hits = 0;
+        }
+        if (__ballot(hits != 0) == 0) continue;
+        // places for the wave's hits: one addition for all
+        const uint32_t mine = __popc(hits);
+        uint32_t upto = mine;
 #pragma unroll
-            for (int i = 0; i < kRounds; ++i) {
+        for (int off = 1; off < kWave; off *= 2) {
+            const uint32_t o = __shfl_up(upto, off, kWave);
+            if (lane >= off) upto += o;
+        }
+        uint32_t at = 0;
+        if (lane == kWave - 1) at = atomicAdd(&n_found, upto);
+        at = __builtin_amdgcn_readlane(at, kWave - 1) + upto - mine;
 #pragma unroll
-                for (int e = 0; e < E; ++e) {
-                    const float x = r.Get(raw[i], e);
-                    const bool in = (x >= al && x <= ah) || (x >= bl && x <= bh);
-                    hits |= in ? 1u << (i * E + e) : 0u;
-                }
-            }
-            // places for the wave's hits: one addition for all
-            const uint32_t mine = __popc(hits);
-            uint32_t upto = mine;
+        for (int i = 0; i < kRounds; ++i) {
 #pragma unroll
-            for (int off = 1; off < kWave; off *= 2) {
-                const uint32_t o = __shfl_up(upto, off, kWave);
-                if (lane >= off) upto += o;
-            }
-            uint32_t at = 0;
-            if (lane == kWave - 1 && upto != 0) at = atomicAdd(&state->n, upto);
-            at = __builtin_amdgcn_readlane(at, kWave - 1) + upto - mine;
-#pragma unroll
-            for (int i = 0; i < kRounds; ++i) {
-#pragma unroll
-                for (int e = 0; e < E; ++e) {
-                    if (hits >> (i * E + e) & 1) {
-                        if (at < kList) list[at] = Key(r.Get(raw[i], e), r.Index(unit[i], e));
-                        ++at;
-                    }
+            for (int e = 0; e < E; ++e) {
+                if (hits >> (i * E + e) & 1) {
+                    if (at < kList) found[at] = Key(r.Get(raw[i], e), r.Index(unit[i], e));
+                    ++at;
                 }
             }
         }
     }
+    // one addition to the row's count for the workgroup
+    __syncthreads();
+    const uint32_t total = n_found;
+    if (total == 0) return;
+    if (threadIdx.x == 0) base = atomicAdd(&state->n, total);
+    __syncthreads();
+    for (uint32_t i = threadIdx.x; i < total && base + i < kList; i += kGatherThreads) list[base + i] = found[i];
 }
 
 // Workgroups of the first pass a row: as many as fill the device at 2 a compute unit,
@@ -1038,15 +1093,13 @@ int Parts(int64_t n_rows, int64_t vocab, int bytes) {
     if (parts > kMaxParts) parts = kMaxParts;
     return static_cast<int>(parts < 1 ? 1 : parts);
 }
-// Workgroups of the gather a row: 4 a compute unit, 64 segments a wave at least.
-int GatherParts(int64_t n_rows, int64_t vocab, int bytes) {
-    int64_t parts = (static_cast<int64_t>(ComputeUnits()) * 4 + n_rows - 1) / n_rows;
-    const int64_t most = (vocab * bytes / 128 + kGatherThreads - 1) / kGatherThreads;
-    if (parts > most) parts = most;
-    return static_cast<int>(parts < 1 ? 1 : parts);
-}
 int64_t Segments(int64_t vocab, int bytes) {  // one more where the row is not aligned
     return (vocab * bytes + 127) / 128 + 1;
+}
+// Workgroups of the gather a row.
+int GatherParts(int64_t vocab, int bytes, int look) {
+    const int each = kGatherThreads * look;
+    return static_cast<int>((Segments(vocab, bytes) + each - 1) / each);
 }
 
 // Rows that one round of launches takes, which is what the workspace is for.
@@ -1074,8 +1127,13 @@ mlk_status Launch(SampleArgs p, int64_t n_rows, char* workspace, hipStream_t s) 
             p.largest = reinterpret_cast<float*>(p.part + rows * p.parts * kPartBytes);
             hipLaunchKernelGGL(SampleBins<T>, dim3(static_cast<unsigned>(rows * p.parts)), dim3(kThreads), 0, s, p);
             hipLaunchKernelGGL((SampleChoose<T, kCuts>), grid, block, 0, s, p);
-            const int parts = GatherParts(rows, p.vocab, kBytes);
-            hipLaunchKernelGGL(SampleGather<T>, dim3(static_cast<unsigned>(rows * parts)), dim3(kGatherThreads), 0, s, p, parts);
+            // where those of one look are more than the device holds at once (5 a compute unit), of
+            // four (512 fp32 rows of top-k: 36 us, with four 9)
+            const bool many = rows * GatherParts(p.vocab, kBytes, 1) > 5 * ComputeUnits();
+            const int parts = GatherParts(p.vocab, kBytes, many ? 4 : 1);
+            const dim3 gather(static_cast<unsigned>(rows * parts)), threads(kGatherThreads);
+            if (!many) hipLaunchKernelGGL((SampleGather<T, 1>), gather, threads, 0, s, p, parts);
+            else hipLaunchKernelGGL((SampleGather<T, 4>), gather, threads, 0, s, p, parts);
             hipLaunchKernelGGL((SampleChoose<T, kFinish>), grid, block, 0, s, p);
         }
         const mlk_status st = CheckLaunch("SampleChoose");
