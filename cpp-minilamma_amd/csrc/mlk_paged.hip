@@ -305,6 +305,13 @@ mlk_status CheckPaged(const char* fn, const mlk_paged_cache* cache, const mlk_pa
 
 namespace {
 
+Scores ScoresOf(const mlk_attention_scores* s) {
+    if (s == nullptr) return {};
+    // (a window of over 2^30 positions, the longest sequence, limits nothing)
+    return {s->slopes, s->prefix_len, s->first, s->softcap,
+            s->window > (1 << 30) || s->window < 0 ? 0 : static_cast<int32_t>(s->window)};
+}
+
 // Score functions and masks of an attention call; they are read while out is written.
 mlk_status CheckScores(const char* fn, const mlk_attention_scores* scores, const void* out, Scores* to) {
     if (scores == nullptr) return Fail(MLK_ERR_INVALID, "%s: scores must not be null", fn);
@@ -317,9 +324,7 @@ mlk_status CheckScores(const char* fn, const mlk_attention_scores* scores, const
         if (!Aligned(p, 4)) return Fail(MLK_ERR_INVALID, "%s: slopes, prefix_len and first must be 4-byte aligned", fn);
         if (p != nullptr && p == out) return Fail(MLK_ERR_INVALID, "%s: out may not alias slopes, prefix_len or first", fn);
     }
-    // (a window of over 2^30 positions, the longest sequence, limits nothing)
-    *to = {scores->slopes, scores->prefix_len, scores->first, scores->softcap,
-           scores->window > (1 << 30) ? 0 : static_cast<int32_t>(scores->window)};
+    *to = ScoresOf(scores);
     return MLK_OK;
 }
 
@@ -524,7 +529,7 @@ int64_t mlk_attention_paged_workspace_bytes(int64_t n_seqs, int64_t n_tokens,
                                             int32_t n_heads, int32_t n_kv_heads,
                                             int32_t head_dim) {
     return AttendWorkspace(n_seqs, n_tokens, max_new_tokens, max_seq_len, n_heads, n_kv_heads,
-                           head_dim, false);
+                           head_dim, false, {});
 }
 
 mlk_status mlk_attention_packed(int32_t type, const void* q, int64_t q_row_stride, const void* k,
@@ -560,26 +565,25 @@ mlk_status mlk_attention_packed_scored(int32_t type, const mlk_attention_scores*
 int64_t mlk_attention_paged_scored_workspace_bytes(int64_t n_seqs, int64_t n_tokens,
                                                    int64_t max_new_tokens, int64_t max_seq_len,
                                                    int32_t n_heads, int32_t n_kv_heads,
-                                                   int32_t head_dim, int64_t window) {
-    (void)window;
+                                                   int32_t head_dim,
+                                                   const mlk_attention_scores* scores) {
     return AttendWorkspace(n_seqs, n_tokens, max_new_tokens, max_seq_len, n_heads, n_kv_heads,
-                           head_dim, false);
+                           head_dim, false, ScoresOf(scores));
 }
 
 int64_t mlk_attention_packed_scored_workspace_bytes(int64_t n_seqs, int64_t n_tokens,
                                                     int64_t max_seq_len, int32_t n_heads,
                                                     int32_t n_kv_heads, int32_t head_dim,
-                                                    int64_t window) {
-    (void)window;
+                                                    const mlk_attention_scores* scores) {
     return AttendWorkspace(n_seqs, n_tokens, max_seq_len, max_seq_len, n_heads, n_kv_heads,
-                           head_dim, true);
+                           head_dim, true, ScoresOf(scores));
 }
 
 int64_t mlk_attention_packed_workspace_bytes(int64_t n_seqs, int64_t n_tokens,
                                              int64_t max_seq_len, int32_t n_heads,
                                              int32_t n_kv_heads, int32_t head_dim) {
     return AttendWorkspace(n_seqs, n_tokens, max_seq_len, max_seq_len, n_heads, n_kv_heads,
-                           head_dim, true);
+                           head_dim, true, {});
 }
 
 }  // extern "C"

@@ -245,7 +245,9 @@ struct RaggedParams {
     int64_t q_row;
     void* out;
     int32_t n_heads, n_kv_heads, group;
-    float factor;  // scale * log2 e
+    float factor;  // scale * log2 e; with a cap, scale / cap
+    Scores scores;  // what kScored kernels take into account, the others have none
+    float cap;     // softcap * log2 e
     int32_t vec;   // rows of q, K and V 16-byte aligned, head_dim % 8 == 0
     // tile kernel: chunk c of a row is positions c * chunk .. of it
     int32_t chunk, n_chunks;
@@ -264,25 +266,81 @@ struct RaggedParams {
     int32_t* err;
 };
 
+// ---------------------------------------------------- score functions
+// Scores after cap and bias are kept times log2 e, which is what the weights' exp2 takes.
+
+// tanh(x): Lambert's continued fraction x / (1 + x^2 / (3 + x^2 / (5 + ..))), to x^5 over
+// x^4: within 2^-22 of itself for |x| <= 1.  Beyond, (1 - e) / (1 + e) of e = exp(-2 |x|),
+// which is at most 0.14: no digits are lost.
+__device__ inline float TanhNear(float x) {
+    const float t = x * x;
+    return x * fmaf(t + 105.0f, t, 945.0f) * __builtin_amdgcn_rcpf(fmaf(fmaf(15.0f, t, 420.0f), t, 945.0f));
+}
+__device__ inline float TanhFar(float x) {
+    const float e = __builtin_amdgcn_exp2f(fabsf(x) * (-2.0f * kLog2e));
+    return copysignf((1.0f - e) * __builtin_amdgcn_rcpf(1.0f + e), x);
+}
+
+// N raw scores of one row, q . k times the row's 2^e, at positions j(i): factor is p.factor
+// for that row; slope: log2 e times the head's.  Whole waves call it.
+template <int N, typename J>
+__device__ inline void Score(const RaggedParams& p, float factor, float slope, int32_t pos, float* x, const J& j) {
+    if (p.cap > 0.0f) {
+        bool far = false;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            x[i] *= factor;
+            far |= !(fabsf(x[i]) <= 1.0f);
+        }
+        if (__ballot(far) != 0) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) x[i] = p.cap * (fabsf(x[i]) <= 1.0f ? TanhNear(x[i]) : TanhFar(x[i]));
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; ++i) x[i] = p.cap * TanhNear(x[i]);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) x[i] *= factor;
+    }
+    if (p.scores.slopes != nullptr) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) x[i] = fmaf(-slope, fabsf(static_cast<float>(pos - j(i))), x[i]);
+    }
+}
+__device__ inline float SlopeOf(const RaggedParams& p, int h) {
+    return p.scores.slopes != nullptr ? p.scores.slopes[h] * kLog2e : 0.0f;
+}
+
 // Rows of a KV head that the few-row kernel takes: two blocks of 16, one where
 // two would not leave registers for the tile in flight.
 inline int FewMost(int head_dim) { return head_dim <= 128 ? 32 : 16; }
 constexpr int kFewKeys = 32;   // positions of its unit of work
+constexpr int kTileAlign = 64;  // positions that a tile's chunks begin at multiples of
 constexpr int kFewHeads = 8;   // most KV heads of its workgroup
 
-// Launches on `stream`; type and cache_type choose the instance.
+// The kernels are built for each head_dim, plain and with score functions and masks, in
+// source files of their own; type and cache_type choose the instance.
+template <int HD, bool kScored>
+mlk_status LaunchFewAt(const RaggedParams& p, dim3 grid, int32_t type, int32_t cache_type, hipStream_t stream);
+template <int HD, bool kScored>
+mlk_status LaunchTileAt(const RaggedParams& p, dim3 grid, int64_t n_slots, int32_t type,
+                        int32_t cache_type, hipStream_t stream);
+template <template <int, bool> class F, bool kScored, typename... Args>
+inline mlk_status ByDim(int head_dim, const Args&... a) {
+    if (head_dim <= 64) return F<64, kScored>::Run(a...);
+    if (head_dim <= 128) return F<128, kScored>::Run(a...);
+    return F<256, kScored>::Run(a...);
+}
+
 // Waves of a few-row workgroup: 8, or 4 where the registers of 8 would not do.
 inline int FewWaves(int head_dim, int few_rows) { return head_dim <= 128 && few_rows <= 16 ? 8 : 4; }
 // Most workgroups of a launch (512 threads each, below 2^32 in all), and of a call:
 // what is not split goes over as many launches as it takes.
 constexpr int64_t kMaxBlocks = 1 << 22, kMaxCallBlocks = int64_t{1} << 35;
-int64_t TileBlocks(const RaggedParams& p);
-mlk_status LaunchFew(const RaggedParams& p, int32_t type, int32_t cache_type, hipStream_t stream);
 // Rows of a tile: 8 waves' 32 each, 4 waves' where a row's results take twice the
 // registers.
 __host__ __device__ constexpr int TileRows(int head_dim) { return head_dim <= 128 ? 256 : 128; }
-mlk_status LaunchTile(const RaggedParams& p, int32_t type, int32_t cache_type, hipStream_t stream);
-
 // f.template Run<A, C>() for the types.
 template <typename F>
 mlk_status ByType(int32_t type, int32_t cache_type, const F& f) {
@@ -308,25 +366,50 @@ struct FewWork {
     int32_t s, units;
 };
 
+// The unit that a sequence's first begins at: those before hold no position that any of
+// its new tokens sees.
+template <bool kScored>
+__device__ inline int32_t FewFirst(const RaggedParams& p, const Seq& q) {
+    if constexpr (!kScored) {
+        return 0;
+    } else {
+        int32_t lo = 0;
+        if (p.scores.window > 0 && q.len - q.n - p.scores.window + 1 > 0) lo = q.len - q.n - p.scores.window + 1;
+        if (p.scores.first != nullptr) {
+            int32_t least = INT32_MAX;
+            for (int i = 0; i < q.n; ++i) {
+                const int32_t f = p.scores.first[q.t0 + i];
+                least = f < least ? f : least;
+            }
+            lo = least > lo ? least : lo;
+        }
+        return (lo < q.len ? lo : q.len - 1) / kFewKeys;
+    }
+}
+__device__ inline int32_t FewHeld(const Seq& q, int32_t first) {  // units with positions
+    return (q.len + kFewKeys - 1) / kFewKeys - first;
+}
 // (A short sequence counts kFewRun units, what it costs; those past its length
 // hold nothing.)
 constexpr int kFewRun = 8;
+template <bool kScored>
 __device__ inline int32_t FewUnits(const RaggedParams& p, int s) {
     Seq q;
     if (s >= p.batch.n_seqs || !LoadSeq(p.batch, s, &q)) return 0;
     if (q.n == 0 || static_cast<int64_t>(q.n) * p.group > p.few_rows) return 0;
-    const int32_t units = (q.len + kFewKeys - 1) / kFewKeys;
+    const int32_t units = FewHeld(q, FewFirst<kScored>(p, q));
     return units > kFewRun ? units : kFewRun;
 }
 
 // Units of all sequences, and of those before sequence `upto` (a whole wave;
 // every lane gets them).
+template <bool kScored>
 __device__ inline int64_t CountFewUnits(const RaggedParams& p, int upto, int64_t* before) {
     const int lane = static_cast<int>(threadIdx.x) % kWave;
     int64_t total = 0;
     *before = 0;
     for (int s0 = 0; s0 < p.batch.n_seqs; s0 += kWave) {
-        int64_t u = FewUnits(p, s0 + lane), b = s0 + lane < upto ? u : 0;
+        int64_t u = FewUnits<kScored>(p, s0 + lane), b = s0 + lane < upto ? u : 0;
         for (int off = kWave / 2; off > 0; off /= 2) {
             u += __shfl_xor(u, off, kWave);
             b += __shfl_xor(b, off, kWave);
@@ -352,19 +435,20 @@ __device__ inline void DivideFew(const RaggedParams& p, int64_t total, FewWork* 
 }
 
 // The sequence of a worker's first unit (a whole wave; false: nothing to do).
+template <bool kScored>
 __device__ inline bool FindFewWork(const RaggedParams& p, int64_t worker, FewWork* w) {
     const int lane = static_cast<int>(threadIdx.x) % kWave;
     if (p.batch.n_seqs == 1) {
         w->s = 0;
         w->before = 0;
-        w->units = FewUnits(p, 0);
+        w->units = FewUnits<kScored>(p, 0);
         DivideFew(p, w->units, w);
         return worker * w->share < static_cast<int64_t>(w->units) * (p.n_kv_heads / w->heads);
     }
     int64_t before = 0, total = 0;
-    if (p.batch.n_seqs > kWave) total = CountFewUnits(p, 0, &before);
+    if (p.batch.n_seqs > kWave) total = CountFewUnits<kScored>(p, 0, &before);
     for (int s0 = 0; s0 < p.batch.n_seqs; s0 += kWave) {
-        const int32_t mine = FewUnits(p, s0 + lane);
+        const int32_t mine = FewUnits<kScored>(p, s0 + lane);
         int64_t sum = mine;  // of lanes 0 .. lane
         for (int off = 1; off < kWave; off *= 2) {
             const int64_t v = __shfl_up(sum, off, kWave);
@@ -395,6 +479,16 @@ __device__ inline bool FindFewWork(const RaggedParams& p, int64_t worker, FewWor
 __device__ inline int64_t FewPartial(const RaggedParams& p, int64_t worker, int place, int head,
                                      int m) {
     return ((worker * 2 + place) * kFewHeads + head) * p.few_rows + m;
+}
+// With scores, chunk 0 of the row tile from row m0 on begins here: no row of it sees
+// positions before by its window.
+__device__ inline int32_t TileBase(const RaggedParams& p, const Seq& q, int64_t m0) {
+    const int64_t lo = q.len - q.n + m0 / p.group - p.scores.window + 1;
+    return p.scores.window > 0 && lo > 0 ? static_cast<int32_t>(lo) / kTileAlign * kTileAlign : 0;
+}
+// The chunk of a tile that position lo, or the base where that is later, lies in.
+__device__ inline int32_t TileFirstChunk(const RaggedParams& p, int32_t base, int32_t lo) {
+    return (lo > base ? lo - base : 0) / p.chunk;
 }
 __device__ inline int64_t TilePartial(const RaggedParams& p, int32_t t, int h) {
     return (static_cast<int64_t>(t) * p.n_heads + h) * p.n_chunks;

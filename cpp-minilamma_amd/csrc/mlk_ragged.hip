@@ -5,8 +5,8 @@
 // Token row t at position p of its sequence, head h on KV head h / (H / KV):
 //   s_j = scale (q . k_j), j <= p;  w = softmax(s);  out = sum_j w_j v_j.
 // Sequences of few rows (new tokens x query heads of a group, at most FewMost)
-// are bound by the bytes of K and V (mlk_ragged_few.hip); the others by the
-// matrix cores (mlk_ragged_tile.hip).  A batch of both kinds runs both kernels,
+// are bound by the bytes of K and V (mlk_ragged_few.h); the others by the
+// matrix cores (mlk_ragged_tile.h).  A batch of both kinds runs both kernels,
 // each leaving the other's sequences alone.
 #include "mlk_ragged.h"
 
@@ -27,6 +27,7 @@ constexpr int kAhead = 4;
 struct JoinRow {
     int64_t base, next, step;
     int32_t t, h, n;
+    bool blind;  // sees nothing: zeros
 };
 
 template <typename A, int L>
@@ -85,7 +86,7 @@ __device__ inline void Join(const RaggedParams& p, const JoinRow& row, int part_
     for (int i = 1; i < per_row; ++i) o += sums[g + i][lane];
     typename A::Bits* out = static_cast<typename A::Bits*>(p.out) +
                             (static_cast<int64_t>(row.t) * p.n_heads + row.h) * hd;
-    const float inv = 1.0f / l;
+    const float inv = row.blind ? 0.0f : 1.0f / l;
     if (p.vec) {  // out is 16-byte aligned, head_dim a multiple of 8
         if (4 * lane < hd) {
             typedef typename A::Bits Out4 __attribute__((ext_vector_type(4)));
@@ -108,7 +109,7 @@ __device__ inline void Join(const RaggedParams& p, const JoinRow& row, int part_
 // 8B heads, bf16, by sequence and by worker: 16384 sequences of lengths to 1024 21.5
 // and 6.7 ms, 1024 of them 0.50 and 0.46; 64 of lengths to 8192 191 and 195 us, one
 // of 8191 in fp32 27 and 38.)
-template <typename A, int L, bool kByWorker>
+template <typename A, int L, bool kByWorker, bool kScored>
 __global__ __launch_bounds__(kThreads) void JoinFew(const RaggedParams p, int per_row,
                                                     int per_place) {
     constexpr int NG = kThreads / L;
@@ -121,7 +122,7 @@ __global__ __launch_bounds__(kThreads) void JoinFew(const RaggedParams p, int pe
     FewWork work;
     int64_t head0 = 0, heads = p.n_kv_heads;
     if constexpr (kByWorker) {
-        if (!FindFewWork(p, place, &work)) return;
+        if (!FindFewWork<kScored>(p, place, &work)) return;
         const int64_t blocks = p.n_kv_heads / work.heads, unit = place * work.share;
         const int64_t block = (unit - work.before * blocks) / work.units;
         const int64_t u0 = work.before * blocks + block * work.units;
@@ -130,7 +131,7 @@ __global__ __launch_bounds__(kThreads) void JoinFew(const RaggedParams p, int pe
         heads = work.heads;
     } else {
         work.s = place;
-        work.units = FewUnits(p, place);
+        work.units = FewUnits<kScored>(p, place);
         if (work.units == 0) return;
     }
     Seq q;
@@ -139,14 +140,14 @@ __global__ __launch_bounds__(kThreads) void JoinFew(const RaggedParams p, int pe
     if (first >= rows * heads) return;  // none of the workgroup's rows is one
     if constexpr (!kByWorker) {
         work.before = 0;
-        DivideFew(p, p.batch.n_seqs == 1 ? work.units : CountFewUnits(p, work.s, &work.before), &work);
+        DivideFew(p, p.batch.n_seqs == 1 ? work.units : CountFewUnits<kScored>(p, work.s, &work.before), &work);
     }
     const int m = static_cast<int>(in_place % rows);
     JoinRow row{};
     if (in_place < rows * heads) {
         const int64_t kvh = head0 + in_place / rows;
         const int64_t u0 = work.before * (p.n_kv_heads / work.heads) + kvh / work.heads * work.units;
-        const int32_t held = (q.len + kFewKeys - 1) / kFewKeys;  // units with positions
+        const int32_t held = FewHeld(q, FewFirst<kScored>(p, q));
         const int64_t w0 = u0 / work.share, w1 = (u0 + held - 1) / work.share;
         const int head = static_cast<int>(kvh % work.heads);
         if (w1 > w0) {
@@ -156,13 +157,17 @@ __global__ __launch_bounds__(kThreads) void JoinFew(const RaggedParams p, int pe
             row.base = FewPartial(p, w0, u0 == w0 * work.share ? 0 : 1, head, m);
             row.next = FewPartial(p, w0 + 1, 0, head, m);
             row.step = 2 * kFewHeads * p.few_rows;
+            if constexpr (kScored) {
+                const Seen seen = SeenBy(p.scores, work.s, row.t, q.len - q.n + m / p.group, q.len);
+                row.blind = seen.lo > seen.hi;
+            }
         }
     }
     Join<A, L>(p, row, g % per_row, per_row, sums);
 }
 
 // Tile kernel's rows: blockIdx.x = token * per_token + place of its heads.
-template <typename A, int L>
+template <typename A, int L, bool kScored>
 __global__ __launch_bounds__(kThreads) void JoinTile(const RaggedParams p, int per_row,
                                                      int per_token) {
     constexpr int NG = kThreads / L;
@@ -174,12 +179,23 @@ __global__ __launch_bounds__(kThreads) void JoinTile(const RaggedParams p, int p
     Seq q;
     if (!LoadSeq(p.batch, s, &q) || t < q.t0 || t >= q.t0 + q.n) return;
     const int32_t pos = q.len - q.n + (t - q.t0);
-    if (static_cast<int64_t>(q.n) * p.group <= p.few_rows || pos < p.chunk) return;
-    JoinRow row{0, 0, 1, t, h, 0};
+    if (static_cast<int64_t>(q.n) * p.group <= p.few_rows || (!kScored && pos < p.chunk)) return;
+    JoinRow row{0, 0, 1, t, h, 0, false};
     if (h < p.n_heads) {
         row.base = TilePartial(p, t, h);
-        row.next = row.base + 1;
         row.n = pos / p.chunk + 1;
+        if constexpr (kScored) {
+            // the row's tile, and which of its chunks have a part of the row
+            const int64_t m = static_cast<int64_t>(t - q.t0) * p.group + h % p.group;
+            const int rows = TileRows(p.rows.head_dim);
+            const int32_t base = TileBase(p, q, m / rows * rows);
+            const Seen seen = SeenBy(p.scores, s, t, pos, q.len);
+            const int32_t c0 = TileFirstChunk(p, base, seen.lo);
+            row.base += c0;
+            row.n = seen.lo > seen.hi ? 0 : (seen.hi - base) / p.chunk - c0 + 1;
+            if (row.n <= 1) row.n = 0;  // written by the tile
+        }
+        row.next = row.base + 1;
     }
     Join<A, L>(p, row, g % per_row, per_row, sums);
 }
@@ -214,29 +230,89 @@ inline int64_t JoinTileBlocks(const RaggedParams& p) {
     return JoinTilePerToken(p) * p.batch.n_tokens;
 }
 
-template <typename A, int L>
+template <typename A, int L, bool kScored>
 void StartJoinFew(const RaggedParams& p, hipStream_t s) {
     const dim3 grid(static_cast<unsigned>(JoinFewBlocks(p))), block(kThreads);
     const int per_row = JoinFewPerRow(p), n = static_cast<int>(JoinFewPerPlace(p));
-    if (JoinByWorker(p)) hipLaunchKernelGGL((JoinFew<A, L, true>), grid, block, 0, s, p, per_row, n);
-    else hipLaunchKernelGGL((JoinFew<A, L, false>), grid, block, 0, s, p, per_row, n);
+    if (JoinByWorker(p)) hipLaunchKernelGGL((JoinFew<A, L, true, kScored>), grid, block, 0, s, p, per_row, n);
+    else hipLaunchKernelGGL((JoinFew<A, L, false, kScored>), grid, block, 0, s, p, per_row, n);
 }
-template <typename A>
+template <typename A, bool kScored>
 mlk_status LaunchJoinFew(const RaggedParams& p, hipStream_t s) {
-    if (JoinGroups(p) == 8) StartJoinFew<A, 32>(p, s);
-    else StartJoinFew<A, 64>(p, s);
+    if (JoinGroups(p) == 8) StartJoinFew<A, 32, kScored>(p, s);
+    else StartJoinFew<A, 64, kScored>(p, s);
     return CheckLaunch("JoinFew");
 }
 
-template <typename A>
+template <typename A, bool kScored>
 mlk_status LaunchJoinTile(const RaggedParams& p, hipStream_t s) {
     const dim3 grid(static_cast<unsigned>(JoinTileBlocks(p))), block(kThreads);
     const int per_row = PerRow(JoinGroups(p), p.n_chunks);
     const int n = static_cast<int>(JoinTilePerToken(p));
-    if (JoinGroups(p) == 8) hipLaunchKernelGGL((JoinTile<A, 32>), grid, block, 0, s, p, per_row, n);
-    else hipLaunchKernelGGL((JoinTile<A, 64>), grid, block, 0, s, p, per_row, n);
+    if (JoinGroups(p) == 8) hipLaunchKernelGGL((JoinTile<A, 32, kScored>), grid, block, 0, s, p, per_row, n);
+    else hipLaunchKernelGGL((JoinTile<A, 64, kScored>), grid, block, 0, s, p, per_row, n);
     return CheckLaunch("JoinTile");
 }
+
+// ------------------------------------------------------------ the kernels' launches
+
+template <int HD, bool kScored>
+struct FewAt {
+    static mlk_status Run(const RaggedParams& p, dim3 grid, int32_t type, int32_t cache_type, hipStream_t s) {
+        return LaunchFewAt<HD, kScored>(p, grid, type, cache_type, s);
+    }
+};
+template <int HD, bool kScored>
+struct TileAt {
+    static mlk_status Run(const RaggedParams& p, dim3 grid, int64_t slots, int32_t type, int32_t cache_type, hipStream_t s) {
+        return LaunchTileAt<HD, kScored>(p, grid, slots, type, cache_type, s);
+    }
+};
+
+template <bool kScored>
+mlk_status LaunchFew(const RaggedParams& p, int32_t type, int32_t cache_type, hipStream_t stream) {
+    if (p.workers != 0) {
+        return ByDim<FewAt, kScored>(p.rows.head_dim, p, dim3(static_cast<unsigned>(p.workers)), type,
+                            cache_type, stream);
+    }
+    RaggedParams part = p;
+    const int64_t most = kMaxBlocks / p.n_kv_heads;  // sequences of a launch
+    mlk_status st = MLK_OK;
+    for (part.taken = 0; part.taken < p.batch.n_seqs && st == MLK_OK; part.taken += most) {
+        const int64_t left = p.batch.n_seqs - part.taken;
+        const dim3 grid(static_cast<unsigned>((left < most ? left : most) * p.n_kv_heads));
+        st = ByDim<FewAt, kScored>(p.rows.head_dim, part, grid, type, cache_type, stream);
+    }
+    return st;
+}
+
+// Row tiles of a batch: sequence s owns the slots from start[s] * group / rows
+// + s on, at least as many as it has tiles, whatever the lengths.
+int64_t TileSlots(int64_t n_seqs, int64_t n_tokens, int32_t group, int rows) {
+    return n_tokens * group / rows + n_seqs;
+}
+int64_t TileBlocks(const RaggedParams& p) {
+    return TileSlots(p.batch.n_seqs, p.batch.n_tokens, p.group, TileRows(p.rows.head_dim)) *
+           p.n_chunks * p.n_kv_heads;
+}
+
+template <bool kScored>
+mlk_status LaunchTile(const RaggedParams& p, int32_t type, int32_t cache_type, hipStream_t stream) {
+    const int64_t slots = TileSlots(p.batch.n_seqs, p.batch.n_tokens, p.group,
+                                    TileRows(p.rows.head_dim));
+    RaggedParams part = p;
+    const int64_t per_slot = static_cast<int64_t>(p.n_chunks) * p.n_kv_heads;
+    const int64_t most = kMaxBlocks / per_slot;  // row tiles of a launch
+    mlk_status st = MLK_OK;
+    for (part.taken = 0; part.taken < slots && st == MLK_OK; part.taken += most) {
+        const int64_t here = slots - part.taken < most ? slots - part.taken : most;
+        const dim3 grid(static_cast<unsigned>(here * per_slot));
+        st = ByDim<TileAt, kScored>(p.rows.head_dim, part, grid, slots, type, cache_type, stream);
+    }
+    return st;
+}
+
+// ------------------------------------------------------------ the plan
 
 int64_t Larger(int64_t a, int64_t b) { return a > b ? a : b; }
 int64_t RoundUp(int64_t a, int64_t to) { return (a + to - 1) / to * to; }
@@ -260,10 +336,19 @@ constexpr int64_t kTileMost = 64;      // most chunks of a tile row
 constexpr int64_t kTileFixed = 300;    // what a tile's start and end cost, in positions
 constexpr int64_t kTileJoin = 300;     // what the join costs
 
-Plan MakePlan(int64_t n_seqs, int64_t n_tokens, int64_t max_new, int64_t max_len, int32_t n_heads,
-              int32_t n_kv_heads, int32_t head_dim, bool packed) {
+// Positions that the rows of `tokens` neighbouring tokens see at most, of max_len, from a
+// multiple of `align` on.
+int64_t SpanOf(const Scores& scores, int64_t max_len, int64_t tokens, int64_t align) {
+    if (scores.window == 0 || scores.prefix != nullptr) return max_len;
+    const int64_t span = scores.window + tokens + align;
+    return span < max_len ? span : max_len;
+}
+
+Plan MakePlan(int64_t n_seqs, int64_t n_tokens, int64_t max_new, int64_t longest, int32_t n_heads,
+              int32_t n_kv_heads, int32_t head_dim, bool packed, const Scores& scores) {
     Plan plan;
     const int64_t group = n_heads / n_kv_heads, cus = ComputeUnits();
+    int64_t max_len = SpanOf(scores, longest, max_new, kFewKeys);
     const int64_t most = FewMost(head_dim), max_rows = max_new * group;
     plan.tile = max_rows > most;
     // a mixed batch of short sequences is left to the tile kernel alone
@@ -290,6 +375,7 @@ Plan MakePlan(int64_t n_seqs, int64_t n_tokens, int64_t max_new, int64_t max_len
         // prompts: n = 1 120, 2 160; all of the 8B heads).
         // The tiles are estimated: in a mixed batch all sequences but one bring one token,
         // in others each but one has half a tile more than its rows fill.
+        max_len = SpanOf(scores, longest, TileRows(head_dim) / group + 1, kTileAlign);
         const bool mixed = plan.few_rows > 0;
         const int64_t rows = (n_tokens - (mixed ? n_seqs - 1 : 0)) * group;
         const int64_t each = TileRows(head_dim);
@@ -325,7 +411,8 @@ bool Multiple8(int64_t a) { return a % 8 == 0; }
 }  // namespace
 
 int64_t AttendWorkspace(int64_t n_seqs, int64_t n_tokens, int64_t max_new, int64_t max_len,
-                        int32_t n_heads, int32_t n_kv_heads, int32_t head_dim, bool packed) {
+                        int32_t n_heads, int32_t n_kv_heads, int32_t head_dim, bool packed,
+                        const Scores& scores) {
     if (n_seqs <= 0 || n_tokens <= 0 || max_new <= 0 || max_len <= 0 || n_heads <= 0 ||
         n_kv_heads <= 0 || n_heads % n_kv_heads != 0 || n_heads > 65536 || head_dim <= 0 ||
         head_dim > 256 || n_seqs > kMaxSeqs || n_tokens > kMaxTokens || max_len > (1 << 30)) {
@@ -335,15 +422,16 @@ int64_t AttendWorkspace(int64_t n_seqs, int64_t n_tokens, int64_t max_new, int64
     if (max_new > max_len) max_new = max_len;
     if (max_new > n_tokens) max_new = n_tokens;
     return PlanBytes(
-        MakePlan(n_seqs, n_tokens, max_new, max_len, n_heads, n_kv_heads, head_dim, packed),
+        MakePlan(n_seqs, n_tokens, max_new, max_len, n_heads, n_kv_heads, head_dim, packed, scores),
         head_dim);
 }
 
-mlk_status Attend(const AttendArgs& a) {
+template <bool kScored>
+mlk_status AttendAs(const AttendArgs& a) {
     const int32_t hd = a.rows.head_dim;
     const Ragged& b = a.batch;
     Plan plan = MakePlan(b.n_seqs, b.n_tokens, b.max_new, b.max_len, a.n_heads, a.n_kv_heads, hd,
-                         b.table == nullptr);
+                         b.table == nullptr, a.scores);
     if (static_cast<int64_t>(a.workspace_bytes) < PlanBytes(plan, hd)) {  // no split
         plan.few_workers = plan.few_partials = plan.tile_partials = 0;
         plan.chunk = b.max_len;
@@ -358,7 +446,10 @@ mlk_status Attend(const AttendArgs& a) {
     p.n_heads = a.n_heads;
     p.n_kv_heads = a.n_kv_heads;
     p.group = a.n_heads / a.n_kv_heads;
-    p.factor = a.scale * kLog2e;
+    const bool capped = a.scores.softcap > 0.0f;
+    p.factor = capped ? a.scale / a.scores.softcap : a.scale * kLog2e;
+    p.scores = a.scores;
+    p.cap = a.scores.softcap * kLog2e;
     p.vec = hd % 8 == 0 && Multiple8(a.q_row) && Multiple8(a.rows.k_row) &&
             Multiple8(a.rows.v_row) && Multiple8(a.rows.page_stride) && Aligned(a.q, 16) &&
             Aligned(a.rows.k, 16) && Aligned(a.rows.v, 16) && Aligned(a.out, 16);
@@ -392,24 +483,27 @@ mlk_status Attend(const AttendArgs& a) {
                     static_cast<long long>(blocks));
     }
     if (plan.few_rows > 0) {
-        mlk_status st = LaunchFew(few, a.type, a.cache_type, a.stream);
+        mlk_status st = LaunchFew<kScored>(few, a.type, a.cache_type, a.stream);
         if (st == MLK_OK && few.workers > 0) {
-            st = a.type == MLK_F32   ? LaunchJoinFew<F32>(few, a.stream)
-                 : a.type == MLK_F16 ? LaunchJoinFew<F16>(few, a.stream)
-                                     : LaunchJoinFew<BF16>(few, a.stream);
+            st = a.type == MLK_F32   ? LaunchJoinFew<F32, kScored>(few, a.stream)
+                 : a.type == MLK_F16 ? LaunchJoinFew<F16, kScored>(few, a.stream)
+                                     : LaunchJoinFew<BF16, kScored>(few, a.stream);
         }
         if (st != MLK_OK) return st;
     }
     if (plan.tile) {
-        mlk_status st = LaunchTile(tile, a.type, a.cache_type, a.stream);
+        mlk_status st = LaunchTile<kScored>(tile, a.type, a.cache_type, a.stream);
         if (st == MLK_OK && tile.n_chunks > 1) {
-            st = a.type == MLK_F32   ? LaunchJoinTile<F32>(tile, a.stream)
-                 : a.type == MLK_F16 ? LaunchJoinTile<F16>(tile, a.stream)
-                                     : LaunchJoinTile<BF16>(tile, a.stream);
+            st = a.type == MLK_F32   ? LaunchJoinTile<F32, kScored>(tile, a.stream)
+                 : a.type == MLK_F16 ? LaunchJoinTile<F16, kScored>(tile, a.stream)
+                                     : LaunchJoinTile<BF16, kScored>(tile, a.stream);
         }
         return st;
     }
     return MLK_OK;
 }
+
+mlk_status Attend(const AttendArgs& a) { return AttendAs<false>(a); }
+mlk_status AttendScored(const AttendArgs& a) { return AttendAs<true>(a); }
 
 }  // namespace mlk

@@ -1,4 +1,4 @@
-// mlk_ragged_few.hip -- ragged attention of few rows per sequence: decode steps
+// mlk_ragged_few.h -- ragged attention of few rows per sequence: decode steps
 // and short chunks, bound by the bytes of K and V.
 //
 // A workgroup takes a range of units of 32 positions, whatever sequences and
@@ -37,7 +37,15 @@
 // by its access pattern.  A single fp32 sequence (67 MB, 26 us) is far from its
 // bytes: length, page, row and join each wait for the one before.
 // Instances: head_dim 64, 128 and 256; another runs on the next one, padded.
+// kScored: with score functions and masks (mlk_attention_scores).  Positions before the first
+// that a sequence's tokens see are no one's work; the scores are capped and biased as they
+// leave the products (bytes bound the kernel still: 64 bf16 sequences of 8B heads 190 us, capped
+// @@).
+#pragma once
+
 #include "mlk_ragged.h"
+
+#include <climits>
 
 namespace mlk {
 namespace {
@@ -109,7 +117,7 @@ __device__ inline void RowOffsets(const FewRows& r, int32_t j, int64_t* ko, int6
     }
 }
 
-template <typename A, typename C, int HD, int NB, int kWaves, Lie kLie>
+template <typename A, typename C, int HD, int NB, int kWaves, Lie kLie, bool kScored>
 __global__ __launch_bounds__(kWaves * kWave) void AttnFew(const RaggedParams p) {
     constexpr int kThreads = kWaves * kWave;
     typedef Pieces<A, C> P;
@@ -135,12 +143,12 @@ __global__ __launch_bounds__(kWaves * kWave) void AttnFew(const RaggedParams p) 
     if (p.workers == 0) {
         work.heads = 1;
         work.s = static_cast<int>(p.taken + blockIdx.x / p.n_kv_heads);
-        work.units = FewUnits(p, work.s);
+        work.units = FewUnits<kScored>(p, work.s);
         work.before = 0;
         unit = static_cast<int64_t>(blockIdx.x % p.n_kv_heads) * work.units;
         end = unit + work.units;
     } else {
-        if (!FindFewWork(p, blockIdx.x, &work)) return;
+        if (!FindFewWork<kScored>(p, blockIdx.x, &work)) return;
         unit = blockIdx.x * work.share;
         end = unit + work.share;
     }
@@ -152,7 +160,7 @@ __global__ __launch_bounds__(kWaves * kWave) void AttnFew(const RaggedParams p) 
         while (work.units == 0 || unit >= (work.before + work.units) * blocks) {
             work.before += work.units;
             if (++work.s >= p.batch.n_seqs) return;
-            work.units = FewUnits(p, work.s);
+            work.units = FewUnits<kScored>(p, work.s);
         }
         const int s = __builtin_amdgcn_readfirstlane(work.s);
         const int32_t units = __builtin_amdgcn_readfirstlane(work.units);
@@ -167,9 +175,10 @@ __global__ __launch_bounds__(kWaves * kWave) void AttnFew(const RaggedParams p) 
         if (!LoadSeq(p.batch, s, &loaded)) return;
         const Seq q = loaded;
         const int rows = q.n * p.group;
-        const int32_t j_begin = u0 * kFewKeys;
+        const int32_t u_first = __builtin_amdgcn_readfirstlane(FewFirst<kScored>(p, q));
+        const int32_t j_begin = (u_first + u0) * kFewKeys;
         if (j_begin >= q.len) continue;
-        const int32_t j_end = q.len - j_begin > (u1 - u0) * kFewKeys ? u1 * kFewKeys : q.len;
+        const int32_t j_end = q.len - j_begin > (u1 - u0) * kFewKeys ? (u_first + u1) * kFewKeys : q.len;
         const bool split = u0 != 0 || j_end < q.len;
 
         const FewRows fr{&p.rows,
@@ -183,6 +192,9 @@ __global__ __launch_bounds__(kWaves * kWave) void AttnFew(const RaggedParams p) 
         constexpr int NQR = kF32 ? HD / 16 : HD / 32;  // runs of q a lane holds
         constexpr int NQW = kF32 ? 4 : (sizeof(AB) == 4 ? 8 : 4);
         int32_t pos[NB];
+        // kScored: what the row sees, and all rows do; its head's slope
+        [[maybe_unused]] int32_t row_lo[NB], row_hi[NB], all_lo = 0, all_hi = INT32_MAX;
+        [[maybe_unused]] float slope[NB];
         uint32_t raw[NB][NQR][NQW];
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
@@ -190,6 +202,23 @@ __global__ __launch_bounds__(kWaves * kWave) void AttnFew(const RaggedParams p) 
             const bool real = m < rows;
             const int i = real ? m / p.group : 0;
             pos[nb] = real ? q.len - q.n + i : -1;
+            if constexpr (kScored) {
+                const Seen seen = real ? SeenBy(p.scores, s, q.t0 + i, pos[nb], q.len) : Seen{0, -1};
+                row_lo[nb] = seen.lo;
+                row_hi[nb] = seen.hi;
+                slope[nb] = SlopeOf(p, kvh * p.group + (real ? m % p.group : 0));
+                int32_t lo = real ? seen.lo : 0, hi = real ? seen.hi : INT32_MAX;
+#pragma unroll
+                for (int off = 8; off > 0; off /= 2) {
+                    const int32_t a = __shfl_xor(lo, off, kWave), b = __shfl_xor(hi, off, kWave);
+                    lo = a > lo ? a : lo;
+                    hi = b < hi ? b : hi;
+                }
+                lo = __builtin_amdgcn_readfirstlane(lo);
+                hi = __builtin_amdgcn_readfirstlane(hi);
+                all_lo = lo > all_lo ? lo : all_lo;
+                all_hi = hi < all_hi ? hi : all_hi;
+            }
             const AB* qr = static_cast<const AB*>(p.q) + static_cast<int64_t>(q.t0 + i) * p.q_row +
                            static_cast<int64_t>(kvh * p.group + (real ? m % p.group : 0)) * hd;
 #pragma unroll
@@ -373,18 +402,33 @@ __global__ __launch_bounds__(kWaves * kWave) void AttnFew(const RaggedParams p) 
             }
             if (jn < j_end) load_k(jn);
 
-            const bool masked = j0 + KT - 1 > first_pos || j0 + KT > j_end;
+            const bool masked = kScored ? j0 + KT - 1 > all_hi || j0 < all_lo || j0 + KT > j_end
+                                        : j0 + KT - 1 > first_pos || j0 + KT > j_end;
             float w[NB][4 * NBK];
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb) {
                 float top = -INFINITY;
+                if constexpr (kScored) {
+                    float x[4 * NBK];
+#pragma unroll
+                    for (int i = 0; i < 4 * NBK; ++i) x[i] = sc[nb][i / 4][i % 4];
+                    Score<4 * NBK>(p, factor[nb], slope[nb], pos[nb], x, [&](int i) {
+                        return j0 + 16 * (i / 4) + 4 * g4 + i % 4;
+                    });
+#pragma unroll
+                    for (int i = 0; i < 4 * NBK; ++i) sc[nb][i / 4][i % 4] = x[i];
+                }
 #pragma unroll
                 for (int b = 0; b < NBK; ++b) {
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
                         float x = sc[nb][b][r];
                         const int32_t j = j0 + 16 * b + 4 * g4 + r;
-                        if (masked && (j > pos[nb] || j >= j_end)) x = -INFINITY;
+                        if constexpr (kScored) {
+                            if (masked && (j > row_hi[nb] || j < row_lo[nb] || j >= j_end)) x = -INFINITY;
+                        } else {
+                            if (masked && (j > pos[nb] || j >= j_end)) x = -INFINITY;
+                        }
                         w[nb][4 * b + r] = x;
                         top = fmaxf(top, x);
                     }
@@ -393,7 +437,7 @@ __global__ __launch_bounds__(kWaves * kWave) void AttnFew(const RaggedParams p) 
                 const float mn = fmaxf(m[nb], top);
                 const float base = mn == -INFINITY ? 0.0f : mn;
                 if (__ballot(mn != m[nb]) != 0) {
-                    const float alpha = __builtin_amdgcn_exp2f((m[nb] - base) * factor[nb]);
+                    const float alpha = __builtin_amdgcn_exp2f(kScored ? m[nb] - base : (m[nb] - base) * factor[nb]);
                     l[nb] *= alpha;
 #pragma unroll
                     for (int e = 0; e < NI; ++e) o[nb][e] *= alpha;
@@ -403,7 +447,7 @@ __global__ __launch_bounds__(kWaves * kWave) void AttnFew(const RaggedParams p) 
                 float sum = 0.0f;
 #pragma unroll
                 for (int i = 0; i < 4 * NBK; ++i) {
-                    w[nb][i] = __builtin_amdgcn_exp2f(fmaf(w[nb][i] - base, factor[nb], kW));
+                    w[nb][i] = __builtin_amdgcn_exp2f(kScored ? w[nb][i] - base + kW : fmaf(w[nb][i] - base, factor[nb], kW));
                     sum += w[nb][i];
                 }
                 l[nb] += sum;
@@ -463,11 +507,13 @@ __global__ __launch_bounds__(kWaves * kWave) void AttnFew(const RaggedParams p) 
             }
         }
         if (bad && p.err != nullptr) RaiseFlag(p.err, 1);
+        if constexpr (!kScored) {
 #pragma unroll
-        for (int nb = 0; nb < NB; ++nb) m[nb] *= factor[nb];  // as the joins take it
+            for (int nb = 0; nb < NB; ++nb) m[nb] *= factor[nb];  // as the joins take it
+        }
 
         const int32_t masked_from0 = (first_pos < j_end ? first_pos : j_end) - KT;
-        const int32_t masked_from = masked_from0 > j_begin ? masked_from0 : j_begin;
+        const int32_t masked_from = masked_from0 > j_begin && !kScored ? masked_from0 : j_begin;
         const int place = first ? 0 : 1;
         if (along == 1) {
             // the wave has its head's positions to itself
@@ -482,8 +528,13 @@ __global__ __launch_bounds__(kWaves * kWave) void AttnFew(const RaggedParams p) 
                 AB* out = static_cast<AB*>(p.out) + (static_cast<int64_t>(q.t0 + i) * p.n_heads + h) * hd;
                 float* part = p.part_o + at * hd;
                 if (split && g4 == 0) p.part_ml[at] = make_float2(m[nb], lt);
-                const float inv = split ? 1.0f : 1.0f / lt;
-                const int32_t last = pos[nb] < j_end ? pos[nb] : j_end - 1;
+                float inv = split ? 1.0f : 1.0f / lt;
+                int32_t last = pos[nb] < j_end ? pos[nb] : j_end - 1, from = masked_from;
+                if constexpr (kScored) {
+                    if (row_lo[nb] > row_hi[nb]) inv = 0.0f;  // it sees nothing
+                    last = row_hi[nb] < j_end ? row_hi[nb] : j_end - 1;
+                    from = row_lo[nb] > from ? row_lo[nb] : from;
+                }
 #pragma unroll
                 for (int n = 0; n < Tile::NVR; ++n) {
 #pragma unroll
@@ -495,8 +546,8 @@ __global__ __launch_bounds__(kWaves * kWave) void AttnFew(const RaggedParams p) 
                         if (any_special) {
                             for (int e = 0; e < Tile::VE; ++e) {
                                 if (d0 + e < hd) {
-                                    x[e] += NonFiniteSum<C>(p.rows, fr.table, fr.t0, vb, masked_from,
-                                                            last, d0 + e);
+                                    x[e] += NonFiniteSum<C>(p.rows, fr.table, fr.t0, vb, from, last,
+                                                            d0 + e);
                                 }
                             }
                         }
@@ -548,12 +599,14 @@ __global__ __launch_bounds__(kWaves * kWave) void AttnFew(const RaggedParams p) 
                     sum += so[w][row][d];
                 }
                 const int i = row / p.group, h = (head0 + hb) * p.group + row % p.group;
+                Seen seen{0, first_pos + i};
+                if constexpr (kScored) seen = SeenBy(p.scores, s, q.t0 + i, first_pos + i, q.len);
                 if (special) {
-                    const int32_t last = first_pos + i < j_end ? first_pos + i : j_end - 1;
+                    const int32_t last = seen.hi < j_end ? seen.hi : j_end - 1;
                     sum += NonFiniteSum<C>(p.rows, fr.table, fr.t0,
                                            static_cast<const CB*>(p.rows.v) +
                                                static_cast<int64_t>(head0 + hb) * hd,
-                                           masked_from, last, d);
+                                           seen.lo > masked_from ? seen.lo : masked_from, last, d);
                 }
                 if (split) {
                     const int64_t at = FewPartial(p, blockIdx.x, place, hb, row);
@@ -562,7 +615,7 @@ __global__ __launch_bounds__(kWaves * kWave) void AttnFew(const RaggedParams p) 
                 } else {
                     AB* out = static_cast<AB*>(p.out) +
                               (static_cast<int64_t>(q.t0 + i) * p.n_heads + h) * hd;
-                    out[d] = A::Put(sum / lt);
+                    out[d] = A::Put(kScored && seen.lo > seen.hi ? 0.0f : sum / lt);
                 }
             }
             __syncthreads();  // the next pair writes over what was read here
@@ -570,54 +623,38 @@ __global__ __launch_bounds__(kWaves * kWave) void AttnFew(const RaggedParams p) 
     }
 }
 
-template <typename A, typename C, int HD, int NB, int kWaves>
-void Start(const RaggedParams& p, dim3 grid, hipStream_t s) {
+template <typename A, typename C, int HD, int NB, int kWaves, bool kScored>
+void StartFew(const RaggedParams& p, dim3 grid, hipStream_t s) {
     const dim3 block(kWaves * kWave);
     switch (LieOf(p, HD)) {
-        case kFull: hipLaunchKernelGGL((AttnFew<A, C, HD, NB, kWaves, kFull>), grid, block, 0, s, p); break;
-        case kPadded: hipLaunchKernelGGL((AttnFew<A, C, HD, NB, kWaves, kPadded>), grid, block, 0, s, p); break;
-        default: hipLaunchKernelGGL((AttnFew<A, C, HD, NB, kWaves, kScalar>), grid, block, 0, s, p); break;
+        case kFull: hipLaunchKernelGGL((AttnFew<A, C, HD, NB, kWaves, kFull, kScored>), grid, block, 0, s, p); break;
+        case kPadded: hipLaunchKernelGGL((AttnFew<A, C, HD, NB, kWaves, kPadded, kScored>), grid, block, 0, s, p); break;
+        default: hipLaunchKernelGGL((AttnFew<A, C, HD, NB, kWaves, kScalar, kScored>), grid, block, 0, s, p); break;
     }
 }
 
-template <typename A, typename C, int HD>
-mlk_status Launch(const RaggedParams& p, dim3 grid, hipStream_t s) {
-    if constexpr (HD <= 128) {
-        if (p.few_rows <= 16) Start<A, C, HD, 1, 8>(p, grid, s);
-        else Start<A, C, HD, 2, 4>(p, grid, s);
-    } else {
-        Start<A, C, HD, 1, 4>(p, grid, s);
-    }
-    return CheckLaunch("AttnFew");
-}
-
-struct ByDim {
+template <int HD, bool kScored>
+struct FewByType {
     const RaggedParams& p;
     dim3 grid;
     hipStream_t stream;
     template <typename A, typename C>
     mlk_status Run() const {
-        if (p.rows.head_dim <= 64) return Launch<A, C, 64>(p, grid, stream);
-        if (p.rows.head_dim <= 128) return Launch<A, C, 128>(p, grid, stream);
-        return Launch<A, C, 256>(p, grid, stream);
+        if constexpr (HD <= 128) {
+            if (p.few_rows <= 16) StartFew<A, C, HD, 1, 8, kScored>(p, grid, stream);
+            else StartFew<A, C, HD, 2, 4, kScored>(p, grid, stream);
+        } else {
+            StartFew<A, C, HD, 1, 4, kScored>(p, grid, stream);
+        }
+        return CheckLaunch("AttnFew");
     }
 };
 
 }  // namespace
 
-mlk_status LaunchFew(const RaggedParams& p, int32_t type, int32_t cache_type, hipStream_t stream) {
-    if (p.workers != 0) {
-        return ByType(type, cache_type, ByDim{p, dim3(static_cast<unsigned>(p.workers)), stream});
-    }
-    RaggedParams part = p;
-    const int64_t most = kMaxBlocks / p.n_kv_heads;  // sequences of a launch
-    mlk_status st = MLK_OK;
-    for (part.taken = 0; part.taken < p.batch.n_seqs && st == MLK_OK; part.taken += most) {
-        const int64_t left = p.batch.n_seqs - part.taken;
-        const dim3 grid(static_cast<unsigned>((left < most ? left : most) * p.n_kv_heads));
-        st = ByType(type, cache_type, ByDim{part, grid, stream});
-    }
-    return st;
+template <int HD, bool kScored>
+mlk_status LaunchFewAt(const RaggedParams& p, dim3 grid, int32_t type, int32_t cache_type, hipStream_t stream) {
+    return ByType(type, cache_type, FewByType<HD, kScored>{p, grid, stream});
 }
 
 }  // namespace mlk

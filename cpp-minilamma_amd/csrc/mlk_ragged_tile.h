@@ -1,4 +1,4 @@
-// mlk_ragged_tile.hip -- ragged attention of many rows per sequence: whole
+// mlk_ragged_tile.h -- ragged attention of many rows per sequence: whole
 // prompts and chunks of them, bound by the matrix cores.
 //
 // A workgroup takes 256 rows (128 with a head_dim over 128) of one sequence and
@@ -29,7 +29,14 @@
 // no one resource is full, the two kinds of phase overlap partly.
 // Instances: head_dim 64, 128 and 256; another runs on the next one, padded, at that
 // one's cost (4096 packed bf16 tokens of 8 heads: 80 in 90 us, 128 in 83).
+// kScored: with score functions and masks.  A tile's positions run from the first that any of
+// its rows sees (chunks from what the window alone leaves, so that the join knows them);
+// waves pass over tiles of positions that none of their rows sees.  @@
+#pragma once
+
 #include "mlk_ragged.h"
+
+#include <climits>
 
 namespace mlk {
 namespace {
@@ -56,7 +63,7 @@ struct TileShape {
     static constexpr int NW = NK == 3 ? 8 : 4;         // dwords a chunk has in memory
 };
 
-template <typename A, typename C, int HD, Lie kLie>
+template <typename A, typename C, int HD, Lie kLie, bool kScored>
 __global__ __launch_bounds__((TileShape<A, C, HD>::kThreads), HD <= 128 ? 2 : 1) void AttnTile(const RaggedParams p, int64_t n_slots) {
     typedef Pieces<A, C> P;
     typedef typename P::M M;
@@ -93,11 +100,15 @@ __global__ __launch_bounds__((TileShape<A, C, HD>::kThreads), HD <= 128 ? 2 : 1)
     if (m0 < 0 || m0 >= rows || rows <= p.few_rows) return;
     const int64_t m_last = (m0 + kRows < rows ? m0 + kRows : rows) - 1;
     const int32_t first = q.len - q.n;  // position of the sequence's first new token
-    const int32_t lo = first + static_cast<int32_t>(m0 / group);
+    [[maybe_unused]] const int32_t lo = first + static_cast<int32_t>(m0 / group);
     const int32_t hi = first + static_cast<int32_t>(m_last / group);
-    const int32_t j_begin = chunk * p.chunk;
-    if (j_begin > hi) return;
-    const int32_t j_end = hi + 1 - j_begin < p.chunk ? hi + 1 : j_begin + p.chunk;
+    // kScored: chunk 0 begins at `base`; the tile's rows see up to `most`
+    const int32_t base0 = kScored ? TileBase(p, q, m0) : 0;
+    const int32_t most = kScored ? SeenBy({nullptr, p.scores.prefix, nullptr, 0.0f, 0}, s, 0, hi, q.len).hi : hi;
+    const int64_t chunk_at = base0 + static_cast<int64_t>(chunk) * p.chunk;
+    if (chunk_at > most) return;
+    int32_t j_begin = static_cast<int32_t>(chunk_at);
+    const int32_t j_end = most + 1 - j_begin < p.chunk ? most + 1 : j_begin + p.chunk;
 
     const int32_t* table =
         p.batch.table == nullptr ? nullptr : p.batch.table + s * p.batch.table_stride;
@@ -113,9 +124,58 @@ __global__ __launch_bounds__((TileShape<A, C, HD>::kThreads), HD <= 128 ? 2 : 1)
     // positions that all rows of the wave attend to: up to wave_lo; that any does: below
     // wave_hi
     const int64_t w0 = m0 + 32 * wave;
-    const int32_t wave_lo = w0 <= m_last ? first + static_cast<int32_t>(w0 / group) : -1;
+    int32_t wave_lo = w0 <= m_last ? first + static_cast<int32_t>(w0 / group) : -1;
     const int64_t w1 = w0 + 31 < m_last ? w0 + 31 : m_last;
-    const int32_t wave_hi = w0 <= m_last ? first + static_cast<int32_t>(w1 / group) + 1 : 0;
+    int32_t wave_hi = w0 <= m_last ? first + static_cast<int32_t>(w1 / group) + 1 : 0;
+    // kScored: what this lane's row sees; from where all rows of the wave see, and any does
+    int32_t row_lo = 0, row_hi = pos, wave_from = 0, wave_any = 0;
+    // positions that all rows of the tile see: all_lo .. all_hi
+    int32_t all_lo = 0, all_hi = lo;
+    float slope = 0.0f;
+    if constexpr (kScored) {
+        const Seen seen = real ? SeenBy(p.scores, s, q.t0 + tok, pos, q.len) : Seen{0, -1};
+        row_lo = seen.lo;
+        row_hi = seen.hi;
+        slope = SlopeOf(p, h);
+        const bool sees = seen.lo <= seen.hi;
+        int32_t least_lo = sees ? seen.lo : INT32_MAX, most_lo = real ? seen.lo : 0;
+        int32_t least_hi = real ? seen.hi : INT32_MAX, most_hi = sees ? seen.hi : -1;
+#pragma unroll
+        for (int off = 16; off > 0; off /= 2) {
+            const int32_t a = __shfl_xor(least_lo, off, kWave), b = __shfl_xor(most_lo, off, kWave);
+            const int32_t c = __shfl_xor(least_hi, off, kWave), d = __shfl_xor(most_hi, off, kWave);
+            least_lo = a < least_lo ? a : least_lo;
+            most_lo = b > most_lo ? b : most_lo;
+            least_hi = c < least_hi ? c : least_hi;
+            most_hi = d > most_hi ? d : most_hi;
+        }
+        wave_any = __builtin_amdgcn_readfirstlane(least_lo);
+        wave_from = __builtin_amdgcn_readfirstlane(most_lo);
+        wave_lo = __builtin_amdgcn_readfirstlane(least_hi);
+        wave_hi = __builtin_amdgcn_readfirstlane(most_hi) + 1;
+        __shared__ int32_t bounds[3];  // least and most first position, least last one
+        if (tid == 0) {
+            bounds[0] = INT32_MAX;
+            bounds[1] = 0;
+            bounds[2] = INT32_MAX;
+        }
+        __syncthreads();
+        if (lane == 0 && w0 <= m_last) {
+            atomicMin(&bounds[0], wave_any);
+            atomicMax(&bounds[1], wave_from);
+            atomicMin(&bounds[2], wave_lo);
+        }
+        __syncthreads();
+        all_lo = bounds[1];
+        all_hi = bounds[2];
+        if (chunk == 0 && real && !sees && half == 0) {  // a row that sees nothing
+            AB* out = static_cast<AB*>(p.out) + (static_cast<int64_t>(q.t0 + tok) * p.n_heads + h) * hd;
+            for (int d = 0; d < hd; ++d) out[d] = A::Put(0.0f);
+        }
+        const int32_t from = bounds[0] / kTileAlign * kTileAlign;
+        if (from >= j_end) return;  // none of the rows has a part here
+        if (from > j_begin) j_begin = from;
+    }
 
     float factor = p.factor;
     u32x4 qf[NS][NQ];
@@ -216,7 +276,8 @@ __global__ __launch_bounds__((TileShape<A, C, HD>::kThreads), HD <= 128 ? 2 : 1)
         }
     };
     auto put_v = [&](int32_t j0, uint16_t* dst) {
-        if (j0 + KT - 1 > lo || j0 + KT > j_end) {  // some row does not attend to all of it
+        // some row does not attend to all of it
+        if (j0 + KT - 1 > all_hi || j0 + KT > j_end || (kScored && j0 < all_lo)) {
 #pragma unroll
             for (int i = 0; i < NCH; ++i) special |= OnlyFinite<C, T::NW>(gv[i]);
         }
@@ -272,13 +333,26 @@ __global__ __launch_bounds__((TileShape<A, C, HD>::kThreads), HD <= 128 ? 2 : 1)
             __builtin_amdgcn_sched_group_barrier(0x008, NM, 0);
             if (i + kDeep < kSteps) __builtin_amdgcn_sched_group_barrier(0x100, NK, 0);
         }
-        if (j0 + KT - 1 > wave_lo || j0 + KT > j_end) {
-            const int32_t last = (pos < j_end ? pos : j_end - 1) - j0 - 4 * half;
+        if constexpr (kScored) {
+#pragma unroll
+            for (int b = 0; b < NKB; ++b) {
+                float x[16];
+#pragma unroll
+                for (int r = 0; r < 16; ++r) x[r] = sc[b][r];
+                Score<16>(p, factor, slope, pos - j0 - 4 * half, x, [&](int r) { return 32 * b + 8 * (r / 4) + r % 4; });
+#pragma unroll
+                for (int r = 0; r < 16; ++r) sc[b][r] = x[r];
+            }
+        }
+        if (j0 + KT - 1 > wave_lo || j0 + KT > j_end || (kScored && j0 < wave_from)) {
+            const int32_t last = (row_hi < j_end ? row_hi : j_end - 1) - j0 - 4 * half;
+            const int32_t from = row_lo - j0 - 4 * half;
 #pragma unroll
             for (int b = 0; b < NKB; ++b) {
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
-                    sc[b][r] = 32 * b + 8 * (r / 4) + r % 4 > last ? -INFINITY : sc[b][r];
+                    const int at = 32 * b + 8 * (r / 4) + r % 4;
+                    sc[b][r] = at > last || (kScored && at < from) ? -INFINITY : sc[b][r];
                 }
                 asm volatile("" : "+v"(sc[b]));  // a branch: else every tile pays for the mask
             }
@@ -292,25 +366,28 @@ __global__ __launch_bounds__((TileShape<A, C, HD>::kThreads), HD <= 128 ? 2 : 1)
         const float mn = fmaxf(mx, Max32(top));
         const float from = mn == -INFINITY ? 0.0f : mn;
         if (__ballot(mn != mx) != 0) {
-            const float alpha = __builtin_amdgcn_exp2f((mx - from) * factor);
+            const float alpha = __builtin_amdgcn_exp2f(kScored ? mx - from : (mx - from) * factor);
             l *= alpha;
 #pragma unroll
             for (int d = 0; d < ND; ++d) o[d] *= alpha;
             mx = mn;
         }
-        // The weights' exponents are (score - maximum) * factor + W.  With the maximum in
-        // the addend that is one instruction a score, off by the addend's rounding: up
-        // to kLarge at most 2^-11, like the score's own.  Beyond it the difference is taken
-        // first: the largest weight is 2^W however large the scores are.
-        const float base = from * factor;
-        float off = static_cast<float>(P::W) - base;
-        if (__ballot(fabsf(base) > kLarge) != 0) {
-            off = static_cast<float>(P::W);
+        float off = static_cast<float>(P::W);
+        if constexpr (!kScored) {
+            // The weights' exponents are (score - maximum) * factor + W.  With the maximum in
+            // the addend that is one instruction a score, off by the addend's rounding: up
+            // to kLarge at most 2^-11, like the score's own.  Beyond it the difference is taken
+            // first: the largest weight is 2^W however large the scores are.
+            const float base = from * factor;
+            off = static_cast<float>(P::W) - base;
+            if (__ballot(fabsf(base) > kLarge) != 0) {
+                off = static_cast<float>(P::W);
 #pragma unroll
-            for (int b = 0; b < NKB; ++b) {
+                for (int b = 0; b < NKB; ++b) {
 #pragma unroll
-                for (int r = 0; r < 16; ++r) sc[b][r] -= from;
-                asm volatile("" : "+v"(sc[b]));  // a branch, as above
+                    for (int r = 0; r < 16; ++r) sc[b][r] -= from;
+                    asm volatile("" : "+v"(sc[b]));  // a branch, as above
+                }
             }
         }
         float sum[4] = {0, 0, 0, 0};
@@ -318,7 +395,7 @@ __global__ __launch_bounds__((TileShape<A, C, HD>::kThreads), HD <= 128 ? 2 : 1)
         for (int b = 0; b < NKB; ++b) {
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
-                sc[b][r] = __builtin_amdgcn_exp2f(fmaf(sc[b][r], factor, off));
+                sc[b][r] = __builtin_amdgcn_exp2f(kScored ? sc[b][r] - from + off : fmaf(sc[b][r], factor, off));
                 sum[r % 4] += sc[b][r];
             }
         }
@@ -366,7 +443,7 @@ __global__ __launch_bounds__((TileShape<A, C, HD>::kThreads), HD <= 128 ? 2 : 1)
             load(j0 + KT, vb, p.rows.v_row, gv);
             find(j0 + 2 * KT);
         }
-        if (j0 < wave_hi) compute(j0, sk[buf], sv[buf]);
+        if (j0 < wave_hi && (!kScored || j0 + KT > wave_any)) compute(j0, sk[buf], sv[buf]);
         const int other = T::NBUF == 1 ? 0 : buf ^ 1;
         if constexpr (T::NBUF == 1) __syncthreads();
         if (more) {
@@ -386,12 +463,21 @@ __global__ __launch_bounds__((TileShape<A, C, HD>::kThreads), HD <= 128 ? 2 : 1)
     if (bad && p.err != nullptr) RaiseFlag(p.err, 1);
     special = __syncthreads_or(special);
     l = Sum32(l);
-    if (!real || pos < j_begin) return;
-    const int32_t last = pos < j_end ? pos : j_end - 1;
-    const int32_t masked_from = (lo < j_end ? lo : j_end) - KT;
-    const bool split = pos >= p.chunk;
+    if (!real) return;
+    const int32_t last = row_hi < j_end ? row_hi : j_end - 1;
+    int32_t masked_from = (lo < j_end ? lo : j_end) - KT;
+    bool split = pos >= p.chunk;
+    if constexpr (kScored) {
+        if (row_lo > row_hi) return;
+        const int32_t c0 = TileFirstChunk(p, base0, row_lo), c1 = (row_hi - base0) / p.chunk;
+        if (chunk < c0 || chunk > c1) return;
+        masked_from = row_lo;
+        split = c0 != c1;
+    } else {
+        if (pos < j_begin) return;
+    }
     const int64_t at = split ? TilePartial(p, q.t0 + tok, h) + chunk : 0;
-    if (split && half == 0) p.part_ml[at] = make_float2(mx * factor, l);
+    if (split && half == 0) p.part_ml[at] = make_float2(kScored ? mx : mx * factor, l);
     const float inv = split ? 1.0f : 1.0f / l;
     AB* out = static_cast<AB*>(p.out) + (static_cast<int64_t>(q.t0 + tok) * p.n_heads + h) * hd;
     float* part = p.part_o + at * hd;
@@ -440,57 +526,30 @@ __global__ __launch_bounds__((TileShape<A, C, HD>::kThreads), HD <= 128 ? 2 : 1)
     }
 }
 
-template <typename A, typename C, int HD>
-mlk_status Launch(const RaggedParams& p, dim3 grid, int64_t n_slots, hipStream_t s) {
-    constexpr int kThreads = TileShape<A, C, HD>::kThreads;
-    const dim3 block(kThreads);
-    switch (LieOf(p, HD)) {
-        case kFull: hipLaunchKernelGGL((AttnTile<A, C, HD, kFull>), grid, block, 0, s, p, n_slots); break;
-        case kPadded: hipLaunchKernelGGL((AttnTile<A, C, HD, kPadded>), grid, block, 0, s, p, n_slots); break;
-        default: hipLaunchKernelGGL((AttnTile<A, C, HD, kScalar>), grid, block, 0, s, p, n_slots); break;
-    }
-    return CheckLaunch("AttnTile");
-}
-
-struct ByDim {
+template <int HD, bool kScored>
+struct TileByType {
     const RaggedParams& p;
     dim3 grid;
     int64_t n_slots;
     hipStream_t stream;
     template <typename A, typename C>
     mlk_status Run() const {
-        if (p.rows.head_dim <= 64) return Launch<A, C, 64>(p, grid, n_slots, stream);
-        if (p.rows.head_dim <= 128) return Launch<A, C, 128>(p, grid, n_slots, stream);
-        return Launch<A, C, 256>(p, grid, n_slots, stream);
+        const dim3 block(TileShape<A, C, HD>::kThreads);
+        switch (LieOf(p, HD)) {
+            case kFull: hipLaunchKernelGGL((AttnTile<A, C, HD, kFull, kScored>), grid, block, 0, stream, p, n_slots); break;
+            case kPadded: hipLaunchKernelGGL((AttnTile<A, C, HD, kPadded, kScored>), grid, block, 0, stream, p, n_slots); break;
+            default: hipLaunchKernelGGL((AttnTile<A, C, HD, kScalar, kScored>), grid, block, 0, stream, p, n_slots); break;
+        }
+        return CheckLaunch("AttnTile");
     }
 };
 
-// Row tiles of a batch: sequence s owns the slots from start[s] * group / rows
-// + s on, at least as many as it has tiles, whatever the lengths.
-int64_t TileSlots(int64_t n_seqs, int64_t n_tokens, int32_t group, int rows) {
-    return n_tokens * group / rows + n_seqs;
-}
-
 }  // namespace
 
-int64_t TileBlocks(const RaggedParams& p) {
-    return TileSlots(p.batch.n_seqs, p.batch.n_tokens, p.group, TileRows(p.rows.head_dim)) *
-           p.n_chunks * p.n_kv_heads;
-}
-
-mlk_status LaunchTile(const RaggedParams& p, int32_t type, int32_t cache_type, hipStream_t stream) {
-    const int64_t slots = TileSlots(p.batch.n_seqs, p.batch.n_tokens, p.group,
-                                    TileRows(p.rows.head_dim));
-    RaggedParams part = p;
-    const int64_t per_slot = static_cast<int64_t>(p.n_chunks) * p.n_kv_heads;
-    const int64_t most = kMaxBlocks / per_slot;  // row tiles of a launch
-    mlk_status st = MLK_OK;
-    for (part.taken = 0; part.taken < slots && st == MLK_OK; part.taken += most) {
-        const int64_t here = slots - part.taken < most ? slots - part.taken : most;
-        const dim3 grid(static_cast<unsigned>(here * per_slot));
-        st = ByType(type, cache_type, ByDim{part, grid, slots, stream});
-    }
-    return st;
+template <int HD, bool kScored>
+mlk_status LaunchTileAt(const RaggedParams& p, dim3 grid, int64_t n_slots, int32_t type,
+                        int32_t cache_type, hipStream_t stream) {
+    return ByType(type, cache_type, TileByType<HD, kScored>{p, grid, n_slots, stream});
 }
 
 }  // namespace mlk

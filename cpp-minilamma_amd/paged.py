@@ -90,14 +90,14 @@ lib.mlk_attention_paged_scored.argtypes = _CB + [C.POINTER(ScoresStruct), _i32, 
                                                  _i32, _f, _vp, C.c_size_t, _vp, _vp]
 lib.mlk_attention_paged_scored.restype = C.c_int
 lib.mlk_attention_paged_scored_workspace_bytes.argtypes = [_i64, _i64, _i64, _i64, _i32, _i32,
-                                                           _i32, _i64]
+                                                           _i32, C.POINTER(ScoresStruct)]
 lib.mlk_attention_paged_scored_workspace_bytes.restype = _i64
 lib.mlk_attention_packed_scored.argtypes = [_i32, C.POINTER(ScoresStruct), _vp, _i64, _vp, _i64,
                                             _vp, _i64, _vp, _i64, _i64, _i64, _i32, _i32, _i32, _f,
                                             _vp, _vp, C.c_size_t, _vp, _vp]
 lib.mlk_attention_packed_scored.restype = C.c_int
 lib.mlk_attention_packed_scored_workspace_bytes.argtypes = [_i64, _i64, _i64, _i32, _i32, _i32,
-                                                            _i64]
+                                                            C.POINTER(ScoresStruct)]
 lib.mlk_attention_packed_scored_workspace_bytes.restype = _i64
 
 
@@ -239,7 +239,7 @@ def attention_scored_workspace_bytes(cache, batch, scores, n_heads):
     c, b = cache.struct, batch.struct
     return int(lib.mlk_attention_paged_scored_workspace_bytes(
         b.n_seqs, b.n_tokens, b.max_new_tokens, b.max_seq_len, n_heads, c.n_kv_heads, c.head_dim,
-        scores.struct.window))
+        C.byref(scores.struct)))
 
 
 def attention_scored(cache, batch, scores, q, out, n_heads, type, scale=None, q_row_stride=None,
@@ -257,7 +257,7 @@ def attention_packed_scored_workspace_bytes(scores, n_seqs, n_tokens, max_seq_le
                                             n_kv_heads, head_dim):
     """Bytes of the optional workspace of attention_packed_scored()."""
     return int(lib.mlk_attention_packed_scored_workspace_bytes(
-        n_seqs, n_tokens, max_seq_len, n_heads, n_kv_heads, head_dim, scores.struct.window))
+        n_seqs, n_tokens, max_seq_len, n_heads, n_kv_heads, head_dim, C.byref(scores.struct)))
 
 
 def attention_packed_scored(type, scores, q, k, v, seq_start, n_seqs, n_tokens, max_seq_len,

@@ -570,15 +570,16 @@ mlk_status mlk_attention_packed_scored(int32_t type, const mlk_attention_scores*
                                        int64_t max_seq_len, int32_t n_heads, int32_t n_kv_heads,
                                        int32_t head_dim, float scale, void* out, void* workspace,
                                        size_t workspace_bytes, int32_t* err, void* stream);
-/* Bytes of their optional workspaces; window as in mlk_attention_scores. */
+/* Bytes of their optional workspaces (scores NULL: as the plain calls'). */
 int64_t mlk_attention_paged_scored_workspace_bytes(int64_t n_seqs, int64_t n_tokens,
                                                    int64_t max_new_tokens, int64_t max_seq_len,
                                                    int32_t n_heads, int32_t n_kv_heads,
-                                                   int32_t head_dim, int64_t window);
+                                                   int32_t head_dim,
+                                                   const mlk_attention_scores* scores);
 int64_t mlk_attention_packed_scored_workspace_bytes(int64_t n_seqs, int64_t n_tokens,
                                                     int64_t max_seq_len, int32_t n_heads,
                                                     int32_t n_kv_heads, int32_t head_dim,
-                                                    int64_t window);
+                                                    const mlk_attention_scores* scores);
 
 /* ------------------------------------------------------------ sampling */
 
