@@ -358,6 +358,17 @@ __global__ __launch_bounds__(kWaves * kWave) void AttnFew(const RaggedParams p) 
             }
         }
 
+        // scores that Score has gone over have no factor left
+        const bool as_they_are = !kScored || AsTheyAre(p);
+        [[maybe_unused]] float raw_factor[NB];
+        if constexpr (kScored) {
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb) {
+                raw_factor[nb] = factor[nb];
+                if (!as_they_are) factor[nb] = 1.0f;
+            }
+        }
+
         f32x4 o[NB][NI];
         float m[NB], l[NB];
 #pragma unroll
@@ -408,11 +419,11 @@ __global__ __launch_bounds__(kWaves * kWave) void AttnFew(const RaggedParams p) 
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb) {
                 float top = -INFINITY;
-                if constexpr (kScored) {
+                if (kScored && !as_they_are) {
                     float x[4 * NBK];
 #pragma unroll
                     for (int i = 0; i < 4 * NBK; ++i) x[i] = sc[nb][i / 4][i % 4];
-                    Score<4 * NBK>(p, factor[nb], slope[nb], pos[nb], x, [&](int i) {
+                    Score<4 * NBK>(p, raw_factor[nb], slope[nb], pos[nb], x, [&](int i) {
                         return j0 + 16 * (i / 4) + 4 * g4 + i % 4;
                     });
 #pragma unroll
@@ -437,7 +448,7 @@ __global__ __launch_bounds__(kWaves * kWave) void AttnFew(const RaggedParams p) 
                 const float mn = fmaxf(m[nb], top);
                 const float base = mn == -INFINITY ? 0.0f : mn;
                 if (__ballot(mn != m[nb]) != 0) {
-                    const float alpha = __builtin_amdgcn_exp2f(kScored ? m[nb] - base : (m[nb] - base) * factor[nb]);
+                    const float alpha = __builtin_amdgcn_exp2f((m[nb] - base) * factor[nb]);
                     l[nb] *= alpha;
 #pragma unroll
                     for (int e = 0; e < NI; ++e) o[nb][e] *= alpha;
@@ -447,7 +458,7 @@ __global__ __launch_bounds__(kWaves * kWave) void AttnFew(const RaggedParams p) 
                 float sum = 0.0f;
 #pragma unroll
                 for (int i = 0; i < 4 * NBK; ++i) {
-                    w[nb][i] = __builtin_amdgcn_exp2f(kScored ? w[nb][i] - base + kW : fmaf(w[nb][i] - base, factor[nb], kW));
+                    w[nb][i] = __builtin_amdgcn_exp2f(fmaf(w[nb][i] - base, factor[nb], kW));
                     sum += w[nb][i];
                 }
                 l[nb] += sum;
@@ -507,10 +518,8 @@ __global__ __launch_bounds__(kWaves * kWave) void AttnFew(const RaggedParams p) 
             }
         }
         if (bad && p.err != nullptr) RaiseFlag(p.err, 1);
-        if constexpr (!kScored) {
 #pragma unroll
-            for (int nb = 0; nb < NB; ++nb) m[nb] *= factor[nb];  // as the joins take it
-        }
+        for (int nb = 0; nb < NB; ++nb) m[nb] *= factor[nb];  // as the joins take it
 
         const int32_t masked_from0 = (first_pos < j_end ? first_pos : j_end) - KT;
         const int32_t masked_from = masked_from0 > j_begin && !kScored ? masked_from0 : j_begin;

@@ -213,6 +213,11 @@ __global__ __launch_bounds__((TileShape<A, C, HD>::kThreads), HD <= 128 ? 2 : 1)
         }
     }
 
+    // scores that Score has gone over have no factor left
+    const bool as_they_are = !kScored || AsTheyAre(p);
+    [[maybe_unused]] const float raw_factor = factor;
+    if (!as_they_are) factor = 1.0f;
+
     // staging: chunk tid + kThreads * i of the tile; a wave's 64 chunks are kPer
     // neighbouring rows
     constexpr int kChunks = HD / 8, kPer = kWave / kChunks;
@@ -333,13 +338,13 @@ __global__ __launch_bounds__((TileShape<A, C, HD>::kThreads), HD <= 128 ? 2 : 1)
             __builtin_amdgcn_sched_group_barrier(0x008, NM, 0);
             if (i + kDeep < kSteps) __builtin_amdgcn_sched_group_barrier(0x100, NK, 0);
         }
-        if constexpr (kScored) {
+        if (kScored && !as_they_are) {
 #pragma unroll
             for (int b = 0; b < NKB; ++b) {
                 float x[16];
 #pragma unroll
                 for (int r = 0; r < 16; ++r) x[r] = sc[b][r];
-                Score<16>(p, factor, slope, pos - j0 - 4 * half, x, [&](int r) { return 32 * b + 8 * (r / 4) + r % 4; });
+                Score<16>(p, raw_factor, slope, pos - j0 - 4 * half, x, [&](int r) { return 32 * b + 8 * (r / 4) + r % 4; });
 #pragma unroll
                 for (int r = 0; r < 16; ++r) sc[b][r] = x[r];
             }
@@ -366,28 +371,25 @@ __global__ __launch_bounds__((TileShape<A, C, HD>::kThreads), HD <= 128 ? 2 : 1)
         const float mn = fmaxf(mx, Max32(top));
         const float from = mn == -INFINITY ? 0.0f : mn;
         if (__ballot(mn != mx) != 0) {
-            const float alpha = __builtin_amdgcn_exp2f(kScored ? mx - from : (mx - from) * factor);
+            const float alpha = __builtin_amdgcn_exp2f((mx - from) * factor);
             l *= alpha;
 #pragma unroll
             for (int d = 0; d < ND; ++d) o[d] *= alpha;
             mx = mn;
         }
-        float off = static_cast<float>(P::W);
-        if constexpr (!kScored) {
-            // The weights' exponents are (score - maximum) * factor + W.  With the maximum in
-            // the addend that is one instruction a score, off by the addend's rounding: up
-            // to kLarge at most 2^-11, like the score's own.  Beyond it the difference is taken
-            // first: the largest weight is 2^W however large the scores are.
-            const float base = from * factor;
-            off = static_cast<float>(P::W) - base;
-            if (__ballot(fabsf(base) > kLarge) != 0) {
-                off = static_cast<float>(P::W);
+        // The weights' exponents are (score - maximum) * factor + W.  With the maximum in
+        // the addend that is one instruction a score, off by the addend's rounding: up
+        // to kLarge at most 2^-11, like the score's own.  Beyond it the difference is taken
+        // first: the largest weight is 2^W however large the scores are.
+        const float base = from * factor;
+        float off = static_cast<float>(P::W) - base;
+        if (__ballot(fabsf(base) > kLarge) != 0) {
+            off = static_cast<float>(P::W);
 #pragma unroll
-                for (int b = 0; b < NKB; ++b) {
+            for (int b = 0; b < NKB; ++b) {
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) sc[b][r] -= from;
-                    asm volatile("" : "+v"(sc[b]));  // a branch, as above
-                }
+                for (int r = 0; r < 16; ++r) sc[b][r] -= from;
+                asm volatile("" : "+v"(sc[b]));  // a branch, as above
             }
         }
         float sum[4] = {0, 0, 0, 0};
@@ -395,7 +397,7 @@ __global__ __launch_bounds__((TileShape<A, C, HD>::kThreads), HD <= 128 ? 2 : 1)
         for (int b = 0; b < NKB; ++b) {
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
-                sc[b][r] = __builtin_amdgcn_exp2f(kScored ? sc[b][r] - from + off : fmaf(sc[b][r], factor, off));
+                sc[b][r] = __builtin_amdgcn_exp2f(fmaf(sc[b][r], factor, off));
                 sum[r % 4] += sc[b][r];
             }
         }
@@ -477,7 +479,7 @@ __global__ __launch_bounds__((TileShape<A, C, HD>::kThreads), HD <= 128 ? 2 : 1)
         if (pos < j_begin) return;
     }
     const int64_t at = split ? TilePartial(p, q.t0 + tok, h) + chunk : 0;
-    if (split && half == 0) p.part_ml[at] = make_float2(kScored ? mx : mx * factor, l);
+    if (split && half == 0) p.part_ml[at] = make_float2(mx * factor, l);
     const float inv = split ? 1.0f : 1.0f / l;
     AB* out = static_cast<AB*>(p.out) + (static_cast<int64_t>(q.t0 + tok) * p.n_heads + h) * hd;
     float* part = p.part_o + at * hd;
