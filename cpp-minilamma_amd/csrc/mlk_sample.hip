@@ -118,6 +118,10 @@ __device__ inline int32_t BinOf(const How& h, float x, double* f) {
     *f = fma(v, h.c, -(t - kRound));
     return static_cast<int32_t>(__double2loint(t));
 }
+__device__ inline int32_t BinOf(const How& h, float x) {
+    double f;
+    return BinOf(h, x, &f);
+}
 
 // exp(f / kPerUnit) 2^42 as a whole number.
 __device__ inline uint64_t Weight(double f) {
@@ -280,8 +284,7 @@ __global__ __launch_bounds__(kThreads) void SampleBins(const SampleArgs p) {
         }
         if (all > so_far) {  // (uniform) the ring moves on: what it now holds anew was far below
             so_far = all;
-            double f;
-            const int32_t to = BinOf(h, all, &f);
+            const int32_t to = BinOf(h, all);
             if (some) {
                 const int32_t fresh = to - top < kBins ? to - top : kBins;
                 for (int32_t i = lane; i < fresh; i += kWave) mass[(to - i) & (kBins - 1)] = 0;
@@ -293,6 +296,7 @@ __global__ __launch_bounds__(kThreads) void SampleBins(const SampleArgs p) {
         auto add = [&](auto counts) {
 #pragma unroll
             for (int a = 0; a < kAhead; ++a) {
+                if (b + a >= w1) break;
 #pragma unroll
                 for (int e = 0; e < E; ++e) {
                     double f;
@@ -376,7 +380,7 @@ struct Choice {
     uint32_t code[kList];  // their bins, and where in them: CodeOf
     uint64_t bin[kBins];   // masses or counts of the bins; of a search's ranges
     uint64_t sum[kBins];   // of the weights up to and with bin i, of the largest bin's middle
-    uint16_t segment[kChunk];
+    uint16_t some[kList];  // segments to look through; places in the list that a search is left with
     uint64_t few[kWave];
     double edge[2 * kPerUnit];  // exp(-i / kPerUnit), and exp(-i)
     uint64_t scan_u[kChooseWaves], scan_v[kChooseWaves];
@@ -480,7 +484,7 @@ struct Chooser {
             uint32_t at = 0;
             if (Lane() == 0) at = atomicAdd(&s.n_segments, static_cast<uint32_t>(__popcll(mask)));
             at = __builtin_amdgcn_readfirstlane(at) + __popcll(mask & ((uint64_t{1} << Lane()) - 1));
-            if (hit) s.segment[at] = static_cast<uint16_t>(i * kChooseThreads + Tid());
+            if (hit) s.some[at] = static_cast<uint16_t>(i * kChooseThreads + Tid());
         }
         __syncthreads();
         return static_cast<int>(s.n_segments);
@@ -508,7 +512,7 @@ struct Chooser {
             const int n = Segments(c0, segments, low);
 #pragma unroll 1
             for (int j = Tid(); j < n * kEach; j += kChooseThreads) {
-                const int32_t i = r.Index((c0 + s.segment[j / kEach]) * kSegment, j % kEach);
+                const int32_t i = r.Index((c0 + s.some[j / kEach]) * kSegment, j % kEach);
                 const float x = i >= 0 && i < r.vocab ? T::Get(r.x[i]) : -INFINITY;
                 if (x >= low && x <= high) f(x, i);
             }
@@ -603,56 +607,88 @@ struct Chooser {
     // bound: by equal ranges of the bin, then (equal logits) by ranges of the keys that are
     // left, until a wave holds them.
     __device__ Place Select(int n, int bin, Bound what, uint64_t bound) {
-        const Span span{bin, bin};
-        uint64_t lo = 0, hi = kLastKey, before = 0;
-        int range = -1;   // of the bin, once it is known
-        uint64_t left = static_cast<uint64_t>(n);  // no fewer than are left
-        auto has = [&](uint64_t key, uint32_t code) {
-            return range < 0 || (static_cast<int>(code % kBins) == range && key >= lo && key <= hi);
-        };
-        while (left > kWave) {
-            uint64_t base = 0, held;
-            int shift = 0;
-            if (range >= 0) {  // how far apart the keys are
-                uint64_t least = kNoKey, most = 0;
-                InList(n, span, [&](int, double, uint64_t key, uint32_t code) {
-                    if (!has(key, code)) return;
-                    least = key < least ? key : least;
-                    most = key > most ? key : most;
-                });
-                MinMax(&least, &most);
-                base = least;
-                while ((most - least) >> shift >= kBins) ++shift;
-            }
-            ClearBins();
-            __syncthreads();
-            InList(n, span, [&](int, double place, uint64_t key, uint32_t code) {
-                if (!has(key, code)) return;
-                AddTo(range >= 0 ? static_cast<int>((key - base) >> shift) : static_cast<int>(code % kBins),
-                      what == kCount ? 1 : Weight(place));
-            });
-            const int at = Narrow(what, bound, &before, &held);
-            if (range < 0) {
-                range = at;
-            } else {
-                lo = base + (static_cast<uint64_t>(at) << shift);
-                hi = lo + ((uint64_t{1} << shift) - 1);
-            }
-            // a weight is at least exp(-1 / 64), 0.9845
-            left = what == kCount ? held : static_cast<uint64_t>(static_cast<double>(held) * (1 / (0.984 * kOne)));
-        }
+        uint64_t before = 0, held, least = kNoKey, most = 0;
+        ClearBins();
         if (Tid() == 0) s.n_few = 0;
         __syncthreads();
-        InList(n, span, [&](int, double, uint64_t key, uint32_t code) {
-            if (has(key, code)) s.few[atomicAdd(&s.n_few, 1u)] = key;
-        });
+        if (n > kWave) {
+            InList(n, {bin, bin}, [&](int, double place, uint64_t, uint32_t code) {
+                AddTo(static_cast<int>(code % kBins), what == kCount ? 1 : Weight(place));
+            });
+        }
+        const uint32_t code = static_cast<uint32_t>(bin) * kBins + (n > kWave ? Narrow(what, bound, &before, &held) : 0);
+        // that range's (of a short list, the bin's) places
+#pragma unroll 2
+        for (int i0 = 0; i0 < n; i0 += kChooseThreads) {
+            const int i = i0 + Tid();
+            bool in = i < n && (n > kWave ? s.code[i] == code : s.code[i] / kBins == static_cast<uint32_t>(bin));
+            uint64_t mask = __ballot(in);
+            if (mask == 0) continue;
+            const uint64_t key = in ? s.list[i] : kNoKey;
+            in = in && key <= limit;
+            mask = __ballot(in);
+            uint32_t at = 0;
+            if (Lane() == 0) at = atomicAdd(&s.n_few, static_cast<uint32_t>(__popcll(mask)));
+            at = __builtin_amdgcn_readfirstlane(at) + __popcll(mask & ((uint64_t{1} << Lane()) - 1));
+            if (in) {
+                s.some[at] = static_cast<uint16_t>(i);
+                least = key < least ? key : least;
+                most = key > most ? key : most;
+            }
+        }
+        __syncthreads();
+        int m = static_cast<int>(s.n_few);
+        uint64_t lo = 0, hi = kLastKey;
+        while (m > kWave) {
+            MinMax(&least, &most);
+            int shift = 0;
+            while ((most - least) >> shift >= kBins) ++shift;
+            ClearBins();
+            __syncthreads();
+            for (int i = Tid(); i < m; i += kChooseThreads) {
+                double place;
+                const uint64_t key = s.list[s.some[i]];
+                BinOfKey(key, &place);
+                AddTo(static_cast<int>((key - least) >> shift), what == kCount ? 1 : Weight(place));
+            }
+            __syncthreads();
+            const int at = Narrow(what, bound, &before, &held);
+            lo = least + (static_cast<uint64_t>(at) << shift);
+            hi = lo + ((uint64_t{1} << shift) - 1);
+            least = kNoKey;
+            most = 0;
+            // what is left, in place: all have read theirs before any writes
+            uint16_t mine[kList / kChooseThreads];
+            int count = 0;
+            for (int i = Tid(); i < m; i += kChooseThreads) {
+                const uint16_t index = s.some[i];
+                const uint64_t key = s.list[index];
+                if (key < lo || key > hi) continue;
+                least = key < least ? key : least;
+                most = key > most ? key : most;
+#pragma unroll
+                for (int j = 0; j < kList / kChooseThreads; ++j) mine[j] = j == count ? index : mine[j];
+                ++count;
+            }
+            if (Tid() == 0) s.n_few = 0;
+            __syncthreads();
+            if (count > 0) {
+                const uint32_t to = atomicAdd(&s.n_few, static_cast<uint32_t>(count));
+#pragma unroll
+                for (int j = 0; j < kList / kChooseThreads; ++j) {
+                    if (j < count) s.some[to + j] = mine[j];
+                }
+            }
+            __syncthreads();
+            m = static_cast<int>(s.n_few);
+        }
         // one wave: every lane an element, its place by comparison with all others
         if (Tid() < kWave) {
-            const int m = static_cast<int>(s.n_few);
             const bool real = Tid() < m;
-            const uint64_t key = real ? s.few[Tid()] : ~uint64_t{0};
+            const uint64_t key = s.list[m > 0 ? s.some[real ? Tid() : 0] : 0];
+            s.few[Tid()] = key;
             double place;
-            BinOfKey(real ? key : s.few[0], &place);
+            BinOfKey(key, &place);
             const uint64_t own = Weight(place), one = what == kCount ? 1 : own;
             s.bin[Tid()] = one;  // (this wave alone is here)
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -1088,7 +1124,7 @@ __global__ __launch_bounds__(kGatherThreads) void SampleGather(const SampleArgs 
 int Parts(int64_t n_rows, int64_t vocab, int bytes) {
     const int64_t blocks = (vocab * bytes + 1023) / 1024;
     int64_t parts = (static_cast<int64_t>(ComputeUnits()) * 2 + n_rows - 1) / n_rows;
-    const int64_t most = blocks / (kAhead * kWaves);
+    const int64_t most = (blocks + kAhead * kWaves - 1) / (kAhead * kWaves);
     if (parts > most) parts = most;
     if (parts > kMaxParts) parts = kMaxParts;
     return static_cast<int>(parts < 1 ? 1 : parts);
