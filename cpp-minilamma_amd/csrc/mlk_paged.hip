@@ -529,7 +529,7 @@ int64_t mlk_attention_paged_workspace_bytes(int64_t n_seqs, int64_t n_tokens,
                                             int32_t n_heads, int32_t n_kv_heads,
                                             int32_t head_dim) {
     return AttendWorkspace(n_seqs, n_tokens, max_new_tokens, max_seq_len, n_heads, n_kv_heads,
-                           head_dim, false, {});
+                           head_dim, false, {}, false);
 }
 
 mlk_status mlk_attention_packed(int32_t type, const void* q, int64_t q_row_stride, const void* k,
@@ -568,7 +568,7 @@ int64_t mlk_attention_paged_scored_workspace_bytes(int64_t n_seqs, int64_t n_tok
                                                    int32_t head_dim,
                                                    const mlk_attention_scores* scores) {
     return AttendWorkspace(n_seqs, n_tokens, max_new_tokens, max_seq_len, n_heads, n_kv_heads,
-                           head_dim, false, ScoresOf(scores));
+                           head_dim, false, ScoresOf(scores), true);
 }
 
 int64_t mlk_attention_packed_scored_workspace_bytes(int64_t n_seqs, int64_t n_tokens,
@@ -576,14 +576,14 @@ int64_t mlk_attention_packed_scored_workspace_bytes(int64_t n_seqs, int64_t n_to
                                                     int32_t n_kv_heads, int32_t head_dim,
                                                     const mlk_attention_scores* scores) {
     return AttendWorkspace(n_seqs, n_tokens, max_seq_len, max_seq_len, n_heads, n_kv_heads,
-                           head_dim, true, ScoresOf(scores));
+                           head_dim, true, ScoresOf(scores), true);
 }
 
 int64_t mlk_attention_packed_workspace_bytes(int64_t n_seqs, int64_t n_tokens,
                                              int64_t max_seq_len, int32_t n_heads,
                                              int32_t n_kv_heads, int32_t head_dim) {
     return AttendWorkspace(n_seqs, n_tokens, max_seq_len, max_seq_len, n_heads, n_kv_heads,
-                           head_dim, true, {});
+                           head_dim, true, {}, false);
 }
 
 }  // extern "C"

@@ -345,7 +345,8 @@ int64_t SpanOf(const Scores& scores, int64_t max_len, int64_t tokens, int64_t al
 }
 
 Plan MakePlan(int64_t n_seqs, int64_t n_tokens, int64_t max_new, int64_t longest, int32_t n_heads,
-              int32_t n_kv_heads, int32_t head_dim, bool packed, const Scores& scores) {
+              int32_t n_kv_heads, int32_t head_dim, bool packed, const Scores& scores,
+              bool scored) {
     Plan plan;
     const int64_t group = n_heads / n_kv_heads, cus = ComputeUnits();
     int64_t max_len = SpanOf(scores, longest, max_new, kFewKeys);
@@ -392,7 +393,11 @@ Plan MakePlan(int64_t n_seqs, int64_t n_tokens, int64_t max_new, int64_t longest
         for (int64_t n = 1; n <= kTileMost && (n == 1 || (n - 1) * kTileLeast < max_len); ++n) {
             grid.n_chunks = static_cast<int32_t>(n);
             if (n > 1 && (TileBlocks(grid) > kMaxBlocks || JoinTileBlocks(grid) > kMaxBlocks)) break;
-            const int64_t chunk = RoundUp((max_len + n - 1) / n, kTileLeast);
+            // (a window's span is short: rounded to whole tiles, its chunks stay alike; 900 fp32
+            // tokens over fp16, a window of 1000, the whole call: two chunks of 576 123 us, of 768
+            // and 329 137)
+            int64_t chunk = RoundUp((max_len + n - 1) / n, scored ? kTileAlign : kTileLeast);
+            if (chunk < kTileLeast) chunk = kTileLeast;
             const int64_t cost = ((tiles < 1 ? 1 : tiles) * n + cus - 1) / cus * (chunk + kTileFixed) +
                                  (n > 1 ? kTileJoin : 0);
             if (cost < best) {
@@ -412,7 +417,7 @@ bool Multiple8(int64_t a) { return a % 8 == 0; }
 
 int64_t AttendWorkspace(int64_t n_seqs, int64_t n_tokens, int64_t max_new, int64_t max_len,
                         int32_t n_heads, int32_t n_kv_heads, int32_t head_dim, bool packed,
-                        const Scores& scores) {
+                        const Scores& scores, bool scored) {
     if (n_seqs <= 0 || n_tokens <= 0 || max_new <= 0 || max_len <= 0 || n_heads <= 0 ||
         n_kv_heads <= 0 || n_heads % n_kv_heads != 0 || n_heads > 65536 || head_dim <= 0 ||
         head_dim > 256 || n_seqs > kMaxSeqs || n_tokens > kMaxTokens || max_len > (1 << 30)) {
@@ -422,7 +427,8 @@ int64_t AttendWorkspace(int64_t n_seqs, int64_t n_tokens, int64_t max_new, int64
     if (max_new > max_len) max_new = max_len;
     if (max_new > n_tokens) max_new = n_tokens;
     return PlanBytes(
-        MakePlan(n_seqs, n_tokens, max_new, max_len, n_heads, n_kv_heads, head_dim, packed, scores),
+        MakePlan(n_seqs, n_tokens, max_new, max_len, n_heads, n_kv_heads, head_dim, packed, scores,
+                 scored),
         head_dim);
 }
 
@@ -431,7 +437,7 @@ mlk_status AttendAs(const AttendArgs& a) {
     const int32_t hd = a.rows.head_dim;
     const Ragged& b = a.batch;
     Plan plan = MakePlan(b.n_seqs, b.n_tokens, b.max_new, b.max_len, a.n_heads, a.n_kv_heads, hd,
-                         b.table == nullptr, a.scores);
+                         b.table == nullptr, a.scores, kScored);
     if (static_cast<int64_t>(a.workspace_bytes) < PlanBytes(plan, hd)) {  // no split
         plan.few_workers = plan.few_partials = plan.tile_partials = 0;
         plan.chunk = b.max_len;
