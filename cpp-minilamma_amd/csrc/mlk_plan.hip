@@ -21,12 +21,18 @@
 namespace mlk {
 namespace {
 
-constexpr int kScanThreads = 1024, kPer = 4;        // sequences a thread takes
-constexpr int kScanSeqs = kScanThreads * kPer;      // of a step of the scan
-constexpr int kRowThreads = 256, kRowsEach = 1024;  // rows of a workgroup
+constexpr int kPer = 4;  // sequences a thread takes of a step of the scan
+constexpr int kRowThreads = 256;
 constexpr int64_t kMaxPages = 1 << 30;
-// Rows that the scanning workgroup works out itself, without a second launch.
-constexpr int64_t kOwnRows = 16384;
+// A step of up to kOwnRows rows (or pages) for each of a workgroup's threads is that one
+// workgroup's whole work: the smallest of few waves, which wait less for each other (a prompt of
+// 6: 3.8 us, with 16 waves 5.5).  A larger one's rows have a launch of their own (8186 rows
+// of 256 sequences, in one 6.2 us, in two 8.7 and what lies between two launches).
+constexpr int kOwnThreads = 256, kScanThreads = 1024;
+constexpr int64_t kOwnRows = 8;
+inline bool IsOwn(int threads, int64_t n_seqs, int64_t rows) {
+    return n_seqs <= threads * kPer && rows <= threads * kOwnRows;
+}
 
 struct Pool {
     int32_t *table, *len, *free_pages, *n_free;
@@ -41,6 +47,7 @@ struct PlanArgs {
     int32_t *start, *positions, *seq;
     int64_t* slots;
     int32_t* base;  // [n_seqs + 1]: pages popped before each sequence's; last: *n_free before
+    bool wide;      // len, fresh and start are 16-byte aligned
     int32_t* err;
 };
 
@@ -48,8 +55,32 @@ struct ReleaseArgs {
     Pool pool;
     const int32_t* keep;
     int32_t* before;  // [n_seqs + 2]: pages given back before each sequence's, in all; *n_free
+    bool wide;        // len and keep are 16-byte aligned
     int32_t* err;
 };
+
+// A thread's kPer neighbouring elements of an array of n, from s on, as one load or store where
+// the array is 16-byte aligned (`wide`) and has them all; `none` past its end.
+static_assert(kPer == 4, "an int4");
+__device__ inline void Load4(const int32_t* p, int s, int n, bool wide, int32_t none, int32_t (&v)[kPer]) {
+    if (wide && s + kPer <= n) {
+        const int4 x = *reinterpret_cast<const int4*>(p + s);
+        v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w;
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) v[i] = s + i < n ? p[s + i] : none;
+}
+__device__ inline void Store4(int32_t* p, int s, int n, bool wide, const int32_t (&v)[kPer]) {
+    if (wide && s + kPer <= n) {
+        *reinterpret_cast<int4*>(p + s) = make_int4(v[0], v[1], v[2], v[3]);
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+        if (s + i < n) p[s + i] = v[i];
+    }
+}
 
 __device__ inline int32_t PagesOf(int64_t len, int32_t shift) {
     return static_cast<int32_t>((len + (int64_t{1} << shift) - 1) >> shift);
@@ -67,29 +98,30 @@ __device__ inline uint32_t Sum(uint32_t a, uint32_t b) {
     return c < 0x7FFFFFFFu ? c : 0x7FFFFFFFu;
 }
 
-// Sum over the workgroup's earlier threads; *total: over all.  `scratch` is reused
-// after the caller's next barrier.
-__device__ inline uint32_t ScanBefore(uint32_t v, uint32_t* scratch, uint32_t* total) {
-    constexpr int kWaves = kScanThreads / kWave;
+// Sums over the workgroup's earlier threads; *total: over all.  `scratch` holds a pair a wave and
+// is reused after the caller's next barrier.
+template <int kThreads>
+__device__ inline uint2 ScanBefore(uint2 v, uint2* scratch, uint2* total) {
+    constexpr int kWaves = kThreads / kWave;
     const int lane = static_cast<int>(threadIdx.x) % kWave, wave = static_cast<int>(threadIdx.x) / kWave;
-    uint32_t sum = v;
+    uint2 sum = v;
 #pragma unroll
     for (int off = 1; off < kWave; off *= 2) {
-        const uint32_t o = __shfl_up(sum, off, kWave);
-        if (lane >= off) sum = Sum(sum, o);
+        const uint32_t x = __shfl_up(sum.x, off, kWave), y = __shfl_up(sum.y, off, kWave);
+        if (lane >= off) sum = make_uint2(Sum(sum.x, x), Sum(sum.y, y));
     }
     if (lane == kWave - 1) scratch[wave] = sum;
-    uint32_t up = __shfl_up(sum, 1, kWave);
-    if (lane == 0) up = 0;
+    uint2 up = make_uint2(__shfl_up(sum.x, 1, kWave), __shfl_up(sum.y, 1, kWave));
+    if (lane == 0) up = make_uint2(0, 0);
     __syncthreads();
-    uint32_t before = 0, all = 0;
+    uint2 before = make_uint2(0, 0), all = make_uint2(0, 0);
 #pragma unroll
     for (int i = 0; i < kWaves; ++i) {
         if (i == wave) before = all;
-        all = Sum(all, scratch[i]);
+        all = make_uint2(Sum(all.x, scratch[i].x), Sum(all.y, scratch[i].y));
     }
     *total = all;
-    return Sum(before, up);
+    return make_uint2(Sum(before.x, up.x), Sum(before.y, up.y));
 }
 
 // Largest s of 0 .. n - 1 with start[s] <= x (start[0] <= x, non-decreasing).
@@ -101,6 +133,19 @@ __device__ inline int Find(const int32_t* start, int n, int32_t x) {
         else hi = mid;
     }
     return lo;
+}
+
+// The same by a whole wave, which looks at 64 places at once: a load for each 64-th part.
+__device__ inline int FindByWave(const int32_t* start, int n, int32_t x) {
+    const int lane = static_cast<int>(threadIdx.x) % kWave;
+    int from = 0;
+    for (;;) {
+        const int step = (n + kWave - 1) / kWave, at = lane * step;
+        const int c = __popcll(__ballot(at < n && start[from + at] <= x));
+        from += (c - 1) * step;  // (lane 0's place is one)
+        if (step == 1) return __builtin_amdgcn_readfirstlane(from);
+        n = n - (c - 1) * step < step ? n - (c - 1) * step : step;
+    }
 }
 
 // Token row t, the k-th of sequence s, which held `len` positions; its new pages
@@ -126,11 +171,11 @@ __device__ inline bool PutRow(const PlanArgs& p, int32_t t, int s, int32_t len, 
     return in;
 }
 
-template <bool kOwn>
-__global__ __launch_bounds__(kScanThreads) void PlanScan(const PlanArgs p) {
-    __shared__ uint32_t sums[3][kScanThreads / kWave];
-    __shared__ int32_t s_start[kOwn ? kScanSeqs + 1 : 1], s_len[kOwn ? kScanSeqs : 1],
-        s_base[kOwn ? kScanSeqs : 1];
+template <int kThreads, bool kOwn>
+__global__ __launch_bounds__(kThreads) void PlanScan(const PlanArgs p) {
+    constexpr int kSeqs = kThreads * kPer;
+    __shared__ uint2 sums[2][kThreads / kWave];
+    __shared__ int32_t s_start[kOwn ? kSeqs + 1 : 1], s_len[kOwn ? kSeqs : 1], s_base[kOwn ? kSeqs : 1];
     __shared__ uint32_t taken;
     const Pool& o = p.pool;
     const int tid = static_cast<int>(threadIdx.x);
@@ -138,64 +183,67 @@ __global__ __launch_bounds__(kScanThreads) void PlanScan(const PlanArgs p) {
     const int32_t free = FreePages(o, &bad);
     if (tid == 0) taken = 0;
     uint32_t pages = 0, asked = 0, rows = 0;  // of earlier steps of the scan
-    for (int s0 = 0; s0 < o.n_seqs; s0 += kScanSeqs) {
+    for (int s0 = 0; s0 < o.n_seqs; s0 += kSeqs) {
         int32_t len[kPer], n[kPer], need[kPer];
-        uint32_t my_pages = 0, my_asked = 0;
+        uint2 mine = make_uint2(0, 0);
+        const int my_s = s0 + tid * kPer;
+        Load4(o.len, my_s, o.n_seqs, p.wide, 0, len);
+        Load4(p.fresh, my_s, o.n_seqs, p.wide, 0, n);
 #pragma unroll
         for (int i = 0; i < kPer; ++i) {
-            const int s = s0 + tid * kPer + i;
-            len[i] = n[i] = need[i] = 0;
-            if (s < o.n_seqs) {
-                len[i] = o.len[s];
-                n[i] = p.fresh[s];
-            }
             const int64_t to = static_cast<int64_t>(len[i]) + n[i];
+            need[i] = 0;
             if (len[i] < 0 || n[i] < 0 || to > p.max_len) {
                 bad = true;
                 n[i] = 0;
             } else {
                 need[i] = PagesOf(to, o.page_shift) - PagesOf(len[i], o.page_shift);
             }
-            my_pages = Sum(my_pages, need[i]);
-            my_asked = Sum(my_asked, n[i]);
+            mine = make_uint2(Sum(mine.x, need[i]), Sum(mine.y, n[i]));
         }
-        uint32_t all_pages, all_asked, all_rows;
-        uint32_t a = Sum(pages, ScanBefore(my_pages, sums[0], &all_pages));
-        uint32_t b = Sum(asked, ScanBefore(my_asked, sums[1], &all_asked));
+        uint2 all;
+        const uint2 before = ScanBefore<kThreads>(mine, sums[0], &all);
+        uint32_t a = Sum(pages, before.x), b = Sum(asked, before.y), r = b;
         int32_t base[kPer];
         uint32_t my_rows = 0, top = 0;
+        bool refused = false;
 #pragma unroll
         for (int i = 0; i < kPer; ++i) {
             base[i] = static_cast<int32_t>(a);
             a = Sum(a, need[i]);
             b = Sum(b, n[i]);
             if ((need[i] != 0 && a > static_cast<uint32_t>(free)) || b > static_cast<uint32_t>(p.n_tokens)) {
+                refused |= n[i] != 0;
                 n[i] = need[i] = 0;
             }
             if (need[i] != 0) top = a;
             my_rows += n[i];
         }
         if (top != 0) atomicMax(&taken, top);
-        uint32_t r = rows + ScanBefore(my_rows, sums[2], &all_rows);
+        // (where all are taken in, here and before, their rows are what was asked for)
+        if (__syncthreads_or(refused || rows != asked)) {
+            r = rows + ScanBefore<kThreads>(make_uint2(my_rows, 0), sums[1], &mine).x;
+            rows += mine.x;
+        } else {
+            rows = Sum(rows, all.y);
+        }
+        int32_t start[kPer];
 #pragma unroll
         for (int i = 0; i < kPer; ++i) {
-            const int s = s0 + tid * kPer + i;
-            if (s < o.n_seqs) {
-                p.start[s] = static_cast<int32_t>(r);
-                if (n[i] != 0) o.len[s] = len[i] + n[i];
-                if constexpr (kOwn) {
-                    s_start[s] = static_cast<int32_t>(r);
-                    s_len[s] = len[i];
-                    s_base[s] = base[i];
-                } else {
-                    p.base[s] = base[i];
-                }
-            }
+            start[i] = static_cast<int32_t>(r);
             r += n[i];
+            if constexpr (kOwn) {
+                s_start[my_s + i] = start[i];
+                s_len[my_s + i] = len[i];
+                s_base[my_s + i] = base[i];
+            }
+            len[i] += n[i];
         }
-        pages = Sum(pages, all_pages);
-        asked = Sum(asked, all_asked);
-        rows += all_rows;
+        Store4(p.start, my_s, o.n_seqs, p.wide, start);
+        Store4(o.len, my_s, o.n_seqs, p.wide, len);
+        if constexpr (!kOwn) Store4(p.base, my_s, o.n_seqs, true, base);
+        pages = Sum(pages, all.x);
+        asked = Sum(asked, all.y);
         __syncthreads();
     }
     if (tid == 0) {
@@ -204,7 +252,7 @@ __global__ __launch_bounds__(kScanThreads) void PlanScan(const PlanArgs p) {
         if constexpr (!kOwn) p.base[o.n_seqs] = free;
     }
     if constexpr (kOwn) {
-        for (int t = tid; t < static_cast<int>(rows); t += kScanThreads) {
+        for (int t = tid; t < static_cast<int>(rows); t += kThreads) {
             const int s = Find(s_start, o.n_seqs, t);
             if (!PutRow(p, t, s, s_len[s], t - s_start[s], free - s_base[s])) bad = true;
         }
@@ -212,29 +260,34 @@ __global__ __launch_bounds__(kScanThreads) void PlanScan(const PlanArgs p) {
     if (bad) RaiseFlag(p.err, 1);
 }
 
-// Token rows of a step, kRowsEach a workgroup; the starts of as many sequences from
-// its first row's on lie in shared memory.
+// Token rows of a step, one a thread; the starts of as many sequences from its first row's on
+// lie in shared memory.
 __global__ __launch_bounds__(kRowThreads) void PlanRows(const PlanArgs p) {
-    __shared__ int32_t s_start[kRowsEach + 1];
+    __shared__ int32_t s_start[kRowThreads + 1];
     const Pool& o = p.pool;
     const int tid = static_cast<int>(threadIdx.x);
-    const int32_t t0 = static_cast<int32_t>(blockIdx.x) * kRowsEach, rows = p.start[o.n_seqs];
+    const int32_t t0 = static_cast<int32_t>(blockIdx.x) * kRowThreads, t = t0 + tid;
+    const int32_t rows = p.start[o.n_seqs], free = p.base[o.n_seqs];
     if (t0 >= rows) return;
-    const int first = Find(p.start, o.n_seqs, t0);
-    const int here = o.n_seqs - first < kRowsEach ? o.n_seqs - first : kRowsEach;
+    const int first = FindByWave(p.start, o.n_seqs, t0);
+    const int here = o.n_seqs - first < kRowThreads ? o.n_seqs - first : kRowThreads;
     for (int i = tid; i <= here; i += kRowThreads) s_start[i] = p.start[first + i];
     __syncthreads();
-    const int32_t free = p.base[o.n_seqs];
-    bool bad = false;
-    for (int i = tid; i < kRowsEach && t0 + i < rows; i += kRowThreads) {
-        const int32_t t = t0 + i;
-        // (sequences without rows can lie between: then it is further on)
-        const int s = t < s_start[here] ? first + Find(s_start, here, t)
-                                        : first + here + Find(p.start + first + here, o.n_seqs - first - here, t);
-        const int32_t from = p.start[s], len = o.len[s] - (p.start[s + 1] - from);
-        if (!PutRow(p, t, s, len, t - from, free - p.base[s])) bad = true;
+    if (t >= rows) return;
+    // (sequences without rows can lie between: then it is further on)
+    int s;
+    int32_t from, to;
+    if (t < s_start[here]) {
+        const int i = Find(s_start, here, t);
+        s = first + i;
+        from = s_start[i];
+        to = s_start[i + 1];
+    } else {
+        s = first + here + Find(p.start + first + here, o.n_seqs - first - here, t);
+        from = p.start[s];
+        to = p.start[s + 1];
     }
-    if (bad) RaiseFlag(p.err, 1);
+    if (!PutRow(p, t, s, o.len[s] - (to - from), t - from, free - p.base[s])) RaiseFlag(p.err, 1);
 }
 
 // The i-th of `total` pages given back, sequence s's k-th; `kept` pages stay.
@@ -249,51 +302,51 @@ __device__ inline bool PutPage(const ReleaseArgs& p, int32_t i, int s, int32_t k
     return at < o.n_pages && page >= 0 && page < o.n_pages;
 }
 
-template <bool kOwn>
-__global__ __launch_bounds__(kScanThreads) void ReleaseScan(const ReleaseArgs p) {
-    __shared__ uint32_t sums[kScanThreads / kWave];
-    __shared__ int32_t s_before[kOwn ? kScanSeqs : 1], s_kept[kOwn ? kScanSeqs : 1];
+template <int kThreads, bool kOwn>
+__global__ __launch_bounds__(kThreads) void ReleaseScan(const ReleaseArgs p) {
+    constexpr int kSeqs = kThreads * kPer;
+    __shared__ uint2 sums[kThreads / kWave];
+    __shared__ int32_t s_before[kOwn ? kSeqs : 1], s_kept[kOwn ? kSeqs : 1];
     const Pool& o = p.pool;
     const int tid = static_cast<int>(threadIdx.x);
     bool bad = false;
     const int32_t free = FreePages(o, &bad);
     uint32_t pages = 0;
-    for (int s0 = 0; s0 < o.n_seqs; s0 += kScanSeqs) {
-        int32_t gone[kPer], kept[kPer];
+    for (int s0 = 0; s0 < o.n_seqs; s0 += kSeqs) {
+        int32_t gone[kPer], kept[kPer], keep[kPer], len[kPer];
         uint32_t mine = 0;
+        const int my_s = s0 + tid * kPer;
+        Load4(p.keep, my_s, o.n_seqs, p.wide, -1, keep);
+        Load4(o.len, my_s, o.n_seqs, p.wide, 0, len);
 #pragma unroll
         for (int i = 0; i < kPer; ++i) {
-            const int s = s0 + tid * kPer + i;
             gone[i] = kept[i] = 0;
-            if (s < o.n_seqs) {
-                const int32_t keep = p.keep[s], len = o.len[s];
-                if (keep >= 0) {
-                    if (keep > len || len > o.table_stride << o.page_shift) {
-                        bad = true;
-                    } else {
-                        kept[i] = PagesOf(keep, o.page_shift);
-                        gone[i] = PagesOf(len, o.page_shift) - kept[i];
-                        o.len[s] = keep;
-                    }
+            if (keep[i] >= 0) {
+                if (keep[i] > len[i] || len[i] > o.table_stride << o.page_shift) {
+                    bad = true;
+                } else {
+                    kept[i] = PagesOf(keep[i], o.page_shift);
+                    gone[i] = PagesOf(len[i], o.page_shift) - kept[i];
+                    len[i] = keep[i];
                 }
             }
             mine += gone[i];
         }
-        uint32_t all, at = pages + ScanBefore(mine, sums, &all);
+        uint2 all;
+        uint32_t at = pages + ScanBefore<kThreads>(make_uint2(mine, 0), sums, &all).x;
+        int32_t before[kPer];
 #pragma unroll
         for (int i = 0; i < kPer; ++i) {
-            const int s = s0 + tid * kPer + i;
-            if (s < o.n_seqs) {
-                if constexpr (kOwn) {
-                    s_before[s] = static_cast<int32_t>(at);
-                    s_kept[s] = kept[i];
-                } else {
-                    p.before[s] = static_cast<int32_t>(at);
-                }
-            }
+            before[i] = static_cast<int32_t>(at);
             at += gone[i];
+            if constexpr (kOwn) {
+                s_before[my_s + i] = before[i];
+                s_kept[my_s + i] = kept[i];
+            }
         }
-        pages += all;
+        Store4(o.len, my_s, o.n_seqs, p.wide, len);
+        if constexpr (!kOwn) Store4(p.before, my_s, o.n_seqs, true, before);
+        pages += all.x;
         __syncthreads();
     }
     const int32_t total = static_cast<int32_t>(pages);
@@ -306,7 +359,7 @@ __global__ __launch_bounds__(kScanThreads) void ReleaseScan(const ReleaseArgs p)
         }
     }
     if constexpr (kOwn) {
-        for (int i = tid; i < total; i += kScanThreads) {
+        for (int i = tid; i < total; i += kThreads) {
             const int s = Find(s_before, o.n_seqs, i);
             if (!PutPage(p, i, s, s_kept[s], i - s_before[s], free, total)) bad = true;
         }
@@ -314,16 +367,33 @@ __global__ __launch_bounds__(kScanThreads) void ReleaseScan(const ReleaseArgs p)
     if (bad) RaiseFlag(p.err, 1);
 }
 
+// Pages given back, one a thread at a time; the sums of as many sequences from the first page's
+// on lie in shared memory.
 __global__ __launch_bounds__(kRowThreads) void ReleasePages(const ReleaseArgs p) {
+    __shared__ int32_t s_before[kRowThreads];
     const Pool& o = p.pool;
+    const int tid = static_cast<int>(threadIdx.x);
     const int32_t total = p.before[o.n_seqs], free = p.before[o.n_seqs + 1];
     const int64_t step = static_cast<int64_t>(gridDim.x) * kRowThreads;
     bool bad = false;
-    for (int64_t i = static_cast<int64_t>(blockIdx.x) * kRowThreads + threadIdx.x; i < total; i += step) {
-        const int s = Find(p.before, o.n_seqs, static_cast<int32_t>(i));
+    for (int64_t i0 = static_cast<int64_t>(blockIdx.x) * kRowThreads; i0 < total; i0 += step) {
+        const int first = FindByWave(p.before, o.n_seqs, static_cast<int32_t>(i0));
+        const int here = o.n_seqs - first < kRowThreads ? o.n_seqs - first : kRowThreads;
+        __syncthreads();
+        if (tid < here) s_before[tid] = p.before[first + tid];
+        __syncthreads();
+        const int64_t i = i0 + tid;
+        if (i >= total) continue;
+        const int32_t x = static_cast<int32_t>(i);
+        const int at = Find(s_before, here, x);
+        int s = first + at;
+        int32_t before = s_before[at];
+        if (at == here - 1) {  // (sequences that gave none back can lie between: then further on)
+            s += Find(p.before + s, o.n_seqs - s, x);
+            before = p.before[s];
+        }
         // (a sequence that gave pages back now has the length it kept)
-        const int32_t kept = PagesOf(o.len[s], o.page_shift);
-        if (!PutPage(p, static_cast<int32_t>(i), s, kept, static_cast<int32_t>(i) - p.before[s], free, total)) bad = true;
+        if (!PutPage(p, x, s, PagesOf(o.len[s], o.page_shift), x - before, free, total)) bad = true;
     }
     if (bad) RaiseFlag(p.err, 1);
 }
@@ -426,16 +496,21 @@ mlk_status mlk_paged_plan(const mlk_paged_pool* pool, const int32_t* new_tokens,
     p.seq = token_seq;
     p.slots = slots;
     p.base = static_cast<int32_t*>(workspace);
+    p.wide = Aligned(pool->seq_len, 16) && Aligned(new_tokens, 16) && Aligned(token_start, 16);
     p.err = err;
     const hipStream_t s = AsStream(stream);
-    if (p.pool.n_seqs <= kScanSeqs && n_tokens <= kOwnRows) {
-        hipLaunchKernelGGL(PlanScan<true>, dim3(1), dim3(kScanThreads), 0, s, p);
+    if (IsOwn(kOwnThreads, p.pool.n_seqs, n_tokens)) {
+        hipLaunchKernelGGL((PlanScan<kOwnThreads, true>), dim3(1), dim3(kOwnThreads), 0, s, p);
         return CheckLaunch("PlanScan");
     }
-    hipLaunchKernelGGL(PlanScan<false>, dim3(1), dim3(kScanThreads), 0, s, p);
+    if (IsOwn(kScanThreads, p.pool.n_seqs, n_tokens)) {
+        hipLaunchKernelGGL((PlanScan<kScanThreads, true>), dim3(1), dim3(kScanThreads), 0, s, p);
+        return CheckLaunch("PlanScan");
+    }
+    hipLaunchKernelGGL((PlanScan<kScanThreads, false>), dim3(1), dim3(kScanThreads), 0, s, p);
     st = CheckLaunch("PlanScan");
     if (st != MLK_OK || n_tokens == 0) return st;
-    const dim3 grid(static_cast<unsigned>((n_tokens + kRowsEach - 1) / kRowsEach));
+    const dim3 grid(static_cast<unsigned>((n_tokens + kRowThreads - 1) / kRowThreads));
     hipLaunchKernelGGL(PlanRows, grid, dim3(kRowThreads), 0, s, p);
     return CheckLaunch("PlanRows");
 }
@@ -457,16 +532,21 @@ mlk_status mlk_paged_release(const mlk_paged_pool* pool, const int32_t* keep, vo
     if (st != MLK_OK) return st;
     p.keep = keep;
     p.before = static_cast<int32_t*>(workspace);
+    p.wide = Aligned(pool->seq_len, 16) && Aligned(keep, 16);
     p.err = err;
     const hipStream_t s = AsStream(stream);
     // pages that can come back at once
     const int64_t entries = pool->n_seqs * pool->table_stride;
     const int64_t most = entries < pool->n_pages ? entries : pool->n_pages;
-    if (p.pool.n_seqs <= kScanSeqs && most <= kOwnRows) {
-        hipLaunchKernelGGL(ReleaseScan<true>, dim3(1), dim3(kScanThreads), 0, s, p);
+    if (IsOwn(kOwnThreads, p.pool.n_seqs, most)) {
+        hipLaunchKernelGGL((ReleaseScan<kOwnThreads, true>), dim3(1), dim3(kOwnThreads), 0, s, p);
         return CheckLaunch("ReleaseScan");
     }
-    hipLaunchKernelGGL(ReleaseScan<false>, dim3(1), dim3(kScanThreads), 0, s, p);
+    if (IsOwn(kScanThreads, p.pool.n_seqs, most)) {
+        hipLaunchKernelGGL((ReleaseScan<kScanThreads, true>), dim3(1), dim3(kScanThreads), 0, s, p);
+        return CheckLaunch("ReleaseScan");
+    }
+    hipLaunchKernelGGL((ReleaseScan<kScanThreads, false>), dim3(1), dim3(kScanThreads), 0, s, p);
     st = CheckLaunch("ReleaseScan");
     if (st != MLK_OK) return st;
     hipLaunchKernelGGL(ReleasePages, dim3(GridFor(most, kRowThreads, 8)), dim3(kRowThreads), 0, s, p);
