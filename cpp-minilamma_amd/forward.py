@@ -230,18 +230,18 @@ class DeviceModel:
         buf = self.__dict__.pop("_scratch", None)
         return buf if buf is not None and buf.nbytes >= n else DeviceBuffer(n, np.uint8)
 
-    def forward(self, tokens, positions=None, pos0=0, all_logits=False, stream=None):
-        """ForwardBatch: the logits of the last token ([vocab]) or of every
-        token ([T, vocab]) as numpy."""
+    def _logits_of(self, tokens, positions, pos0, rows, more, stream):
+        """The forward's logits of its last `rows` tokens on the device, on `stream`:
+        (the scratch they lie in, their address, that of `more` bytes behind them)."""
         c = self.config
         D, V, T = c["dim"], c["vocab"], len(tokens)
-        rows = T if all_logits else 1
-        sizes = [T * 4, 0 if positions is None else T * 4, T * D * 4, rows * D * 4, rows * V * 4]
+        sizes = [T * 4, 0 if positions is None else T * 4, T * D * 4, rows * D * 4, rows * V * 4,
+                 more]
         at = [0]
         for n in sizes:
             at.append(at[-1] + (n + 255) // 256 * 256)
         buf = self._take(at[-1])
-        ids, d_pos, x, h, out = (buf.ptr + a for a in at[:-1])
+        ids, d_pos, x, h, out, behind = (buf.ptr + a for a in at[:-1])
         ids_pos = np.zeros(at[2] // 4, np.int32)  # one copy for both
         ids_pos[:T] = np.ascontiguousarray(tokens, np.int32).ravel()[:T]
         if positions is None:
@@ -256,10 +256,50 @@ class DeviceModel:
         self._embed(ids, T, x, stream)
         self._layers(x, T, d_pos, pos0, max_ctx, stream, None)
         self._logits(x + (T - rows) * D * 4, rows, h, out, stream)
+        return buf, out, behind
+
+    def _download(self, buf, ptr, a, stream):
+        """Waits for `stream`, copies `a` from ptr and keeps buf for the next call."""
         if stream is not None:  # (the copy below waits for the null stream alone)
             check(lib.mlk_stream_synchronize(_sp(stream)), "forward")
-        res = np.empty((rows, V), np.float32)
-        check(lib.mlk_memcpy(res.ctypes.data, out, res.nbytes, D2H), "download")
+        check(lib.mlk_memcpy(a.ctypes.data, ptr, a.nbytes, D2H), "download")
         if buf.nbytes <= self._KEPT_SCRATCH:
             self._scratch = buf
+        return a
+
+    def forward(self, tokens, positions=None, pos0=0, all_logits=False, stream=None):
+        """ForwardBatch: the logits of the last token ([vocab]) or of every
+        token ([T, vocab]) as numpy."""
+        rows = len(tokens) if all_logits else 1
+        buf, out, _ = self._logits_of(tokens, positions, pos0, rows, 0, stream)
+        res = self._download(buf, out, np.empty((rows, self.config["vocab"]), np.float32), stream)
         return res if all_logits else res[0]
+
+    def choose(self, tokens, uniform, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0,
+               positions=None, pos0=0, stream=None):
+        """The token that follows `tokens`, chosen on the device from its uniform
+        number in [0, 1) (sampling.sample), and its share of what was kept; for an
+        array of n uniform numbers, those that follow each of the last n tokens, as
+        two arrays.  The settings are numbers, or arrays of n.  Eight bytes a row come
+        back instead of its logits."""
+        from . import sampling
+        u = np.atleast_1d(np.asarray(uniform, np.float32))
+        n, V = u.size, self.config["vocab"]
+        if u.ndim != 1 or not 1 <= n <= len(tokens):
+            raise ValueError(f"{n} uniform numbers for {len(tokens)} tokens")
+        given = np.empty((7, n), np.float32)  # u and the settings, then tokens and shares
+        given[0], given[1], given[3], given[4] = u, temperature, top_p, min_p
+        given.view(np.int32)[2] = top_k
+        need = sampling.workspace_bytes("f32", n, V)
+        head = (given.nbytes + 255) // 256 * 256
+        buf, out, at = self._logits_of(tokens, positions, pos0, n, head + need, stream)
+        check(lib.mlk_memcpy(at, given.ctypes.data, 5 * 4 * n, H2D), "upload")
+        row = [at + 4 * n * i for i in range(7)]
+        sampling.sample("f32", out, n, V, row[0], row[5], sampling.Sampling(*row[1:5]), row[6],
+                        workspace=at + head, workspace_bytes=need, stream=stream)
+        got = self._download(buf, row[5], np.empty((2, n), np.float32), stream)
+        ids, shares = got[0].view(np.int32), got[1]
+        if (ids < 0).any():
+            raise ValueError("a row has no token to choose: NaN, or only -infinity, or a setting "
+                             "out of its range")
+        return (int(ids[0]), float(shares[0])) if np.ndim(uniform) == 0 else (ids, shares)
