@@ -38,6 +38,7 @@ constexpr int kChooseThreads = 256, kChooseWaves = kChooseThreads / kWave;  // t
 constexpr int kBins = 1024;     // of a histogram, a power of two
 constexpr int kPerUnit = 32;    // bins of a temperature
 constexpr int kList = 4096;     // elements gathered at once
+constexpr int kFewAll = kChooseThreads;  // of a list that is put in order as a whole
 constexpr int kChunk = 1024;    // segments looked at at once
 constexpr int kEach = kBins / kChooseThreads;  // neighbouring bins a thread has
 constexpr int kMaxParts = 48;   // workgroups of a row
@@ -67,9 +68,12 @@ struct RowState {
     int32_t top;     // its largest bin
     float largest;   // logit
     float al, ah, bl, bh;  // logits to gather: al .. ah and bl .. bh
-    uint32_t live;   // 0: its token is chosen
+    uint32_t live;   // kChosen: its token is; kAll: what is gathered is all that can be kept
     uint32_t n;      // how many were gathered
+    uint64_t reach;  // the sum that top-p asks for; with a top-k, 0: it follows from that
+    uint64_t unused;
 };
+constexpr uint32_t kChosen = 0, kLive = 1, kAll = 2;
 constexpr int64_t kStateBytes = sizeof(RowState) + kBins * 8 + kList * 8;
 
 struct SampleArgs {
@@ -103,6 +107,10 @@ __device__ inline How HowOf(const SampleArgs& a, int64_t row) {
     h.m = a.how.min_p != nullptr ? a.how.min_p[row] : 0.0f;
     h.u = h.t == 0.0f ? 0.0f : a.u[row];
     h.bad = !(h.t >= 0.0f) || !(h.u >= 0.0f && h.u < 1.0f) || h.p != h.p || h.m != h.m;
+    if (h.m > 1.0f) {  // none weighs as much: the first alone
+        h.k = 1;
+        h.m = 0.0f;
+    }
     if (h.k <= 0 || h.k >= a.vocab) h.k = 0;
     const float t = fmaxf(h.t, 0x1p-14f);
     h.c = kPerUnit / static_cast<double>(t);
@@ -618,7 +626,6 @@ struct Chooser {
         }
         const uint32_t code = static_cast<uint32_t>(bin) * kBins + (n > kWave ? Narrow(what, bound, &before, &held) : 0);
         // that range's (of a short list, the bin's) places
-#pragma unroll 2
         for (int i0 = 0; i0 < n; i0 += kChooseThreads) {
             const int i = i0 + Tid();
             bool in = i < n && (n > kWave ? s.code[i] == code : s.code[i] / kBins == static_cast<uint32_t>(bin));
@@ -779,6 +786,12 @@ __device__ inline uint64_t Share(double u, uint64_t sum) {
     return static_cast<uint64_t>(u * static_cast<double>(sum));
 }
 
+// The least whole sum that is at least p of `sum`.
+__device__ inline uint64_t Reach(float p, uint64_t sum) {
+    const double x = ceil(static_cast<double>(p) * static_cast<double>(sum));
+    return x > 1.0 ? static_cast<uint64_t>(x) : 1;
+}
+
 // The passes after the first.  kCuts: which logits to gather; kFinish: the choice from what was
 // gathered; kSmall: the choice from a row that the list holds whole, without any of the others.
 enum Pass { kCuts, kFinish, kSmall };
@@ -797,13 +810,17 @@ __global__ __launch_bounds__(kChooseThreads) void SampleChoose(const SampleArgs 
     int32_t top = INT32_MIN;
     uint64_t best = kNoKey;
     float largest = -INFINITY;
+    bool all_held = kPass_ == kSmall && p.vocab <= kFewAll;  // in the list, and few
+    uint64_t row_reach = 0;
     if constexpr (kPass_ == kFinish) {
         const RowState at = *state;
 #pragma unroll
         for (int i = 0; i < kEach; ++i) s.bin[tid + i * kChooseThreads] = state_bin[tid + i * kChooseThreads];
-        if (at.live == 0) return;
+        if (at.live == kChosen) return;
         top = at.top;
         largest = at.largest;
+        all_held = at.live == kAll && at.n <= kFewAll;
+        row_reach = at.reach;
     } else if constexpr (kPass_ == kCuts) {
         // lane i of each wave: part i
         const char* parts = p.part + row * p.parts * kPartBytes;
@@ -874,7 +891,7 @@ __global__ __launch_bounds__(kChooseThreads) void SampleChoose(const SampleArgs 
     }
     if constexpr (kPass_ != kFinish) {
         const bool none = h.bad || flags != kSome;
-        if (kPass_ == kCuts && tid == 0) state->live = none || h.t == 0.0f ? 0 : 1;
+        if (kPass_ == kCuts && tid == 0) state->live = none || h.t == 0.0f ? kChosen : kLive;
         if (none || h.t == 0.0f) {
             if (tid == 0) {
                 p.tokens[row] = none ? -1 : static_cast<int32_t>(best);
@@ -896,6 +913,55 @@ __global__ __launch_bounds__(kChooseThreads) void SampleChoose(const SampleArgs 
         }
     }
     __syncthreads();
+    if (kPass_ != kCuts && all_held) {
+        // all that can be kept is in the list, an element a thread: in order by comparison with all
+        // others, and every cut is a count
+        const int n = kPass_ == kSmall ? p.vocab : static_cast<int>(state->n);
+        uint64_t key = kNoKey, w = 0;
+        if (tid < n) {
+            key = kPass_ == kSmall ? s.list[tid] : state_list[tid];
+            double f;
+            const int b = ch.BinOfKey(key, &f);
+            if (key <= kLastKey && b >= 0 && b < kBins) w = ch.Scaled(Weight(f), b);
+            if (w == 0) key = kNoKey;
+        }
+        __syncthreads();
+        s.bin[tid] = key;
+        s.list[kFewAll + tid] = kNoKey;
+        s.sum[tid] = 0;
+        __syncthreads();
+        int rank = 0;
+#pragma unroll 8
+        for (int i = 0; i < n; ++i) rank += s.bin[i] < key ? 1 : 0;
+        if (key != kNoKey) {
+            s.list[kFewAll + rank] = key;
+            s.sum[rank] = w;
+        }
+        __syncthreads();
+        w = s.sum[tid];
+        uint64_t all;
+        const uint64_t upto = ScanBlock(w, s.scan_u, &all);
+        s.sum[tid] = upto;
+        int kept = __syncthreads_count(w != 0);
+        const uint64_t first = s.sum[0];
+        if (h.k != 0 && h.k < kept) kept = h.k;
+        if (h.p < 1.0f) {
+            const uint64_t sum = row_reach != 0 ? row_reach : Reach(h.p, s.sum[kept - 1]);
+            const int before = __syncthreads_count(tid < kept && upto < sum);
+            if (before + 1 < kept) kept = before + 1;
+        }
+        if (h.m > 0.0f) {
+            const int enough = __syncthreads_count(w != 0 && static_cast<double>(w) >= static_cast<double>(h.m) * static_cast<double>(first));
+            if (enough < kept) kept = enough > 1 ? enough : 1;
+        }
+        const uint64_t whole = s.sum[kept - 1], bound = Share(h.u, whole);
+        const int at = __syncthreads_count(tid < kept && upto <= bound);
+        if (tid == (at < kept ? at : kept - 1)) {
+            p.tokens[row] = static_cast<int32_t>(s.list[kFewAll + tid]);
+            if (p.prob != nullptr) p.prob[row] = static_cast<float>(static_cast<double>(w) / static_cast<double>(whole));
+        }
+        return;
+    }
     // Three places are looked for in turn, each where its cut is asked for: the top-k's, the
     // top-p's (with the sum that min-p leaves) and the token's.  The row is gathered once for
     // the first two as a rule, or once for the last two.
@@ -931,12 +997,11 @@ __global__ __launch_bounds__(kChooseThreads) void SampleChoose(const SampleArgs 
             kept = s.sum[last];
             uint64_t low = kept;  // what is kept will weigh low .. kept
             if (by_p) {
-                const double x = ceil(static_cast<double>(h.p) * static_cast<double>(kept));
-                reach = x > 1.0 ? static_cast<uint64_t>(x) : 1;
+                reach = Reach(h.p, kept);
                 p_bin = ch.FirstBins(last, true, reach, reach).lo;
             }
             if (by_m) {
-                least = fmin(static_cast<double>(h.m), 1.0) * ch.WeightOf(largest);  // its equals are kept
+                least = static_cast<double>(h.m) * ch.WeightOf(largest);  // its equals are kept
                 const double where = -static_cast<double>(kPerUnit) * log(least / kOne);
                 m.hi = where >= kBins ? kBins - 1 : static_cast<int>(where + 0.51);
                 m.lo = m.hi > 1 ? m.hi - 2 : 0;
@@ -971,7 +1036,18 @@ __global__ __launch_bounds__(kChooseThreads) void SampleChoose(const SampleArgs 
         }
         bool whole = true;  // the list serves the places looked for later too
         if constexpr (kPass_ == kCuts) {
-            if (tid == 0) *state = {top, largest, ch.Lowest(a.hi), ch.Highest(a.lo), ch.Lowest(b.hi), ch.Highest(b.lo), 1, 0};
+            bool is_all = a.lo == 0;
+            if (what == kTopP) {  // whether all up to the last bin are few
+                uint64_t mass = 0, all;
+                for (int i = tid; i <= last; i += kChooseThreads) mass += s.bin[i];
+                ScanBlock(mass, s.scan_u, &all);
+                is_all = static_cast<double>(all) * (1 / (0.984 * kOne)) < 0.9 * kFewAll;
+                if (is_all) a = b = {0, last};
+            }
+            if (tid == 0) {
+                *state = {top, largest, ch.Lowest(a.hi), ch.Highest(a.lo), ch.Lowest(b.hi), ch.Highest(b.lo), is_all ? kAll : kLive, 0,
+                          what == kTopP ? reach : 0, 0};
+            }
             return;
         }
         if (kPass_ == kFinish && first) {  // what was gathered for this
@@ -982,6 +1058,7 @@ __global__ __launch_bounds__(kChooseThreads) void SampleChoose(const SampleArgs 
             __syncthreads();
             if (n > kList) n = -1;
             whole = !(what == kTopK && a.lo != 0);
+            if (what == kTopP && state->live == kAll) whole = true;
         }
         if (n < 0 && look) {
             n = ch.Gather(bin);
@@ -1055,7 +1132,7 @@ __global__ __launch_bounds__(kGatherThreads) void SampleGather(const SampleArgs 
 #pragma unroll
     for (int l = 0; l < kLook; ++l) m[l] = s0 + l * kWave < segments ? largest[s0 + l * kWave] : -INFINITY;
     const RowState at = *state;
-    if (at.live == 0) return;
+    if (at.live == kChosen) return;
     if (threadIdx.x == 0) n_found = 0;
     __syncthreads();
     const float al = at.al, ah = at.ah, bl = at.bl, bh = at.bh, low = fminf(al, bl);

@@ -191,6 +191,21 @@ def test_ties_in_the_middle(mlk, sampling, act, V):
     check(x, how, run(mlk, sampling, x, how, act), act, 0.5)
 
 
+@pytest.mark.parametrize("V", [9, 500, 30000])
+def test_cuts_among_equal_largest_logits(mlk, sampling, V):
+    """Three equal largest logits: min-p of 1 keeps the three, more than 1 the first, a
+    top-k of 2 two, a top-p the fewest that reach it."""
+    x = np.zeros((8, V), np.float32)
+    x[:, [2, V // 2, V - 2]] = 60.0  # all else weighs nothing
+    how = settings(8, m=[1.0, 1.5, 3.0, 1.0, 0, 0, 0, 0], k=[0, 0, 0, 2, 2, 0, 0, 1],
+                   p=[1, 1, 1, 1, 1, 0.5, 0.3, 1], u=[0.99, 0.99, 0.5, 0.99, 0.99, 0.99, 0.99, 0.99])
+    tokens, probs, flag = run(mlk, sampling, x, how)
+    a, b, c = 2, V // 2, V - 2
+    np.testing.assert_array_equal(tokens, [c, a, a, b, b, b, a, a])
+    np.testing.assert_allclose(probs, [1 / 3, 1, 1, 1 / 2, 1 / 2, 1 / 2, 1, 1], rtol=2.0 ** -23)
+    assert flag == 0
+
+
 def test_uniforms_at_the_ends(mlk, sampling):
     rng = np.random.default_rng(5)
     x = logits(rng, 6, 5000)
