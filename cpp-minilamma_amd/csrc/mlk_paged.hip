@@ -313,10 +313,13 @@ Scores ScoresOf(const mlk_attention_scores* s) {
 }
 
 // Score functions and masks of an attention call; they are read while out is written.
-mlk_status CheckScores(const char* fn, const mlk_attention_scores* scores, const void* out, Scores* to) {
+mlk_status CheckScores(const char* fn, const mlk_attention_scores* scores, float scale, const void* out, Scores* to) {
     if (scores == nullptr) return Fail(MLK_ERR_INVALID, "%s: scores must not be null", fn);
-    if (!std::isfinite(scores->softcap) || scores->softcap < 0.0f) {
-        return Fail(MLK_ERR_INVALID, "%s: softcap must be finite and not negative", fn);
+    const float cap = scores->softcap;
+    // (so that neither the cap times log2 e nor the scale over it leaves fp32's range)
+    if (!(cap == 0.0f || (cap >= 0x1p-40f && cap <= 0x1p40f && std::isnormal(scale / cap)))) {
+        return Fail(MLK_ERR_INVALID, "%s: softcap must be 0 or in 2^-40..2^40, and the scale over it "
+                                     "a normal number", fn);
     }
     if (scores->window < 0) return Fail(MLK_ERR_INVALID, "%s: window must not be negative", fn);
     const void* ptrs[3] = {scores->slopes, scores->prefix_len, scores->first};
@@ -520,7 +523,7 @@ mlk_status mlk_attention_paged_scored(const mlk_paged_cache* cache, const mlk_pa
     AttendArgs a;
     mlk_status st = PagedCall(fn, cache, batch, type, q, q_row_stride, out, n_heads, scale,
                               workspace, workspace_bytes, err, stream, &a);
-    if (st == MLK_OK) st = CheckScores(fn, scores, out, &a.scores);
+    if (st == MLK_OK) st = CheckScores(fn, scores, scale, out, &a.scores);
     return st != MLK_OK || a.batch.n_seqs == 0 ? st : AttendScored(a);
 }
 
@@ -558,7 +561,7 @@ mlk_status mlk_attention_packed_scored(int32_t type, const mlk_attention_scores*
     mlk_status st = PackedCall(fn, type, q, q_row_stride, k, k_row_stride, v, v_row_stride,
                                seq_start, n_seqs, n_tokens, max_seq_len, n_heads, n_kv_heads,
                                head_dim, scale, out, workspace, workspace_bytes, err, stream, &a);
-    if (st == MLK_OK) st = CheckScores(fn, scores, out, &a.scores);
+    if (st == MLK_OK) st = CheckScores(fn, scores, scale, out, &a.scores);
     return st != MLK_OK || a.batch.n_seqs == 0 ? st : AttendScored(a);
 }
 

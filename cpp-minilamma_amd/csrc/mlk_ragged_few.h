@@ -380,6 +380,7 @@ __global__ __launch_bounds__(kWaves * kWave) void AttnFew(const RaggedParams p) 
         }
         const int32_t first_pos = q.len - q.n;  // the lowest position of a row
         bool special = false;                   // met a non-finite V in a masked tile
+        [[maybe_unused]] Seen met{INT32_MAX, -1};  // kScored: the first and last such tile's positions
 
         for (; j0 < j_end; j0 += step) {
             const int32_t jn = j0 + step;
@@ -467,7 +468,9 @@ __global__ __launch_bounds__(kWaves * kWave) void AttnFew(const RaggedParams p) 
             if (masked) {
 #pragma unroll
                 for (int j = 0; j < Tile::NKEY; ++j) {
-                    special |= OnlyFinite<C, Tile::NVW>(tile.v[j]);
+                    const bool hit = OnlyFinite<C, Tile::NVW>(tile.v[j]);
+                    special |= hit;
+                    if (kScored && hit) met = {j0 < met.lo ? j0 : met.lo, j0 + KT - 1};
                 }
             }
             if constexpr (kF32) {
@@ -527,6 +530,13 @@ __global__ __launch_bounds__(kWaves * kWave) void AttnFew(const RaggedParams p) 
         if (along == 1) {
             // the wave has its head's positions to itself
             const bool any_special = __ballot(special) != 0;
+            if (kScored && any_special) {
+#pragma unroll
+                for (int off = kWave / 2; off > 0; off /= 2) {
+                    const int32_t a = __shfl_xor(met.lo, off, kWave), b = __shfl_xor(met.hi, off, kWave);
+                    met = {a < met.lo ? a : met.lo, b > met.hi ? b : met.hi};
+                }
+            }
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb) {
                 const float lt = Sum32(Sum16(l[nb]));
@@ -542,7 +552,8 @@ __global__ __launch_bounds__(kWaves * kWave) void AttnFew(const RaggedParams p) 
                 if constexpr (kScored) {
                     if (row_lo[nb] > row_hi[nb]) inv = 0.0f;  // it sees nothing
                     last = row_hi[nb] < j_end ? row_hi[nb] : j_end - 1;
-                    from = row_lo[nb] > from ? row_lo[nb] : from;
+                    last = last < met.hi ? last : met.hi;
+                    from = row_lo[nb] > met.lo ? row_lo[nb] : met.lo;
                 }
 #pragma unroll
                 for (int n = 0; n < Tile::NVR; ++n) {
@@ -597,6 +608,18 @@ __global__ __launch_bounds__(kWaves * kWave) void AttnFew(const RaggedParams p) 
                 }
             }
             special = __syncthreads_or(special);
+            if (kScored && special) {
+                __shared__ int32_t span[2];
+                if (tid == 0) {
+                    span[0] = INT32_MAX;
+                    span[1] = -1;
+                }
+                __syncthreads();
+                atomicMin(&span[0], met.lo);
+                atomicMax(&span[1], met.hi);
+                __syncthreads();
+                met = {span[0], span[1]};
+            }
             for (int u = tid; u < heads * rows * HD; u += kThreads) {
                 const int d = u % HD, row = u / HD % rows, hb = u / HD / rows;
                 if (kLie != kFull && d >= hd) continue;
@@ -610,12 +633,17 @@ __global__ __launch_bounds__(kWaves * kWave) void AttnFew(const RaggedParams p) 
                 const int i = row / p.group, h = (head0 + hb) * p.group + row % p.group;
                 Seen seen{0, first_pos + i};
                 if constexpr (kScored) seen = SeenBy(p.scores, s, q.t0 + i, first_pos + i, q.len);
+                int32_t from = seen.lo > masked_from ? seen.lo : masked_from;
                 if (special) {
-                    const int32_t last = seen.hi < j_end ? seen.hi : j_end - 1;
+                    int32_t last = seen.hi < j_end ? seen.hi : j_end - 1;
+                    if constexpr (kScored) {
+                        last = last < met.hi ? last : met.hi;
+                        from = from > met.lo ? from : met.lo;
+                    }
                     sum += NonFiniteSum<C>(p.rows, fr.table, fr.t0,
                                            static_cast<const CB*>(p.rows.v) +
                                                static_cast<int64_t>(head0 + hb) * hd,
-                                           seen.lo > masked_from ? seen.lo : masked_from, last, d);
+                                           from, last, d);
                 }
                 if (split) {
                     const int64_t at = FewPartial(p, blockIdx.x, place, hb, row);

@@ -223,6 +223,7 @@ __global__ __launch_bounds__((TileShape<A, C, HD>::kThreads), HD <= 128 ? 2 : 1)
     constexpr int kChunks = HD / 8, kPer = kWave / kChunks;
     uint32_t gk[NCH][T::NW], gv[NCH][T::NW];
     bool bad = false, special = false;
+    [[maybe_unused]] Seen met{INT32_MAX, -1};  // kScored: positions of the first and last tile that was
     const int my_r = lane / kChunks, my_c = lane % kChunks;
     auto first_row = [&](int i) { return kPer * wave + kThreads / kChunks * i; };
     // whole tiles whose kPer rows share a page (or are packed): uniform bases; their
@@ -284,7 +285,11 @@ __global__ __launch_bounds__((TileShape<A, C, HD>::kThreads), HD <= 128 ? 2 : 1)
         // some row does not attend to all of it
         if (j0 + KT - 1 > all_hi || j0 + KT > j_end || (kScored && j0 < all_lo)) {
 #pragma unroll
-            for (int i = 0; i < NCH; ++i) special |= OnlyFinite<C, T::NW>(gv[i]);
+            for (int i = 0; i < NCH; ++i) {
+                const bool hit = OnlyFinite<C, T::NW>(gv[i]);
+                special |= hit;
+                if (kScored && hit) met = {j0 < met.lo ? j0 : met.lo, j0 + KT - 1};
+            }
         }
         put(dst, gv);
     };
@@ -464,16 +469,29 @@ __global__ __launch_bounds__((TileShape<A, C, HD>::kThreads), HD <= 128 ? 2 : 1)
     }
     if (bad && p.err != nullptr) RaiseFlag(p.err, 1);
     special = __syncthreads_or(special);
+    if (kScored && special) {
+        __shared__ int32_t span[2];
+        if (tid == 0) {
+            span[0] = INT32_MAX;
+            span[1] = -1;
+        }
+        __syncthreads();
+        atomicMin(&span[0], met.lo);
+        atomicMax(&span[1], met.hi);
+        __syncthreads();
+        met = {span[0], span[1]};
+    }
     l = Sum32(l);
     if (!real) return;
-    const int32_t last = row_hi < j_end ? row_hi : j_end - 1;
+    int32_t last = row_hi < j_end ? row_hi : j_end - 1;
     int32_t masked_from = (lo < j_end ? lo : j_end) - KT;
     bool split = pos >= p.chunk;
     if constexpr (kScored) {
         if (row_lo > row_hi) return;
         const int32_t c0 = TileFirstChunk(p, base0, row_lo), c1 = (row_hi - base0) / p.chunk;
         if (chunk < c0 || chunk > c1) return;
-        masked_from = row_lo;
+        masked_from = row_lo > met.lo ? row_lo : met.lo;
+        last = last < met.hi ? last : met.hi;
         split = c0 != c1;
     } else {
         if (pos < j_begin) return;

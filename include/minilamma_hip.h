@@ -546,7 +546,7 @@ int64_t mlk_paged_plan_workspace_bytes(int64_t n_seqs);
  * documents side by side in one sequence, where each token's own begins; it may
  * lie behind the token's last position: a token that sees nothing gets zeros. */
 typedef struct {
-    float softcap;              /* finite, >= 0 */
+    float softcap;              /* 0, or 2^-40 .. 2^40 with scale / softcap a normal number */
     const float* slopes;        /* device [n_heads] or NULL */
     int64_t window;             /* >= 0 */
     const int32_t* prefix_len;  /* device [n_seqs] or NULL */

@@ -336,6 +336,46 @@ def test_unseen_positions_do_not_reach_a_token(mlk, paged, act, ct, value, hd, n
 
 
 @pytest.mark.parametrize("act,ct", PAIRS)
+@pytest.mark.parametrize("n", [3, 400])
+def test_non_finite_values_far_apart(mlk, paged, act, ct, n):
+    """V infinite at positions thousands apart, in tiles that tokens of one document see
+    and those of the next do not: each token gets what it sees, sum and sign."""
+    H, KV, hd, m = 4, 2, 64, 3500
+    rng = np.random.default_rng(21)
+    batch = Batch([n, 1], [m, 900], 16)
+    pages = Pages(mlk, paged, batch, KV, hd, ct, rng)
+    masks = Masks(batch, H, cap=20.0)
+    masks.first = np.zeros(batch.T, np.int32)
+    masks.first[n // 2:n] = 2900  # the second half of the new tokens: a document of their own
+    places = {(5, 0): np.inf, (1700, 1): -np.inf, (2890, 2): np.inf, (2950, 3): np.inf, (10, 4): np.inf,
+              (2000, 4): -np.inf, (m - 2, 5): -np.inf}
+    view = pages.view(1)
+    for (pos, d), x in places.items():
+        pg, r = batch.slots(0, m)
+        view[pg[pos], r[pos], 0, d] = to_type(np.float32([x]), ct)[0]
+    pages.upload(mlk, paged)
+    q = to_type(rng.standard_normal((batch.T, H, hd)), act)
+    got = values(run_paged(mlk, paged, batch, pages, masks, q, H, act), act).reshape(batch.T, KV, H // KV, hd)
+    for t, s, p in batch.rows():
+        see = masks.see(t, s, p)
+        bad = {}
+        for (pos, d), x in places.items():
+            if s == 0 and pos < len(see) and see[pos]:
+                bad.setdefault(d, set()).add(x)
+        for d in range(hd):
+            g = got[t, 0, :, d]
+            if d not in bad:
+                assert np.isfinite(g).all(), (t, d)
+            elif len(bad[d]) > 1:
+                assert np.isnan(g).all(), (t, d)
+            elif act != "f32":
+                assert (g == next(iter(bad[d]))).all(), (t, d)
+            else:  # fp32's pieces may meet it as inf - inf
+                assert not np.isfinite(g).any(), (t, d)
+        assert np.isfinite(got[t, 1]).all()
+
+
+@pytest.mark.parametrize("act,ct", PAIRS)
 def test_large_scores_are_capped(mlk, paged, act, ct):
     """Scores hundreds of times the cap, of either sign: tanh at its ends."""
     H, KV, hd = 4, 2, 64

@@ -100,6 +100,7 @@ def make(paged, **kw):
 SCORES = [
     (dict(softcap=-1.0), "softcap"), (dict(softcap=float("nan")), "softcap"),
     (dict(softcap=float("inf")), "softcap"), (dict(window=-1), "window"),
+    (dict(softcap=1e-13), "softcap"), (dict(softcap=2e12), "softcap"),
     (dict(slopes=FAKE + 2), "4-byte aligned"), (dict(prefix_len=FAKE + 1), "4-byte aligned"),
     (dict(first=FAKE + 3), "4-byte aligned"), (dict(first=6 * FAKE), "may not alias"),
     (dict(slopes=6 * FAKE), "may not alias"),
@@ -131,6 +132,8 @@ def test_scored_calls_check_the_rest_as_the_plain_ones_do(mlk, paged):
                                       8, 6 * FAKE)
     with pytest.raises(ValueError, match="workspace_bytes"):
         paged.attention_scored(cache, batch, scores, 5 * FAKE, 6 * FAKE, 4, "f16", workspace=FAKE)
+    with pytest.raises(mlk.MlkError, match="softcap"):  # the scale over it is not a normal number
+        paged.attention_scored(cache, batch, scores, 5 * FAKE, 6 * FAKE, 4, "f16", scale=1e-37)
     assert mlk.lib.mlk_attention_packed_scored(0, None, FAKE, 32, FAKE, 16, FAKE, 16, FAKE, 1, 1,
                                                1, 4, 2, 8, 1.0, 9 * FAKE, None, 0, None,
                                                None) == mlk.MLK_ERR_INVALID
