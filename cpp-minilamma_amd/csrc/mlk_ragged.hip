@@ -101,7 +101,7 @@ __device__ inline void Join(const RaggedParams& p, const JoinRow& row, int part_
     }
 }
 
-// Few-row kernel's rows, a place's after the other's: blockIdx.x = place * per_place
+// Few-row kernel's rows, a place's after the other's: block = place * per_place
 // + place of its rows.  A place is a sequence, all heads; or, in batches of more
 // sequences than workers, a worker, standing for the one (sequence, block of heads)
 // that it is the second to hold a part of: others have no parts to join, and looking
@@ -110,14 +110,13 @@ __device__ inline void Join(const RaggedParams& p, const JoinRow& row, int part_
 // and 6.7 ms, 1024 of them 0.50 and 0.46; 64 of lengths to 8192 191 and 195 us, one
 // of 8191 in fp32 27 and 38.)
 template <typename A, int L, bool kByWorker, bool kScored>
-__global__ __launch_bounds__(kThreads) void JoinFew(const RaggedParams p, int per_row,
-                                                    int per_place) {
+__device__ inline void JoinFewRows(const RaggedParams& p, uint32_t block, int per_row, int per_place,
+                                   f32x4 (*sums)[L]) {
     constexpr int NG = kThreads / L;
-    __shared__ f32x4 sums[NG][L];
     const int g = static_cast<int>(threadIdx.x) / L;
     const int rows_here = NG / per_row;
-    const int place = static_cast<int>(blockIdx.x / per_place);
-    const int64_t first = static_cast<int64_t>(blockIdx.x % per_place) * rows_here;
+    const int place = static_cast<int>(block / per_place);
+    const int64_t first = static_cast<int64_t>(block % per_place) * rows_here;
     const int64_t in_place = first + g / per_row;
     FewWork work;
     int64_t head0 = 0, heads = p.n_kv_heads;
@@ -166,15 +165,14 @@ __global__ __launch_bounds__(kThreads) void JoinFew(const RaggedParams p, int pe
     Join<A, L>(p, row, g % per_row, per_row, sums);
 }
 
-// Tile kernel's rows: blockIdx.x = token * per_token + place of its heads.
+// Tile kernel's rows: block = token * per_token + place of its heads.
 template <typename A, int L, bool kScored>
-__global__ __launch_bounds__(kThreads) void JoinTile(const RaggedParams p, int per_row,
-                                                     int per_token) {
+__device__ inline void JoinTileRows(const RaggedParams& p, uint32_t block, int per_row, int per_token,
+                                    f32x4 (*sums)[L]) {
     constexpr int NG = kThreads / L;
-    __shared__ f32x4 sums[NG][L];
     const int g = static_cast<int>(threadIdx.x) / L;
-    const int32_t t = static_cast<int32_t>(blockIdx.x / per_token);
-    const int32_t h = static_cast<int32_t>(blockIdx.x % per_token) * (NG / per_row) + g / per_row;
+    const int32_t t = static_cast<int32_t>(block / per_token);
+    const int32_t h = static_cast<int32_t>(block % per_token) * (NG / per_row) + g / per_row;
     const int s = LastSeq(p.batch, t, [](int32_t a, int) { return a; });
     Seq q;
     if (!LoadSeq(p.batch, s, &q) || t < q.t0 || t >= q.t0 + q.n) return;
@@ -230,28 +228,73 @@ inline int64_t JoinTileBlocks(const RaggedParams& p) {
     return JoinTilePerToken(p) * p.batch.n_tokens;
 }
 
-template <typename A, int L, bool kScored>
-void StartJoinFew(const RaggedParams& p, hipStream_t s) {
-    const dim3 grid(static_cast<unsigned>(JoinFewBlocks(p))), block(kThreads);
-    const int per_row = JoinFewPerRow(p), n = static_cast<int>(JoinFewPerPlace(p));
-    if (JoinByWorker(p)) hipLaunchKernelGGL((JoinFew<A, L, true, kScored>), grid, block, 0, s, p, per_row, n);
-    else hipLaunchKernelGGL((JoinFew<A, L, false, kScored>), grid, block, 0, s, p, per_row, n);
+template <typename A, int L, bool kByWorker, bool kScored>
+__global__ __launch_bounds__(kThreads) void JoinFew(const RaggedParams p, int per_row, int per_place) {
+    __shared__ f32x4 sums[kThreads / L][L];
+    JoinFewRows<A, L, kByWorker, kScored>(p, blockIdx.x, per_row, per_place, sums);
 }
-template <typename A, bool kScored>
-mlk_status LaunchJoinFew(const RaggedParams& p, hipStream_t s) {
-    if (JoinGroups(p) == 8) StartJoinFew<A, 32, kScored>(p, s);
-    else StartJoinFew<A, 64, kScored>(p, s);
-    return CheckLaunch("JoinFew");
+template <typename A, int L, bool kScored>
+__global__ __launch_bounds__(kThreads) void JoinTile(const RaggedParams p, int per_row, int per_token) {
+    __shared__ f32x4 sums[kThreads / L][L];
+    JoinTileRows<A, L, kScored>(p, blockIdx.x, per_row, per_token, sums);
 }
 
-template <typename A, bool kScored>
-mlk_status LaunchJoinTile(const RaggedParams& p, hipStream_t s) {
-    const dim3 grid(static_cast<unsigned>(JoinTileBlocks(p))), block(kThreads);
-    const int per_row = PerRow(JoinGroups(p), p.n_chunks);
-    const int n = static_cast<int>(JoinTilePerToken(p));
-    if (JoinGroups(p) == 8) hipLaunchKernelGGL((JoinTile<A, 32, kScored>), grid, block, 0, s, p, per_row, n);
-    else hipLaunchKernelGGL((JoinTile<A, 64, kScored>), grid, block, 0, s, p, per_row, n);
-    return CheckLaunch("JoinTile");
+// Both, where a mixed batch leaves both: the few-row kernel's rows by the first few_blocks
+// workgroups, the tile kernel's by the others.  Neither waits for the other, and each is a chain
+// of loads (calls with one launch for each and with one for both: 32 sequences of 8B heads, one
+// of 1023 new tokens, 170.1 and 163.6 us; 64 with a window of 1024, 116.6 and 110.8).
+struct JoinParams {
+    RaggedParams few, tile;
+    uint32_t few_blocks;
+    int few_per_row, few_per_place, tile_per_row, tile_per_token;
+};
+template <typename A, int L, bool kByWorker, bool kScored>
+__global__ __launch_bounds__(kThreads) void JoinBoth(const JoinParams p) {
+    __shared__ f32x4 sums[kThreads / L][L];
+    if (blockIdx.x < p.few_blocks) {
+        JoinFewRows<A, L, kByWorker, kScored>(p.few, blockIdx.x, p.few_per_row, p.few_per_place, sums);
+    } else {
+        JoinTileRows<A, L, kScored>(p.tile, blockIdx.x - p.few_blocks, p.tile_per_row, p.tile_per_token, sums);
+    }
+}
+
+// `few`, `tile`: null where those rows have no parts.
+template <typename A, int L, bool kScored>
+void StartJoin(const RaggedParams* few, const RaggedParams* tile, hipStream_t s) {
+    JoinParams p{};
+    int64_t blocks = 0;
+    if (few != nullptr) {
+        p.few = *few;
+        p.few_per_row = JoinFewPerRow(*few);
+        p.few_per_place = static_cast<int>(JoinFewPerPlace(*few));
+        blocks = JoinFewBlocks(*few);
+        p.few_blocks = static_cast<uint32_t>(blocks);
+    }
+    if (tile != nullptr) {
+        p.tile = *tile;
+        p.tile_per_row = PerRow(JoinGroups(*tile), tile->n_chunks);
+        p.tile_per_token = static_cast<int>(JoinTilePerToken(*tile));
+        blocks += JoinTileBlocks(*tile);
+    }
+    const dim3 grid(static_cast<unsigned>(blocks)), block(kThreads);
+    const bool by_worker = few != nullptr && JoinByWorker(*few);
+    if (few == nullptr) {
+        hipLaunchKernelGGL((JoinTile<A, L, kScored>), grid, block, 0, s, p.tile, p.tile_per_row, p.tile_per_token);
+    } else if (tile == nullptr) {
+        if (by_worker) hipLaunchKernelGGL((JoinFew<A, L, true, kScored>), grid, block, 0, s, p.few, p.few_per_row, p.few_per_place);
+        else hipLaunchKernelGGL((JoinFew<A, L, false, kScored>), grid, block, 0, s, p.few, p.few_per_row, p.few_per_place);
+    } else {
+        if (by_worker) hipLaunchKernelGGL((JoinBoth<A, L, true, kScored>), grid, block, 0, s, p);
+        else hipLaunchKernelGGL((JoinBoth<A, L, false, kScored>), grid, block, 0, s, p);
+    }
+}
+template <bool kScored>
+mlk_status LaunchJoin(const RaggedParams* few, const RaggedParams* tile, int32_t type, hipStream_t s) {
+    const bool narrow = JoinGroups(few != nullptr ? *few : *tile) == 8;
+    if (type == MLK_F32) (narrow ? StartJoin<F32, 32, kScored> : StartJoin<F32, 64, kScored>)(few, tile, s);
+    else if (type == MLK_F16) (narrow ? StartJoin<F16, 32, kScored> : StartJoin<F16, 64, kScored>)(few, tile, s);
+    else (narrow ? StartJoin<BF16, 32, kScored> : StartJoin<BF16, 64, kScored>)(few, tile, s);
+    return CheckLaunch("Join");
 }
 
 // ------------------------------------------------------------ the kernels' launches
@@ -488,25 +531,13 @@ mlk_status AttendAs(const AttendArgs& a) {
         return Fail(MLK_ERR_INVALID, "attention: %lld workgroups exceed a call's 2^35",
                     static_cast<long long>(blocks));
     }
-    if (plan.few_rows > 0) {
-        mlk_status st = LaunchFew<kScored>(few, a.type, a.cache_type, a.stream);
-        if (st == MLK_OK && few.workers > 0) {
-            st = a.type == MLK_F32   ? LaunchJoinFew<F32, kScored>(few, a.stream)
-                 : a.type == MLK_F16 ? LaunchJoinFew<F16, kScored>(few, a.stream)
-                                     : LaunchJoinFew<BF16, kScored>(few, a.stream);
-        }
-        if (st != MLK_OK) return st;
-    }
-    if (plan.tile) {
-        mlk_status st = LaunchTile<kScored>(tile, a.type, a.cache_type, a.stream);
-        if (st == MLK_OK && tile.n_chunks > 1) {
-            st = a.type == MLK_F32   ? LaunchJoinTile<F32, kScored>(tile, a.stream)
-                 : a.type == MLK_F16 ? LaunchJoinTile<F16, kScored>(tile, a.stream)
-                                     : LaunchJoinTile<BF16, kScored>(tile, a.stream);
-        }
-        return st;
-    }
-    return MLK_OK;
+    mlk_status st = MLK_OK;
+    if (plan.few_rows > 0) st = LaunchFew<kScored>(few, a.type, a.cache_type, a.stream);
+    if (plan.tile && st == MLK_OK) st = LaunchTile<kScored>(tile, a.type, a.cache_type, a.stream);
+    if (st != MLK_OK) return st;
+    const bool join_few = plan.few_rows > 0 && few.workers > 0, join_tile = plan.tile && tile.n_chunks > 1;
+    if (!join_few && !join_tile) return MLK_OK;
+    return LaunchJoin<kScored>(join_few ? &few : nullptr, join_tile ? &tile : nullptr, a.type, a.stream);
 }
 
 mlk_status Attend(const AttendArgs& a) { return AttendAs<false>(a); }
