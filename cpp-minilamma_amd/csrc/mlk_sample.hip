@@ -5,26 +5,34 @@
 // with w_i = exp((x_i - x_1) / T) and C_n = w_1 + .. + w_n, the tokens kept are the
 // first n = max(1, min(n_k, n_p, n_m)), and the one chosen is the first with C_i >
 // u C_n.  Each cut, and the choice itself, is the place in that order where a count
-// or a sum crosses a bound.  A row is not sorted for it: bins of 1/16 of a
-// temperature (b = rint(16 x / T), whatever the row's maximum is) say in which bin
-// each bound is crossed, and only that bin's elements, or the few above the last
-// cut, are put in order.
+// or a sum crosses a bound.  A row is not sorted for it: bins of 1/32 of a
+// temperature (b = rint(32 x / T), whatever the row's maximum is) say in which bin
+// each bound is crossed, and only the elements of those bins are looked at again.
 //
-// Bins (one read of the logits, many workgroups a row): every wave has a histogram of
-// its own in shared memory, a ring of the 512 bins up to the largest it has met (32
-// temperatures; what drops out weighs below 2^-46 of the row's largest), so nothing
-// waits for the maximum.  A weight is kept relative to its bin's middle, exp(f / 16)
-// with |f| <= 1/2: a polynomial of degree 6 in float64 (Taylor's, within 2^-47), as a
-// whole number of 2^-42.  Sums of whole numbers depend on no order: the row's bins
-// are the same for every division of the work.  Rows with a top-k count instead, and
-// evaluate no weights.  The largest of every 128 bytes is noted for the second pass.
+// SampleBins (the one read of all logits, up to kMaxParts workgroups a row): every wave
+// has a histogram of its own in shared memory, a ring of the 1024 bins up to the largest
+// it has met (32 temperatures; what drops out weighs below 2^-45 of the row's largest), so
+// nothing waits for the maximum.  A weight is kept relative to its bin's middle, exp(f / 32)
+// with |f| <= 1/2: a polynomial of degree 5 in float64 (Taylor's, within 2^-45), as a
+// whole number of 2^-42.  Sums of whole numbers depend on no order: a row's bins, and so its
+// token, are the same for every division of the work and every batch.  Rows with a top-k
+// count instead, and evaluate no weights.  The largest of every 128 bytes is noted.
 //
-// Choice (one workgroup a row): the parts' bins are added, a scan over the 512 finds
-// the bins where the bounds are crossed, and the elements of those bins are gathered
-// (128 bytes are read again only if their largest lies in the bins looked for),
-// sorted in shared memory, and their sums scanned.  Bins of too many elements for that (nearly
-// equal logits, high temperatures) are narrowed by the digits of the order's key
-// (logit bits, then index), pass by pass over the row.
+// SampleChoose, kCuts (a workgroup a row): the parts' bins are added and scanned, which gives
+// the bins where the bounds are crossed.  SampleGather (many a row): the logits of those bins
+// into a list; 128 bytes are read again only if their largest reaches the lowest bin looked
+// for.  SampleChoose, kFinish (a workgroup a row): where the list is all that can be kept and
+// no longer than kFewAll, it is put in order by comparison and every cut is a count; else
+// the crossing is found in its bin by 1024 equal ranges of the bin, then (equal logits) of the
+// keys.  A bin of more elements than the list holds (nearly equal logits, high temperatures)
+// is narrowed by the digits of the order's key (logit bits, then index), pass by pass over
+// the row.  Rows of up to kList logits are one launch, kSmall, with everything in the list.
+//
+// What bounds it: 512 fp32 rows of 128256 of mixed settings (263 MB, 54 us at a copy's rate)
+// 133 us: SampleBins 74 (with a top-k, or at temperature 0, 55: the bytes; weights cost
+// the rest, float64 and additions in shared memory), cuts 8, gather 29, finish 14.  64 bf16
+// rows 59 us, one fp32 row 32, 6 fp32 rows of 131 7: four launches, one for small rows,
+// each a chain of loads, scans and barriers.
 #include "mlk_paged.h"
 
 #include <cmath>
@@ -64,14 +72,14 @@ constexpr int64_t kPartBytes = sizeof(Part) + kBins * 8;
 
 // What the second pass leaves of a row for the two that follow, then the kBins masses (or
 // counts) of its bins, then kList keys.
-struct RowState {
+struct RowState {  // 48 bytes
     int32_t top;     // its largest bin
     float largest;   // logit
     float al, ah, bl, bh;  // logits to gather: al .. ah and bl .. bh
     uint32_t live;   // kChosen: its token is; kAll: what is gathered is all that can be kept
     uint32_t n;      // how many were gathered
     uint64_t reach;  // the sum that top-p asks for; with a top-k, 0: it follows from that
-    uint64_t unused;
+    uint64_t unused;  // (whole 16 bytes)
 };
 constexpr uint32_t kChosen = 0, kLive = 1, kAll = 2;
 constexpr int64_t kStateBytes = sizeof(RowState) + kBins * 8 + kList * 8;
