@@ -26,13 +26,15 @@
 // the crossing is found in its bin by 1024 equal ranges of the bin, then (equal logits) of the
 // keys.  A bin of more elements than the list holds (nearly equal logits, high temperatures)
 // is narrowed by the digits of the order's key (logit bits, then index), pass by pass over
-// the row.  Rows of up to kList logits are one launch, kSmall, with everything in the list.
+// the row.  Of few rows the three are one launch, kOneLaunch, in which every workgroup of the
+// gathering adds up the bins for itself and the one that ends last finishes.  Rows of up to
+// kList logits are one launch alone, kSmall, with everything in the list.
 //
-// What bounds it: 512 fp32 rows of 128256 of mixed settings (263 MB, 54 us at a copy's rate)
-// 133 us: SampleBins 74 (with a top-k, or at temperature 0, 55: the bytes; weights cost
-// the rest, float64 and additions in shared memory), cuts 8, gather 29, finish 14.  64 bf16
-// rows 59 us, one fp32 row 32, 6 fp32 rows of 131 7: four launches, one for small rows,
-// each a chain of loads, scans and barriers.
+// What bounds it: 512 fp32 rows of 128256 of mixed settings (263 MB, 56 us at a copy's rate)
+// 127 us: SampleBins 71 (with a top-k, or at temperature 0, 55: the bytes; weights cost
+// the rest, float64 and additions in shared memory), cuts 8, gather 33, finish 20, as each takes
+// by itself.  64 bf16 rows 58 us, one fp32 row 28, 6 fp32 rows of 131 7: a few launches, each a
+// chain of loads, scans and barriers.
 #include "mlk_paged.h"
 
 #include <cmath>
@@ -79,7 +81,8 @@ struct RowState {  // 48 bytes
     uint32_t live;   // kChosen: its token is; kAll: what is gathered is all that can be kept
     uint32_t n;      // how many were gathered
     uint64_t reach;  // the sum that top-p asks for; with a top-k, 0: it follows from that
-    uint64_t unused;  // (whole 16 bytes)
+    uint32_t done;   // kOneLaunch: workgroups of the row that have gathered theirs
+    uint32_t unused;  // (whole 16 bytes)
 };
 constexpr uint32_t kChosen = 0, kLive = 1, kAll = 2;
 constexpr int64_t kStateBytes = sizeof(RowState) + kBins * 8 + kList * 8;
@@ -239,6 +242,11 @@ __global__ __launch_bounds__(kThreads) void SampleBins(const SampleArgs p) {
     const int part = static_cast<int>(blockIdx.x % p.parts);
     const How h = HowOf(p, row);
     if (h.bad) return;  // the second pass sees that too
+    if (part == 0 && tid == 0) {
+        RowState* state = reinterpret_cast<RowState*>(p.state + row * kStateBytes);
+        state->n = 0;
+        state->done = 0;
+    }
     const RowUnits<T> r(p, row);
     const int32_t units = r.Units(), blocks = (units + kWave - 1) / kWave;
     const int32_t b0 = static_cast<int32_t>(static_cast<int64_t>(blocks) * part / p.parts);
@@ -800,15 +808,99 @@ __device__ inline uint64_t Reach(float p, uint64_t sum) {
     return x > 1.0 ? static_cast<uint64_t>(x) : 1;
 }
 
+// The row's logits in the two spans of `at`, in any order, into `found` (of more than kList not
+// all); *n_found: how many.  8 lanes to each 128 bytes whose largest is no lower; a wave looks at
+// 64 kLook segments.  `hits`: room for 64 kLook a wave.
+template <typename T, int kLook>
+__device__ inline void GatherPart(const RowUnits<T>& r, const float* largest, int part, const RowState& at,
+                                  uint64_t* found, uint16_t* hits_of, uint32_t* n_found) {
+    constexpr int E = RowUnits<T>::E, kGroups = kWave / kSegment, kRounds = 32 / E;
+    const int lane = static_cast<int>(threadIdx.x) % kWave;
+    const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / kWave);
+    const int32_t units = r.Units(), segments = (units + kSegment - 1) / kSegment;
+    uint16_t* hit_segment = hits_of + wave * kLook * kWave;
+    const int32_t s0 = (part * kChooseWaves + wave) * kLook * kWave + lane;
+    float m[kLook];
+#pragma unroll
+    for (int l = 0; l < kLook; ++l) m[l] = s0 + l * kWave < segments ? largest[s0 + l * kWave] : -INFINITY;
+    if (threadIdx.x == 0) *n_found = 0;
+    __syncthreads();
+    const float al = at.al, ah = at.ah, bl = at.bl, bh = at.bh, low = fminf(al, bl);
+    int n = 0;
+#pragma unroll
+    for (int l = 0; l < kLook; ++l) {
+        const bool hit = m[l] >= low;
+        const uint64_t mask = __ballot(hit);
+        if (hit) hit_segment[n + __popcll(mask & ((uint64_t{1} << lane) - 1))] = static_cast<uint16_t>(s0 + l * kWave);
+        n += __popcll(mask);
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    for (int g = 0; g < n; g += kGroups * kRounds) {
+        u32x4 raw[kRounds];
+        int32_t unit[kRounds];
+#pragma unroll
+        for (int i = 0; i < kRounds; ++i) {
+            const int j = g + i * kGroups + lane / kSegment;
+            unit[i] = j < n ? hit_segment[j] * kSegment + lane % kSegment : units;
+            raw[i] = r.Load(unit[i], unit[i] < units);
+        }
+        uint32_t hits = 0;
+#pragma unroll
+        for (int i = 0; i < kRounds; ++i) {
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                const float x = r.Get(raw[i], e);
+                const bool in = (x >= al && x <= ah) || (x >= bl && x <= bh);
+                hits |= in ? 1u << (i * E + e) : 0u;
+            }
+        }
+        if (__ballot(hits != 0) == 0) continue;
+        // places for the wave's hits: one addition for all
+        const uint32_t mine = __popc(hits);
+        uint32_t upto = mine;
+#pragma unroll
+        for (int off = 1; off < kWave; off *= 2) {
+            const uint32_t o = __shfl_up(upto, off, kWave);
+            if (lane >= off) upto += o;
+        }
+        uint32_t to = 0;
+        if (lane == kWave - 1) to = atomicAdd(n_found, upto);
+        to = __builtin_amdgcn_readlane(to, kWave - 1) + upto - mine;
+#pragma unroll
+        for (int i = 0; i < kRounds; ++i) {
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                if (hits >> (i * E + e) & 1) {
+                    if (to < kList) found[to] = Key(r.Get(raw[i], e), r.Index(unit[i], e));
+                    ++to;
+                }
+            }
+        }
+    }
+    __syncthreads();
+}
+
+// What a workgroup found, behind what others have put there: one addition to the row's count.
+__device__ inline void AddToList(RowState* state, const uint64_t* found, uint32_t total, uint32_t* base) {
+    uint64_t* list = reinterpret_cast<uint64_t*>(state + 1) + kBins;
+    if (total == 0) return;
+    if (threadIdx.x == 0) *base = atomicAdd(&state->n, total);
+    __syncthreads();
+    for (uint32_t i = threadIdx.x; i < total && *base + i < kList; i += kChooseThreads) list[*base + i] = found[i];
+}
+
 // The passes after the first.  kCuts: which logits to gather; kFinish: the choice from what was
-// gathered; kSmall: the choice from a row that the list holds whole, without any of the others.
-enum Pass { kCuts, kFinish, kSmall };
+// gathered; kOneLaunch: these and the gathering between them, by as many workgroups as gather,
+// each of which finds the cuts for itself; the last to have gathered goes on; kSmall: the choice
+// from a row that the list holds whole, without any of the others.
+enum Pass { kCuts, kFinish, kOneLaunch, kSmall };
 
 template <typename T, Pass kPass_>
-__global__ __launch_bounds__(kChooseThreads) void SampleChoose(const SampleArgs p) {
+__global__ __launch_bounds__(kChooseThreads) void SampleChoose(const SampleArgs p, int gather_parts) {
     __shared__ Choice s;
     const int tid = static_cast<int>(threadIdx.x);
-    const int64_t row = blockIdx.x;
+    const int64_t row = kPass_ == kOneLaunch ? blockIdx.x / gather_parts : blockIdx.x;
+    const int gather_part = kPass_ == kOneLaunch ? static_cast<int>(blockIdx.x % gather_parts) : 0;
     const How h = HowOf(p, row);
     const RowUnits<T> units(p, row);
     RowState* state = reinterpret_cast<RowState*>(p.state + row * kStateBytes);
@@ -829,7 +921,7 @@ __global__ __launch_bounds__(kChooseThreads) void SampleChoose(const SampleArgs 
         largest = at.largest;
         all_held = at.live == kAll && at.n <= kFewAll;
         row_reach = at.reach;
-    } else if constexpr (kPass_ == kCuts) {
+    } else if constexpr (kPass_ == kCuts || kPass_ == kOneLaunch) {
         // lane i of each wave: part i
         const char* parts = p.part + row * p.parts * kPartBytes;
         static_assert(kMaxParts <= kWave, "a lane a part");
@@ -869,7 +961,7 @@ __global__ __launch_bounds__(kChooseThreads) void SampleChoose(const SampleArgs 
 #pragma unroll
                 for (int e = 0; e < kEach; ++e) {
                     s.bin[tid + e * kChooseThreads] = sum[e];
-                    state_bin[tid + e * kChooseThreads] = sum[e];
+                    if (kPass_ == kCuts) state_bin[tid + e * kChooseThreads] = sum[e];
                 }
             }
         }
@@ -901,7 +993,7 @@ __global__ __launch_bounds__(kChooseThreads) void SampleChoose(const SampleArgs 
         const bool none = h.bad || flags != kSome;
         if (kPass_ == kCuts && tid == 0) state->live = none || h.t == 0.0f ? kChosen : kLive;
         if (none || h.t == 0.0f) {
-            if (tid == 0) {
+            if (tid == 0 && gather_part == 0) {
                 p.tokens[row] = none ? -1 : static_cast<int32_t>(best);
                 if (p.prob != nullptr) p.prob[row] = none ? 0.0f : 1.0f;
                 if (none) RaiseFlag(p.err, 1);
@@ -921,10 +1013,9 @@ __global__ __launch_bounds__(kChooseThreads) void SampleChoose(const SampleArgs 
         }
     }
     __syncthreads();
-    if (kPass_ != kCuts && all_held) {
-        // all that can be kept is in the list, an element a thread: in order by comparison with all
-        // others, and every cut is a count
-        const int n = kPass_ == kSmall ? p.vocab : static_cast<int>(state->n);
+    // Where all that can be kept is in the list and few, an element a thread: in order by comparison
+    // with all others, and every cut is a count.
+    auto in_order = [&](int n) {
         uint64_t key = kNoKey, w = 0;
         if (tid < n) {
             key = kPass_ == kSmall ? s.list[tid] : state_list[tid];
@@ -968,6 +1059,9 @@ __global__ __launch_bounds__(kChooseThreads) void SampleChoose(const SampleArgs 
             p.tokens[row] = static_cast<int32_t>(s.list[kFewAll + tid]);
             if (p.prob != nullptr) p.prob[row] = static_cast<float>(static_cast<double>(w) / static_cast<double>(whole));
         }
+    };
+    if (kPass_ != kCuts && all_held) {
+        in_order(kPass_ == kSmall ? p.vocab : static_cast<int>(state->n));
         return;
     }
     // Three places are looked for in turn, each where its cut is asked for: the top-k's, the
@@ -982,7 +1076,7 @@ __global__ __launch_bounds__(kChooseThreads) void SampleChoose(const SampleArgs 
     bool by_p = h.p < 1.0f, by_m = h.m > 0.0f;
     Span m{0, 0};
     int p_bin = 0;
-    bool first = true;
+    bool first = true, whole_list = false;
 #pragma unroll 1
     for (int what = h.k != 0 ? kTopK : kTopP; what <= kToken; ++what) {
         Span a, b;      // bins to gather, if there is no list
@@ -1043,7 +1137,7 @@ __global__ __launch_bounds__(kChooseThreads) void SampleChoose(const SampleArgs 
             a = b = {bin, bin};
         }
         bool whole = true;  // the list serves the places looked for later too
-        if constexpr (kPass_ == kCuts) {
+        if ((kPass_ == kCuts || kPass_ == kOneLaunch) && first) {
             bool is_all = a.lo == 0;
             if (what == kTopP) {  // whether all up to the last bin are few
                 uint64_t mass = 0, all;
@@ -1052,21 +1146,43 @@ __global__ __launch_bounds__(kChooseThreads) void SampleChoose(const SampleArgs 
                 is_all = static_cast<double>(all) * (1 / (0.984 * kOne)) < 0.9 * kFewAll;
                 if (is_all) a = b = {0, last};
             }
-            if (tid == 0) {
-                *state = {top, largest, ch.Lowest(a.hi), ch.Highest(a.lo), ch.Lowest(b.hi), ch.Highest(b.lo), is_all ? kAll : kLive, 0,
-                          what == kTopP ? reach : 0, 0};
+            const RowState at{top, largest, ch.Lowest(a.hi), ch.Highest(a.lo), ch.Lowest(b.hi), ch.Highest(b.lo), is_all ? kAll : kLive, 0,
+                              what == kTopP ? reach : 0, 0, 0};
+            if constexpr (kPass_ == kCuts) {
+                if (tid == 0) *state = at;
+                return;
             }
-            return;
+            GatherPart<T, 1>(units, ch.largest, gather_part, at, s.list, s.some, &s.n_list);
+            AddToList(state, s.list, s.n_list, &s.n_few);
+            __syncthreads();  // (one thread's release and acquire then are the workgroup's)
+            if (tid == 0) {
+                s.n_few = __hip_atomic_fetch_add(&state->done, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) + 1;
+                s.n_list = __hip_atomic_load(&state->n, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            }
+            __syncthreads();
+            if (s.n_few != static_cast<uint32_t>(gather_parts)) return;
+            n = static_cast<int>(s.n_list);
+            if (is_all) {
+                row_reach = at.reach;
+                if (n <= kFewAll) {
+                    in_order(n);
+                    return;
+                }
+            }
+            whole_list = is_all;
         }
-        if (kPass_ == kFinish && first) {  // what was gathered for this
+        if ((kPass_ == kFinish || kPass_ == kOneLaunch) && first) {  // what was gathered for this
             first = false;
-            n = static_cast<int>(state->n);
+            if constexpr (kPass_ == kFinish) {
+                n = static_cast<int>(state->n);
+                whole_list = state->live == kAll;
+            }
 #pragma unroll 4
             for (int i = tid; i < (n < kList ? n : kList); i += kChooseThreads) ch.PutInList(i, state_list[i]);
             __syncthreads();
             if (n > kList) n = -1;
             whole = !(what == kTopK && a.lo != 0);
-            if (what == kTopP && state->live == kAll) whole = true;
+            if (what == kTopP && whole_list) whole = true;
         }
         if (n < 0 && look) {
             n = ch.Gather(bin);
@@ -1116,92 +1232,19 @@ __global__ __launch_bounds__(kChooseThreads) void SampleChoose(const SampleArgs 
     }
 }
 
-// Between kCuts and kFinish: the row's logits in the two spans found, in any order, 8 lanes to
-// each 128 bytes whose largest is no lower.  A wave looks at 64 kLook segments.
-constexpr int kGatherThreads = 256;
+// Between kCuts and kFinish: what a row's workgroup finds goes to the row's list.
 template <typename T, int kLook>
-__global__ __launch_bounds__(kGatherThreads) void SampleGather(const SampleArgs p, int parts) {
-    constexpr int E = RowUnits<T>::E, kGroups = kWave / kSegment, kRounds = 32 / E;
-    __shared__ uint64_t found[kList];  // (of more the row's list is of no use)
-    __shared__ int32_t hits_of[kGatherThreads / kWave][kLook * kWave];
+__global__ __launch_bounds__(kChooseThreads) void SampleGather(const SampleArgs p, int parts) {
+    __shared__ uint64_t found[kList];
+    __shared__ uint16_t hits[kChooseWaves * kLook * kWave];
     __shared__ uint32_t n_found, base;
-    const int lane = static_cast<int>(threadIdx.x) % kWave;
-    const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / kWave);
     const int64_t row = blockIdx.x / parts;
     const int part = static_cast<int>(blockIdx.x % parts);
     RowState* state = reinterpret_cast<RowState*>(p.state + row * kStateBytes);
-    uint64_t* list = reinterpret_cast<uint64_t*>(state + 1) + kBins;
-    const float* largest = p.largest + row * p.segments;
-    const RowUnits<T> r(p, row);
-    const int32_t units = r.Units(), segments = (units + kSegment - 1) / kSegment;
-    int32_t* hit_segment = hits_of[wave];
-    const int32_t s0 = (part * (kGatherThreads / kWave) + wave) * kLook * kWave + lane;
-    float m[kLook];
-#pragma unroll
-    for (int l = 0; l < kLook; ++l) m[l] = s0 + l * kWave < segments ? largest[s0 + l * kWave] : -INFINITY;
     const RowState at = *state;
     if (at.live == kChosen) return;
-    if (threadIdx.x == 0) n_found = 0;
-    __syncthreads();
-    const float al = at.al, ah = at.ah, bl = at.bl, bh = at.bh, low = fminf(al, bl);
-    int n = 0;
-#pragma unroll
-    for (int l = 0; l < kLook; ++l) {
-        const bool hit = m[l] >= low;
-        const uint64_t mask = __ballot(hit);
-        if (hit) hit_segment[n + __popcll(mask & ((uint64_t{1} << lane) - 1))] = s0 + l * kWave;
-        n += __popcll(mask);
-    }
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    for (int g = 0; g < n; g += kGroups * kRounds) {
-        u32x4 raw[kRounds];
-        int32_t unit[kRounds];
-#pragma unroll
-        for (int i = 0; i < kRounds; ++i) {
-            const int j = g + i * kGroups + lane / kSegment;
-            unit[i] = j < n ? hit_segment[j] * kSegment + lane % kSegment : units;
-            raw[i] = r.Load(unit[i], unit[i] < units);
-        }
-        uint32_t hits = 0;
-#pragma unroll
-        for (int i = 0; i < kRounds; ++i) {
-#pragma unroll
-            for (int e = 0; e < E; ++e) {
-                const float x = r.Get(raw[i], e);
-                const bool in = (x >= al && x <= ah) || (x >= bl && x <= bh);
-                hits |= in ? 1u << (i * E + e) : 0u;
-            }
-        }
-        if (__ballot(hits != 0) == 0) continue;
-        // places for the wave's hits: one addition for all
-        const uint32_t mine = __popc(hits);
-        uint32_t upto = mine;
-#pragma unroll
-        for (int off = 1; off < kWave; off *= 2) {
-            const uint32_t o = __shfl_up(upto, off, kWave);
-            if (lane >= off) upto += o;
-        }
-        uint32_t at = 0;
-        if (lane == kWave - 1) at = atomicAdd(&n_found, upto);
-        at = __builtin_amdgcn_readlane(at, kWave - 1) + upto - mine;
-#pragma unroll
-        for (int i = 0; i < kRounds; ++i) {
-#pragma unroll
-            for (int e = 0; e < E; ++e) {
-                if (hits >> (i * E + e) & 1) {
-                    if (at < kList) found[at] = Key(r.Get(raw[i], e), r.Index(unit[i], e));
-                    ++at;
-                }
-            }
-        }
-    }
-    // one addition to the row's count for the workgroup
-    __syncthreads();
-    const uint32_t total = n_found;
-    if (total == 0) return;
-    if (threadIdx.x == 0) base = atomicAdd(&state->n, total);
-    __syncthreads();
-    for (uint32_t i = threadIdx.x; i < total && base + i < kList; i += kGatherThreads) list[base + i] = found[i];
+    GatherPart<T, kLook>(RowUnits<T>(p, row), p.largest + row * p.segments, part, at, found, hits, &n_found);
+    AddToList(state, found, n_found, &base);
 }
 
 // Workgroups of the first pass a row: as many as fill the device at 2 a compute unit,
@@ -1219,7 +1262,7 @@ int64_t Segments(int64_t vocab, int bytes) {  // one more where the row is not a
 }
 // Workgroups of the gather a row.
 int GatherParts(int64_t vocab, int bytes, int look) {
-    const int each = kGatherThreads * look;
+    const int each = kChooseThreads * look;
     return static_cast<int>((Segments(vocab, bytes) + each - 1) / each);
 }
 
@@ -1239,7 +1282,7 @@ mlk_status Launch(SampleArgs p, int64_t n_rows, char* workspace, hipStream_t s) 
         const int64_t rows = n_rows - from < most ? n_rows - from : most;
         const dim3 grid(static_cast<unsigned>(rows));
         if (p.vocab <= kList) {
-            hipLaunchKernelGGL((SampleChoose<T, kSmall>), grid, block, 0, s, p);
+            hipLaunchKernelGGL((SampleChoose<T, kSmall>), grid, block, 0, s, p, 1);
         } else {
             p.parts = Parts(rows, p.vocab, kBytes);
             p.segments = static_cast<int32_t>((Segments(p.vocab, kBytes) + 3) / 4 * 4);
@@ -1247,15 +1290,23 @@ mlk_status Launch(SampleArgs p, int64_t n_rows, char* workspace, hipStream_t s) 
             p.part = p.state + rows * kStateBytes;
             p.largest = reinterpret_cast<float*>(p.part + rows * p.parts * kPartBytes);
             hipLaunchKernelGGL(SampleBins<T>, dim3(static_cast<unsigned>(rows * p.parts)), dim3(kThreads), 0, s, p);
-            hipLaunchKernelGGL((SampleChoose<T, kCuts>), grid, block, 0, s, p);
-            // where those of one look are more than the device holds at once (5 a compute unit), of
-            // four (512 fp32 rows of top-k: 36 us, with four 9)
-            const bool many = rows * GatherParts(p.vocab, kBytes, 1) > 5 * ComputeUnits();
-            const int parts = GatherParts(p.vocab, kBytes, many ? 4 : 1);
-            const dim3 gather(static_cast<unsigned>(rows * parts)), threads(kGatherThreads);
-            if (!many) hipLaunchKernelGGL((SampleGather<T, 1>), gather, threads, 0, s, p, parts);
-            else hipLaunchKernelGGL((SampleGather<T, 4>), gather, threads, 0, s, p, parts);
-            hipLaunchKernelGGL((SampleChoose<T, kFinish>), grid, block, 0, s, p);
+            const int looks = GatherParts(p.vocab, kBytes, 1);
+            // as long as each compute unit has one workgroup of it (fp32 rows of 128256: 1 row 32.2 us by
+            // the three launches, 27.7 by one, 16 rows 39.6 and 37.4, 32 rows 43.8 and 45.9; bf16,
+            // half the bytes: 32 rows 53.1 and 50.9, 64 rows 58.0 and 59.2)
+            if (rows * looks <= ComputeUnits()) {
+                hipLaunchKernelGGL((SampleChoose<T, kOneLaunch>), dim3(static_cast<unsigned>(rows * looks)), block, 0, s, p, looks);
+            } else {
+                hipLaunchKernelGGL((SampleChoose<T, kCuts>), grid, block, 0, s, p, 1);
+                // where those of one look are more than the device holds at once (5 a compute unit), of
+                // four (512 fp32 rows of top-k: 36 us, with four 9)
+                const bool many = rows * looks > 5 * ComputeUnits();
+                const int parts = GatherParts(p.vocab, kBytes, many ? 4 : 1);
+                const dim3 gather(static_cast<unsigned>(rows * parts));
+                if (!many) hipLaunchKernelGGL((SampleGather<T, 1>), gather, block, 0, s, p, parts);
+                else hipLaunchKernelGGL((SampleGather<T, 4>), gather, block, 0, s, p, parts);
+                hipLaunchKernelGGL((SampleChoose<T, kFinish>), grid, block, 0, s, p, 1);
+            }
         }
         const mlk_status st = CheckLaunch("SampleChoose");
         if (st != MLK_OK) return st;

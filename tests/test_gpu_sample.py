@@ -294,6 +294,31 @@ def test_a_rows_choice_does_not_depend_on_the_others(mlk, sampling, act):
         np.testing.assert_array_equal(p.view(np.uint32), all_p[some].view(np.uint32))
 
 
+@pytest.mark.parametrize("act", ["f32", "bf16"])
+def test_hard_rows_choose_alike_in_large_and_small_batches(mlk, sampling, act):
+    """Rows of equal, few, masked and cut-off logits, 30 at a time and all at once: the
+    same tokens and bits, those of the definition where it is clear."""
+    rng = np.random.default_rng(14)
+    V = 20001
+    hard = np.stack([
+        np.full(V, 1.5, np.float32), np.full(V, -30000.0, np.float32),
+        rng.integers(-3, 3, V).astype(np.float32), rng.integers(0, 2, V).astype(np.float32) * 40,
+        np.where(rng.random(V) < 0.9, -np.inf, rng.standard_normal(V)).astype(np.float32),
+        np.where(np.arange(V) == 17, 0.0, -np.inf).astype(np.float32), np.full(V, -np.inf, np.float32),
+        rng.standard_normal(V).astype(np.float32) * 1e-5, logits(rng, 1, V, 0.3)[0],
+        rng.standard_normal(V).astype(np.float32) * 1000])
+    x = np.repeat(hard, len(MIX), axis=0)
+    x = np.concatenate([x, x])
+    how = mixed(rng, len(x))
+    all_t, all_p, flag = run(mlk, sampling, x, how, act)
+    assert flag != 0  # of the rows that have no logit
+    for a in range(0, len(x), 30):
+        t, p, _ = run(mlk, sampling, x[a:a + 30], how[a:a + 30], act)
+        np.testing.assert_array_equal(t, all_t[a:a + 30])
+        np.testing.assert_array_equal(p.view(np.uint32), all_p[a:a + 30].view(np.uint32))
+    check(x[:170], how[:170], (all_t[:170], all_p[:170], flag), act, 0.3)
+
+
 def test_large_and_far_apart_logits(mlk, sampling):
     """Logits of 10^4 and beyond, all far below 0, spread over 10^5 temperatures."""
     rng = np.random.default_rng(11)
