@@ -39,10 +39,9 @@
 // Instances: head_dim 64, 128 and 256; another runs on the next one, padded.
 // kScored: with score functions and masks (mlk_attention_scores).  Positions before the first
 // that a sequence's tokens see are no one's work; the scores are capped and biased as they
-// leave the products (bytes bound the kernel still: 64 bf16 sequences of 8B heads, 1.09 GB, 191 us, capped
-// 196, 5.6 TB/s; 256 sequences of one token with a window of 1024, 115 MB with what else the
-// batch has, 35: the share of each worker is 1 or 2 tiles, and what it waits for is page,
-// row and join in turn).
+// leave the products (bytes bound the kernel still: 64 bf16 sequences of 8B heads, 1.09 GB, 196 us capped, 5.6
+// TB/s; 18 fp32 over fp16 sequences with a window of 1000, 74 MB, 35 us: a wave has
+// two or three tiles, and waits for length, page and rows in turn before the first).
 #pragma once
 
 #include "mlk_ragged.h"
