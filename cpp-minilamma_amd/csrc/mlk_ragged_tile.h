@@ -32,7 +32,7 @@
 // kScored: with score functions and masks.  A tile's positions run from the first that any of
 // its rows sees (chunks from what the window alone leaves, so that the join knows them);
 // waves pass over tiles of positions that none of their rows sees.  7001 bf16 tokens of 70B
-// heads in documents (120 GFLOP of what the masks leave): 253 us, capped or not, and 190 to
+// heads in documents (120 GFLOP of what the masks leave): 252 us, 214 without the cap, and 190 to
 // 232 as the plain kernel's own sequences: tiles of 256 rows (32 tokens) across an edge of
 // documents take both in.
 #pragma once

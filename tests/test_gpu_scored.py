@@ -228,6 +228,32 @@ def test_many_sequences(mlk, paged):
         check(batch, pages.of, masks, q, got, H, hd, "bf16", rows=set(rng.integers(0, batch.T, 60)))
 
 
+@pytest.mark.parametrize("act,ct", PAIRS)
+@pytest.mark.parametrize("ones", [7, 600])
+def test_chunks_beside_single_tokens(mlk, paged, ones, act, ct):
+    """Both kinds of rows with parts to join, in batches of fewer and of more sequences than
+    workers; the plain entry over the same ones."""
+    H, KV, hd = 8, 2, 64
+    rng = np.random.default_rng(15)
+    counts = [1] * ones + [130] + [1] * ones
+    lens = [int(n) for n in rng.integers(600 if ones == 7 else 1, 2000 if ones == 7 else 700, 2 * ones + 1)]
+    lens[ones] = 1900
+    batch = Batch(counts, lens, 32)
+    pages = Pages(mlk, paged, batch, KV, hd, ct, rng)
+    q = to_type(rng.standard_normal((batch.T, H, hd)), act)
+    rows = set(rng.integers(0, batch.T, 20)) | {ones, ones + 64, ones + 129}
+    for kw in (dict(window=1000, cap=10.0), dict(bias=True, prefix="random")):
+        masks = Masks(batch, H, **kw)
+        got = run_paged(mlk, paged, batch, pages, masks, q, H, act)
+        check(batch, pages.of, masks, q, got, H, hd, act, rows=rows)
+    dev = batch.device(mlk, paged)
+    out = mlk.DeviceBuffer.from_array(np.full((batch.T, H, hd), 7, NP[act]))
+    ws = mlk.DeviceBuffer(max(paged.attention_workspace_bytes(pages.handle, dev, H, act), 16), np.uint8)
+    paged.attention(pages.handle, dev, mlk.DeviceBuffer.from_array(q), out, H, act, workspace=ws)
+    mlk.synchronize()
+    check(batch, pages.of, Masks(batch, H), q, out.download(), H, hd, act, rows=rows)
+
+
 # ------------------------------------------------------------------ packed
 
 def run_packed(mlk, paged, batch, masks, q, k, v, H, KV, hd, act, strides=(None,) * 3,
