@@ -21,7 +21,7 @@
 // SampleChoose, kCuts (a workgroup a row): the parts' bins are added and scanned, which gives
 // the bins where the bounds are crossed.  SampleGather (many a row): the logits of those bins
 // into a list; 128 bytes are read again only if their largest reaches the lowest bin looked
-// for.  SampleChoose, kFinish (a workgroup a row): where the list is all that can be kept and
+// for.  SampleChoose, kFinish (a workgroup a row, of twice the threads where rows are few): where the list is all that can be kept and
 // no longer than kFewAll, it is put in order by comparison and every cut is a count; else
 // the crossing is found in its bin by 1024 equal ranges of the bin, then (equal logits) of the
 // keys.  A bin of more elements than the list holds (nearly equal logits, high temperatures)
@@ -33,7 +33,7 @@
 // What bounds it: 512 fp32 rows of 128256 of mixed settings (263 MB, 56 us at a copy's rate)
 // 127 us: SampleBins 71 (with a top-k, or at temperature 0, 55: the bytes; weights cost
 // the rest, float64 and additions in shared memory), cuts 8, gather 33, finish 20, as each takes
-// by itself.  64 bf16 rows 58 us, one fp32 row 28, 6 fp32 rows of 131 7: a few launches, each a
+// by itself.  64 bf16 rows 54 us, one fp32 row 28, 6 fp32 rows of 131 7: a few launches, each a
 // chain of loads, scans and barriers.
 #include "mlk_paged.h"
 
@@ -50,7 +50,7 @@ constexpr int kPerUnit = 32;    // bins of a temperature
 constexpr int kList = 4096;     // elements gathered at once
 constexpr int kFewAll = kChooseThreads;  // of a list that is put in order as a whole
 constexpr int kChunk = 1024;    // segments looked at at once
-constexpr int kEach = kBins / kChooseThreads;  // neighbouring bins a thread has
+constexpr int kWideThreads = 512, kMostWaves = kWideThreads / kWave;  // of kFinish where rows are few
 constexpr int kMaxParts = 48;   // workgroups of a row
 constexpr int64_t kMaxVocab = 1 << 20, kMaxRows = 1 << 20;
 constexpr double kOne = 0x1p42;  // a weight of 1
@@ -378,7 +378,7 @@ __global__ __launch_bounds__(kThreads) void SampleBins(const SampleArgs p) {
 // ------------------------------------------------------------ second pass
 
 // Inclusive sums over the workgroup's threads, in a fixed order; *total over all.
-template <typename V>
+template <int kWaves, typename V>
 __device__ inline V ScanBlock(V v, V* scratch, V* total) {
     const int lane = static_cast<int>(threadIdx.x) % kWave, wave = static_cast<int>(threadIdx.x) / kWave;
 #pragma unroll
@@ -391,7 +391,7 @@ __device__ inline V ScanBlock(V v, V* scratch, V* total) {
     __syncthreads();
     V before = 0, all = 0;
 #pragma unroll
-    for (int i = 0; i < kChooseWaves; ++i) {
+    for (int i = 0; i < kWaves; ++i) {
         if (i == wave) before = all;
         all += scratch[i];
     }
@@ -407,7 +407,7 @@ struct Choice {
     uint16_t some[kList];  // segments to look through; places in the list that a search is left with
     uint64_t few[kWave];
     double edge[2 * kPerUnit];  // exp(-i / kPerUnit), and exp(-i)
-    uint64_t scan_u[kChooseWaves], scan_v[kChooseWaves];
+    uint64_t scan_u[kMostWaves], scan_v[kMostWaves];
     int32_t found[2];
     uint32_t n_list, n_segments, n_few;
     uint64_t word[3];
@@ -427,8 +427,9 @@ struct Span {
     __device__ bool Has(int b) const { return b >= lo && b <= hi; }
 };
 
-template <typename T>
+template <typename T, int kT>  // kT threads
 struct Chooser {
+    static constexpr int kW = kT / kWave, kEach = kBins / kT;  // neighbouring bins a thread has
     const SampleArgs& p;
     const How& h;
     Choice& s;
@@ -494,21 +495,21 @@ struct Chooser {
         __syncthreads();
         if (Tid() == 0) s.n_segments = 0;
         __syncthreads();
-        float m[kChunk / kChooseThreads];
+        float m[kChunk / kT];
 #pragma unroll
-        for (int i = 0; i < kChunk / kChooseThreads; ++i) {
-            const int32_t seg = c0 + i * kChooseThreads + Tid();
+        for (int i = 0; i < kChunk / kT; ++i) {
+            const int32_t seg = c0 + i * kT + Tid();
             m[i] = seg < segments ? largest[seg] : -INFINITY;
         }
 #pragma unroll
-        for (int i = 0; i < kChunk / kChooseThreads; ++i) {
+        for (int i = 0; i < kChunk / kT; ++i) {
             const bool hit = m[i] >= low;
             const uint64_t mask = __ballot(hit);
             if (mask == 0) continue;
             uint32_t at = 0;
             if (Lane() == 0) at = atomicAdd(&s.n_segments, static_cast<uint32_t>(__popcll(mask)));
             at = __builtin_amdgcn_readfirstlane(at) + __popcll(mask & ((uint64_t{1} << Lane()) - 1));
-            if (hit) s.some[at] = static_cast<uint16_t>(i * kChooseThreads + Tid());
+            if (hit) s.some[at] = static_cast<uint16_t>(i * kT + Tid());
         }
         __syncthreads();
         return static_cast<int>(s.n_segments);
@@ -529,14 +530,14 @@ struct Chooser {
     // largest is no lower than those.
     template <typename F>
     __device__ void Near(const Span& span, const F& f) {
-        constexpr int kEach = kSegment * RowUnits<T>::E;  // elements of a segment
+        constexpr int kElements = kSegment * RowUnits<T>::E;  // of a segment
         const float low = Lowest(span.hi), high = Highest(span.lo);
         const int32_t segments = (r.Units() + kSegment - 1) / kSegment;
         for (int32_t c0 = 0; c0 < segments; c0 += kChunk) {
             const int n = Segments(c0, segments, low);
 #pragma unroll 1
-            for (int j = Tid(); j < n * kEach; j += kChooseThreads) {
-                const int32_t i = r.Index((c0 + s.some[j / kEach]) * kSegment, j % kEach);
+            for (int j = Tid(); j < n * kElements; j += kT) {
+                const int32_t i = r.Index((c0 + s.some[j / kElements]) * kSegment, j % kElements);
                 const float x = i >= 0 && i < r.vocab ? T::Get(r.x[i]) : -INFINITY;
                 if (x >= low && x <= high) f(x, i);
             }
@@ -557,7 +558,7 @@ struct Chooser {
     template <typename F>
     __device__ void InList(int n, const Span& span, const F& f) {
 #pragma unroll 2
-        for (int i = Tid(); i < n; i += kChooseThreads) {
+        for (int i = Tid(); i < n; i += kT) {
             const uint32_t code = s.code[i];
             if (!span.Has(static_cast<int>(code / kBins))) continue;
             const uint64_t key = s.list[i];
@@ -583,14 +584,14 @@ struct Chooser {
         }
         __syncthreads();
 #pragma unroll
-        for (int i = 0; i < kChooseWaves; ++i) {
+        for (int i = 0; i < kW; ++i) {
             *lo = s.scan_u[i] < *lo ? s.scan_u[i] : *lo;
             *hi = s.scan_v[i] > *hi ? s.scan_v[i] : *hi;
         }
     }
 
     __device__ void ClearBins() {
-        for (int i = Tid(); i < kBins; i += kChooseThreads) s.bin[i] = 0;
+        for (int i = Tid(); i < kBins; i += kT) s.bin[i] = 0;
     }
     __device__ void AddTo(int range, uint64_t w) {
         atomicAdd(reinterpret_cast<ull*>(&s.bin[range]), static_cast<ull>(w));
@@ -605,7 +606,7 @@ struct Chooser {
             w[i] = s.bin[Tid() * kEach + i];
             mine += w[i];
         }
-        uint64_t sum = *before + ScanBlock(mine, s.scan_u, &all) - mine;
+        uint64_t sum = *before + ScanBlock<kW>(mine, s.scan_u, &all) - mine;
         all += *before;
         // (a bound past the end: the last place)
         if (what == kPass ? bound >= all : bound > all) bound = what == kPass ? all - 1 : all;
@@ -642,7 +643,7 @@ struct Chooser {
         }
         const uint32_t code = static_cast<uint32_t>(bin) * kBins + (n > kWave ? Narrow(what, bound, &before, &held) : 0);
         // that range's (of a short list, the bin's) places
-        for (int i0 = 0; i0 < n; i0 += kChooseThreads) {
+        for (int i0 = 0; i0 < n; i0 += kT) {
             const int i = i0 + Tid();
             bool in = i < n && (n > kWave ? s.code[i] == code : s.code[i] / kBins == static_cast<uint32_t>(bin));
             uint64_t mask = __ballot(in);
@@ -668,7 +669,7 @@ struct Chooser {
             while ((most - least) >> shift >= kBins) ++shift;
             ClearBins();
             __syncthreads();
-            for (int i = Tid(); i < m; i += kChooseThreads) {
+            for (int i = Tid(); i < m; i += kT) {
                 double place;
                 const uint64_t key = s.list[s.some[i]];
                 BinOfKey(key, &place);
@@ -681,16 +682,16 @@ struct Chooser {
             least = kNoKey;
             most = 0;
             // what is left, in place: all have read theirs before any writes
-            uint16_t mine[kList / kChooseThreads];
+            uint16_t mine[kList / kT];
             int count = 0;
-            for (int i = Tid(); i < m; i += kChooseThreads) {
+            for (int i = Tid(); i < m; i += kT) {
                 const uint16_t index = s.some[i];
                 const uint64_t key = s.list[index];
                 if (key < lo || key > hi) continue;
                 least = key < least ? key : least;
                 most = key > most ? key : most;
 #pragma unroll
-                for (int j = 0; j < kList / kChooseThreads; ++j) mine[j] = j == count ? index : mine[j];
+                for (int j = 0; j < kList / kT; ++j) mine[j] = j == count ? index : mine[j];
                 ++count;
             }
             if (Tid() == 0) s.n_few = 0;
@@ -698,7 +699,7 @@ struct Chooser {
             if (count > 0) {
                 const uint32_t to = atomicAdd(&s.n_few, static_cast<uint32_t>(count));
 #pragma unroll
-                for (int j = 0; j < kList / kChooseThreads; ++j) {
+                for (int j = 0; j < kList / kT; ++j) {
                     if (j < count) s.some[to + j] = mine[j];
                 }
             }
@@ -774,7 +775,7 @@ struct Chooser {
             w[i] = Scaled(s.bin[Tid() * kEach + i], Tid() * kEach + i);
             mine += w[i];
         }
-        uint64_t sum = ScanBlock(mine, s.scan_u, &all) - mine;
+        uint64_t sum = ScanBlock<kW>(mine, s.scan_u, &all) - mine;
 #pragma unroll
         for (int i = 0; i < kEach; ++i) {
             sum += w[i];
@@ -786,7 +787,7 @@ struct Chooser {
     __device__ Span FirstBins(int last, bool reach, uint64_t x, uint64_t y) {
         if (Tid() < 2) s.found[Tid()] = last;
         __syncthreads();
-        for (int i = Tid(); i < last; i += kChooseThreads) {
+        for (int i = Tid(); i < last; i += kT) {
             const uint64_t sum = s.sum[i], before = Below(i);
             if (reach ? sum >= x && before < x : sum > x && (i == 0 || before <= x)) s.found[0] = i;
             if (reach ? sum >= y && before < y : sum > y && (i == 0 || before <= y)) s.found[1] = i;
@@ -895,8 +896,9 @@ __device__ inline void AddToList(RowState* state, const uint64_t* found, uint32_
 // from a row that the list holds whole, without any of the others.
 enum Pass { kCuts, kFinish, kOneLaunch, kSmall };
 
-template <typename T, Pass kPass_>
-__global__ __launch_bounds__(kChooseThreads) void SampleChoose(const SampleArgs p, int gather_parts) {
+template <typename T, Pass kPass_, int kT = kChooseThreads>
+__global__ __launch_bounds__(kT) void SampleChoose(const SampleArgs p, int gather_parts) {
+    constexpr int kW = kT / kWave, kEach = kBins / kT;
     __shared__ Choice s;
     const int tid = static_cast<int>(threadIdx.x);
     const int64_t row = kPass_ == kOneLaunch ? blockIdx.x / gather_parts : blockIdx.x;
@@ -915,7 +917,7 @@ __global__ __launch_bounds__(kChooseThreads) void SampleChoose(const SampleArgs 
     if constexpr (kPass_ == kFinish) {
         const RowState at = *state;
 #pragma unroll
-        for (int i = 0; i < kEach; ++i) s.bin[tid + i * kChooseThreads] = state_bin[tid + i * kChooseThreads];
+        for (int i = 0; i < kEach; ++i) s.bin[tid + i * kT] = state_bin[tid + i * kT];
         if (at.live == kChosen) return;
         top = at.top;
         largest = at.largest;
@@ -953,22 +955,22 @@ __global__ __launch_bounds__(kChooseThreads) void SampleChoose(const SampleArgs 
                     const int32_t from = static_cast<int32_t>(s.few[i]) + tid;
 #pragma unroll
                     for (int e = 0; e < kEach; ++e) {
-                        const int32_t at = from + e * kChooseThreads;
+                        const int32_t at = from + e * kT;
                         const uint64_t m = bins[at >= 0 ? at : 0];
                         sum[e] += at >= 0 ? m : 0;
                     }
                 }
 #pragma unroll
                 for (int e = 0; e < kEach; ++e) {
-                    s.bin[tid + e * kChooseThreads] = sum[e];
-                    if (kPass_ == kCuts) state_bin[tid + e * kChooseThreads] = sum[e];
+                    s.bin[tid + e * kT] = sum[e];
+                    if (kPass_ == kCuts) state_bin[tid + e * kT] = sum[e];
                 }
             }
         }
     } else {
         bool nan = false;
 #pragma unroll 4
-        for (int i = tid; i < p.vocab; i += kChooseThreads) {
+        for (int i = tid; i < p.vocab; i += kT) {
             const float x = T::Get(units.x[i]);
             const uint64_t key = x > -INFINITY ? Key(x, i) : kNoKey;
             nan |= x != x;
@@ -976,9 +978,9 @@ __global__ __launch_bounds__(kChooseThreads) void SampleChoose(const SampleArgs 
             s.list[i] = key;
             best = key < best ? key : best;
         }
-        for (int i = tid; i < kBins; i += kChooseThreads) s.bin[i] = 0;
+        for (int i = tid; i < kBins; i += kT) s.bin[i] = 0;
         if (tid == 0) s.word[0] = kNoKey;
-        largest = BlockMax<kChooseWaves>(largest, reinterpret_cast<float*>(s.scan_u));
+        largest = BlockMax<kW>(largest, reinterpret_cast<float*>(s.scan_u));
         flags = (largest > -INFINITY ? kSome : 0) | (__syncthreads_or(nan) ? kNan : 0);
         if (h.t == 0.0f) {
             atomicMin(reinterpret_cast<ull*>(&s.word[0]), static_cast<ull>(best));
@@ -1001,10 +1003,10 @@ __global__ __launch_bounds__(kChooseThreads) void SampleChoose(const SampleArgs 
             return;
         }
     }
-    Chooser<T> ch{p, h, s, units, p.largest + row * p.segments, top, kLastKey};
+    Chooser<T, kT> ch{p, h, s, units, p.largest + row * p.segments, top, kLastKey};
     ch.MakeEdges();
     if constexpr (kPass_ == kSmall) {
-        for (int i = tid; i < p.vocab; i += kChooseThreads) {
+        for (int i = tid; i < p.vocab; i += kT) {
             const uint64_t key = s.list[i];
             s.code[i] = ch.CodeOf(key);
             double place;
@@ -1030,16 +1032,16 @@ __global__ __launch_bounds__(kChooseThreads) void SampleChoose(const SampleArgs 
         s.sum[tid] = 0;
         __syncthreads();
         int rank = 0;
-#pragma unroll 8
-        for (int i = 0; i < n; ++i) rank += s.bin[i] < key ? 1 : 0;
         if (key != kNoKey) {
+#pragma unroll 8
+            for (int i = 0; i < n; ++i) rank += s.bin[i] < key ? 1 : 0;
             s.list[kFewAll + rank] = key;
             s.sum[rank] = w;
         }
         __syncthreads();
         w = s.sum[tid];
         uint64_t all;
-        const uint64_t upto = ScanBlock(w, s.scan_u, &all);
+        const uint64_t upto = ScanBlock<kW>(w, s.scan_u, &all);
         s.sum[tid] = upto;
         int kept = __syncthreads_count(w != 0);
         const uint64_t first = s.sum[0];
@@ -1141,8 +1143,8 @@ __global__ __launch_bounds__(kChooseThreads) void SampleChoose(const SampleArgs 
             bool is_all = a.lo == 0;
             if (what == kTopP) {  // whether all up to the last bin are few
                 uint64_t mass = 0, all;
-                for (int i = tid; i <= last; i += kChooseThreads) mass += s.bin[i];
-                ScanBlock(mass, s.scan_u, &all);
+                for (int i = tid; i <= last; i += kT) mass += s.bin[i];
+                ScanBlock<kW>(mass, s.scan_u, &all);
                 is_all = static_cast<double>(all) * (1 / (0.984 * kOne)) < 0.9 * kFewAll;
                 if (is_all) a = b = {0, last};
             }
@@ -1178,7 +1180,7 @@ __global__ __launch_bounds__(kChooseThreads) void SampleChoose(const SampleArgs 
                 whole_list = state->live == kAll;
             }
 #pragma unroll 4
-            for (int i = tid; i < (n < kList ? n : kList); i += kChooseThreads) ch.PutInList(i, state_list[i]);
+            for (int i = tid; i < (n < kList ? n : kList); i += kT) ch.PutInList(i, state_list[i]);
             __syncthreads();
             if (n > kList) n = -1;
             whole = !(what == kTopK && a.lo != 0);
@@ -1203,7 +1205,7 @@ __global__ __launch_bounds__(kChooseThreads) void SampleChoose(const SampleArgs 
 #pragma unroll
             for (int i = 0; i < 3; ++i) {
                 uint64_t all;
-                ScanBlock(sum[i], s.scan_u, &all);
+                ScanBlock<kW>(sum[i], s.scan_u, &all);
                 if (m.lo + i <= m.hi) kept += ch.Scaled(all, m.lo + i);
             }
         }
@@ -1291,9 +1293,10 @@ mlk_status Launch(SampleArgs p, int64_t n_rows, char* workspace, hipStream_t s) 
             p.largest = reinterpret_cast<float*>(p.part + rows * p.parts * kPartBytes);
             hipLaunchKernelGGL(SampleBins<T>, dim3(static_cast<unsigned>(rows * p.parts)), dim3(kThreads), 0, s, p);
             const int looks = GatherParts(p.vocab, kBytes, 1);
-            // as long as each compute unit has one workgroup of it (fp32 rows of 128256: 1 row 32.2 us by
-            // the three launches, 27.7 by one, 16 rows 39.6 and 37.4, 32 rows 43.8 and 45.9; bf16,
-            // half the bytes: 32 rows 53.1 and 50.9, 64 rows 58.0 and 59.2)
+            // as long as each compute unit has one workgroup of it (fp32 rows of 128256: 1 row 32.3 us by
+            // the three launches, 27.9 by one, 8 rows 37.2 and 36.6, 16 rows 37.6 and 37.7; of 32000: 64
+            // rows 31.6 and 28.8; bf16 rows of 128256, half the bytes: 16 rows 49.0 and 46.7, 32 rows 49.5
+            // and 51.1)
             if (rows * looks <= ComputeUnits()) {
                 hipLaunchKernelGGL((SampleChoose<T, kOneLaunch>), dim3(static_cast<unsigned>(rows * looks)), block, 0, s, p, looks);
             } else {
@@ -1305,7 +1308,12 @@ mlk_status Launch(SampleArgs p, int64_t n_rows, char* workspace, hipStream_t s) 
                 const dim3 gather(static_cast<unsigned>(rows * parts));
                 if (!many) hipLaunchKernelGGL((SampleGather<T, 1>), gather, block, 0, s, p, parts);
                 else hipLaunchKernelGGL((SampleGather<T, 4>), gather, block, 0, s, p, parts);
-                hipLaunchKernelGGL((SampleChoose<T, kFinish>), grid, block, 0, s, p, 1);
+                // twice the threads where a compute unit has one row at most (rows of 128256, mixed
+                // settings, the whole call: 64 in fp32 50.7 us with 256, 46.0 with 512, 256 of them 84.2 and
+                // 81.0; 64 in bf16 58.4 and 54.0; 512 rows, with twice the threads in the other passes
+                // too, 127 and 137)
+                if (rows <= ComputeUnits()) hipLaunchKernelGGL((SampleChoose<T, kFinish, kWideThreads>), grid, dim3(kWideThreads), 0, s, p, 1);
+                else hipLaunchKernelGGL((SampleChoose<T, kFinish>), grid, block, 0, s, p, 1);
             }
         }
         const mlk_status st = CheckLaunch("SampleChoose");
