@@ -367,3 +367,31 @@ def test_replays_choose_as_calls_do(mlk, sampling):
         call(eager, None)
         mlk.synchronize()
         np.testing.assert_array_equal(got, eager.download())
+
+
+@pytest.mark.parametrize("rows,V", [(1, 128256), (5, 50257), (70, 50257), (300, 9000), (9, 131)])
+def test_calls_at_once_over_any_workspace(mlk, sampling, rows, V):
+    """Two streams, a workspace each, full of ones: what a call alone chooses."""
+    rng = np.random.default_rng(V + rows)
+    up = mlk.DeviceBuffer.from_array
+    how = mixed(rng, rows)
+    x = [logits(rng, rows, V) for _ in range(2)]
+    alone = [run(mlk, sampling, a, how) for a in x]
+    f = {n: up(np.array([h[n] for h in how], np.int32 if n == "k" else np.float32))
+         for n in ("t", "k", "p", "m", "u")}
+    s = sampling.Sampling(f["t"], f["k"], f["p"], f["m"])
+    need = sampling.workspace_bytes("f32", rows, V)
+    streams = [mlk.Stream() for _ in range(2)]
+    d = [up(a) for a in x]
+    ws = [up(np.full(need, 255, np.uint8)) for _ in range(2)]
+    tokens = [[up(np.zeros(rows, np.int32)) for _ in range(8)] for _ in range(2)]
+    probs = [[up(np.zeros(rows, np.float32)) for _ in range(8)] for _ in range(2)]
+    for i in range(8):
+        for j in range(2):
+            sampling.sample("f32", d[j], rows, V, f["u"], tokens[j][i], how=s, prob=probs[j][i],
+                            workspace=ws[j], stream=streams[j].handle)
+    for j in range(2):
+        streams[j].synchronize()
+        for i in range(8):
+            np.testing.assert_array_equal(tokens[j][i].download(), alone[j][0])
+            np.testing.assert_array_equal(probs[j][i].download().view(np.uint32), alone[j][1].view(np.uint32))
