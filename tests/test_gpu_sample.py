@@ -395,3 +395,24 @@ def test_calls_at_once_over_any_workspace(mlk, sampling, rows, V):
         for i in range(8):
             np.testing.assert_array_equal(tokens[j][i].download(), alone[j][0])
             np.testing.assert_array_equal(probs[j][i].download().view(np.uint32), alone[j][1].view(np.uint32))
+
+
+def test_rows_past_32_bits(mlk, sampling):
+    """Rows 3 * 2^29 logits apart."""
+    rng = np.random.default_rng(17)
+    up = mlk.DeviceBuffer.from_array
+    for V in (40003, 1000):
+        rows, stride = 4, 3 << 29
+        x, how = logits(rng, rows, V), mixed(rng, rows)
+        alone = run(mlk, sampling, x, how)
+        far = mlk.DeviceBuffer(4 * ((rows - 1) * stride + V), np.uint8)
+        for r in range(rows):
+            one = np.ascontiguousarray(x[r])
+            mlk.check(mlk.lib.mlk_memcpy(far.offset(4 * r * stride), one.ctypes.data, one.nbytes, mlk.H2D))
+        f = {n: up(np.array([h[n] for h in how], np.int32 if n == "k" else np.float32))
+             for n in ("t", "k", "p", "m", "u")}
+        tokens, ws = up(np.zeros(rows, np.int32)), mlk.DeviceBuffer(sampling.workspace_bytes("f32", rows, V), np.uint8)
+        sampling.sample("f32", far, rows, V, f["u"], tokens, how=sampling.Sampling(f["t"], f["k"], f["p"], f["m"]),
+                        row_stride=stride, workspace=ws)
+        mlk.synchronize()
+        np.testing.assert_array_equal(tokens.download(), alone[0])

@@ -254,6 +254,34 @@ def test_chunks_beside_single_tokens(mlk, paged, ones, act, ct):
     check(batch, pages.of, Masks(batch, H), q, out.download(), H, hd, act, rows=rows)
 
 
+class FarPages(Pages):
+    """Pages 2^29 elements apart."""
+
+    def upload(self, mlk, paged):
+        n, page, KV, hd = self.shape
+        stride, size = 1 << 29, self.host[0].itemsize
+        self.bufs = [mlk.DeviceBuffer(((n - 1) * stride + self.row) * size, np.uint8) for _ in range(2)]
+        for buf, a in zip(self.bufs, self.host):
+            for i in range(n):
+                one = np.ascontiguousarray(a[i, :self.row])
+                mlk.check(mlk.lib.mlk_memcpy(buf.offset(i * stride * size), one.ctypes.data, one.nbytes, mlk.H2D))
+        self.handle = paged.PagedCache(*self.bufs, self.t, n, page, KV, hd, page_stride=stride)
+
+
+@pytest.mark.parametrize("counts,lens", [([1, 2], [700, 300]), ([70, 1], [400, 650])])
+def test_offsets_past_32_bits(mlk, paged, counts, lens):
+    H, KV, hd = 8, 2, 128
+    rng = np.random.default_rng(16)
+    batch = Batch(counts, lens, 64)
+    pages = FarPages(mlk, paged, batch, KV, hd, "bf16", rng)
+    assert batch.n_pages > 8 and batch.table.max() >= 8
+    q = to_type(rng.standard_normal((batch.T, H, hd)), "bf16")
+    for kw in (dict(cap=10.0, window=250), dict(bias=True)):
+        masks = Masks(batch, H, **kw)
+        got = run_paged(mlk, paged, batch, pages, masks, q, H, "bf16")
+        check(batch, pages.of, masks, q, got, H, hd, "bf16", rows=some_rows(rng, batch, H))
+
+
 # ------------------------------------------------------------------ packed
 
 def run_packed(mlk, paged, batch, masks, q, k, v, H, KV, hd, act, strides=(None,) * 3,
