@@ -1301,12 +1301,17 @@ mlk_status Launch(SampleArgs p, int64_t n_rows, char* workspace, hipStream_t s) 
                 hipLaunchKernelGGL((SampleChoose<T, kOneLaunch>), dim3(static_cast<unsigned>(rows * looks)), block, 0, s, p, looks);
             } else {
                 hipLaunchKernelGGL((SampleChoose<T, kCuts>), grid, block, 0, s, p, 1);
-                // where those of one look are more than the device holds at once (5 a compute unit), of
-                // four (512 fp32 rows of top-k: 36 us, with four 9)
-                const bool many = rows * looks > 5 * ComputeUnits();
-                const int parts = GatherParts(p.vocab, kBytes, many ? 4 : 1);
+                // the fewest looks a workgroup that leave no more than 5 of them to a compute unit: rows with
+                // much to gather go over more of them, but the start of one with nothing to gather costs as
+                // well (the whole call, rows of 128256 with one look, two and four: 128 in fp32 of mixed settings
+                // 59.2, 57.2 and 64.7 us, of top-k 43.6, 38.0 and 36.3; 256 in bf16 of mixed settings 80.1,
+                // 84.2 and 98.0, of top-k 48.5, 42.8 and 41.9)
+                const int most_groups = 5 * ComputeUnits();
+                const int look = rows * looks <= most_groups ? 1 : rows * GatherParts(p.vocab, kBytes, 2) <= most_groups ? 2 : 4;
+                const int parts = GatherParts(p.vocab, kBytes, look);
                 const dim3 gather(static_cast<unsigned>(rows * parts));
-                if (!many) hipLaunchKernelGGL((SampleGather<T, 1>), gather, block, 0, s, p, parts);
+                if (look == 1) hipLaunchKernelGGL((SampleGather<T, 1>), gather, block, 0, s, p, parts);
+                else if (look == 2) hipLaunchKernelGGL((SampleGather<T, 2>), gather, block, 0, s, p, parts);
                 else hipLaunchKernelGGL((SampleGather<T, 4>), gather, block, 0, s, p, parts);
                 // twice the threads where a compute unit has one row at most (rows of 128256, mixed
                 // settings, the whole call: 64 in fp32 50.7 us with 256, 46.0 with 512, 256 of them 84.2 and

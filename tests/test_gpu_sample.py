@@ -319,6 +319,23 @@ def test_hard_rows_choose_alike_in_large_and_small_batches(mlk, sampling, act):
     check(x[:170], how[:170], (all_t[:170], all_p[:170], flag), act, 0.3)
 
 
+@pytest.mark.parametrize("act,rows", [("f32", 220), ("f32", 500), ("bf16", 400), ("bf16", 700)])
+def test_batches_of_every_division(mlk, sampling, act, rows):
+    """Batches whose rows are gathered by fewer workgroups each: as 20 of them choose."""
+    rng = np.random.default_rng(rows)
+    V = 50257
+    some = logits(rng, 20, V)
+    some[3:6] = np.round(some[3:6])
+    some[7, 100:] = -np.inf
+    how = mixed(rng, 20)
+    few_t, few_p, _ = run(mlk, sampling, some, how, act)
+    at = rng.integers(0, 20, rows)
+    t, p, _ = run(mlk, sampling, some[at], [how[i] for i in at], act)
+    np.testing.assert_array_equal(t, few_t[at])
+    np.testing.assert_array_equal(p.view(np.uint32), few_p[at].view(np.uint32))
+    check(some, how, (few_t, few_p, 0), act, 0.7)
+
+
 def test_large_and_far_apart_logits(mlk, sampling):
     """Logits of 10^4 and beyond, all far below 0, spread over 10^5 temperatures."""
     rng = np.random.default_rng(11)
