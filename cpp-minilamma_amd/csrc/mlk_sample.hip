@@ -845,36 +845,31 @@ __device__ inline void GatherPart(const RowUnits<T>& r, const float* largest, in
             unit[i] = j < n ? hit_segment[j] * kSegment + lane % kSegment : units;
             raw[i] = r.Load(unit[i], unit[i] < units);
         }
-        uint32_t hits = 0;
+        // which lanes' elements are in a span, then places for all of the wave's by one addition
+        uint64_t in[kRounds * E];
+        uint32_t all = 0;
 #pragma unroll
         for (int i = 0; i < kRounds; ++i) {
 #pragma unroll
             for (int e = 0; e < E; ++e) {
                 const float x = r.Get(raw[i], e);
-                const bool in = (x >= al && x <= ah) || (x >= bl && x <= bh);
-                hits |= in ? 1u << (i * E + e) : 0u;
+                in[i * E + e] = __ballot((x >= al && x <= ah) || (x >= bl && x <= bh));
+                all += __popcll(in[i * E + e]);
             }
         }
-        if (__ballot(hits != 0) == 0) continue;
-        // places for the wave's hits: one addition for all
-        const uint32_t mine = __popc(hits);
-        uint32_t upto = mine;
-#pragma unroll
-        for (int off = 1; off < kWave; off *= 2) {
-            const uint32_t o = __shfl_up(upto, off, kWave);
-            if (lane >= off) upto += o;
-        }
+        if (all == 0) continue;
         uint32_t to = 0;
-        if (lane == kWave - 1) to = atomicAdd(n_found, upto);
-        to = __builtin_amdgcn_readlane(to, kWave - 1) + upto - mine;
+        if (lane == 0) to = atomicAdd(n_found, all);
+        to = __builtin_amdgcn_readfirstlane(to);
 #pragma unroll
         for (int i = 0; i < kRounds; ++i) {
 #pragma unroll
             for (int e = 0; e < E; ++e) {
-                if (hits >> (i * E + e) & 1) {
-                    if (to < kList) found[to] = Key(r.Get(raw[i], e), r.Index(unit[i], e));
-                    ++to;
-                }
+                const uint64_t mask = in[i * E + e];
+                if (mask == 0) continue;
+                const uint32_t at = to + __builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(mask >> 32), __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(mask), 0));
+                if (__builtin_amdgcn_inverse_ballot_w64(mask) && at < kList) found[at] = Key(r.Get(raw[i], e), r.Index(unit[i], e));
+                to += __popcll(mask);
             }
         }
     }
