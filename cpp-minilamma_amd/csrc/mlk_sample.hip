@@ -31,9 +31,9 @@
 // kList logits are one launch alone, kSmall, with everything in the list.
 //
 // What bounds it: 512 fp32 rows of 128256 of mixed settings (263 MB, 56 us at a copy's rate)
-// 127 us: SampleBins 71 (with a top-k, or at temperature 0, 55: the bytes; weights cost
-// the rest, float64 and additions in shared memory), cuts 8, gather 33, finish 20, as each takes
-// by itself.  64 bf16 rows 54 us, one fp32 row 28, 6 fp32 rows of 131 7: a few launches, each a
+// 122 us: SampleBins 70 (with a top-k, or at temperature 0, 55: the bytes; weights cost
+// the rest, float64 and additions in shared memory), cuts 8, gather 28, finish 20, as each takes
+// by itself.  64 bf16 rows 53 us, one fp32 row 28, 6 fp32 rows of 131 7: a few launches, each a
 // chain of loads, scans and barriers.
 #include "mlk_paged.h"
 
