@@ -1151,7 +1151,11 @@ __global__ __launch_bounds__(kT) void SampleChoose(const SampleArgs p, int gathe
             }
             GatherPart<T, 1>(units, ch.largest, gather_part, at, s.list, s.some, &s.n_list);
             AddToList(state, s.list, s.n_list, &s.n_few);
-            __syncthreads();  // (one thread's release and acquire then are the workgroup's)
+            // every wave's part of the list has arrived; one thread's release and acquire then are the
+            // workgroup's (by all of them they cost more than the launches that this saves: 64 bf16 rows
+            // 90 us for 59)
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            __syncthreads();
             if (tid == 0) {
                 s.n_few = __hip_atomic_fetch_add(&state->done, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) + 1;
                 s.n_list = __hip_atomic_load(&state->n, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
