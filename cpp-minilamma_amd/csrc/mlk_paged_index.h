@@ -72,8 +72,9 @@ MLK_HD inline Seen SeenBy(const Scores& m, int s, int32_t t, int32_t pos, int32_
         if (f > v.lo) v.lo = f;
     }
     if (m.prefix != nullptr) {
-        const int32_t n = ReadIndex(m.prefix + s), last = (n < len ? n : len) - 1;
-        if (last > v.hi) v.hi = last;
+        // (compared before one is taken off: it may be of any value)
+        const int32_t n = ReadIndex(m.prefix + s), end = n < len ? n : len;
+        if (end > v.hi) v.hi = end - 1;
     }
     return v;
 }
