@@ -476,12 +476,12 @@ struct Chooser {
     }
 
     // Logits no smaller (larger) than any of bin `bin`, to within a thousandth of a bin and a
-    // rounding.
+    // rounding; -infinity is below all (bins of the highest temperatures reach past the numbers).
     __device__ float Lowest(int bin) const {
         const double b = static_cast<double>(top) - bin;
         if (!(h.c > 0.0) || b <= -0x1p28) return -0x1.fffffep127f;
         const double x = (b - 0.501) / h.c;
-        return static_cast<float>(x - fabs(x) * 0x1p-23);
+        return fmaxf(static_cast<float>(x - fabs(x) * 0x1p-23), -0x1.fffffep127f);
     }
     __device__ float Highest(int bin) const {
         const double b = static_cast<double>(top) - bin;
