@@ -168,6 +168,12 @@ __device__ inline uint64_t Key(float x, int32_t i) {
 
 constexpr uint64_t kNoKey = ~uint64_t{0}, kLastKey = kNoKey - 1;  // past every element's
 
+// The least logit that weighs anything beside a row's (or a part's) largest: all numbers do as
+// far as their bins say, but beside infinity only its equals.
+__device__ inline float LeastOf(float largest) {
+    return largest < INFINITY ? -0x1.fffffep127f : INFINITY;
+}
+
 // A row as units of 16 bytes from the last 16-byte boundary at or before it.
 template <typename T>
 struct RowUnits {
@@ -310,13 +316,26 @@ __global__ __launch_bounds__(kThreads) void SampleBins(const SampleArgs p) {
             so_far = all;
             const int32_t to = BinOf(h, all);
             if (some) {
-                const int32_t fresh = to - top < kBins ? to - top : kBins;
+                // (beside infinity all that was before is)
+                const int32_t fresh = all < INFINITY && to - top < kBins ? to - top : kBins;
                 for (int32_t i = lane; i < fresh; i += kWave) mass[(to - i) & (kBins - 1)] = 0;
             }
             top = to;
             some = true;
         }
         if (!some) continue;
+        if (so_far == INFINITY) {  // its equals count alone, each the same
+            uint32_t n = 0;
+#pragma unroll
+            for (int a = 0; a < kAhead; ++a) {
+#pragma unroll
+                for (int e = 0; e < E; ++e) n += v[a][e] == INFINITY ? 1 : 0;
+            }
+            double f;
+            const int32_t at = BinOf(h, INFINITY, &f) & (kBins - 1);
+            if (n != 0) atomicAdd(reinterpret_cast<ull*>(&mass[at]), static_cast<ull>(h.k != 0 ? n : n * Weight(f)));
+            continue;
+        }
         auto add = [&](auto counts) {
 #pragma unroll
             for (int a = 0; a < kAhead; ++a) {
@@ -359,6 +378,8 @@ __global__ __launch_bounds__(kThreads) void SampleBins(const SampleArgs p) {
         if (best_of[w] < best) best = best_of[w];
         most = fmaxf(most, largest_of[w]);
     }
+    // (a wave that met an infinity has the largest bin; those that met none count for nothing then)
+    const float least = LeastOf(most);
     Part* out = reinterpret_cast<Part*>(p.part + blockIdx.x * kPartBytes);
     if (tid == 0) *out = {all_top, flags, best, most, {}};
     if (h.t == 0.0f || !(flags & kSome)) return;
@@ -367,7 +388,7 @@ __global__ __launch_bounds__(kThreads) void SampleBins(const SampleArgs p) {
         const int32_t at = all_top - i;
         uint64_t sum = 0;
         for (int w = 0; w < kWaves; ++w) {
-            if ((flags_of[w] & kSome) && static_cast<uint32_t>(tops[w] - at) < kBins) {
+            if ((flags_of[w] & kSome) && largest_of[w] >= least && static_cast<uint32_t>(tops[w] - at) < kBins) {
                 sum += hist[w][at & (kBins - 1)];
             }
         }
@@ -436,6 +457,7 @@ struct Chooser {
     RowUnits<T> r;
     const float* largest;
     int32_t top;
+    float least;     // of the row's logits, what is smaller weighs nothing
     uint64_t limit;  // keys past it are cut off by top-k
 
     __device__ int Tid() const { return static_cast<int>(threadIdx.x); }
@@ -479,9 +501,9 @@ struct Chooser {
     // rounding; -infinity is below all (bins of the highest temperatures reach past the numbers).
     __device__ float Lowest(int bin) const {
         const double b = static_cast<double>(top) - bin;
-        if (!(h.c > 0.0) || b <= -0x1p28) return -0x1.fffffep127f;
+        if (!(h.c > 0.0) || b <= -0x1p28) return least;
         const double x = (b - 0.501) / h.c;
-        return fmaxf(static_cast<float>(x - fabs(x) * 0x1p-23), -0x1.fffffep127f);
+        return fmaxf(static_cast<float>(x - fabs(x) * 0x1p-23), least);
     }
     __device__ float Highest(int bin) const {
         const double b = static_cast<double>(top) - bin;
@@ -927,7 +949,8 @@ __global__ __launch_bounds__(kT) void SampleChoose(const SampleArgs p, int gathe
             Part part{INT32_MIN, 0, ~uint64_t{0}, -INFINITY, {}};
             if (lane < p.parts) part = *reinterpret_cast<const Part*>(parts + lane * kPartBytes);
             flags = (__ballot(part.flags & kSome) != 0 ? kSome : 0) | (__ballot(part.flags & kNan) != 0 ? kNan : 0);
-            if (!(part.flags & kSome)) part.top = INT32_MIN;
+            const bool infinite = __ballot(part.largest == INFINITY) != 0;  // then other parts count for nothing
+            if (!(part.flags & kSome) || (infinite && part.largest < INFINITY)) part.top = INT32_MIN;
             top = part.top;
             best = part.best;
             largest = part.largest;
@@ -998,11 +1021,12 @@ __global__ __launch_bounds__(kT) void SampleChoose(const SampleArgs p, int gathe
             return;
         }
     }
-    Chooser<T, kT> ch{p, h, s, units, p.largest + row * p.segments, top, kLastKey};
+    Chooser<T, kT> ch{p, h, s, units, p.largest + row * p.segments, top, LeastOf(largest), kLastKey};
     ch.MakeEdges();
     if constexpr (kPass_ == kSmall) {
         for (int i = tid; i < p.vocab; i += kT) {
-            const uint64_t key = s.list[i];
+            uint64_t key = s.list[i];
+            if (Logit(static_cast<uint32_t>(key >> 32)) < ch.least) s.list[i] = key = kNoKey;
             s.code[i] = ch.CodeOf(key);
             double place;
             const int b = ch.BinOfKey(key, &place);

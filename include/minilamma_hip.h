@@ -603,9 +603,9 @@ typedef struct {
  * and the token is the first of them with C_i > uniform C_n; prob (NULL: not
  * wanted) is its share w_i / C_n.  uniform = 0 chooses the largest logit, as does
  * temperature 0 (uniform is then not looked at).  A logit of -infinity is never
- * chosen; logits of +infinity share all the weight.  Weights below 2^-44 (30
+ * chosen; logits of +infinity share all the weight, beside whatever else.  Weights below 2^-44 (30
  * temperatures below the largest) may count as 0; temperatures below 2^-14 count
- * as 2^-14, logits of over 2^24 temperatures in size as that.
+ * as 2^-14, finite logits of over 2^24 temperatures in size as that (their order stays).
  * The weights are added as whole numbers: a row's token depends on
  * neither the other rows nor how the work is divided, run for run.
  * A row that has a NaN, or only -infinities, or a setting that is a NaN, a negative

@@ -1,4 +1,5 @@
-"""The sampler at the ends of its ranges: temperatures up to the largest number."""
+"""The sampler at the ends of its ranges: temperatures up to the largest number, infinities
+beside logits of any size."""
 from __future__ import annotations
 
 import importlib
@@ -33,3 +34,24 @@ def test_a_masked_logit_is_not_chosen_at_the_highest_temperatures(mlk, sampling,
                        p=list(np.resize([1, 1, 1, 1, 0.93, 0.93, 0.55], rows)),
                        m=list(np.resize([0, 0.1, 0.2, 0, 0], rows)))
         check(x, how, run(mlk, sampling, x, how, act), act, 1.0)
+
+
+@pytest.mark.parametrize("act", ["f32", "bf16"])
+@pytest.mark.parametrize("V", [200, 3000, 5000, 128256])
+@pytest.mark.parametrize("t", [1e-30, 2.0 ** -14, 0.01, 1.0, 1e38, LARGEST, float("inf")])
+def test_infinities_share_all_the_weight(mlk, sampling, t, V, act):
+    """Beside logits of ordinary size, of over 2^24 temperatures and of the largest number."""
+    rng = np.random.default_rng(V)
+    for rows in (16, 290) if V <= 5000 else (16,):
+        x = rng.standard_normal((rows, V)).astype(np.float32)
+        n = rng.integers(1, 4, rows)
+        for r in range(rows):
+            at = rng.choice(V, n[r] + 20, replace=False)
+            x[r, at] = [3e38, 60000.0, -np.inf, 2000.0][r % 4]
+            x[r, at[:n[r]]] = np.inf
+        u = np.resize(np.float32([0.1, 0.4, 0.6, 0.95]), rows)
+        how = settings(rows, t=t, u=u, k=list(np.resize([0, 50, 0, 2, 0, 30000, 0], rows)),
+                       p=list(np.resize([1, 1, 0.9, 1, 0.6], rows)), m=list(np.resize([0, 0, 0.1], rows)))
+        got = run(mlk, sampling, x, how, act)
+        # (an infinity over an infinite temperature: as over the largest)
+        check(x, [dict(h, t=min(t, LARGEST)) for h in how], got, act, 1.0)
