@@ -492,9 +492,10 @@ struct Chooser {
         s.code[at] = CodeOf(key);
     }
     __device__ uint64_t Below(int bin) const { return bin > 0 ? s.sum[bin - 1] : 0; }
-    // Whole weights of a bin as those of the largest bin's middle.
+    // Whole weights of a bin as those of the largest bin's middle; of that bin itself they stay as
+    // they are (float64 holds no sum of over 2^53: of equal logits all bounds are exact).
     __device__ uint64_t Scaled(uint64_t w, int bin) {
-        return static_cast<uint64_t>(rint(static_cast<double>(w) * Edge(bin)));
+        return bin == 0 ? w : static_cast<uint64_t>(rint(static_cast<double>(w) * Edge(bin)));
     }
 
     // Logits no smaller (larger) than any of bin `bin`, to within a thousandth of a bin and a
@@ -783,6 +784,7 @@ struct Chooser {
 
     // A bound on the sum over all as one on whole weights within bin `bin`.
     __device__ uint64_t InBin(uint64_t bound, int bin, bool reach) const {
+        if (bin == 0) return bound;
         const uint64_t below = Below(bin);
         const double in = bound > below ? static_cast<double>(bound - below) / Edge(bin) : 0.0;
         return static_cast<uint64_t>(reach ? ceil(in) : in);
@@ -821,14 +823,35 @@ struct Chooser {
     }
 };
 
-__device__ inline uint64_t Share(double u, uint64_t sum) {
-    return static_cast<uint64_t>(u * static_cast<double>(sum));
+// The largest whole number of at most a * sum for a in [0, 1), exactly; *rest: whether it is less.
+__device__ inline uint64_t Times(float a, uint64_t sum, bool* rest) {
+    const uint32_t bits = __float_as_uint(fabsf(a)), e = bits >> 23;  // a = m 2^-shift; -0 is 0
+    const uint32_t m = e == 0 ? bits : (bits & 0x7FFFFFu) | 0x800000u;
+    const uint32_t shift = 149 - (e == 0 ? 0 : e - 1);  // 24 .. 149
+    // m * sum = high 2^32 + low
+    const uint64_t p = uint64_t{m} * static_cast<uint32_t>(sum), high = uint64_t{m} * (sum >> 32) + (p >> 32);
+    const uint32_t low = static_cast<uint32_t>(p);
+    if (shift < 32) {
+        *rest = low << (32 - shift) != 0;
+        return high << (32 - shift) | low >> shift;
+    }
+    const uint32_t s = shift - 32;
+    const uint64_t x = s < 64 ? high >> s : 0;
+    *rest = low != 0 || (s < 64 ? x << s : 0) != high;
+    return x;
 }
 
-// The least whole sum that is at least p of `sum`.
+__device__ inline uint64_t Share(float u, uint64_t sum) {
+    bool rest;
+    return Times(u, sum, &rest);
+}
+
+// The least whole sum that is at least p (below 1) of `sum`, 1 or more.
 __device__ inline uint64_t Reach(float p, uint64_t sum) {
-    const double x = ceil(static_cast<double>(p) * static_cast<double>(sum));
-    return x > 1.0 ? static_cast<uint64_t>(x) : 1;
+    if (!(p > 0.0f)) return 1;
+    bool rest;
+    const uint64_t x = Times(p, sum, &rest);
+    return rest || x == 0 ? x + 1 : x;
 }
 
 // The row's logits in the two spans of `at`, in any order, into `found` (of more than kList not
@@ -1091,7 +1114,7 @@ __global__ __launch_bounds__(kT) void SampleChoose(const SampleArgs p, int gathe
     enum { kTopK, kTopP, kToken };
     int last = kBins - 1;       // no element of a later bin can be chosen
     int n = kPass_ == kSmall ? p.vocab : -1;  // elements of the list, where it has all that is needed
-    const double u = h.u;
+    const float u = h.u;
     uint64_t kept = 0, reach = 0;
     double least = 0.0;
     bool by_p = h.p < 1.0f, by_m = h.m > 0.0f;

@@ -55,3 +55,29 @@ def test_infinities_share_all_the_weight(mlk, sampling, t, V, act):
         got = run(mlk, sampling, x, how, act)
         # (an infinity over an infinite temperature: as over the largest)
         check(x, [dict(h, t=min(t, LARGEST)) for h in how], got, act, 1.0)
+
+
+@pytest.mark.parametrize("V", [4098, 50258, 100000, 150000, 1048574])
+def test_bounds_that_equal_a_sum(mlk, sampling, V):
+    """Equal logits whose weight is an odd whole number: u V and p V are whole, and so is the
+    first place behind them (float64's 53 bits do not hold such sums)."""
+    for value in (0.1, 1.3, -7.77, 3.14):
+        x = np.full((8, V), value, np.float32)
+        how = settings(8, u=[0.5, 0.25, 0.75, 0.125, 1 - 2.0 ** -24, 1 - 2.0 ** -24, 0.5, 0.5],
+                       p=[1, 1, 1, 1, 0.5, 0.25, 0.5, 1], k=[0, 0, 0, 0, 0, 0, 4096, 4094])
+        check(x, how, run(mlk, sampling, x, how), need_clear=1.0)
+
+
+@pytest.mark.parametrize("rows", [3, 300])
+def test_bounds_that_equal_a_sum_beside_others(mlk, sampling, rows):
+    """n equal logits far above all others: the draw at i / n is the next of them."""
+    V = 60000
+    n = 50002
+    x = np.full((rows, V), -100.0, np.float32)
+    x[:, 9000:9000 + n] = 2.3
+    how = settings(rows, u=0.5, p=list(np.resize([1.0, 1.0, 0.5], rows)), k=list(np.resize([0, n, 0], rows)))
+    tokens, probs, flag = run(mlk, sampling, x, how)
+    want = np.resize([9000 + n // 2, 9000 + n // 2, 9000 + n // 4], rows)
+    np.testing.assert_array_equal(tokens, want)
+    np.testing.assert_allclose(probs, np.resize([1 / n, 1 / n, 2 / n], rows), rtol=2.0 ** -22)
+    assert flag == 0
