@@ -283,7 +283,9 @@ class DeviceModel:
         two arrays.  The settings are numbers, or arrays of n.  Eight bytes a row come
         back instead of its logits."""
         from . import sampling
-        u = np.atleast_1d(np.asarray(uniform, np.float32))
+        wide = np.atleast_1d(np.asarray(uniform, np.float64))
+        u = wide.astype(np.float32)
+        u[(u == 1) & (wide < 1)] = np.nextafter(np.float32(1), np.float32(0))  # rounded up to 1
         n, V = u.size, self.config["vocab"]
         if u.ndim != 1 or not 1 <= n <= len(tokens):
             raise ValueError(f"{n} uniform numbers for {len(tokens)} tokens")
