@@ -291,7 +291,8 @@ class DeviceModel:
             raise ValueError(f"{n} uniform numbers for {len(tokens)} tokens")
         given = np.empty((7, n), np.float32)  # u and the settings, then tokens and shares
         given[0], given[1], given[3], given[4] = u, temperature, top_p, min_p
-        given.view(np.int32)[2] = top_k
+        # (more than int32 counts is all, as 0 and what is below are)
+        given.view(np.int32)[2] = np.maximum(np.minimum(top_k, 2 ** 31 - 1), 0)
         need = sampling.workspace_bytes("f32", n, V)
         head = (given.nbytes + 255) // 256 * 256
         buf, out, at = self._logits_of(tokens, positions, pos0, n, head + need, stream)

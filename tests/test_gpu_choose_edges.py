@@ -1,4 +1,4 @@
-"""DeviceModel.choose with settings that float32 does not hold as they are."""
+"""DeviceModel.choose with settings that float32 and int32 do not hold as they are."""
 from __future__ import annotations
 
 import importlib
@@ -33,3 +33,14 @@ def test_uniform_numbers_next_to_one(fwd):
     for u in (1.0, 1 + 2.0 ** -30, -2.0 ** -60, float("nan")):
         with pytest.raises(ValueError, match="no token to choose"):
             dm.choose(tokens, u)
+
+
+def test_top_k_past_32_bits(fwd):
+    """A top-k of more tokens than int32 counts keeps all; a negative one does too."""
+    model, tokens, _, _ = tiny_model()
+    dm = fwd.DeviceModel(model)
+    want = dm.choose(tokens, [0.9, 0.95])
+    for k in (2 ** 40, 2 ** 32 + 1, -2 ** 40, np.array([2 ** 32 + 1, 2 ** 63 - 1]), [2 ** 32 + 1, -2 ** 62]):
+        got = dm.choose(tokens, [0.9, 0.95], top_k=k)
+        for a, b in zip(got, want):
+            np.testing.assert_array_equal(a, b)
