@@ -472,8 +472,10 @@ mlk_status mlk_paged_plan(const mlk_paged_pool* pool, const int32_t* new_tokens,
         return Fail(MLK_ERR_INVALID, "%s: max_seq_len must be in 1..2^30 and at most table_stride "
                                      "* page_size", fn);
     }
-    if (pool->n_seqs == 0) return MLK_OK;
-    if (new_tokens == nullptr || token_start == nullptr || !Aligned(new_tokens, 4) ||
+    // (no sequences: of the outputs only token_start[0] is written, where it is given)
+    const bool none = pool->n_seqs == 0;
+    if (none && token_start == nullptr) return MLK_OK;
+    if ((new_tokens == nullptr && !none) || token_start == nullptr || !Aligned(new_tokens, 4) ||
         !Aligned(token_start, 4) || !Aligned(positions, 4) || !Aligned(token_seq, 4)) {
         return Fail(MLK_ERR_INVALID, "%s: new_tokens and token_start must be 4-byte aligned device "
                                      "arrays, as positions and token_seq where given", fn);
@@ -483,12 +485,12 @@ mlk_status mlk_paged_plan(const mlk_paged_pool* pool, const int32_t* new_tokens,
     const void* ins[5] = {pool->page_table, pool->seq_len, pool->free_pages, pool->n_free, new_tokens};
     for (int i = 0; i < 4; ++i) {
         bool same = false;
-        for (int j = 0; j < 5; ++j) same |= outs[i] == ins[j];
+        for (int j = 0; j < 5; ++j) same |= outs[i] != nullptr && outs[i] == ins[j];
         for (int j = 0; j < i; ++j) same |= outs[i] != nullptr && outs[i] == outs[j];
         if (same) return Fail(MLK_ERR_INVALID, "%s: an output may not alias another or the pool", fn);
     }
     if (new_tokens == pool->seq_len) return Fail(MLK_ERR_INVALID, "%s: new_tokens may not alias seq_len", fn);
-    st = CheckWorkspace(fn, workspace, workspace_bytes, pool->n_seqs);
+    if (!none) st = CheckWorkspace(fn, workspace, workspace_bytes, pool->n_seqs);
     if (st != MLK_OK) return st;
     p.fresh = new_tokens;
     p.n_tokens = static_cast<int32_t>(n_tokens);
@@ -501,7 +503,7 @@ mlk_status mlk_paged_plan(const mlk_paged_pool* pool, const int32_t* new_tokens,
     p.wide = Aligned(pool->seq_len, 16) && Aligned(new_tokens, 16) && Aligned(token_start, 16);
     p.err = err;
     const hipStream_t s = AsStream(stream);
-    if (IsOwn(kOwnThreads, p.pool.n_seqs, n_tokens)) {
+    if (none || IsOwn(kOwnThreads, p.pool.n_seqs, n_tokens)) {
         hipLaunchKernelGGL((PlanScan<kOwnThreads, true>), dim3(1), dim3(kOwnThreads), 0, s, p);
         return CheckLaunch("PlanScan");
     }

@@ -495,8 +495,9 @@ typedef struct {
  *   token_seq   [n_tokens]     its sequence,
  *   slots       [n_tokens]     its cache row, page * page_size + position %
  *                              page_size (-1: page outside [0, n_pages))
- * (the last three may be NULL; rows behind the last token are left as they
- * are).  With need_s the pages that sequence s starts, it is taken in where it
+ * (the last three may be NULL; rows behind the last token are left as they are;
+ * with no sequences only token_start[0] is written, 0, and it may be NULL too).
+ * With need_s the pages that sequence s starts, it is taken in where it
  * starts none or need_0 + .. + need_s <= *n_free, and new_tokens[0] + .. +
  * new_tokens[s] <= n_tokens: first come, first served, no sequence overtakes one
  * that had to wait for pages.  One that is not taken in brings no token rows
