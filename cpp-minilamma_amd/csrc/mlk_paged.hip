@@ -571,7 +571,7 @@ int64_t mlk_attention_paged_scored_workspace_bytes(int64_t n_seqs, int64_t n_tok
                                                    int32_t head_dim,
                                                    const mlk_attention_scores* scores) {
     return AttendWorkspace(n_seqs, n_tokens, max_new_tokens, max_seq_len, n_heads, n_kv_heads,
-                           head_dim, false, ScoresOf(scores), true);
+                           head_dim, false, ScoresOf(scores), scores != nullptr);
 }
 
 int64_t mlk_attention_packed_scored_workspace_bytes(int64_t n_seqs, int64_t n_tokens,
@@ -579,7 +579,7 @@ int64_t mlk_attention_packed_scored_workspace_bytes(int64_t n_seqs, int64_t n_to
                                                     int32_t n_kv_heads, int32_t head_dim,
                                                     const mlk_attention_scores* scores) {
     return AttendWorkspace(n_seqs, n_tokens, max_seq_len, max_seq_len, n_heads, n_kv_heads,
-                           head_dim, true, ScoresOf(scores), true);
+                           head_dim, true, ScoresOf(scores), scores != nullptr);
 }
 
 int64_t mlk_attention_packed_workspace_bytes(int64_t n_seqs, int64_t n_tokens,
