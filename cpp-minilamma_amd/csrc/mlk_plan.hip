@@ -293,6 +293,7 @@ __global__ __launch_bounds__(kRowThreads) void PlanRows(const PlanArgs p) {
 }
 
 // The i-th of `total` pages given back, sequence s's k-th; `kept` pages stay.
+// (An entry that is no page goes back too: every page has its place by the lengths alone.)
 __device__ inline bool PutPage(const ReleaseArgs& p, int32_t i, int s, int32_t kept, int32_t k,
                                int32_t free, int32_t total) {
     const Pool& o = p.pool;

@@ -525,6 +525,9 @@ mlk_status mlk_paged_plan(const mlk_paged_pool* pool, const int32_t* new_tokens,
  * was.  keep[s] over seq_len[s], or a length outside 0 .. table_stride *
  * page_size, leaves the sequence as it is and raises *err.  Pages that do not
  * fit the stack (the same page held twice) are dropped and raise *err.
+ * An entry outside [0, n_pages) goes back as it is and raises *err: the pool is
+ * then damaged, a later plan hands the entry out again (its rows get slot -1, and
+ * *err is raised each time), until the caller sets the pool up anew.
  * Pages that sequences share are not counted: a shared page is given back by
  * one of them alone.  workspace as above.
  */
