@@ -824,8 +824,12 @@ struct Chooser {
 };
 
 // The largest whole number of at most a * sum for a in [0, 1), exactly; *rest: whether it is less.
-__device__ inline uint64_t Times(float a, uint64_t sum, bool* rest) {
-    const uint32_t bits = __float_as_uint(fabsf(a)), e = bits >> 23;  // a = m 2^-shift; -0 is 0
+// (The arguments are all lanes' the same: scalar work.)
+__device__ inline uint64_t Times(float a, uint64_t all_sum, bool* rest) {
+    const uint32_t bits = __builtin_amdgcn_readfirstlane(__float_as_uint(a)) & 0x7FFFFFFFu;  // -0 is 0
+    const uint64_t sum = static_cast<uint64_t>(__builtin_amdgcn_readfirstlane(static_cast<uint32_t>(all_sum >> 32))) << 32 |
+                         static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<uint32_t>(all_sum)));
+    const uint32_t e = bits >> 23;  // a = m 2^-shift
     const uint32_t m = e == 0 ? bits : (bits & 0x7FFFFFu) | 0x800000u;
     const uint32_t shift = 149 - (e == 0 ? 0 : e - 1);  // 24 .. 149
     // m * sum = high 2^32 + low
