@@ -14,7 +14,7 @@
 // its position and slot.  The row at a page's first position enters it in the
 // table; the pages a sequence held before are read there, the new ones popped by
 // index, so no row waits for another.  Integer work; what it costs is latency: plan and
-// release of 262144 rows of 4096 sequences (4.4 MB, 0.9 us at a copy's rate) take 23.4 us,
+// release of 262144 rows of 4096 sequences (4.4 MB, 0.9 us at a copy's rate) take 23.4 to 24.0 us,
 // their four kernels 7.9, 5.8, 3.2 and 6.6; of 6 rows of one sequence 9.5, two launches.
 #include "mlk_paged.h"
 

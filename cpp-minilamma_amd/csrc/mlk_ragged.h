@@ -272,7 +272,7 @@ struct RaggedParams {
 // tanh(x) / x as a polynomial in x^2 for |x| <= kTanhNear: relative errors up to 1.1e-7, the
 // least that five terms allow (fitted in float64 by reweighted least squares).  Capped scores
 // rarely come near the cap, and there it costs half of what a division does (7001 packed bf16
-// tokens in documents, 70B heads: with a quotient of polynomials 333 us, so 252).
+// tokens in documents, 70B heads: with a quotient of polynomials 333 us, so 252 to 259).
 constexpr float kTanhNear = 0.625f;
 constexpr float kTanh[5] = {0.999999893f, -0.333319542f, 0.13304526f, -0.0518218663f, 0.0150509447f};
 // Beyond: (1 - e) / (1 + e) of e = exp(-2 |x|), which is at most 0.29 there.

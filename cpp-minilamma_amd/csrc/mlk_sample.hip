@@ -31,9 +31,9 @@
 // kList logits are one launch alone, kSmall, with everything in the list.
 //
 // What bounds it: 512 fp32 rows of 128256 of mixed settings (263 MB, 56 us at a copy's rate)
-// 122 us: SampleBins 70 (with a top-k, or at temperature 0, 55: the bytes; weights cost
+// 123 to 130 us: SampleBins 67 to 70 (with a top-k, or at temperature 0, 55: the bytes; weights cost
 // the rest, float64 and additions in shared memory), cuts 8, gather 28, finish 20, as each takes
-// by itself.  64 bf16 rows 53 us, one fp32 row 28, 6 fp32 rows of 131 7: a few launches, each a
+// by itself.  64 bf16 rows 54 us, one fp32 row 28, 6 fp32 rows of 131 7: a few launches, each a
 // chain of loads, scans and barriers.
 #include "mlk_paged.h"
 
@@ -1343,7 +1343,7 @@ mlk_status Launch(SampleArgs p, int64_t n_rows, char* workspace, hipStream_t s) 
             p.largest = reinterpret_cast<float*>(p.part + rows * p.parts * kPartBytes);
             hipLaunchKernelGGL(SampleBins<T>, dim3(static_cast<unsigned>(rows * p.parts)), dim3(kThreads), 0, s, p);
             const int looks = GatherParts(p.vocab, kBytes, 1);
-            // as long as each compute unit has one workgroup of it (fp32 rows of 128256: 1 row 32.3 us by
+            // as long as each compute unit has one workgroup of it; at that edge it can be the slower (fp32 rows of 128256: 1 row 32.3 us by
             // the three launches, 27.9 by one, 8 rows 37.2 and 36.6, 16 rows 37.6 and 37.7; of 32000: 64
             // rows 31.6 and 28.8; bf16 rows of 128256, half the bytes: 16 rows 49.0 and 46.7, 32 rows 49.5
             // and 51.1)
