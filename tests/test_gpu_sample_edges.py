@@ -1,5 +1,6 @@
 """The sampler at the ends of its ranges: temperatures up to the largest number, infinities
-beside logits of any size."""
+beside logits of any size, bounds that fall exactly on a sum of equal weights, and more rows
+than a round of launches takes."""
 from __future__ import annotations
 
 import importlib
@@ -7,7 +8,7 @@ import importlib
 import numpy as np
 import pytest
 
-from test_gpu_sample import check, run, settings
+from test_gpu_sample import check, logits, mixed, run, settings
 
 pytestmark = pytest.mark.gpu
 
@@ -80,4 +81,20 @@ def test_bounds_that_equal_a_sum_beside_others(mlk, sampling, rows):
     want = np.resize([9000 + n // 2, 9000 + n // 2, 9000 + n // 4], rows)
     np.testing.assert_array_equal(tokens, want)
     np.testing.assert_allclose(probs, np.resize([1 / n, 1 / n, 2 / n], rows), rtol=2.0 ** -22)
+    assert flag == 0
+
+
+@pytest.mark.parametrize("act", ["f32", "bf16"])
+def test_more_rows_than_a_round_takes(mlk, sampling, act):
+    """2100 rows, more than twice the 1024 that a round of launches works on, and a last round of
+    few: as 60 of them choose."""
+    rng = np.random.default_rng(41)
+    V, rows = 4999, 2100
+    x, how = logits(rng, 60, V), mixed(rng, 60)
+    few = run(mlk, sampling, x, how, act)
+    check(x, how, few, act, 0.7)
+    at = rng.integers(0, 60, rows)
+    tokens, probs, flag = run(mlk, sampling, x[at], [how[i] for i in at], act, stride=V + 3, offset=1)
+    np.testing.assert_array_equal(tokens, few[0][at])
+    np.testing.assert_array_equal(probs.view(np.uint32), few[1][at].view(np.uint32))
     assert flag == 0
